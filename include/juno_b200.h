@@ -115,7 +115,15 @@ int juno_sgemv_f32(juno_ctx *ctx, const float *a_host, const float *x_host, int6
  * Replaces the per-request float[L][pos*kvDim] heap cache and the scalar gqa()
  * of LlamaTransformerHandler.java:670-733,1678-1730.  A pool holds `n_pages`
  * pages of `page_tokens` (16) positions for every layer; kv_dtype 0 = FP16,
- * 1 = FP32 (the reference's storage type). */
+ * 1 = FP32 (the reference's storage type), 3 = 4 bits (JUNO_KV_Q4).
+ *
+ * 4-bit pages hold 5 bits an element: a group is 32 neighbouring dimensions of one position and key/value head, and its values are
+ * m + d q with m its least value in FP16, d a fifteenth of its range in BF16 (0 for a range below 2^-80) and q the nearest whole number
+ * in [0, 15], half-way cases to the even one.  Values beyond the range of FP16, infinities too, are held as its largest; a NaN makes
+ * its group NaN.  head_dim 64 or 128, up to 8 query heads to a key/value head. */
+#define JUNO_KV_F16 0
+#define JUNO_KV_F32 1
+#define JUNO_KV_Q4 3
 int juno_kvpool_create(juno_ctx *ctx, int32_t n_layers, int32_t n_kv_heads, int32_t head_dim,
                        int32_t n_pages, int32_t kv_dtype, juno_kvpool **out);
 int juno_kvpool_free(juno_kvpool *p);
@@ -156,6 +164,53 @@ int juno_attn_decode(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, ju
  * No counterpart in the reference. */
 int juno_attn_decode_static(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs,
                             int32_t n_heads, const float *q_dev, float *out_dev);
+
+/* ── cache pages from device memory ─────────────────────────────────────────────
+ * The same operators for hosts that keep activations on the GPU: pointers are device memory (of the context's device, or
+ * managed), work is enqueued on `stream` (a cudaStream_t, NULL = the context's stream; cudaStreamLegacy and cudaStreamPerThread by their
+ * handles) and the call returns before it is done.  Calls of one context take effect in the order in which they are made, whatever their
+ * streams are: a call on another stream waits for what the context's stream has, and the context's stream waits for it.  The caller's own
+ * work on q, k, v and results is ordered by that stream only.  A stream that is being captured, or one of another device, gives
+ * JUNO_ERR_INVALID_ARG: a graph would hold the page table of the moment.  Working memory belongs to the context and grows with the largest
+ * call.  Arrays of sequences, positions, counts and lengths are host memory and are not used after the call.  n <= 4096.
+ * Not for pools of a model. */
+
+/* Writes counts[i] positions of keys and values, the first at positions[i] (at most the sequence's length), for every
+ * sequence, which may be there once.  k_dev and v_dev have rows of ld elements, n_kv_heads*head_dim of them used: the rows of seqs[0],
+ * then those of seqs[1] and so on.  counts[i] may be 0.  Any kv_dtype.  The weights of positions that are written start at zero. */
+int juno_kv_append_device(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs,
+                          const int32_t *positions, const int32_t *counts, const float *k_dev, const float *v_dev,
+                          int64_t ld, void *stream);
+/* The values that the pages hold for cached positions, rows as above.  Any kv_dtype. */
+int juno_kv_read_device(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs,
+                        const int32_t *positions, const int32_t *counts, float *k_dev, float *v_dev, int64_t ld,
+                        void *stream);
+/* out[i] = gqa(q[i], first lens[i] positions of seqs[i]); lens NULL = all cached ones.  A row of no positions is zero.  A sequence may be
+ * there several times (the rows of a prompt) unless it keeps weights.  Rows of q and out lie ldq and ldo elements apart.  JUNO_KV_Q4
+ * pools. */
+int juno_attn_decode_device(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs,
+                            const int32_t *lens, int32_t n_heads, const float *q_dev, int64_t ldq, float *out_dev,
+                            int64_t ldo, void *stream);
+
+/* Accumulated attention weight.  juno_kvpool_track gives a JUNO_KV_Q4 pool room for the weights of n_seqs sequences of up to
+ * max_tokens positions (n_layers*n_kv_heads*max_tokens FP32 each); once per pool.  juno_seq_track has a sequence keep them, zeros at
+ * first: from then on each decode attention over it adds, for every layer, key/value head and attended position, the softmax weights that
+ * the head's query heads gave to that position.  A fork of such a sequence has weights of its own, a copy.  JUNO_ERR_OOM when the
+ * room is taken. */
+int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens);
+int juno_seq_track(juno_seq *s);
+/* The weights of the first counts[i] positions of each sequence at one layer, w_dev [n][n_kv_heads][ld]; store != 0 sets them (a
+ * sequence that comes from elsewhere), each sequence once then. */
+int juno_kv_weights_device(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs,
+                           const int32_t *counts, float *w_dev, int64_t ld, int32_t store, void *stream);
+/* Cuts sequences that keep weights down to `keep` positions: in every layer and key/value head the newest `recent` (at most keep) stay, and
+ * of the older ones those of most weight, the earlier of two equal ones (a NaN counts least).  They move to the front in order, with
+ * their weights, and the sequence's length is `keep`; pages behind return to the pool.  Pages shared with a fork are left to it, which takes fresh ones
+ * (JUNO_ERR_OOM, and nothing has changed, when there are not enough).  Shorter sequences stay as they are.  From then on the cached
+ * positions of different heads are different tokens, in order: keys carry their rotation, so attention and further appends go on.
+ * kept_dev (or NULL): int32 [n_layers][n][n_kv_heads][keep], the places before, ascending, -1 behind a shorter sequence's. */
+int juno_kv_evict(juno_ctx *ctx, juno_kvpool *p, int32_t n, juno_seq *const *seqs, int32_t keep, int32_t recent,
+                  int32_t *kept_dev, void *stream);
 
 /* ── forward-pass operator (boundaries B and C) ───────────────────────────────
  * juno_model_* replaces the device half of LlamaTransformerHandler

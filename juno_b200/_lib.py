@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libjuno_b200.so")
 
 OK, ERR_INVALID_ARG, ERR_OOM, ERR_CUDA, ERR_NCCL, ERR_TIMEOUT, ERR_CLOSED, ERR_UNSUPPORTED = 0, -1, -2, -3, -4, -5, -6, -7
 TYPE_F32, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 8, 12, 14
+KV_F16, KV_F32, KV_Q4 = 0, 1, 3
 
 (T_TOKEN_EMBD, T_OUTPUT_NORM, T_OUTPUT, T_ATTN_NORM, T_FFN_NORM, T_ATTN_Q, T_ATTN_K, T_ATTN_V, T_ATTN_OUT,
  T_FFN_GATE, T_FFN_UP, T_FFN_DOWN) = range(12)
@@ -81,6 +82,13 @@ SIGNATURES = {
     "juno_seq_append_kv": (C.c_int, [P, I32, I32, I32, P, P]),
     "juno_attn_decode": (C.c_int, [P, P, I32, I32, PP, I32, P, P]),
     "juno_attn_decode_static": (C.c_int, [P, P, I32, I32, PP, I32, P, P]),
+    "juno_kvpool_track": (C.c_int, [P, I32, I32]),
+    "juno_seq_track": (C.c_int, [P]),
+    "juno_kv_append_device": (C.c_int, [P, P, I32, I32, PP, P, P, P, P, I64, P]),
+    "juno_kv_read_device": (C.c_int, [P, P, I32, I32, PP, P, P, P, P, I64, P]),
+    "juno_kv_weights_device": (C.c_int, [P, P, I32, I32, PP, P, P, I64, I32, P]),
+    "juno_attn_decode_device": (C.c_int, [P, P, I32, I32, PP, P, I32, P, I64, P, I64, P]),
+    "juno_kv_evict": (C.c_int, [P, P, I32, PP, I32, I32, P, P]),
     "juno_tp_slice": (C.c_int, [I32, I32, I32, I32, I32, I32, I32, I32, C.POINTER(I64)]),
     "juno_nccl_unique_id": (C.c_int, [P]),
     "juno_model_create": (C.c_int, [P, C.POINTER(ModelCfg), PP]),

@@ -12,6 +12,8 @@
 #include <type_traits>
 
 #include "attn.cuh"
+#include "cache_ops.cuh"
+#include "q4_pages.cuh"
 
 namespace juno {
 
@@ -904,7 +906,7 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
     JUNO_REQUIRE(n_layers > 0 && n_kv_heads > 0 && n_pages > 0 && max_slots > 0 && max_pages_per_seq > 0,
                  "bad KV pool geometry");
     JUNO_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim %d is not supported (64, 128)", head_dim);
-    JUNO_REQUIRE(dtype == 0 || dtype == 1, "kv_dtype %d (0 = f16, 1 = f32)", dtype);
+    JUNO_REQUIRE(dtype == 0 || dtype == 1 || dtype == kKvQ4, "kv_dtype %d (0 = f16, 1 = f32, 3 = 4 bits)", dtype);
     juno_kvpool *p = new juno_kvpool();
     p->magic = kMagicPool;
     p->ctx = ctx;
@@ -914,25 +916,25 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
     p->n_pages = n_pages;
     p->dtype = dtype;
     p->page_tokens = kPageTokens;
-    p->elem_bytes = dtype == 0 ? 2 : 4;
+    p->elem_bytes = dtype == 0 ? 2 : dtype == 1 ? 4 : 0;  // 4-bit pages are counted in blocks
     p->max_slots = max_slots;
     p->max_pages_per_seq = max_pages_per_seq;
     p->k = p->v = nullptr;
     p->d_table = p->h_table = nullptr;
     p->owned_by_model = 0;
-    const size_t bytes = (size_t)n_layers * n_pages * n_kv_heads * kPageTokens * head_dim * p->elem_bytes;
+    const size_t bytes = (size_t)n_layers * p->page_bytes() * n_pages;
     const size_t tbytes = (size_t)max_slots * max_pages_per_seq * sizeof(int32_t);
     cudaError_t e = cudaMalloc(&p->k, bytes);
-    if (e == cudaSuccess) e = cudaMalloc(&p->v, bytes);
+    if (e == cudaSuccess && dtype != kKvQ4) e = cudaMalloc(&p->v, bytes);
     if (e == cudaSuccess) e = cudaMalloc((void **)&p->d_table, tbytes);
     if (e == cudaSuccess) e = cudaMallocHost((void **)&p->h_table, tbytes);
     if (e == cudaSuccess) e = cudaMemsetAsync(p->d_table, 0, tbytes, ctx->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(p->k, 0, bytes, ctx->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p->v, 0, bytes, ctx->stream);
+    if (e == cudaSuccess && p->v) e = cudaMemsetAsync(p->v, 0, bytes, ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
-        set_error("cudaMalloc of the KV pool (2 x %zu bytes) failed: %s", bytes, cudaGetErrorString(e));
+        set_error("cudaMalloc of the KV pool (%s%zu bytes) failed: %s", dtype == kKvQ4 ? "" : "2 x ", bytes, cudaGetErrorString(e));
         if (p->k) cudaFree(p->k);
         if (p->v) cudaFree(p->v);
         if (p->d_table) cudaFree(p->d_table);
@@ -1026,6 +1028,8 @@ int kvpool_destroy(juno_kvpool *p) {
     cudaFree(p->k);
     cudaFree(p->v);
     if (p->state) cudaFree(p->state);
+    if (p->weights) cudaFree(p->weights);
+    p->weights = nullptr;
     cudaFree(p->d_table);
     cudaFreeHost(p->h_table);
     p->state = nullptr;
@@ -1054,6 +1058,32 @@ int seq_create(juno_kvpool *p, int max_tokens, juno_seq **out) {
     return JUNO_OK;
 }
 
+// Entries [lo, hi] of the sequence's row of the page table, from the mirror to the device.  The calls on a pool of its own return before the device
+// is done with them, and the mirror may have changed again by then: the entries travel with the launch.  A model's calls wait for their work.
+struct TableWords {
+    int32_t v[480];
+};
+static __global__ void table_store_kernel(int32_t *dst, const TableWords w, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = w.v[i];
+}
+int table_store(const juno_kvpool *p, int slot, int lo, int hi, cudaStream_t st) {
+    const size_t at = (size_t)slot * p->max_pages_per_seq;
+    if (p->latent || p->owned_by_model) {
+        JUNO_CUDA_TRY(cudaMemcpyAsync(p->d_table + at + lo, p->h_table + at + lo, (size_t)(hi - lo + 1) * sizeof(int32_t), cudaMemcpyHostToDevice, st));
+        return JUNO_OK;
+    }
+    constexpr int kWords = (int)(sizeof(TableWords) / sizeof(int32_t));
+    for (; lo <= hi; lo += kWords) {
+        TableWords w;
+        const int n = std::min(kWords, hi - lo + 1);
+        memcpy(w.v, p->h_table + at + lo, (size_t)n * sizeof(int32_t));
+        table_store_kernel<<<1, 128, 0, st>>>(p->d_table + at + lo, w, n);
+        JUNO_CUDA_TRY(cudaGetLastError());
+        p->ctx->kernel_launches++;
+    }
+    return JUNO_OK;
+}
+
 // Copies one page (all layers, K and V) to another on the device, ordered on `st`.
 static int page_copy(juno_kvpool *p, int dst, int src, cudaStream_t st) {
     if (p->latent) {
@@ -1064,11 +1094,11 @@ static int page_copy(juno_kvpool *p, int dst, int src, cudaStream_t st) {
         }
         return JUNO_OK;
     }
-    const size_t page_bytes = (size_t)p->n_kv_heads * kPageTokens * p->head_dim * p->elem_bytes;
+    const size_t page_bytes = p->page_bytes();
     for (int layer = 0; layer < p->n_layers; layer++) {
         const size_t d = ((size_t)layer * p->n_pages + dst) * page_bytes, s = ((size_t)layer * p->n_pages + src) * page_bytes;
         JUNO_CUDA_TRY(cudaMemcpyAsync(static_cast<uint8_t *>(p->k) + d, static_cast<const uint8_t *>(p->k) + s, page_bytes, cudaMemcpyDeviceToDevice, st));
-        JUNO_CUDA_TRY(cudaMemcpyAsync(static_cast<uint8_t *>(p->v) + d, static_cast<const uint8_t *>(p->v) + s, page_bytes, cudaMemcpyDeviceToDevice, st));
+        if (p->v) JUNO_CUDA_TRY(cudaMemcpyAsync(static_cast<uint8_t *>(p->v) + d, static_cast<const uint8_t *>(p->v) + s, page_bytes, cudaMemcpyDeviceToDevice, st));
     }
     return JUNO_OK;
 }
@@ -1112,12 +1142,31 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st) {
         lo = std::min(lo, i);
         hi = std::max(hi, i);
     }
-    JUNO_CUDA_TRY(cudaMemcpyAsync(p->d_table + (size_t)s->slot * p->max_pages_per_seq + lo, row + lo,
-                                  (size_t)(hi - lo + 1) * sizeof(int32_t), cudaMemcpyHostToDevice, st));
+    return table_store(p, s->slot, lo, hi, st);
+}
+
+// Gives the sequence one of the pool's weight planes: zeros, or what `src` holds for the positions that both have.
+static int seq_track(juno_seq *s, const juno_seq *src) {
+    juno_kvpool *p = s->pool;
+    JUNO_REQUIRE(s->max_tokens <= p->track_tokens, "a sequence of up to %d positions does not fit the pool's weights (juno_kvpool_track: %d)", s->max_tokens,
+                 p->track_tokens);
+    if (p->free_tracks.empty()) {
+        set_error("no free weights for another sequence");
+        return JUNO_ERR_OOM;
+    }
+    const int track = p->free_tracks.back();
+    const size_t pitch = (size_t)p->track_tokens * sizeof(float), planes = (size_t)p->n_layers * p->n_kv_heads;
+    float *own = p->weights + track * p->track_stride();
+    JUNO_CUDA_TRY(cudaMemsetAsync(own, 0, pitch * planes, p->ctx->stream));
+    if (src && s->len)
+        JUNO_CUDA_TRY(cudaMemcpy2DAsync(own, pitch, p->weights + src->track * p->track_stride(), pitch, (size_t)s->len * sizeof(float), planes,
+                                        cudaMemcpyDeviceToDevice, p->ctx->stream));
+    p->free_tracks.pop_back();
+    s->track = track;
     return JUNO_OK;
 }
 
-static int seq_check(juno_seq *s) {
+int seq_check(const juno_seq *s) {
     if (!s) {
         set_error("sequence is null");
         return JUNO_ERR_INVALID_ARG;
@@ -1179,6 +1228,8 @@ int juno_seq_free(juno_seq *s) {
     for (int pg : s->pages)
         if (--p->page_refs[(size_t)pg] == 0) p->free_pages.push_back(pg);  // a shared page stays with its other holders
     p->free_slots.push_back(s->slot);
+    if (s->track >= 0) p->free_tracks.push_back(s->track);
+    s->track = -1;
     s->pages.clear();
     s->magic = kMagicDead;
     return JUNO_OK;
@@ -1214,19 +1265,57 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
         row[i] = pg;
     }
     s->len = n_tokens;
-    if (n_pg) {
-        cudaError_t e = cudaMemcpyAsync(p->d_table + (size_t)s->slot * p->max_pages_per_seq, row, (size_t)n_pg * sizeof(int32_t),
-                                        cudaMemcpyHostToDevice, p->ctx->stream);
-        if (e != cudaSuccess) {
-            for (int pg : s->pages) p->page_refs[(size_t)pg]--;
-            p->free_slots.push_back(s->slot);
-            s->magic = kMagicDead;
-            delete s;
-            JUNO_CUDA_TRY(e);
-        }
+    int rc = n_pg ? table_store(p, s->slot, 0, n_pg - 1, p->ctx->stream) : JUNO_OK;
+    if (rc == JUNO_OK && src->track >= 0) rc = seq_track(s, src);
+    if (rc != JUNO_OK) {
+        for (int pg : s->pages) p->page_refs[(size_t)pg]--;
+        p->free_slots.push_back(s->slot);
+        s->magic = kMagicDead;
+        delete s;
+        return rc;
     }
     *out = s;
     return JUNO_OK;
+}
+
+int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens) {
+    JUNO_REQUIRE(p, "pool is null");
+    if (p->magic != kMagicPool) {
+        set_error("KV pool is closed");
+        return JUNO_ERR_CLOSED;
+    }
+    if (p->dtype != kKvQ4) {
+        set_error("weights are kept for pools of 4-bit pages");
+        return JUNO_ERR_UNSUPPORTED;
+    }
+    JUNO_REQUIRE(!p->owned_by_model, "this pool belongs to a model");
+    JUNO_REQUIRE(n_seqs >= 1 && n_seqs <= p->max_slots, "n_seqs %d outside [1,%d]", n_seqs, p->max_slots);
+    JUNO_REQUIRE(max_tokens >= 1 && max_tokens <= p->max_pages_per_seq * kPageTokens, "max_tokens %d outside [1,%d]", max_tokens,
+                 p->max_pages_per_seq * kPageTokens);
+    std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
+    JUNO_REQUIRE(!p->weights, "this pool keeps weights already");
+    DeviceGuard g(p->ctx->device);
+    const int room = (max_tokens + kPageTokens - 1) / kPageTokens * kPageTokens;
+    const size_t bytes = (size_t)n_seqs * p->n_layers * p->n_kv_heads * room * sizeof(float);
+    const cudaError_t e = cudaMalloc((void **)&p->weights, bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        p->weights = nullptr;
+        set_error("cudaMalloc of %zu bytes of attention weights failed: %s", bytes, cudaGetErrorString(e));
+        return e == cudaErrorMemoryAllocation ? JUNO_ERR_OOM : JUNO_ERR_CUDA;
+    }
+    p->track_tokens = room;
+    for (int i = n_seqs - 1; i >= 0; i--) p->free_tracks.push_back(i);
+    return JUNO_OK;
+}
+
+int juno_seq_track(juno_seq *s) {
+    JUNO_TRY(seq_check(s));
+    std::lock_guard<std::recursive_mutex> lk(s->pool->ctx->mu);
+    JUNO_REQUIRE(s->pool->weights, "the pool keeps no weights (juno_kvpool_track)");
+    JUNO_REQUIRE(s->track < 0, "this sequence keeps its weights already");
+    DeviceGuard g(s->pool->ctx->device);
+    return seq_track(s, nullptr);
 }
 
 int juno_seq_length(juno_seq *s, int32_t *n_tokens) {
@@ -1245,6 +1334,7 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     JUNO_REQUIRE(!p->latent, "this sequence belongs to a model with latent pages: it has no K and V to append");
     JUNO_REQUIRE(layer >= 0 && layer < p->n_layers, "layer %d out of range", layer);
     JUNO_REQUIRE(pos >= 0 && n_tokens >= 0, "bad position range");
+    JUNO_REQUIRE(p->dtype != kKvQ4 || pos <= s->len, "position %d is not behind the %d cached ones", pos, s->len);
     if (n_tokens == 0) return JUNO_OK;
     std::lock_guard<std::recursive_mutex> lk(c->mu);
     DeviceGuard g(c->device);
@@ -1261,14 +1351,17 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     const size_t total = (size_t)n_tokens * kvdim;
     const unsigned blocks = (unsigned)((total + 255) / 256);
     const int32_t *row = p->d_table + (size_t)s->slot * p->max_pages_per_seq;
-    if (p->dtype == 0)
+    if (p->dtype == kKvQ4) {
+        const CacheRow r{s->slot, pos, 0, s->track};
+        JUNO_TRY(launch_kv_append(c, p, layer, &r, 1, n_tokens, c->stage_x, c->stage_y, kvdim, c->stream));
+    } else if (p->dtype == 0)
         kv_scatter_kernel<__half><<<blocks, 256, 0, c->stream>>>(p->k, p->v, row, p->n_pages, p->n_kv_heads, p->head_dim,
                                                                   layer, pos, n_tokens, c->stage_x, c->stage_y);
     else
         kv_scatter_kernel<float><<<blocks, 256, 0, c->stream>>>(p->k, p->v, row, p->n_pages, p->n_kv_heads, p->head_dim,
                                                                  layer, pos, n_tokens, c->stage_x, c->stage_y);
     JUNO_CUDA_TRY(cudaGetLastError());
-    c->kernel_launches++;
+    if (p->dtype != kKvQ4) c->kernel_launches++;
     JUNO_CUDA_TRY(cudaStreamSynchronize(c->stream));
     c->h2d_bytes += (int64_t)(2 * bytes);
     s->len = std::max(s->len, pos + n_tokens);
@@ -1301,8 +1394,22 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
         max_len = std::max(max_len, seqs[i]->len);
     }
     const int hd = p->head_dim, qdim = n_heads * hd;
-    const int n_splits = attn_pick_splits(c, p, n, max_len);
     const size_t qbytes = (size_t)n * qdim * sizeof(float);
+    if (p->dtype == kKvQ4) {
+        void *px = c->stage_x, *py = c->stage_y;
+        JUNO_TRY(ensure_device(&px, &c->stage_x_bytes, qbytes));
+        c->stage_x = (float *)px;
+        JUNO_TRY(ensure_device(&py, &c->stage_y_bytes, qbytes));
+        c->stage_y = (float *)py;
+        JUNO_CUDA_TRY(cudaMemcpyAsync(c->stage_x, q_host, qbytes, cudaMemcpyHostToDevice, c->stream));
+        JUNO_TRY(q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, c->stream));
+        JUNO_CUDA_TRY(cudaMemcpyAsync(out_host, c->stage_y, qbytes, cudaMemcpyDeviceToHost, c->stream));
+        JUNO_CUDA_TRY(cudaStreamSynchronize(c->stream));
+        c->h2d_bytes += (int64_t)qbytes;
+        c->d2h_bytes += (int64_t)qbytes;
+        return JUNO_OK;
+    }
+    const int n_splits = attn_pick_splits(c, p, n, max_len);
     const size_t scratch = attn_scratch_floats(n, n_heads, hd, n_splits) * sizeof(float);
     const size_t meta_bytes = meta.size() * sizeof(int32_t);
     // stage_x: q | meta ; stage_y: out | scratch
@@ -1363,6 +1470,10 @@ int juno_attn_decode_static(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t 
     JUNO_REQUIRE(n_heads > 0 && n_heads % p->n_kv_heads == 0, "n_heads %d is not a multiple of n_kv_heads %d", n_heads,
                  p->n_kv_heads);
     JUNO_REQUIRE(c->device >= 0 && c->device < 64, "device ordinal %d not supported here", c->device);
+    if (p->dtype == kKvQ4) {
+        set_error("the allocation-free entry point serves FP16 and FP32 pages");
+        return JUNO_ERR_UNSUPPORTED;
+    }
     // Two contexts of one device share the array: the per-device lock is held until this call's kernels have drained.
     std::lock_guard<std::mutex> dev_lock(g_static_attn_mu[c->device]);
     std::lock_guard<std::recursive_mutex> lk(c->mu);

@@ -4,7 +4,11 @@
 
 #include "common.cuh"
 
-// Page layout (both K and V): [layer][page][kv_head][page_tokens=16][head_dim], FP16 or FP32.
+// Page layout (both K and V): [layer][page][kv_head][page_tokens=16][head_dim], FP16 or FP32.  A 4-bit pool has the keys and values of a head and
+// page in one block (q4_pages.cuh): [layer][page][kv_head][block] in `k`, `v` is null.
+//
+// A pool can hold, for up to track_seqs sequences, the attention weight that each cached position has received: [sequence][layer][kv_head][track_tokens]
+// FP32 (juno_kvpool_track).
 //
 // A LATENT pool keeps one row per position and layer instead (attention whose keys and values are linear in a small latent):
 // only `k` exists, layer l is the plane [page][page_tokens][row_width[l]] that starts at element row_off[l], BF16 or FP32.
@@ -14,7 +18,7 @@
 struct juno_kvpool {
     uint32_t magic;
     juno_ctx *ctx;
-    int n_layers, n_kv_heads, head_dim, n_pages, dtype;  // dtype 0 = f16, 1 = f32, 2 = bf16 (latent pools only)
+    int n_layers, n_kv_heads, head_dim, n_pages, dtype;  // dtype 0 = f16, 1 = f32, 2 = bf16 (latent pools only), 3 = 4 bits
     bool latent = false;
     std::vector<int> row_width;
     std::vector<size_t> row_off;
@@ -30,6 +34,14 @@ struct juno_kvpool {
     int32_t *d_table, *h_table;
     std::vector<int> free_slots;
     int owned_by_model;
+    float *weights = nullptr;
+    int track_tokens = 0;
+    std::vector<int> free_tracks;
+    // bytes of a cached position and key/value head, key and value together
+    double row_bytes() const { return dtype == 3 ? 1.25 * head_dim : 2.0 * head_dim * elem_bytes; }
+    // bytes of a page and layer: of keys and of values each, of both together for 4 bits
+    size_t page_bytes() const { return (size_t)n_kv_heads * head_dim * (dtype == 3 ? 20 : page_tokens * elem_bytes); }
+    size_t track_stride() const { return (size_t)n_layers * n_kv_heads * track_tokens; }
 };
 
 struct juno_seq {
@@ -39,6 +51,7 @@ struct juno_seq {
     int len;   // positions written so far (highest position + 1)
     int slot;  // row of the pool's page table
     std::vector<int> pages;
+    int track = -1;  // which of the pool's weight planes this sequence has
 };
 
 namespace juno {
@@ -97,5 +110,8 @@ int seq_create(juno_kvpool *p, int max_tokens, juno_seq **out);
 // Makes the positions [from, upto) of the sequence writable: allocates missing pages and gives the sequence a private
 // copy of every page of the range that it shares with another sequence (copy-on-write, ordered on `st`).
 int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st);
+// Entries [lo, hi] of a row of the page table, from the mirror to the device, ordered on `st`.
+int table_store(const juno_kvpool *p, int slot, int lo, int hi, cudaStream_t st);
+int seq_check(const juno_seq *s);  // JUNO_ERR_CLOSED for a handle that was freed
 
 }  // namespace juno

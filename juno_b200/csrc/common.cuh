@@ -89,6 +89,10 @@ struct juno_ctx {
     size_t stage_x_bytes = 0, stage_y_bytes = 0;
     void *pinned = nullptr;
     size_t pinned_bytes = 0;
+    // working memory of the calls on cache pages that take a stream, and the events that order them (cache_ops.cuh)
+    void *cache_scratch = nullptr;
+    size_t cache_scratch_bytes = 0;
+    cudaEvent_t cache_events[2] = {nullptr, nullptr};
     // per-kernel timing (off by default): event pairs around launches, summed at read time
     bool profiling = false;
     std::vector<juno::ProfSpan> prof_spans;

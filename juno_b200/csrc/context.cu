@@ -249,6 +249,9 @@ int juno_ctx_destroy(juno_ctx *c) {
     if (c->stage_x) cudaFree(c->stage_x);
     if (c->stage_y) cudaFree(c->stage_y);
     if (c->pinned) cudaFreeHost(c->pinned);
+    if (c->cache_scratch) cudaFree(c->cache_scratch);
+    for (cudaEvent_t e : c->cache_events)
+        if (e) cudaEventDestroy(e);
     cudaStreamDestroy(c->stream);
     {
         HostPool &h = host_pool();

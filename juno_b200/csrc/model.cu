@@ -754,6 +754,7 @@ extern "C" int juno_model_finalize(juno_model *m) {
     const int max_pages_per_seq = (f.max_ctx + kPageTokens - 1) / kPageTokens;
     const long long want_pages = (long long)f.max_seqs * max_pages_per_seq;
     JUNO_REQUIRE(want_pages < (1ll << 31), "KV pool too large");
+    JUNO_REQUIRE(f.kv_dtype == 0 || f.kv_dtype == 1, "kv_dtype %d (0 = f16, 1 = f32)", f.kv_dtype);
     JUNO_TRY(kvpool_create(c, f.n_layers, m->kv_loc, hd, (int)want_pages, f.kv_dtype, f.max_seqs, max_pages_per_seq,
                            &m->pool));
     m->pool->owned_by_model = 1;

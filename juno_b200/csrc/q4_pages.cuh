@@ -1,0 +1,52 @@
+// 4-bit cache pages: layout and arithmetic.
+//
+// A group is kQ4Group neighbouring dimensions of one position and key/value head.  Its values are held as m + d q:
+//   lo, hi   least and largest value (clamped to the range of FP16)
+//   m        lo in FP16, d  (hi - lo) / 15 in BF16; 0 where hi - lo is below 2^-80
+//   q        the whole number in [0, 15] nearest to (x - m) / d, ties to the even one, decided exactly
+// d in BF16 has the whole FP32 range and widens with one AND; its 8 bits cost nothing, as q is found for the rounded d (the largest value of
+// a group lies at most 15 d 2^-8 beyond the last number).  m needs the digits more: in FP16 a group far from zero loses what FP16 pages lose.
+// A NaN makes its group NaN (m is NaN, d 0).
+//
+// The pages of a head (16 positions) are one block of 20 * hd bytes, [layer][page][kv_head] in the pool:
+//   keys    codes    word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group
+//           factors  word [position][group]: m in the low half, d in the high one
+//   values  codes    half word [position / 2][u][group][position % 2], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group
+//           factors  as for keys
+// so that lane (g, t) of a warp finds at 16 * lane (8 * lane for heads of 64) what the MMAs of decode attention want of it: for keys of position g its four (two)
+// groups' numbers, for values two positions of unit g.
+#pragma once
+#include <stdint.h>
+#include <string.h>
+
+#include "layout.cuh"
+
+namespace juno {
+
+constexpr int kQ4Group = 32;
+constexpr int kKvQ4 = 3;  // juno_kvpool::dtype
+
+JHD int q4_block_bytes(int hd) { return 20 * hd; }
+JHD int q4_k_code(int hd, int p, int t, int g) { return ((p * 4 + t) * (hd / kQ4Group) + g) * 4; }
+JHD int q4_k_factors(int hd, int p, int g) { return 8 * hd + (p * (hd / kQ4Group) + g) * 4; }
+JHD int q4_v_code(int hd, int p, int u, int g) { return 10 * hd + (((p >> 1) * 8 + u) * (hd / kQ4Group) + g) * 4 + (p & 1) * 2; }
+JHD int q4_v_factors(int hd, int p, int g) { return 18 * hd + (p * (hd / kQ4Group) + g) * 4; }
+// Where number e of the eight of a key word lies: an AND with 0x000f000f leaves numbers 0 and 1 as the halves of an operand register, the
+// next ones follow at 4, 8 and 12 bits.
+JHD int q4_k_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }
+
+// The number of x in a group with offset m and step d (inv is about 1 / d).  s + r is x - m exactly; half-way points (q + 1/2) d have 13 bits and
+// are exact, so that the comparisons decide exactly what the estimate may have missed by one.
+JHD int q4_number(float x, float m, float d, float inv) {
+    if (!(d > 0.f)) return 0;
+    const float s = x - m, a = s - x, r = (x - (s - a)) + (-m - a);
+    const float guess = s * inv + 0.5f;
+    int q = guess >= 15.f ? 15 : guess > 0.f ? (int)guess : 0;
+    const float above = ((float)q + 0.5f) * d, below = ((float)q - 0.5f) * d;
+    if (s > above || (s == above && (r > 0.f || (r == 0.f && (q & 1))))) q++;
+    else if (s < below || (s == below && (r < 0.f || (r == 0.f && (q & 1))))) q--;
+    return q < 0 ? 0 : q > 15 ? 15 : q;
+}
+constexpr float kQ4Most = 65504.f, kQ4Nothing = 8.271806125530277e-25f;  // 2^-80
+
+}  // namespace juno

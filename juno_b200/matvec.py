@@ -172,24 +172,69 @@ class B200MatVec:
         return out
 
 
-class PagedKvCache:
-    """Device-resident paged KV pool + per-request sequences, with the GQA decode attention operator."""
+def _device_ptr(x, name: str, rows: int, width: int, dtype: str = "float32"):
+    """(address, row stride) of a CUDA tensor (anything with data_ptr, dtype, shape and stride) that holds `rows` rows of `width` elements."""
+    if not hasattr(x, "data_ptr"):
+        raise ValueError(f"{name} is not a tensor in device memory")
+    if str(x.dtype).rsplit(".", 1)[-1] != dtype or not x.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor of {dtype} is wanted")
+    if x.dim() != 2 or x.shape[0] != rows or x.shape[1] != width or (width > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < width):
+        raise ValueError(f"{name}: shape [{rows}, {width}] with neighbouring elements in a row is wanted, not {list(x.shape)} with strides {list(x.stride())}")
+    return x.data_ptr(), (x.stride(0) if rows > 1 else width)
 
-    def __init__(self, ctx: GpuContext, n_layers: int, n_kv_heads: int, head_dim: int, n_pages: int, kv_dtype: str = "f16"):
+
+class SequenceBatch:
+    """Sequences of one cache in the order in which a step names them."""
+
+    def __init__(self, seqs):
+        self.n = len(seqs)
+        self.handles = (C.c_void_p * self.n)(*[s.value if isinstance(s, C.c_void_p) else s for s in seqs])
+
+
+class PagedKvCache:
+    """Device-resident paged KV pool + per-request sequences, with the GQA decode attention operator.
+
+    kv_dtype "f16", "f32", or "q4": 4-bit pages (JUNO_KV_Q4 in include/juno_b200.h), 5 bits an element.  track_seqs > 0 gives a "q4" pool room for
+    the attention weights of that many sequences of up to track_tokens positions; `evict` cuts such sequences down by them.
+
+    The *_device calls take CUDA tensors and return before the work is done; `stream` is a cudaStream_t as an integer or an object with
+    `cuda_stream`, None the context's stream.  The legacy default stream, whose handle is 0, is meant by 0."""
+
+    def __init__(self, ctx: GpuContext, n_layers: int, n_kv_heads: int, head_dim: int, n_pages: int, kv_dtype: str = "f16",
+                 track_seqs: int = 0, track_tokens: int = 0):
         self.ctx, self._L = ctx, ctx._L
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
         h = C.c_void_p()
         check(self._L.juno_kvpool_create(ctx.handle, n_layers, n_kv_heads, head_dim, n_pages,
-                                         {"f16": 0, "f32": 1}[kv_dtype], C.byref(h)), "juno_kvpool_create")
+                                         {"f16": _lib.KV_F16, "f32": _lib.KV_F32, "q4": _lib.KV_Q4}[kv_dtype], C.byref(h)), "juno_kvpool_create")
         self.handle = h
+        if track_seqs:
+            try:
+                check(self._L.juno_kvpool_track(h, track_seqs, track_tokens), "juno_kvpool_track")
+            except Exception:
+                self.close()
+                raise
 
-    def new_sequence(self, max_tokens: int):
+    def new_sequence(self, max_tokens: int, track: bool = False):
+        """track: the sequence keeps the attention weight that each of its positions receives."""
         h = C.c_void_p()
         check(self._L.juno_kvseq_create(self.handle, max_tokens, C.byref(h)), "juno_kvseq_create")
+        if track:
+            try:
+                check(self._L.juno_seq_track(h), "juno_seq_track")
+            except Exception:
+                self._L.juno_seq_free(h)
+                raise
         return h
 
     def free_sequence(self, seq) -> None:
         check(self._L.juno_seq_free(seq), "juno_seq_free")
+
+    def fork(self, seq, n_tokens: int):
+        """A sequence that starts with the first n_tokens cached positions of another one (juno_seq_fork)."""
+        h = C.c_void_p()
+        check(self._L.juno_seq_fork(seq, int(n_tokens), C.byref(h)), "juno_seq_fork")
+        return h
 
     def length(self, seq) -> int:
         n = C.c_int32()
@@ -208,6 +253,73 @@ class PagedKvCache:
         check(self._L.juno_attn_decode(self.ctx.handle, self.handle, layer, len(seqs), arr, n_heads, _ptr(q), _ptr(out)),
               "juno_attn_decode")
         return out
+
+    # ── device memory in and out ───────────────────────────────────────────────
+    @staticmethod
+    def batch(seqs) -> SequenceBatch:
+        """Sequences that several calls name together; every call takes one in the place of a list."""
+        return seqs if isinstance(seqs, SequenceBatch) else SequenceBatch(seqs)
+
+    @staticmethod
+    def _ints(x, n: int, name: str) -> np.ndarray:
+        a = np.ascontiguousarray(x, dtype=np.int32)
+        if a.shape != (n,):
+            raise ValueError(f"{name}: {n} whole numbers are wanted, not shape {a.shape}")
+        return a
+
+    @staticmethod
+    def _stream(stream):
+        if stream is None:
+            return None
+        return int(getattr(stream, "cuda_stream", stream)) or 1  # cudaStreamLegacy
+
+    def _rows(self, seqs, positions, counts, k, v):
+        b = self.batch(seqs)
+        positions, counts = self._ints(positions, b.n, "positions"), self._ints(counts, b.n, "counts")
+        rows, width = int(counts.sum()), self.n_kv_heads * self.head_dim
+        (kp, ld), (vp, ldv) = _device_ptr(k, "k", rows, width), _device_ptr(v, "v", rows, width)
+        if ld != ldv:
+            raise ValueError(f"the rows of k and v lie {ld} and {ldv} elements apart")
+        return b, positions, counts, kp, vp, ld
+
+    def append_device(self, layer: int, seqs, positions, counts, k, v, stream=None) -> None:
+        """counts[i] new positions of sequence i, the first at positions[i]; k, v: [sum of counts, n_kv_heads * head_dim] (juno_kv_append_device)."""
+        b, positions, counts, kp, vp, ld = self._rows(seqs, positions, counts, k, v)
+        check(self._L.juno_kv_append_device(self.ctx.handle, self.handle, layer, b.n, b.handles, _ptr(positions), _ptr(counts), kp, vp, ld,
+                                            self._stream(stream)), "juno_kv_append_device")
+
+    def read_device(self, layer: int, seqs, positions, counts, k, v, stream=None) -> None:
+        """What the pages hold for cached positions, into k and v (juno_kv_read_device)."""
+        b, positions, counts, kp, vp, ld = self._rows(seqs, positions, counts, k, v)
+        check(self._L.juno_kv_read_device(self.ctx.handle, self.handle, layer, b.n, b.handles, _ptr(positions), _ptr(counts), kp, vp, ld,
+                                          self._stream(stream)), "juno_kv_read_device")
+
+    def attention_device(self, layer: int, seqs, q, n_heads: int, out, lens=None, stream=None) -> None:
+        """Decode attention over 4-bit pages; q, out: [sequences, n_heads * head_dim] (juno_attn_decode_device)."""
+        b = self.batch(seqs)
+        (qp, ldq), (op, ldo) = (_device_ptr(x, name, b.n, n_heads * self.head_dim) for x, name in ((q, "q"), (out, "out")))
+        check(self._L.juno_attn_decode_device(self.ctx.handle, self.handle, layer, b.n, b.handles, None if lens is None else _ptr(self._ints(lens, b.n, "lens")),
+                                              n_heads, qp, ldq, op, ldo, self._stream(stream)), "juno_attn_decode_device")
+
+    def weights_device(self, layer: int, seqs, counts, w, store: bool = False, stream=None) -> None:
+        """The weights of the first counts[i] positions of each sequence into w [sequences, n_kv_heads, at least most counts], or from it
+        (juno_kv_weights_device)."""
+        b = self.batch(seqs)
+        if not (hasattr(w, "data_ptr") and w.dim() == 3 and tuple(w.shape[:2]) == (b.n, self.n_kv_heads) and w.is_contiguous()):
+            raise ValueError(f"w: a contiguous tensor [{b.n}, {self.n_kv_heads}, positions] is wanted")
+        wp, ld = _device_ptr(w.view(b.n * self.n_kv_heads, w.shape[2]), "w", b.n * self.n_kv_heads, w.shape[2])
+        check(self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, _ptr(self._ints(counts, b.n, "counts")), wp, ld,
+                                             1 if store else 0, self._stream(stream)), "juno_kv_weights_device")
+
+    def evict(self, seqs, keep: int, recent: int = 0, kept=None, stream=None) -> None:
+        """Cuts sequences down to the `keep` positions of most weight, the newest `recent` among them, in every layer and key/value head; kept:
+        int32 [n_layers, sequences, n_kv_heads, keep] gets their places (juno_kv_evict)."""
+        b, kp = self.batch(seqs), None
+        if kept is not None:
+            if not (hasattr(kept, "data_ptr") and tuple(kept.shape) == (self.n_layers, b.n, self.n_kv_heads, keep) and kept.is_contiguous()):
+                raise ValueError(f"kept: a contiguous tensor [{self.n_layers}, {b.n}, {self.n_kv_heads}, {keep}] is wanted")
+            kp = _device_ptr(kept.view(-1, keep), "kept", self.n_layers * b.n * self.n_kv_heads, keep, "int32")[0]
+        check(self._L.juno_kv_evict(self.ctx.handle, self.handle, b.n, b.handles, keep, recent, kp, self._stream(stream)), "juno_kv_evict")
 
     def close(self) -> None:
         if self.handle is not None:

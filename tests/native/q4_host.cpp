@@ -1,0 +1,28 @@
+// Test-only host build of the layout and arithmetic of 4-bit cache pages (csrc/q4_pages.cuh): the functions that the device kernels call.
+#include "../../juno_b200/csrc/q4_pages.cuh"
+
+using namespace juno;
+
+extern "C" int q4_host_number(float x, float m, float d) { return q4_number(x, m, d, 1.f / d); }
+extern "C" int q4_host_block_bytes(int hd) { return q4_block_bytes(hd); }
+
+// Marks every half byte of a block that a number takes and every byte of its factors; returns how many were marked twice, or lie outside.
+extern "C" int q4_host_cover(int hd, unsigned char *nibbles) {
+    int twice = 0;
+    const int size = 2 * q4_block_bytes(hd);
+    auto mark = [&](int nibble) {
+        if (nibble < 0 || nibble >= size || nibbles[nibble]++) twice++;
+    };
+    for (int p = 0; p < 16; p++)
+        for (int g = 0; g < hd / kQ4Group; g++) {
+            for (int t = 0; t < 4; t++)
+                for (int e = 0; e < 8; e++) mark(2 * q4_k_code(hd, p, t, g) + q4_k_shift(e) / 4);
+            for (int u = 0; u < 8; u++)
+                for (int i = 0; i < 4; i++) mark(2 * q4_v_code(hd, p, u, g) + i);
+            for (int b = 0; b < 8; b++) {
+                mark(2 * q4_k_factors(hd, p, g) + b);
+                mark(2 * q4_v_factors(hd, p, g) + b);
+            }
+        }
+    return twice;
+}
