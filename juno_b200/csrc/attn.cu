@@ -1402,9 +1402,10 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
         JUNO_TRY(ensure_device(&py, &c->stage_y_bytes, qbytes));
         c->stage_y = (float *)py;
         JUNO_CUDA_TRY(cudaMemcpyAsync(c->stage_x, q_host, qbytes, cudaMemcpyHostToDevice, c->stream));
-        JUNO_TRY(q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, c->stream));
+        JUNO_TRY(q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, WAIT_BLOCKING, c->stream));
         JUNO_CUDA_TRY(cudaMemcpyAsync(out_host, c->stage_y, qbytes, cudaMemcpyDeviceToHost, c->stream));
         JUNO_CUDA_TRY(cudaStreamSynchronize(c->stream));
+        JUNO_TRY(wait_status(c, WAIT_BLOCKING));
         c->h2d_bytes += (int64_t)qbytes;
         c->d2h_bytes += (int64_t)qbytes;
         return JUNO_OK;

@@ -1,4 +1,4 @@
-// Shared-memory loads, mbarriers with bounded waits and bulk copies of the quantised products (qgemv.cu, gemm_quant_tc.cu).
+// Shared-memory loads, mbarriers with bounded waits and bulk copies of the quantised products (qgemv.cu, gemm_quant_tc.cu) and of 4-bit cache pages (q4_attn.cu).
 #pragma once
 #include <stdint.h>
 
@@ -65,12 +65,12 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void *src, unsigned
 // A wait on a weight tile gives up after this many SM cycles (about a fifth of a second); after the first give-up
 // of a warp its later waits are short, so that the kernel still drains the copies it has in flight and returns.
 constexpr long long kQWaitLimitClk = 400000000ll, kQWaitLimitAfterFail = 2000000ll;
-__device__ __forceinline__ void mbar_wait_bounded(uint32_t bar, unsigned parity, unsigned ns, unsigned *err, bool &failed) {
+__device__ __forceinline__ void mbar_wait_bounded(uint32_t bar, unsigned parity, unsigned ns, unsigned *err, bool &failed, unsigned code = 1u) {
     if (mbar_test(bar, parity, 0)) return;
     const long long t0 = clock64(), limit = failed ? kQWaitLimitAfterFail : kQWaitLimitClk;
     while (!mbar_test(bar, parity, ns)) {
         if (clock64() - t0 > limit) {
-            if (!failed && (threadIdx.x & 31) == 0) *reinterpret_cast<volatile unsigned *>(err) = 1u | ((threadIdx.x >> 5) << 8) | (blockIdx.x << 16);
+            if (!failed && (threadIdx.x & 31) == 0) *reinterpret_cast<volatile unsigned *>(err) = code | ((threadIdx.x >> 5) << 8) | (blockIdx.x << 16);
             failed = true;
             return;
         }

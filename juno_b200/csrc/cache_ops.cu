@@ -405,8 +405,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams 
             const uint8_t *b = block_of(r.old_pages, src);
             uint32_t v;
             if (k >= kw && k < kw + hd / 8) {
-                const int half = 2 * (k - kw);
-                const uint8_t *c = b + q4_v_code(hd, src & 15, 0, 0) + 4 * half;
+                const uint8_t *c = b + q4_v_code(hd, src & 15, 2 * (k - kw) / NG, 2 * (k - kw) % NG);
                 v = *reinterpret_cast<const uint16_t *>(c) | (uint32_t) * reinterpret_cast<const uint16_t *>(c + 4) << 16;
             } else {
                 v = *reinterpret_cast<const uint32_t *>(b + at(src, k));
@@ -420,8 +419,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams 
             uint8_t *b = block_of(r.new_pages, dst);
             const uint32_t v = rows_s[idx];
             if (k >= kw && k < kw + hd / 8) {
-                const int half = 2 * (k - kw);
-                uint8_t *c = b + q4_v_code(hd, dst & 15, 0, 0) + 4 * half;
+                uint8_t *c = b + q4_v_code(hd, dst & 15, 2 * (k - kw) / NG, 2 * (k - kw) % NG);
                 *reinterpret_cast<uint16_t *>(c) = (uint16_t)v;
                 *reinterpret_cast<uint16_t *>(c + 4) = (uint16_t)(v >> 16);
             } else {

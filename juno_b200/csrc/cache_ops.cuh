@@ -70,8 +70,9 @@ int cache_words(juno_ctx *c, const int32_t *words, size_t n, int32_t *dst, cudaS
 int launch_kv_append(juno_ctx *c, const juno_kvpool *p, int layer, const CacheRow *rows, int n, int n_tokens, const float *k, const float *v, int64_t ld,
                      cudaStream_t st);
 // Decode attention over 4-bit pages, lens[i] (null: all cached) positions of each sequence; adds to the weights of sequences that keep them.
+// `word`: where its kernel reports a wait that it gave up.
 int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *seqs, const int32_t *lens, int n_heads, const float *q, int64_t ldq, float *out,
-              int64_t ldo, cudaStream_t st);
+              int64_t ldo, WaitWord word, cudaStream_t st);
 
 // No C++ exception crosses the C ABI.
 template <class F>

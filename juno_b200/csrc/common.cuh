@@ -54,6 +54,7 @@ constexpr uint32_t kMagicDead = 0xDEADDEAD;
 // Whose kernels gave up a wait: calls that return when their work is done look at their own word then, and take the failure back, so
 // that it is reported once and by the call it belongs to; work that is only enqueued (juno_gemv_device) has another one.
 enum WaitWord { WAIT_BLOCKING = 0, WAIT_ENQUEUED = 1 };
+constexpr unsigned kErrCacheWait = 9;  // code of a given-up wait on a page of the cache
 constexpr unsigned kErrStackWait = 8;  // code of a given-up wait in a layer stack's kernels (see GemvScratch::qerr)
 
 // Scratch of the host-level MatVec entry points and the word kernels report a given-up wait in.

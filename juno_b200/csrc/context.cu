@@ -75,6 +75,8 @@ int wait_status(juno_ctx *c, WaitWord which) {
     if (!code) return JUNO_OK;
     if ((code & 0xffu) == kErrStackWait)
         set_error("a matrix product gave up waiting inside a kernel (stage %u of block %u)", (code >> 8) & 0xffu, code >> 16);
+    else if ((code & 0xffu) == kErrCacheWait)
+        set_error("decode attention gave up waiting for a page of the cache (warp %u of block %u)", (code >> 8) & 0xffu, code >> 16);
     else if ((code & 0xffu) >= 3u)
         set_error("tensor-parallel rank %u did not deliver its %s within a second (this rank gave up waiting)", (code >> 8) & 0xffu,
                   (code & 0xffu) == 3u ? "partial products" : "greedy pick");
