@@ -252,6 +252,7 @@ int juno_ctx_destroy(juno_ctx *c) {
     if (c->stage_y) cudaFree(c->stage_y);
     if (c->pinned) cudaFreeHost(c->pinned);
     if (c->cache_scratch) cudaFree(c->cache_scratch);
+    if (c->cache_arrived) cudaFree(c->cache_arrived);
     for (cudaEvent_t e : c->cache_events)
         if (e) cudaEventDestroy(e);
     cudaStreamDestroy(c->stream);

@@ -24,6 +24,7 @@ struct Q4AttnParams {
     int64_t ldq, ldo;
     float *out;
     float *part_o, *part_ml;  // [part][head][hd], [part][head][max, sum]
+    unsigned *arrived;        // [row][kv_head]: parts that are done, zero between launches
     float *scores;            // sequences that keep weights: [kv_head][position of all pages][G], log2 domain
     float *weights;
     int track_tokens;
@@ -32,7 +33,12 @@ struct Q4AttnParams {
 
 __device__ __forceinline__ int row_end(const Q4AttnParams &p, int i) { return i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : p.total; }
 
-constexpr int kQ4MinShare = 8, kQ4MaxGroup = 8, kQ4Warps = 4, kQ4Slots = 2, kQ4Tile = 2;  // pages of a tile: a warp's step
+constexpr int kQ4MaxGroup = 8, kQ4Slots = 2, kQ4Tile = 2;  // pages of a tile: a warp's step
+// Warps of a CTA and CTAs on an SM: 16 warps of 128 registers, 12 of 168.
+template <int HPL>
+constexpr int kQ4Warps = HPL == 1 ? 8 : 4;
+template <int HPL>
+constexpr int kQ4Ctas = HPL == 1 ? 2 : 3;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -82,24 +88,49 @@ __device__ __forceinline__ float factor_d(uint32_t f) { return __uint_as_float(f
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
 // eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
-template <int HD>
-constexpr int kQ4Ring = kQ4Warps * kQ4Slots * kQ4Tile * 20 * HD;  // bytes of a CTA's rings
+template <int HD, int HPL>
+struct Q4Smem {  // bytes
+    static constexpr int kRing = kQ4Warps<HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HPL> * kQ4Slots * 8,
+                         kQuery = kMerge + kQ4Warps<HPL> * 4 * HPL * (HD + 2) * 4, kQueryRow = HD + 8,  // halves; the pad keeps the rows on different banks
+        kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kAll = kSums + 4 * HPL * (HD / kQ4Group + 1) * 4;
+};
+
+// The largest score of a (row, head) and the sum of its weights over the row's parts, by all threads of a warp.
+__device__ __forceinline__ float2 row_sums(const Q4AttnParams &p, int i, int share0, int parts, int h, int lane) {
+    float M = -INFINITY, L = 0.f;
+    for (int s = lane; s < parts; s += 32) M = fmaxf(M, __ldcg(p.part_ml + ((size_t)(i + share0 + s) * p.n_heads + h) * 2));
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    for (int s = lane; s < parts; s += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + ((size_t)(i + share0 + s) * p.n_heads + h) * 2));
+        L = fmaf(ml.y, exp2_fast(ml.x - M), L);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+    return make_float2(M, L);
+}
 
 template <int HD, int HPL>
-__global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
-    constexpr int NG = HD / kQ4Group, BLOCK = 20 * HD, FACT = NG * 4, TILE = kQ4Tile * BLOCK;
+__global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
+    constexpr int NG = HD / kQ4Group, BLOCK = 20 * HD, FACT = NG * 4, TILE = kQ4Tile * BLOCK, W = kQ4Warps<HPL>, HEADS = 4 * HPL;
+    using Smem = Q4Smem<HD, HPL>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t = lane & 3;
     const int kvh = blockIdx.x % p.n_kv_heads, share = blockIdx.x / p.n_kv_heads, G = p.n_heads / p.n_kv_heads, h0 = kvh * G;
-    const uint32_t ring = smem_u32(smem) + warp * kQ4Slots * TILE, bars = smem_u32(smem) + kQ4Ring<HD> + warp * kQ4Slots * 8;
-    float *mg_o = reinterpret_cast<float *>(smem + kQ4Ring<HD> + kQ4Warps * kQ4Slots * 8);  // where the warps meet: [warp][head][HD], [warp][head], [warp][head]
-    float *mg_m = mg_o + kQ4Warps * G * HD, *mg_l = mg_m + kQ4Warps * G;
+    const uint32_t ring = smem_u32(smem) + warp * kQ4Slots * TILE, bars = smem_u32(smem) + Smem::kBars + warp * kQ4Slots * 8;
+    float *mg_o = reinterpret_cast<float *>(smem + Smem::kMerge);  // where the warps meet: [warp][head][HD], [warp][head], [warp][head]
+    float *mg_m = mg_o + W * G * HD, *mg_l = mg_m + W * G;
+    __half *q_s = reinterpret_cast<__half *>(smem + Smem::kQuery);    // [limb][head][kQueryRow]
+    float *sums_s = reinterpret_cast<float *>(smem + Smem::kSums);  // [head][group], [head]
+    __shared__ int last_s;
     if (lane == 0) {
         for (int s = 0; s < kQ4Slots; s++) mbar_init(bars + s * 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
     }
     __syncwarp();
+    pdl_launch_dependents();
+    pdl_wait();
     const uint8_t *plane = p.pool + ((size_t)p.layer * p.n_pages * p.n_kv_heads + kvh) * BLOCK;
     const size_t page_bytes = (size_t)p.n_kv_heads * BLOCK;
     const uint64_t policy = l2_evict_first_policy();
@@ -114,7 +145,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
     const int32_t *table = nullptr;
     int page0 = 0;
     auto place = [&](int tile) {  // of this lane's page among the 16 tiles from `tile`
-        const int pg = kQ4Tile * (warp + kQ4Warps * (tile + (lane >> 1))) + (lane & 1);
+        const int pg = kQ4Tile * (warp + W * (tile + (lane >> 1))) + (lane & 1);
         return pg < part_pages ? table[pg] : 0;
     };
     auto issue = [&] {
@@ -122,7 +153,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
         const int a = __shfl_sync(0xffffffffu, places, at), b = __shfl_sync(0xffffffffu, places, at + 1);
         if (lane == 0) {
             const uint32_t slot = issued % kQ4Slots, bar = bars + slot * 8, to = ring + slot * TILE;
-            const bool two = kQ4Tile * (warp + kQ4Warps * part_issued) + 1 < part_pages;
+            const bool two = kQ4Tile * (warp + W * part_issued) + 1 < part_pages;
             mbar_expect_tx(bar, two ? TILE : BLOCK);
             bulk_g2s(to, plane + a * page_bytes, BLOCK, bar, policy);
             if (two) bulk_g2s(to + BLOCK, plane + b * page_bytes, BLOCK, bar, policy);
@@ -140,7 +171,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
         part_pages = r.upto > 0 ? min(share1, row_end(p, i)) - from : 0;
         table = p.table + (size_t)r.slot * p.max_pages_per_seq + page0;
         const int tiles = (part_pages + kQ4Tile - 1) / kQ4Tile;
-        part_tiles = tiles > warp ? (tiles - warp + kQ4Warps - 1) / kQ4Warps : 0;
+        part_tiles = tiles > warp ? (tiles - warp + W - 1) / W : 0;
         part_issued = 0;
         places = place(0);
         places_next = place(16);
@@ -148,71 +179,58 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
     };
     if (share0 < share1) begin(cache_find(p.rows, share0), share0);
 
-    for (int from = share0; from < share1;) {
+    int from = share0;
+    while (from < share1) {
         const int i = row, to = min(share1, row_end(p, i)), n_tiles = part_tiles, pos_first = page0 << 4;
         const int pos_end = min(r.upto, (to - r.first) << 4);  // of this part, in the row
         const bool track = p.scores && r.track >= 0;
-        // The query: lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8, as the B operand wants them.
+        // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
+        // largest element), in two FP16 limbs.  Elements 2, 3, 6, 7 of eight meet 16 q.
+        for (int head = warp; head < HEADS; head += W) {
+            constexpr int E = HD / 32;  // elements of a lane
+            const float scale = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
+            float y[E], top = 0.f, sum = 0.f;
+            const float *src = p.q + (size_t)i * p.ldq + (size_t)(h0 + head) * HD + E * lane;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                y[e] = head < G ? src[e] * scale : 0.f;
+                sum += y[e];
+                top = fmaxf(top, fabsf(y[e]));
+            }
+#pragma unroll
+            for (int x = 1; x < 32; x <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                if (x < kQ4Group / E) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            }
+            const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127)), up = 13 - e2;
+            const float shift = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float s = (E * lane + e) & 2 ? shift * 0.0625f : shift, y0 = y[e] * s, y1 = y[e + 1] * s;
+                const uint32_t hi = pack_h2(y0, y1);
+                const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                uint32_t *to_q = reinterpret_cast<uint32_t *>(q_s + head * Smem::kQueryRow + E * lane + e);
+                to_q[0] = hi;
+                to_q[HEADS * Smem::kQueryRow / 2] = pack_h2(y0 - hf.x, y1 - hf.y);
+            }
+            if (lane % (kQ4Group / E) == 0) sums_s[head * NG + lane / (kQ4Group / E)] = sum;
+            if (lane == 0) sums_s[HEADS * NG + head] = __uint_as_float((uint32_t)(127 + 24 - up) << 23);
+        }
+        __syncthreads();
+        // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8, as the B operand wants them
         uint32_t qh[NG][4], ql[HPL == 2 ? NG : 1][4];
         float qsum[HPL][NG], back[HPL];  // of this lane's own heads: sums over the groups, and the scale of the scores
-        {
-            const int head = HPL == 1 ? g8 >> 1 : g8;
-            const float *src = p.q + (size_t)i * p.ldq + (size_t)(h0 + head) * HD + 8 * t;
-            const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-            const float scale = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
-            float y[NG][8], top = 0.f, sums[NG];
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                if (head >= G) {
+        for (int g = 0; g < NG; g++) {
+            const __half *from_q = q_s + (HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : g8) * Smem::kQueryRow + g * kQ4Group + 8 * t;
+            lds_words<4>(qh[g], smem_u32(from_q));
+            if constexpr (HPL == 2) lds_words<4>(ql[g], smem_u32(from_q + HEADS * Smem::kQueryRow));
+        }
 #pragma unroll
-                    for (int e = 0; e < 8; e++) y[g][e] = 0.f;
-                } else if (vec) {
-                    const float4 a = *reinterpret_cast<const float4 *>(src + g * kQ4Group), b = *reinterpret_cast<const float4 *>(src + g * kQ4Group + 4);
-                    y[g][0] = a.x; y[g][1] = a.y; y[g][2] = a.z; y[g][3] = a.w;
-                    y[g][4] = b.x; y[g][5] = b.y; y[g][6] = b.z; y[g][7] = b.w;
-                } else {
+        for (int h = 0; h < HPL; h++) {
+            back[h] = sums_s[HEADS * NG + HPL * t + h];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) y[g][e] = src[g * kQ4Group + e];
-                }
-                sums[g] = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    y[g][e] *= scale;
-                    sums[g] += y[g][e];
-                    top = fmaxf(top, fabsf(y[g][e]));
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-                for (int g = 0; g < NG; g++) sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], o);
-            }
-            // the largest element to 2^13 .. 2^14: the second limb then ends at 2^-25, 38 bits below it
-            const int up = top > 0.f && top < INFINITY ? 13 - max(-100, min(100, ilogbf(top))) : 0;
-            const float shift = scalbnf(1.f, up);
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int b = 0; b < 4; b++) {  // registers: MMA 0 (k low, k high), MMA 1 (k low, k high); k high meets 16 q
-                    const float s = b & 1 ? shift * 0.0625f : shift, y0 = y[g][2 * b] * s, y1 = y[g][2 * b + 1] * s;
-                    const uint32_t hi = pack_h2(y0, y1);
-                    const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                    const uint32_t lo = pack_h2(y0 - hf.x, y1 - hf.y);
-                    if constexpr (HPL == 1) {
-                        qh[g][b] = g8 & 1 ? lo : hi;
-                    } else {
-                        qh[g][b] = hi;
-                        ql[g][b] = lo;
-                    }
-                }
-#pragma unroll
-            for (int h = 0; h < HPL; h++) {
-                const int lane_of = HPL == 1 ? 8 * t : 8 * t + 4 * h;  // a lane of the column that holds this lane's head
-                back[h] = scalbnf(1.f, 24 - __shfl_sync(0xffffffffu, up, lane_of));
-#pragma unroll
-                for (int g = 0; g < NG; g++) qsum[h][g] = __shfl_sync(0xffffffffu, sums[g], lane_of);
-            }
+            for (int g = 0; g < NG; g++) qsum[h][g] = sums_s[(HPL * t + h) * NG + g];
         }
         float o[NG][2][4], omin[HPL][NG], m_run[HPL], l_run[HPL], vscale = 0.f;
         uint32_t limit = 0;  // factors above this one ask for another scale
@@ -229,8 +247,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
         }
         constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
-        for (int j = 0; j < n_tiles; j++, pos0 += kQ4Warps * kQ4Tile * kPageTokens) {
-            mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
+        for (int j = 0; j < n_tiles; j++, pos0 += W * kQ4Tile * kPageTokens) {
+            mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 1000, p.err, failed, kErrCacheWait);
             if (__any_sync(0xffffffffu, failed)) {
                 failed = true;
                 break;
@@ -275,7 +293,6 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
 #pragma unroll
                     for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], back[h], off[h][x]);
             }
-            const bool tail = pos0 + kQ4Tile * kPageTokens > pos_end;
             if (track) {
                 float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
 #pragma unroll
@@ -292,15 +309,23 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     lds_words<NG>(f[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * FACT);
-                    if (tail && pos0 + 16 * u + 8 * x + g8 >= pos_end) {  // behind the end: whatever their place holds
-#pragma unroll
-                        for (int h = 0; h < HPL; h++) s[h][u][x] = -INFINITY;
-#pragma unroll
-                        for (int g = 0; g < NG; g++) f[u][x][g] = 0u;
-                    }
-#pragma unroll
-                    for (int g = 0; g < NG; g++) steps = max(steps, f[u][x][g]);
                 }
+            if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
+#pragma unroll
+                for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
+#pragma unroll
+                        for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
+#pragma unroll
+                        for (int g = 0; g < NG; g++) f[u][x][g] = on ? f[u][x][g] : 0u;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                for (int g = 0; g < NG; g++) steps = max(steps, max(f[u][0][g], f[u][1][g]));
             // a larger score than any before, or a step beyond the scale's range: seldom after the first tiles
             steps &= 0xffff0000u;
             float top[HPL];
@@ -317,7 +342,7 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
                 steps = __reduce_max_sync(0xffffffffu, steps);
                 if (steps > limit) {  // the largest step to 2^10 .. 2^11, up to 2^15 in range
                     const int e = max((int)(steps >> 23) - 127, -100);
-                    const float next = scalbnf(1.f, 10 - e);
+                    const float next = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
                     vfix = vscale == 0.f ? 0.f : next / vscale;
                     vscale = next;
                     limit = (uint32_t)(e + 4 + 127) << 23 | 0x7fffffu;
@@ -426,15 +451,14 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
             }
         }
         __syncthreads();
-        const int end = row_end(p, i);
-        const bool whole = first >= share0 && end <= share1;
-        for (int idx = tid; idx < G * HD; idx += kQ4Warps * 32) {
+        const int end = row_end(p, i), share_a = first / p.share, parts = (end - 1) / p.share - share_a + 1;
+        for (int idx = tid; idx < G * HD; idx += W * 32) {
             const int g = idx / HD, d = idx - g * HD;
             float M = -INFINITY, L = 0.f, acc = 0.f;
 #pragma unroll
-            for (int w = 0; w < kQ4Warps; w++) M = fmaxf(M, mg_m[w * G + g]);
+            for (int w = 0; w < W; w++) M = fmaxf(M, mg_m[w * G + g]);
 #pragma unroll
-            for (int w = 0; w < kQ4Warps; w++) {
+            for (int w = 0; w < W; w++) {
                 const float lw = mg_l[w * G + g];
                 if (lw == 0.f) continue;  // a warp without pages
                 const float fw = exp2_fast(mg_m[w * G + g] - M);
@@ -442,13 +466,40 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
                 acc = fmaf(mg_o[((size_t)w * G + g) * HD + d], fw, acc);
             }
             const size_t part = (size_t)(i + share) * p.n_heads + h0 + g;
-            if (whole)
+            if (parts == 1)
                 p.out[(size_t)i * p.ldo + (h0 + g) * HD + d] = pos_end > 0 ? acc / L : 0.f;
             else
                 p.part_o[part * HD + d] = acc;
-            if (d == 0 && (!whole || track)) {
-                p.part_ml[part * 2] = M;
-                p.part_ml[part * 2 + 1] = L;
+            if (d == 0 && (parts > 1 || track)) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(M, L);
+        }
+        if (parts > 1) {  // whoever is last puts the parts together, in their order
+            __syncthreads();
+            if (tid == 0) {
+                __threadfence();
+                unsigned *arrived = p.arrived + (size_t)i * p.n_kv_heads + kvh;
+                last_s = atomicAdd(arrived, 1u) == (unsigned)parts - 1;
+                if (last_s) {
+                    *arrived = 0;
+                    __threadfence();
+                }
+            }
+            __syncthreads();
+            if (last_s) {
+                for (int g = warp; g < G; g += W) {
+                    const float2 ml = row_sums(p, i, share_a, parts, h0 + g, lane);
+                    if (lane == 0) mg_m[g] = ml.x, mg_l[g] = 1.f / ml.y;
+                }
+                __syncthreads();
+                const size_t stride = (size_t)p.n_heads * HD;
+                for (int idx = tid; idx < G * HD; idx += W * 32) {
+                    const int g = idx / HD;
+                    const float *from_o = p.part_o + (size_t)(i + share_a) * stride + (size_t)h0 * HD + idx, *from_m = p.part_ml + ((size_t)(i + share_a) * p.n_heads + h0 + g) * 2;
+                    const float M = mg_m[g];
+                    float acc = 0.f;
+#pragma unroll 8
+                    for (int s = 0; s < parts; s++) acc = fmaf(__ldcg(from_o + s * stride), exp2_fast(__ldcg(from_m + (size_t)s * p.n_heads * 2) - M), acc);
+                    p.out[(size_t)i * p.ldo + (size_t)h0 * HD + idx] = acc * mg_l[g];
+                }
             }
         }
         __syncthreads();  // the warps' results have been read
@@ -457,70 +508,33 @@ __global__ void __launch_bounds__(kQ4Warps * 32, HPL == 1 ? 4 : 3) q4_attn_kerne
             break;
         }
     }
-    if (failed)
+    if (failed) {  // the parts that are left count as done, so that the next launch finds zeros
         for (unsigned j = ring_open((int)issued, (int)used, kQ4Slots); j < issued; j++)
             mbar_wait_bounded(bars + j % kQ4Slots * 8, j / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
-}
-
-// The largest score of a (row, head) and the sum of its weights over the row's parts, by all threads of a warp.
-__device__ __forceinline__ float2 row_sums(const Q4AttnParams &p, int i, int share0, int parts, int h, int lane) {
-    float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < parts; s += 32) M = fmaxf(M, p.part_ml[((size_t)(i + share0 + s) * p.n_heads + h) * 2]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    for (int s = lane; s < parts; s += 32) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + ((size_t)(i + share0 + s) * p.n_heads + h) * 2);
-        L = fmaf(ml.y, exp2_fast(ml.x - M), L);
+        if (tid == 0)
+            for (int i = cache_find(p.rows, min(p.total - 1, from)); from < share1; from = row_end(p, i++)) {
+                const int parts = (row_end(p, i) - 1) / p.share - cache_row(p.rows, i).first / p.share + 1;
+                unsigned *arrived = p.arrived + (size_t)i * p.n_kv_heads + kvh;
+                if (parts > 1 && atomicAdd(arrived, 1u) == (unsigned)parts - 1) *arrived = 0;
+            }
     }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-    return make_float2(M, L);
 }
 
-// Blocks [0, rows * n_heads): the parts of one (row, head), in their order.  Further blocks, one per kQ4WeightPages pages of all rows and key/value head: the
-// weight that their positions have received.
-constexpr int kQ4MergeThreads = 128, kQ4WeightPages = kQ4MergeThreads / kPageTokens;
-template <int HD>
-__global__ void __launch_bounds__(kQ4MergeThreads) q4_merge_kernel(const __grid_constant__ Q4AttnParams p) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, merges = p.rows.n * p.n_heads;
+// One block per kQ4WeightPages pages of all rows and key/value head: the weight that their positions have received.
+constexpr int kQ4WeightThreads = 128, kQ4WeightPages = kQ4WeightThreads / kPageTokens;
+__global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __grid_constant__ Q4AttnParams p) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __shared__ float2 sums[kQ4MaxGroup];
-    if ((int)blockIdx.x < merges) {
-        constexpr int WAYS = kQ4MergeThreads / HD;
-        __shared__ float acc_s[WAYS][HD];
-        const int i = blockIdx.x / p.n_heads, h = blockIdx.x - i * p.n_heads;
-        const int share0 = cache_row(p.rows, i).first / p.share, parts = (row_end(p, i) - 1) / p.share - share0 + 1;
-        if (parts == 1) return;
-        if (warp == 0) {
-            const float2 ml = row_sums(p, i, share0, parts, h, lane);
-            if (lane == 0) sums[0] = ml;
-        }
-        __syncthreads();
-        const float M = sums[0].x;
-        const int d = tid % HD;
-        float acc = 0.f;
-#pragma unroll 4
-        for (int s = tid / HD; s < parts; s += WAYS) {
-            const size_t part = (size_t)(i + share0 + s) * p.n_heads + h;
-            acc = fmaf(p.part_o[part * HD + d], exp2_fast(p.part_ml[part * 2] - M), acc);
-        }
-        if (WAYS > 1) {
-            acc_s[tid / HD][d] = acc;
-            __syncthreads();
-            if (tid >= HD) return;
-            for (int w = 1; w < WAYS; w++) acc += acc_s[w][d];
-        }
-        p.out[(size_t)i * p.ldo + h * HD + d] = acc / sums[0].y;
-        return;
-    }
-    const int at = blockIdx.x - merges, kvh = at % p.n_kv_heads, page0 = at / p.n_kv_heads * kQ4WeightPages, page1 = min(p.total, page0 + kQ4WeightPages);
+    const int kvh = blockIdx.x % p.n_kv_heads, page0 = blockIdx.x / p.n_kv_heads * kQ4WeightPages, page1 = min(p.total, page0 + kQ4WeightPages);
     const int G = p.n_heads / p.n_kv_heads;
+    pdl_wait();
     for (int i = cache_find(p.rows, page0); i < p.rows.n; i++) {
         const CacheRow r = cache_row(p.rows, i);
         if (r.first >= page1) break;
         if (r.track < 0 || r.upto == 0) continue;
         const int share0 = r.first / p.share, parts = (row_end(p, i) - 1) / p.share - share0 + 1;
         __syncthreads();
-        for (int g = warp; g < G; g += kQ4MergeThreads / 32) {
+        for (int g = warp; g < G; g += kQ4WeightThreads / 32) {
             const float2 ml = row_sums(p, i, share0, parts, kvh * G + g, lane);
             if (lane == 0) sums[g] = make_float2(ml.x, 1.f / ml.y);
         }
@@ -535,17 +549,25 @@ __global__ void __launch_bounds__(kQ4MergeThreads) q4_merge_kernel(const __grid_
 }
 
 template <int HD, int HPL>
-static int launch_q4_attn(const Q4AttnParams &a, unsigned grid, cudaStream_t st) {
-    const int bytes = kQ4Ring<HD> + kQ4Warps * kQ4Slots * 8 + kQ4Warps * 4 * HPL * (HD + 2) * 4;
+static int launch_q4_attn(const Q4AttnParams &a, int shares, cudaStream_t st) {
     static bool set[64] = {false};  // per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!set[dev & 63]) {
-        JUNO_CUDA_TRY(cudaFuncSetAttribute(q4_attn_kernel<HD, HPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        JUNO_CUDA_TRY(cudaFuncSetAttribute(q4_attn_kernel<HD, HPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD, HPL>::kAll));
         set[dev & 63] = true;
     }
-    q4_attn_kernel<HD, HPL><<<grid, kQ4Warps * 32, bytes, st>>>(a);
-    JUNO_CUDA_TRY(cudaGetLastError());
+    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL>, dim3((unsigned)(shares * a.n_kv_heads)), dim3(kQ4Warps<HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
+    return JUNO_OK;
+}
+
+// Zeros, once; every launch leaves them so.
+static int arrival_words(juno_ctx *c, size_t n, cudaStream_t st) {
+    if (c->cache_arrived && c->cache_arrived_bytes >= n * sizeof(unsigned)) return JUNO_OK;
+    void *words = c->cache_arrived;
+    JUNO_TRY(ensure_device(&words, &c->cache_arrived_bytes, std::max<size_t>(n * sizeof(unsigned), 16384)));
+    c->cache_arrived = static_cast<unsigned *>(words);
+    JUNO_CUDA_TRY(cudaMemsetAsync(words, 0, c->cache_arrived_bytes, st));
     return JUNO_OK;
 }
 
@@ -567,12 +589,14 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
         bytes += len;
         JUNO_REQUIRE(pages < (1 << 27), "attention over %lld pages in one call", (long long)pages);
     }
-    // One share for every CTA that the GPU holds at a time, so that all end together; none below two tiles for each warp of four.
-    const int64_t slots = std::max(1, c->sm_count * (G <= 4 ? 4 : 3) / H);
-    const int share = (int)std::max<int64_t>(kQ4MinShare, (pages + slots - 1) / slots);
+    // One share for every CTA that the GPU holds at a time, so that all end together; none below a tile for each warp.
+    const int warps = G <= 4 ? kQ4Warps<1> : kQ4Warps<2>, ctas = G <= 4 ? kQ4Ctas<1> : kQ4Ctas<2>;
+    const int64_t slots = std::max(1, c->sm_count * ctas / H);
+    const int share = (int)std::max<int64_t>(warps * kQ4Tile, (pages + slots - 1) / slots);
     const int shares = (int)((pages + share - 1) / share);
     bool whole = true;  // no row in more than one share
     for (int i = 0; whole && i < n; i++) whole = rows[(size_t)i].first / share == ((i + 1 < n ? rows[(size_t)i + 1].first : (int)pages) - 1) / share;
+    if (!whole) JUNO_TRY(arrival_words(c, (size_t)n * H, st));
     Q4AttnParams a;
     auto padded = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t parts = (size_t)(n + shares), far_b = cache_rows_bytes(n), ml_b = padded(parts * n_heads * 8), o_b = whole ? 0 : padded(parts * n_heads * hd * 4),
@@ -599,21 +623,16 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     a.scores = track ? reinterpret_cast<float *>(scratch + far_b + ml_b + o_b) : nullptr;
     a.weights = p->weights;
     a.track_tokens = p->track_tokens;
+    a.arrived = c->cache_arrived;
     a.err = c->gemv_scratch.qerr + word;
     ProfScope prof(c, st, PROF_ATTN, (double)bytes * H * p->row_bytes());
-    const unsigned grid = (unsigned)(shares * H);
     if (hd == 128)
-        JUNO_TRY(G <= 4 ? (launch_q4_attn<128, 1>(a, grid, st)) : (launch_q4_attn<128, 2>(a, grid, st)));
+        JUNO_TRY(G <= 4 ? (launch_q4_attn<128, 1>(a, shares, st)) : (launch_q4_attn<128, 2>(a, shares, st)));
     else
-        JUNO_TRY(G <= 4 ? (launch_q4_attn<64, 1>(a, grid, st)) : (launch_q4_attn<64, 2>(a, grid, st)));
+        JUNO_TRY(G <= 4 ? (launch_q4_attn<64, 1>(a, shares, st)) : (launch_q4_attn<64, 2>(a, shares, st)));
     c->kernel_launches++;
-    if (whole && !track) return JUNO_OK;
-    const unsigned merge = (unsigned)(n * n_heads + (track ? (pages + kQ4WeightPages - 1) / kQ4WeightPages * H : 0));
-    if (hd == 128)
-        q4_merge_kernel<128><<<merge, kQ4MergeThreads, 0, st>>>(a);
-    else
-        q4_merge_kernel<64><<<merge, kQ4MergeThreads, 0, st>>>(a);
-    JUNO_CUDA_TRY(cudaGetLastError());
+    if (!track) return JUNO_OK;
+    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages + kQ4WeightPages - 1) / kQ4WeightPages * H)), dim3(kQ4WeightThreads), 0, st, a));
     c->kernel_launches++;
     return JUNO_OK;
 }
