@@ -171,9 +171,10 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const RowsParams p) {
         if (sub == 0 && r.track >= 0)
             p.weights[(((size_t)r.track * p.n_layers + p.layer) * H + h) * p.track_tokens + pos] = 0.f;
     }
-    if ((sub & 3) == 0)
-        *reinterpret_cast<uint32_t *>(block + (is_v ? q4_v_factors(HD, pp, g) : q4_k_factors(HD, pp, g))) =
-            (uint32_t)__half_as_ushort(mh) | (uint32_t)__bfloat16_as_ushort(dh) << 16;
+    if ((sub & 3) == 0) {
+        *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))) = __bfloat16_as_ushort(dh);
+        *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))) = __half_as_ushort(mh);
+    }
 }
 
 __device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
@@ -198,8 +199,8 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const RowsParams p) {
     const int pos = r.upto + (int)row - r.first, pp = pos & 15, g = sub >> 2;
     const int page = p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)];
     const uint8_t *block = static_cast<const uint8_t *>(p.kpool) + (((size_t)p.layer * p.n_pages + page) * H + h) * q4_block_bytes(HD);
-    const uint32_t f = *reinterpret_cast<const uint32_t *>(block + (is_v ? q4_v_factors(HD, pp, g) : q4_k_factors(HD, pp, g)));
-    const float m = __half2float(__ushort_as_half((unsigned short)f)), d = __uint_as_float(f & 0xffff0000u);
+    const float m = __half2float(*reinterpret_cast<const __half *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))));
+    const float d = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))));
     float x[8];
     if (is_v) {
 #pragma unroll
@@ -386,45 +387,32 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams 
         done += sum;
         __syncthreads();
     }
-    // the rows: key numbers, key factors, value numbers (half words), value factors
-    extern __shared__ uint32_t rows_s[];  // [kEvictRows][hd * 5 / 16] words
-    const int hd = p.hd, NG = hd / kQ4Group, kw = hd / 8 + NG, words = kw + hd / 8 + NG;
+    // the rows as half words: keys' numbers, values' numbers, and the four kinds of factors
+    extern __shared__ uint16_t rows_s[];  // [kEvictRows][hd * 5 / 8]
+    const int hd = p.hd, NG = hd / kQ4Group, halves = hd * 5 / 8;
     __shared__ float w_s[kEvictRows];
     auto block_of = [&](int list, int pos) {
         return p.pool + (((size_t)layer * p.n_pages + p.pages[list + (pos >> 4)]) * p.n_kv_heads + h) * q4_block_bytes(hd);
     };
-    // word i of a row: where it lies in a block
-    auto at = [&](int pos, int i) {
-        const int pp = pos & 15;
-        return i < hd / 8 ? q4_k_code(hd, pp, 0, 0) + 4 * i : i < kw ? q4_k_factors(hd, pp, 0) + 4 * (i - hd / 8) : q4_v_factors(hd, pp, 0) + 4 * (i - kw - hd / 8);
+    auto at = [&](int pos, int i) {  // half word i of a row: where it lies in a block
+        const int pp = pos & 15, q = hd / 4;
+        if (i < q) return q4_k_code(hd, pp, 0, 0) + 2 * i;
+        if ((i -= q) < q) return q4_v_code(hd, pp, i / NG, i % NG);
+        i -= q;
+        const int kind = i / NG, g = i - kind * NG;
+        return kind == 0 ? q4_k_step(hd, pp, g) : kind == 1 ? q4_k_offset(hd, pp, g) : kind == 2 ? q4_v_step(hd, pp, g) : q4_v_offset(hd, pp, g);
     };
     for (int base = 0; base < r.keep; base += kEvictRows) {
         const int n = min(kEvictRows, r.keep - base);
-        for (int idx = tid; idx < n * words; idx += kEvictThreads) {
-            const int j = idx / words, k = idx - j * words, src = kept[base + j];
-            const uint8_t *b = block_of(r.old_pages, src);
-            uint32_t v;
-            if (k >= kw && k < kw + hd / 8) {
-                const uint8_t *c = b + q4_v_code(hd, src & 15, 2 * (k - kw) / NG, 2 * (k - kw) % NG);
-                v = *reinterpret_cast<const uint16_t *>(c) | (uint32_t) * reinterpret_cast<const uint16_t *>(c + 4) << 16;
-            } else {
-                v = *reinterpret_cast<const uint32_t *>(b + at(src, k));
-            }
-            rows_s[idx] = v;
+        for (int idx = tid; idx < n * halves; idx += kEvictThreads) {
+            const int j = idx / halves, src = kept[base + j];
+            rows_s[idx] = *reinterpret_cast<const uint16_t *>(block_of(r.old_pages, src) + at(src, idx - j * halves));
         }
         if (tid < n) w_s[tid] = w[kept[base + tid]];
         __syncthreads();
-        for (int idx = tid; idx < n * words; idx += kEvictThreads) {
-            const int j = idx / words, k = idx - j * words, dst = base + j;
-            uint8_t *b = block_of(r.new_pages, dst);
-            const uint32_t v = rows_s[idx];
-            if (k >= kw && k < kw + hd / 8) {
-                uint8_t *c = b + q4_v_code(hd, dst & 15, 2 * (k - kw) / NG, 2 * (k - kw) % NG);
-                *reinterpret_cast<uint16_t *>(c) = (uint16_t)v;
-                *reinterpret_cast<uint16_t *>(c + 4) = (uint16_t)(v >> 16);
-            } else {
-                *reinterpret_cast<uint32_t *>(b + at(dst, k)) = v;
-            }
+        for (int idx = tid; idx < n * halves; idx += kEvictThreads) {
+            const int j = idx / halves, dst = base + j;
+            *reinterpret_cast<uint16_t *>(block_of(r.new_pages, dst) + at(dst, idx - j * halves)) = rows_s[idx];
         }
         if (tid < n) w[base + tid] = w_s[tid];
         __syncthreads();

@@ -66,16 +66,20 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// NG words that lie together in shared memory
-template <int NG>
-__device__ __forceinline__ void lds_words(uint32_t (&v)[NG], uint32_t a) {
-    if constexpr (NG == 4)
+// N words that lie together in shared memory
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t a) {
+    if constexpr (N == 1)
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(a));
+    else if constexpr (N == 4)
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
     else
         asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
 }
-__device__ __forceinline__ float factor_m(uint32_t f) { return __half2float(__ushort_as_half((unsigned short)f)); }
-__device__ __forceinline__ float factor_d(uint32_t f) { return __uint_as_float(f & 0xffff0000u); }
+// The steps of groups g and g + 1 (g even) lie in one word; a BF16 number is the upper half of an FP32 one.
+__device__ __forceinline__ float step_of(const uint32_t *words, int g) { return __uint_as_float(g & 1 ? words[g >> 1] & 0xffff0000u : words[g >> 1] << 16); }
+// FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
+__device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
 // A share's pages of one row are tiles of two pages, spread over four warps; each warp has a ring of kQ4Slots tiles that bulk copies fill, the next row's first
 // tiles already while this one's results are put together.  Per page
@@ -92,7 +96,7 @@ template <int HD, int HPL>
 struct Q4Smem {  // bytes
     static constexpr int kRing = kQ4Warps<HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HPL> * kQ4Slots * 8,
                          kQuery = kMerge + kQ4Warps<HPL> * 4 * HPL * (HD + 2) * 4, kQueryRow = HD + 8,  // halves; the pad keeps the rows on different banks
-        kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kAll = kSums + 4 * HPL * (HD / kQ4Group + 1) * 4;
+        kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kBack = kSums + 2 * 4 * HPL * 4 * 2, kAll = kBack + 4 * HPL * 4;
 };
 
 // The largest score of a (row, head) and the sum of its weights over the row's parts, by all threads of a warp.
@@ -110,9 +114,9 @@ __device__ __forceinline__ float2 row_sums(const Q4AttnParams &p, int i, int sha
     return make_float2(M, L);
 }
 
-template <int HD, int HPL>
+template <int HD, int HPL, bool TRACK>
 __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
-    constexpr int NG = HD / kQ4Group, BLOCK = 20 * HD, FACT = NG * 4, TILE = kQ4Tile * BLOCK, W = kQ4Warps<HPL>, HEADS = 4 * HPL;
+    constexpr int NG = HD / kQ4Group, NW = NG / 2, BLOCK = 20 * HD, TILE = kQ4Tile * BLOCK, W = kQ4Warps<HPL>, HEADS = 4 * HPL;
     using Smem = Q4Smem<HD, HPL>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t = lane & 3;
@@ -121,7 +125,8 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
     float *mg_o = reinterpret_cast<float *>(smem + Smem::kMerge);  // where the warps meet: [warp][head][HD], [warp][head], [warp][head]
     float *mg_m = mg_o + W * G * HD, *mg_l = mg_m + W * G;
     __half *q_s = reinterpret_cast<__half *>(smem + Smem::kQuery);    // [limb][head][kQueryRow]
-    float *sums_s = reinterpret_cast<float *>(smem + Smem::kSums);  // [head][group], [head]
+    __half *sums_s = reinterpret_cast<__half *>(smem + Smem::kSums);  // [limb][head][4]: the query's sums over groups, scaled
+    float *back_s = reinterpret_cast<float *>(smem + Smem::kBack);    // [head]: what takes the scale of the scores back
     __shared__ int last_s;
     if (lane == 0) {
         for (int s = 0; s < kQ4Slots; s++) mbar_init(bars + s * 8, 1);
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
     while (from < share1) {
         const int i = row, to = min(share1, row_end(p, i)), n_tiles = part_tiles, pos_first = page0 << 4;
         const int pos_end = min(r.upto, (to - r.first) << 4);  // of this part, in the row
-        const bool track = p.scores && r.track >= 0;
+        const bool track = TRACK && r.track >= 0;
         // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
         // largest element), in two FP16 limbs.  Elements 2, 3, 6, 7 of eight meet 16 q.
         for (int head = warp; head < HEADS; head += W) {
@@ -213,13 +218,19 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                 to_q[0] = hi;
                 to_q[HEADS * Smem::kQueryRow / 2] = pack_h2(y0 - hf.x, y1 - hf.y);
             }
-            if (lane % (kQ4Group / E) == 0) sums_s[head * NG + lane / (kQ4Group / E)] = sum;
-            if (lane == 0) sums_s[HEADS * NG + head] = __uint_as_float((uint32_t)(127 + 24 - up) << 23);
+            if (lane % (kQ4Group / E) == 0) {  // 32 elements of up to 2^14: five powers of two less
+                const float whole = sum * (shift * 0.03125f);
+                const __half hi = __float2half_rn(whole);
+                sums_s[head * 4 + lane / (kQ4Group / E)] = hi;
+                sums_s[(HEADS + head) * 4 + lane / (kQ4Group / E)] = __float2half_rn(whole - __half2float(hi));
+            }
+            if (lane == 0) back_s[head] = __uint_as_float((uint32_t)(127 + 5 - up) << 23);
         }
         __syncthreads();
         // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8, as the B operand wants them
         uint32_t qh[NG][4], ql[HPL == 2 ? NG : 1][4];
-        float qsum[HPL][NG], back[HPL];  // of this lane's own heads: sums over the groups, and the scale of the scores
+        uint32_t qsum[HPL];  // k: the groups
+        float back[HPL];     // of this lane's own heads
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const __half *from_q = q_s + (HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : g8) * Smem::kQueryRow + g * kQ4Group + 8 * t;
@@ -228,12 +239,12 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
         }
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
-            back[h] = sums_s[HEADS * NG + HPL * t + h];
-#pragma unroll
-            for (int g = 0; g < NG; g++) qsum[h][g] = sums_s[(HPL * t + h) * NG + g];
+            const int column = HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : h * HEADS + g8;  // HPL = 2: h is the limb
+            qsum[h] = t < NW ? *reinterpret_cast<const uint32_t *>(sums_s + column * 4 + 2 * t) : 0u;
+            back[h] = back_s[HPL * t + h];
         }
-        float o[NG][2][4], omin[HPL][NG], m_run[HPL], l_run[HPL], vscale = 0.f;
-        uint32_t limit = 0;  // factors above this one ask for another scale
+        float o[NG][2][4], oo[4] = {0.f, 0.f, 0.f, 0.f}, m_run[HPL], l_run[HPL], vscale = 0.f;  // oo: the offsets' part, row g8 = group
+        uint32_t limit = 0;  // largest step in the scale's range, in both halves
 #pragma unroll
         for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -242,8 +253,6 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
         for (int h = 0; h < HPL; h++) {
             m_run[h] = -INFINITY;
             l_run[h] = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; g++) omin[h][g] = 0.f;
         }
         constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
@@ -259,19 +268,27 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++) {
                 const uint32_t base = tile + u * BLOCK;
-                uint32_t k0[NG], k1[NG], f0[NG], f1[NG];
-                lds_words<NG>(k0, base + lane * FACT);
-                lds_words<NG>(k1, base + 32 * FACT + lane * FACT);
-                lds_words<NG>(f0, base + 8 * HD + g8 * FACT);
-                lds_words<NG>(f1, base + 8 * HD + (g8 + 8) * FACT);
-                float off[HPL][2], sum[HPL][2];
+                uint32_t k0[NG], k1[NG], d0[NW], d1[NW], m0[1], m1[1];
+                lds_words<NG>(k0, base + lane * NG * 4);
+                lds_words<NG>(k1, base + (32 + lane) * NG * 4);
+                lds_words<NW>(d0, base + 8 * HD + g8 * NG * 2);
+                lds_words<NW>(d1, base + 8 * HD + (g8 + 8) * NG * 2);
+                lds_words<1>(m0, base + 9 * HD + g8 * NG * 2 + (t % NW) * 4);  // k beyond the groups: once more, times the zeros of qsum
+                lds_words<1>(m1, base + 9 * HD + (g8 + 8) * NG * 2 + (t % NW) * 4);
+                float off[4], sum[HPL][2];
+                mma_f16_first(off, m0[0], m1[0], 0u, 0u, qsum[0], 0u);
+                if constexpr (HPL == 1) {
+                    off[0] += off[1];
+                    off[1] = off[2] + off[3];
+                } else {
+                    mma_f16(off, m0[0], m1[0], 0u, 0u, qsum[1], 0u);
+                }
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
                     float c[4];
                     const uint32_t x0 = k0[g] >> 8, x1 = k1[g] >> 8;
                     mma_f16_first(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, qh[g][0], qh[g][1]);
                     mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, qh[g][2], qh[g][3]);
-                    const float d0 = factor_d(f0[g]), d1 = factor_d(f1[g]), m0 = factor_m(f0[g]), m1 = factor_m(f1[g]);
                     if constexpr (HPL == 1) {
                         c[0] += c[1];
                         c[1] = c[2] + c[3];
@@ -281,17 +298,15 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                     }
 #pragma unroll
                     for (int h = 0; h < HPL; h++) {
-                        const float c0 = c[h], c1 = c[HPL + h];
-                        sum[h][0] = g ? fmaf(d0, c0, sum[h][0]) : d0 * c0;
-                        sum[h][1] = g ? fmaf(d1, c1, sum[h][1]) : d1 * c1;
-                        off[h][0] = g ? fmaf(m0, qsum[h][g], off[h][0]) : m0 * qsum[h][g];
-                        off[h][1] = g ? fmaf(m1, qsum[h][g], off[h][1]) : m1 * qsum[h][g];
+                        sum[h][0] = g ? fmaf(step_of(d0, g), c[h], sum[h][0]) : step_of(d0, g) * c[h];
+                        sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
                     }
                 }
+                // 2^24 of the numbers, 2^-up; the sums' 2^5 2^-up
 #pragma unroll
                 for (int h = 0; h < HPL; h++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], back[h], off[h][x]);
+                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 524288.f, off[x * HPL + h]) * back[h];
             }
             if (track) {
                 float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
@@ -303,49 +318,53 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                         for (int x = 0; x < 2; x++)
                             if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
             }
-            uint32_t f[kQ4Tile][2][NG], steps = 0;
+            uint32_t d[kQ4Tile][2][NW], m[kQ4Tile][2], steps = limit;
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    lds_words<NG>(f[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * FACT);
+                    lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
+                    uint32_t one[1];
+                    lds_words<1>(one, tile + u * BLOCK + 19 * HD + (g8 % NG) * 32 + x * 16 + t * 4);  // rows beyond the groups: again, and not looked at
+                    m[u][x] = one[0];
                 }
             if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
 #pragma unroll
                 for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
+                        const int at = pos0 + 16 * u + 8 * x;
+                        const bool on = at + g8 < pos_end;
 #pragma unroll
                         for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
 #pragma unroll
-                        for (int g = 0; g < NG; g++) f[u][x][g] = on ? f[u][x][g] : 0u;
+                        for (int g = 0; g < NW; g++) d[u][x][g] = on ? d[u][x][g] : 0u;
+                        m[u][x] &= (at + 2 * t < pos_end ? 0xffffu : 0u) | (at + 2 * t + 1 < pos_end ? 0xffff0000u : 0u);
                     }
             }
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
-                for (int g = 0; g < NG; g++) steps = max(steps, max(f[u][0][g], f[u][1][g]));
-            // a larger score than any before, or a step beyond the scale's range: seldom after the first tiles
-            steps &= 0xffff0000u;
+                for (int g = 0; g < NW; g++) steps = __vmaxu2(steps, __vmaxu2(d[u][0][g], d[u][1][g]));
+            // a score far above the reference, or a step beyond the scale's range: seldom after the first tile
             float top[HPL];
-            bool grown = steps > limit;
+            bool grown = steps != limit;
 #pragma unroll
             for (int h = 0; h < HPL; h++) {
                 top[h] = s[h][0][0];
 #pragma unroll
                 for (int u = 0; u < kQ4Tile; u++) top[h] = fmaxf(fmaxf(top[h], s[h][u][0]), s[h][u][1]);
-                grown |= top[h] > m_run[h];
+                grown |= top[h] > m_run[h] + 8.f;
             }
             if (__any_sync(0xffffffffu, grown)) {
                 float fix[HPL], vfix = 1.f;
-                steps = __reduce_max_sync(0xffffffffu, steps);
-                if (steps > limit) {  // the largest step to 2^10 .. 2^11, up to 2^15 in range
-                    const int e = max((int)(steps >> 23) - 127, -100);
-                    const float next = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+                steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
+                if (steps > (limit & 0xffffu)) {  // the largest step to 2^2 .. 2^3, up to 2^7 in range: times weights of up to 2^8
+                    const int e = max((int)(steps >> 7) - 127, -100);
+                    const float next = __uint_as_float((uint32_t)(127 + 2 - e) << 23);
                     vfix = vscale == 0.f ? 0.f : next / vscale;
                     vscale = next;
-                    limit = (uint32_t)(e + 4 + 127) << 23 | 0x7fffffu;
+                    limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
                 }
 #pragma unroll
                 for (int h = 0; h < HPL; h++) {
@@ -355,9 +374,9 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                     fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
                     m_run[h] = mx;
                     l_run[h] *= fix[h];
-#pragma unroll
-                    for (int g = 0; g < NG; g++) omin[h][g] *= fix[h];
                 }
+#pragma unroll
+                for (int x = 0; x < 4; x++) oo[x] *= fix[HPL == 1 ? 0 : x & 1];
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -371,8 +390,8 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
             for (int u = 0; u < kQ4Tile; u++) {
                 const uint32_t base = tile + u * BLOCK + 10 * HD;
                 uint32_t v0[NG], v1[NG];
-                lds_words<NG>(v0, base + lane * FACT);
-                lds_words<NG>(v1, base + 32 * FACT + lane * FACT);
+                lds_words<NG>(v0, base + lane * NG * 4);
+                lds_words<NG>(v1, base + (32 + lane) * NG * 4);
                 float w[HPL][2], ws[HPL][2];
 #pragma unroll
                 for (int h = 0; h < HPL; h++) {
@@ -383,34 +402,35 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                     }
                     l_run[h] += w[h][0] + w[h][1];
                 }
+                // group -1: the weights alone, for the offsets
 #pragma unroll
-                for (int g = 0; g < NG; g++) {
+                for (int g = -1; g < NG; g++) {
                     float hi[HPL][2], lo[HPL][2];
 #pragma unroll
                     for (int h = 0; h < HPL; h++)
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            omin[h][g] = fmaf(w[h][x], factor_m(f[u][x][g]), omin[h][g]);
-                            const float y = ws[h][x] * factor_d(f[u][x][g]);
-                            hi[h][x] = __uint_as_float(__float_as_uint(y) & 0xffffe000u);  // what a half holds
+                            const float y = g < 0 ? w[h][x] : ws[h][x] * step_of(d[u][x], g < 0 ? 0 : g);
+                            hi[h][x] = upper_limb(y);
                             lo[h][x] = y - hi[h][x];
                         }
-                    uint32_t b0, b1;
-                    if constexpr (HPL == 1) {
-                        b0 = transpose8(pack_h2(hi[0][0], lo[0][0]));
-                        b1 = transpose8(pack_h2(hi[0][1], lo[0][1]));
-                    } else {
-                        b0 = transpose8(pack_h2(hi[0][0], hi[1][0]));
-                        b1 = transpose8(pack_h2(hi[0][1], hi[1][1]));
-                    }
-                    const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
-                    mma_f16(o[g][0], v0[g] & kLow, v0[g] & kHigh, v1[g] & kLow, v1[g] & kHigh, b0, b1);
-                    mma_f16(o[g][1], x0 & kLow, x0 & kHigh, x1 & kLow, x1 & kHigh, b0, b1);
-                    if constexpr (HPL == 2) {
-                        b0 = transpose8(pack_h2(lo[0][0], lo[1][0]));
-                        b1 = transpose8(pack_h2(lo[0][1], lo[1][1]));
-                        mma_f16(o[g][0], v0[g] & kLow, v0[g] & kHigh, v1[g] & kLow, v1[g] & kHigh, b0, b1);
-                        mma_f16(o[g][1], x0 & kLow, x0 & kHigh, x1 & kLow, x1 & kHigh, b0, b1);
+#pragma unroll
+                    for (int limb = 0; limb < HPL; limb++) {
+                        uint32_t b0, b1;
+                        if constexpr (HPL == 1) {
+                            b0 = transpose8(pack_h2(hi[0][0], lo[0][0]));
+                            b1 = transpose8(pack_h2(hi[0][1], lo[0][1]));
+                        } else {
+                            b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
+                            b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
+                        }
+                        if (g < 0) {
+                            mma_f16(oo, m[u][0], m[u][0], m[u][1], m[u][1], b0, b1);
+                        } else {
+                            const uint32_t a0 = v0[g < 0 ? 0 : g], a1 = v1[g < 0 ? 0 : g], x0 = a0 >> 8, x1 = a1 >> 8;
+                            mma_f16(o[g < 0 ? 0 : g][0], a0 & kLow, a0 & kHigh, a1 & kLow, a1 & kHigh, b0, b1);
+                            mma_f16(o[g < 0 ? 0 : g][1], x0 & kLow, x0 & kHigh, x1 & kLow, x1 & kHigh, b0, b1);
+                        }
                     }
                 }
             }
@@ -424,12 +444,13 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
-#pragma unroll
-                for (int g = 0; g < NG; g++) omin[h][g] += __shfl_xor_sync(0xffffffffu, omin[h][g], x);
-            }
+            for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
         }
+        float offset[HPL][NG];  // row g of the offsets' part: lanes 4 g + t
+#pragma unroll
+        for (int h = 0; h < HPL; h++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) offset[h][g] = __shfl_sync(0xffffffffu, HPL == 1 ? oo[0] + oo[1] : oo[h], 4 * g + t);
         const float unscale = vscale == 0.f ? 0.f : 16777216.f / vscale;
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
@@ -441,7 +462,7 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const float *c = &o[g][x >> 1][2 * (x & 1)];
-                    v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], x & 1 ? unscale * 0.0625f : unscale, omin[h][g]);
+                    v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], x & 1 ? unscale * 0.0625f : unscale, offset[h][g]);
                 }
                 *reinterpret_cast<float4 *>(mg_o + ((size_t)warp * G + head) * HD + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
             }
@@ -548,17 +569,22 @@ __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __gr
     }
 }
 
-template <int HD, int HPL>
+template <int HD, int HPL, bool TRACK>
 static int launch_q4_attn(const Q4AttnParams &a, int shares, cudaStream_t st) {
     static bool set[64] = {false};  // per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!set[dev & 63]) {
-        JUNO_CUDA_TRY(cudaFuncSetAttribute(q4_attn_kernel<HD, HPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD, HPL>::kAll));
+        JUNO_CUDA_TRY(cudaFuncSetAttribute(q4_attn_kernel<HD, HPL, TRACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD, HPL>::kAll));
         set[dev & 63] = true;
     }
-    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL>, dim3((unsigned)(shares * a.n_kv_heads)), dim3(kQ4Warps<HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
+    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL, TRACK>, dim3((unsigned)(shares * a.n_kv_heads)), dim3(kQ4Warps<HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
     return JUNO_OK;
+}
+
+template <int HD, bool TRACK>
+static int launch_q4_attn(const Q4AttnParams &a, int G, int shares, cudaStream_t st) {
+    return G <= 4 ? launch_q4_attn<HD, 1, TRACK>(a, shares, st) : launch_q4_attn<HD, 2, TRACK>(a, shares, st);
 }
 
 // Zeros, once; every launch leaves them so.
@@ -627,9 +653,9 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     a.err = c->gemv_scratch.qerr + word;
     ProfScope prof(c, st, PROF_ATTN, (double)bytes * H * p->row_bytes());
     if (hd == 128)
-        JUNO_TRY(G <= 4 ? (launch_q4_attn<128, 1>(a, shares, st)) : (launch_q4_attn<128, 2>(a, shares, st)));
+        JUNO_TRY((track ? launch_q4_attn<128, true>(a, G, shares, st) : launch_q4_attn<128, false>(a, G, shares, st)));
     else
-        JUNO_TRY(G <= 4 ? (launch_q4_attn<64, 1>(a, shares, st)) : (launch_q4_attn<64, 2>(a, shares, st)));
+        JUNO_TRY((track ? launch_q4_attn<64, true>(a, G, shares, st) : launch_q4_attn<64, false>(a, G, shares, st)));
     c->kernel_launches++;
     if (!track) return JUNO_OK;
     JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages + kQ4WeightPages - 1) / kQ4WeightPages * H)), dim3(kQ4WeightThreads), 0, st, a));

@@ -9,12 +9,14 @@
 // A NaN makes its group NaN (m is NaN, d 0).
 //
 // The pages of a head (16 positions) are one block of 20 * hd bytes, [layer][page][kv_head] in the pool:
-//   keys    codes    word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group
-//           factors  word [position][group]: m in the low half, d in the high one
-//   values  codes    half word [position / 8][u][position / 2 % 4][group][position % 2], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group
-//           factors  as for keys
-// so that lane (g, t) of a warp finds at 16 * lane (8 * lane for heads of 64) what the MMAs of decode attention want of it: for keys of position g its four (two)
-// groups' numbers, for values two positions of unit g.
+//   keys    codes  word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group
+//           d      half word [position][group]
+//           m      half word [position][group]
+//   values  codes  half word [position / 8][u][position / 2 % 4][group][position % 2], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group
+//           d      half word [position][group]
+//           m      half word [group][position]
+// Every piece lies as the MMAs of decode attention want it: lane (g, t) of a warp finds the numbers of all groups of position g (keys), and of two positions of
+// unit g (values), at 16 * lane (8 * lane for heads of 64); the offsets are operands of an MMA as they are.
 #pragma once
 #include <stdint.h>
 #include <string.h>
@@ -28,9 +30,11 @@ constexpr int kKvQ4 = 3;  // juno_kvpool::dtype
 
 JHD int q4_block_bytes(int hd) { return 20 * hd; }
 JHD int q4_k_code(int hd, int p, int t, int g) { return ((p * 4 + t) * (hd / kQ4Group) + g) * 4; }
-JHD int q4_k_factors(int hd, int p, int g) { return 8 * hd + (p * (hd / kQ4Group) + g) * 4; }
+JHD int q4_k_step(int hd, int p, int g) { return 8 * hd + (p * (hd / kQ4Group) + g) * 2; }
+JHD int q4_k_offset(int hd, int p, int g) { return 9 * hd + (p * (hd / kQ4Group) + g) * 2; }
 JHD int q4_v_code(int hd, int p, int u, int g) { return 10 * hd + ((((p >> 3) * 8 + u) * 4 + (p >> 1 & 3)) * (hd / kQ4Group) + g) * 4 + (p & 1) * 2; }
-JHD int q4_v_factors(int hd, int p, int g) { return 18 * hd + (p * (hd / kQ4Group) + g) * 4; }
+JHD int q4_v_step(int hd, int p, int g) { return 18 * hd + (p * (hd / kQ4Group) + g) * 2; }
+JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (g * 16 + p) * 2; }
 // Where number e of the eight of a key word lies: an AND with 0x000f000f leaves numbers 0 and 1 as the halves of an operand register, the
 // next ones follow at 4, 8 and 12 bits.
 JHD int q4_k_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }

@@ -19,9 +19,11 @@ extern "C" int q4_host_cover(int hd, unsigned char *nibbles) {
                 for (int e = 0; e < 8; e++) mark(2 * q4_k_code(hd, p, t, g) + q4_k_shift(e) / 4);
             for (int u = 0; u < 8; u++)
                 for (int i = 0; i < 4; i++) mark(2 * q4_v_code(hd, p, u, g) + i);
-            for (int b = 0; b < 8; b++) {
-                mark(2 * q4_k_factors(hd, p, g) + b);
-                mark(2 * q4_v_factors(hd, p, g) + b);
+            for (int b = 0; b < 4; b++) {
+                mark(2 * q4_k_step(hd, p, g) + b);
+                mark(2 * q4_k_offset(hd, p, g) + b);
+                mark(2 * q4_v_step(hd, p, g) + b);
+                mark(2 * q4_v_offset(hd, p, g) + b);
             }
         }
     return twice;
