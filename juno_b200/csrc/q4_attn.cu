@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
     __half *q_s = reinterpret_cast<__half *>(smem + Smem::kQuery);    // [limb][head][kQueryRow]
     __half *sums_s = reinterpret_cast<__half *>(smem + Smem::kSums);  // [limb][head][4]: the query's sums over groups, scaled
     float *back_s = reinterpret_cast<float *>(smem + Smem::kBack);    // [head]: what takes the scale of the scores back
-    __shared__ int last_s;
+    int row_a = -1, row_b = -1;             // rows that other shares have parts of, too: the first, the last
+    unsigned before_a = 0u, before_b = 0u;  // thread 0: their parts that were done before
     if (lane == 0) {
         for (int s = 0; s < kQ4Slots; s++) mbar_init(bars + s * 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -169,8 +170,17 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
             places_next = place(part_issued + 16);
         }
     };
+    constexpr int E = HD / 32, QUERIES = (HEADS + W - 1) / W;  // elements of a lane, heads of a warp
+    float query[QUERIES][E];
     auto begin = [&](int i, int from) {  // row i from page `from` of all pages
         row = i;
+#pragma unroll
+        for (int n = 0; n < QUERIES; n++) {
+            const int head = warp + n * W;
+            const float *src = p.q + (size_t)i * p.ldq + (size_t)(h0 + head) * HD + E * lane;
+#pragma unroll
+            for (int e = 0; e < E; e++) query[n][e] = head < G ? src[e] : 0.f;
+        }
         r = cache_row(p.rows, i);
         page0 = from - r.first;
         part_pages = r.upto > 0 ? min(share1, row_end(p, i)) - from : 0;
@@ -191,14 +201,15 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
         const bool track = TRACK && r.track >= 0;
         // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
         // largest element), in two FP16 limbs.  Elements 2, 3, 6, 7 of eight meet 16 q.
-        for (int head = warp; head < HEADS; head += W) {
-            constexpr int E = HD / 32;  // elements of a lane
+#pragma unroll
+        for (int n = 0; n < QUERIES; n++) {
+            const int head = warp + n * W;
+            if (head >= HEADS) break;
             const float scale = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
             float y[E], top = 0.f, sum = 0.f;
-            const float *src = p.q + (size_t)i * p.ldq + (size_t)(h0 + head) * HD + E * lane;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                y[e] = head < G ? src[e] * scale : 0.f;
+                y[e] = query[n][e] * scale;
                 sum += y[e];
                 top = fmaxf(top, fabsf(y[e]));
             }
@@ -473,55 +484,48 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
         }
         __syncthreads();
         const int end = row_end(p, i), share_a = first / p.share, parts = (end - 1) / p.share - share_a + 1;
-        for (int idx = tid; idx < G * HD; idx += W * 32) {
-            const int g = idx / HD, d = idx - g * HD;
-            float M = -INFINITY, L = 0.f, acc = 0.f;
+        for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {  // two dimensions of a head; a head to a warp, whose first lanes have the warps' shares of it
+            const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
+            float mw = lane < W ? mg_m[lane * G + g] : -INFINITY, lw = lane < W ? mg_l[lane * G + g] : 0.f, M = mw;
 #pragma unroll
-            for (int w = 0; w < W; w++) M = fmaxf(M, mg_m[w * G + g]);
+            for (int x = 1; x < W; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+            M = __shfl_sync(0xffffffffu, M, 0);
+            const float fw = lw == 0.f ? 0.f : exp2_fast(mw - M);  // a warp without pages has no share
+            float L = lw * fw, ax = 0.f, ay = 0.f;
+#pragma unroll
+            for (int x = 1; x < W; x <<= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+            L = __shfl_sync(0xffffffffu, L, 0);
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                const float lw = mg_l[w * G + g];
-                if (lw == 0.f) continue;  // a warp without pages
-                const float fw = exp2_fast(mg_m[w * G + g] - M);
-                L = fmaf(lw, fw, L);
-                acc = fmaf(mg_o[((size_t)w * G + g) * HD + d], fw, acc);
+                const float f = __shfl_sync(0xffffffffu, fw, w);
+                const float2 v = *reinterpret_cast<const float2 *>(mg_o + ((size_t)w * G + g) * HD + d);
+                if (f != 0.f) {
+                    ax = fmaf(v.x, f, ax);
+                    ay = fmaf(v.y, f, ay);
+                }
             }
             const size_t part = (size_t)(i + share) * p.n_heads + h0 + g;
-            if (parts == 1)
-                p.out[(size_t)i * p.ldo + (h0 + g) * HD + d] = pos_end > 0 ? acc / L : 0.f;
-            else
-                p.part_o[part * HD + d] = acc;
+            if (parts == 1) {
+                float *to_o = p.out + (size_t)i * p.ldo + (h0 + g) * HD + d;
+                to_o[0] = pos_end > 0 ? ax / L : 0.f;
+                to_o[1] = pos_end > 0 ? ay / L : 0.f;
+            } else {
+                *reinterpret_cast<float2 *>(p.part_o + part * HD + d) = make_float2(ax, ay);
+            }
             if (d == 0 && (parts > 1 || track)) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(M, L);
         }
-        if (parts > 1) {  // whoever is last puts the parts together, in their order
+        // The rows that this share has with others are its first and its last.  Whoever of a row is last puts its parts together, at the end.
+        if (parts > 1) {
             __syncthreads();
+            unsigned before = 0u;
             if (tid == 0) {
                 __threadfence();
-                unsigned *arrived = p.arrived + (size_t)i * p.n_kv_heads + kvh;
-                last_s = atomicAdd(arrived, 1u) == (unsigned)parts - 1;
-                if (last_s) {
-                    *arrived = 0;
-                    __threadfence();
-                }
+                before = atomicAdd(p.arrived + (size_t)i * p.n_kv_heads + kvh, 1u);
             }
-            __syncthreads();
-            if (last_s) {
-                for (int g = warp; g < G; g += W) {
-                    const float2 ml = row_sums(p, i, share_a, parts, h0 + g, lane);
-                    if (lane == 0) mg_m[g] = ml.x, mg_l[g] = 1.f / ml.y;
-                }
-                __syncthreads();
-                const size_t stride = (size_t)p.n_heads * HD;
-                for (int idx = tid; idx < G * HD; idx += W * 32) {
-                    const int g = idx / HD;
-                    const float *from_o = p.part_o + (size_t)(i + share_a) * stride + (size_t)h0 * HD + idx, *from_m = p.part_ml + ((size_t)(i + share_a) * p.n_heads + h0 + g) * 2;
-                    const float M = mg_m[g];
-                    float acc = 0.f;
-#pragma unroll 8
-                    for (int s = 0; s < parts; s++) acc = fmaf(__ldcg(from_o + s * stride), exp2_fast(__ldcg(from_m + (size_t)s * p.n_heads * 2) - M), acc);
-                    p.out[(size_t)i * p.ldo + (size_t)h0 * HD + idx] = acc * mg_l[g];
-                }
-            }
+            if (first < share0)
+                row_a = i, before_a = before;
+            else
+                row_b = i, before_b = before;
         }
         __syncthreads();  // the warps' results have been read
         if (__syncthreads_or(failed)) {
@@ -538,6 +542,62 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                 unsigned *arrived = p.arrived + (size_t)i * p.n_kv_heads + kvh;
                 if (parts > 1 && atomicAdd(arrived, 1u) == (unsigned)parts - 1) *arrived = 0;
             }
+    }
+    for (int which = 0; which < 2; which++) {
+        const int i = which ? row_b : row_a;
+        if (i < 0) continue;
+        const int share_a = cache_row(p.rows, i).first / p.share, parts = (row_end(p, i) - 1) / p.share - share_a + 1;
+        if (!__syncthreads_or(tid == 0 && (which ? before_b : before_a) == (unsigned)parts - 1)) continue;
+        // two dimensions of a head to a thread, a head to a warp, a part's largest score and sum to a lane
+        if (tid == 0) {
+            __threadfence();
+            p.arrived[(size_t)i * p.n_kv_heads + kvh] = 0;
+        }
+        const size_t stride = (size_t)p.n_heads * HD;
+        for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {
+            const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
+            const float2 *from_ml = reinterpret_cast<const float2 *>(p.part_ml) + (size_t)(i + share_a) * p.n_heads + h0 + g;
+            const float *from_o = p.part_o + (size_t)(i + share_a) * stride + (size_t)(h0 + g) * HD + d;
+            constexpr int AHEAD = 8;  // parts asked for before their weights are known
+            float2 v[AHEAD], ml = make_float2(-INFINITY, 0.f);
+            if (lane < parts) ml = __ldcg(from_ml + (size_t)lane * p.n_heads);
+#pragma unroll
+            for (int s = 0; s < AHEAD; s++)
+                if (s < parts) v[s] = __ldcg(reinterpret_cast<const float2 *>(from_o + s * stride));
+            float M = ml.x;
+            for (int s = lane + 32; s < parts; s += 32) M = fmaxf(M, __ldcg(from_ml + (size_t)s * p.n_heads).x);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+            float L = 0.f, ax = 0.f, ay = 0.f;
+            for (int base = 0; base < parts; base += 32) {
+                if (base > 0) ml = base + lane < parts ? __ldcg(from_ml + (size_t)(base + lane) * p.n_heads) : make_float2(-INFINITY, 0.f);
+                const float f = base + lane < parts ? exp2_fast(ml.x - M) : 0.f;
+                L = fmaf(ml.y, f, L);
+                const int n = min(32, parts - base);
+                if (base == 0) {
+#pragma unroll
+                    for (int s = 0; s < AHEAD; s++) {
+                        const float fs = __shfl_sync(0xffffffffu, f, s);
+                        if (s < parts) {
+                            ax = fmaf(v[s].x, fs, ax);
+                            ay = fmaf(v[s].y, fs, ay);
+                        }
+                    }
+                }
+#pragma unroll 12
+                for (int s = base ? 0 : AHEAD; s < n; s++) {
+                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(from_o + (base + s) * stride));
+                    const float fs = __shfl_sync(0xffffffffu, f, s);
+                    ax = fmaf(y.x, fs, ax);
+                    ay = fmaf(y.y, fs, ay);
+                }
+            }
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+            float *to_o = p.out + (size_t)i * p.ldo + (h0 + g) * HD + d;
+            to_o[0] = ax / L;
+            to_o[1] = ay / L;
+        }
     }
 }
 
