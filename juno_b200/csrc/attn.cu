@@ -1221,9 +1221,9 @@ int juno_seq_free(juno_seq *s) {
     JUNO_TRY(seq_check(s));
     juno_kvpool *p = s->pool;
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
-    {
+    if (p->owned_by_model) {
         DeviceGuard g(p->ctx->device);
-        cudaStreamSynchronize(p->ctx->stream);  // no kernel may still read these pages
+        cudaStreamSynchronize(p->ctx->stream);  // no kernel may still read these pages; calls on pools of their own take effect in order
     }
     for (int pg : s->pages)
         if (--p->page_refs[(size_t)pg] == 0) p->free_pages.push_back(pg);  // a shared page stays with its other holders

@@ -106,15 +106,15 @@ struct RowsParams {
     int track_tokens;
 };
 
-// Eight lanes' worth of work: one lane has eight neighbouring dimensions of a key or value, four lanes a group.
+// One lane has eight neighbouring dimensions of a key or value, four lanes a group: what is stored of a position is contiguous but for the values' offsets.
 template <int HD>
-__global__ void __launch_bounds__(256) q4_append_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ RowsParams p) {
     constexpr int LPV = HD / 8;  // lanes per vector
     const int H = p.n_kv_heads, sub = threadIdx.x % LPV;
     const int64_t vec = (int64_t)blockIdx.x * (256 / LPV) + threadIdx.x / LPV, n_vec = (int64_t)p.n_tokens * 2 * H;
     const bool on = vec < n_vec;
-    const int64_t row = on ? vec / (2 * H) : 0;
-    const int which = on ? (int)(vec - row * 2 * H) : 0, is_v = which >= H, h = which - is_v * H;
+    const int row = on ? (int)(vec / (2 * H)) : 0;
+    const int which = on ? (int)(vec - (int64_t)row * 2 * H) : 0, is_v = which >= H, h = which - is_v * H;
     float x[8];
     if (on) {
         const float *src = (is_v ? p.v : p.k) + row * p.ld + h * HD + sub * 8;
@@ -130,41 +130,49 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const RowsParams p) {
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = 0.f;
     }
-    float lo = INFINITY, hi = -INFINITY;
-    bool nan = false;
+    float lo = x[0], hi = x[0];
+    bool odd = x[0] != x[0];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        nan |= x[e] != x[e];
-        x[e] = fminf(fmaxf(x[e], -kQ4Most), kQ4Most);
+    for (int e = 1; e < 8; e++) {
+        odd |= x[e] != x[e];
         lo = fminf(lo, x[e]);
         hi = fmaxf(hi, x[e]);
     }
-    if (nan) hi = INFINITY;  // the group's mark: no clamped value is infinite
+    if (odd || fmaxf(hi, -lo) > kQ4Most) {  // seldom: a NaN, or values beyond what FP16 holds
+        lo = kQ4Most;
+        hi = -kQ4Most;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            x[e] = fminf(fmaxf(x[e], -kQ4Most), kQ4Most);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+        if (odd) hi = INFINITY;  // the group's mark of a NaN: no clamped value is infinite
+    }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    nan = hi == INFINITY;
+    const bool nan = hi == INFINITY;
     const __half mh = nan ? __ushort_as_half(0x7e00) : __float2half_rn(lo);
     const float reach = hi - lo;
     const __nv_bfloat16 dh = __float2bfloat16_rn(nan || reach < kQ4Nothing ? 0.f : __fdiv_rn(reach, 15.f));
-    const float m = __half2float(mh), d = __bfloat162float(dh), inv = __fdiv_rn(1.f, d);
+    const float m = __half2float(mh), d = __bfloat162float(dh), inv = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
     uint32_t q[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) q[e] = (uint32_t)q4_number(x[e], m, d, inv);
     if (!on) return;
-    const CacheRow r = cache_row(p.rows, cache_find(p.rows, (int)row));
-    const int pos = r.upto + (int)row - r.first, pp = pos & 15, g = sub >> 2;
+    const CacheRow r = cache_row(p.rows, cache_find(p.rows, row));
+    const int pos = r.upto + row - r.first, pp = pos & 15, g = sub >> 2;
     const int page = p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)];
     uint8_t *block = static_cast<uint8_t *>(p.kpool) + (((size_t)p.layer * p.n_pages + page) * H + h) * q4_block_bytes(HD);
+    uint32_t w = 0;
     if (is_v) {
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-            *reinterpret_cast<uint16_t *>(block + q4_v_code(HD, pp, 2 * (sub & 3) + u, g)) =
-                (uint16_t)(q[4 * u] | q[4 * u + 1] << 4 | q[4 * u + 2] << 8 | q[4 * u + 3] << 12);
+        for (int e = 0; e < 8; e++) w |= q[e] << (4 * e);
+        *reinterpret_cast<uint32_t *>(block + q4_v_code(HD, pp, 2 * (sub & 3), g)) = w;
     } else {
-        uint32_t w = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++) w |= q[e] << q4_k_shift(e);
         *reinterpret_cast<uint32_t *>(block + q4_k_code(HD, pp, sub & 3, g)) = w;
@@ -177,49 +185,64 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const RowsParams p) {
     }
 }
 
-__device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
-    if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-        reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) dst[e] = x[e];
-    }
-}
-
+// One lane has four neighbouring dimensions, so that a warp's stores are contiguous; kReadRows rows to a lane, whose loads are under way together.
+constexpr int kReadRows = 4;
 template <int HD>
-__global__ void __launch_bounds__(256) q4_read_kernel(const RowsParams p) {
-    constexpr int LPV = HD / 8;
-    const int H = p.n_kv_heads, sub = threadIdx.x % LPV;
+__global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ RowsParams p) {
+    constexpr int LPV = HD / 4;
+    const int H = p.n_kv_heads, sub = threadIdx.x % LPV, piece = sub & 7, g = sub >> 3;
     const int64_t vec = (int64_t)blockIdx.x * (256 / LPV) + threadIdx.x / LPV;
-    if (vec >= (int64_t)p.n_tokens * 2 * H) return;
-    const int64_t row = vec / (2 * H);
-    const int which = (int)(vec - row * 2 * H), is_v = which >= H, h = which - is_v * H;
-    const CacheRow r = cache_row(p.rows, cache_find(p.rows, (int)row));
-    const int pos = r.upto + (int)row - r.first, pp = pos & 15, g = sub >> 2;
-    const int page = p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)];
-    const uint8_t *block = static_cast<const uint8_t *>(p.kpool) + (((size_t)p.layer * p.n_pages + page) * H + h) * q4_block_bytes(HD);
-    const float m = __half2float(*reinterpret_cast<const __half *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))));
-    const float d = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))));
-    float x[8];
-    if (is_v) {
+    const int row0 = (int)(vec / (2 * H)) * kReadRows;
+    if (row0 >= p.n_tokens) return;
+    const int which = (int)(vec % (2 * H)), is_v = which >= H, h = which - is_v * H;
+    int i = cache_find(p.rows, row0), next = i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : INT_MAX;
+    CacheRow r = cache_row(p.rows, i);
+    uint32_t w[kReadRows];
+    float m[kReadRows], d[kReadRows];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const uint32_t w = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, 2 * (sub & 3) + u, g));
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[4 * u + i] = fmaf(d, (float)(w >> (4 * i) & 15u), m);
+    for (int n = 0; n < kReadRows; n++) {
+        const int row = row0 + n;
+        if (row >= p.n_tokens) break;
+        if (row >= next) {
+            i = cache_find(p.rows, row);
+            r = cache_row(p.rows, i);
+            next = i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : INT_MAX;
         }
-    } else {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, sub & 3, g));
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = fmaf(d, (float)(w >> q4_k_shift(e) & 15u), m);
+        const int pos = r.upto + row - r.first, pp = pos & 15;
+        const int page = p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)];
+        const uint8_t *block = static_cast<const uint8_t *>(p.kpool) + (((size_t)p.layer * p.n_pages + page) * H + h) * q4_block_bytes(HD);
+        m[n] = __half2float(*reinterpret_cast<const __half *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))));
+        d[n] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))));
+        // numbers 0..3 of a unit (values), or numbers 0..3 or 4..7 of a word (keys): brought to where a key word has numbers 0..3
+        if (is_v) {
+            const uint32_t u = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g));
+            w[n] = (u & 15u) | (u >> 4 & 15u) << 16 | (u >> 8 & 15u) << 4 | (u >> 12) << 20;
+        } else {
+            w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g)) >> (8 * (piece & 1));
+        }
     }
-    store8((is_v ? p.v : p.k) + row * p.ld + h * HD + sub * 8, x);
+    float *out = (is_v ? p.v : p.k) + (int64_t)row0 * p.ld + h * HD + sub * 4;
+    const bool vec4 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (p.ld & 3) == 0;
+#pragma unroll
+    for (int n = 0; n < kReadRows; n++) {
+        if (row0 + n >= p.n_tokens) break;
+        const float4 x = make_float4(fmaf(d[n], (float)(w[n] & 15u), m[n]), fmaf(d[n], (float)(w[n] >> 16 & 15u), m[n]), fmaf(d[n], (float)(w[n] >> 4 & 15u), m[n]),
+                                     fmaf(d[n], (float)(w[n] >> 20 & 15u), m[n]));
+        float *to = out + n * p.ld;
+        if (vec4) {
+            *reinterpret_cast<float4 *>(to) = x;
+        } else {
+            to[0] = x.x;
+            to[1] = x.y;
+            to[2] = x.z;
+            to[3] = x.w;
+        }
+    }
 }
 
 // FP16 and FP32 pages: eight elements a thread, both directions.
 template <typename T, bool APPEND>
-__global__ void __launch_bounds__(256) rows_kernel(const RowsParams p, int hd) {
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowsParams p, int hd) {
     const int H = p.n_kv_heads, per = hd / 8;
     const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)p.n_tokens * 2 * H * per;
     if (item >= n) return;
@@ -260,7 +283,8 @@ static int launch_rows(juno_ctx *c, const juno_kvpool *p, int layer, const Cache
     a.weights = p->weights;
     a.track_tokens = p->track_tokens;
     const int hd = p->head_dim;
-    const int64_t lanes = (int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8);
+    const int64_t lanes = p->dtype == kKvQ4 && !APPEND ? (int64_t)(n_tokens + kReadRows - 1) / kReadRows * 2 * p->n_kv_heads * (hd / 4)
+                                                       : (int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8);
     const unsigned blocks = (unsigned)((lanes + 255) / 256);
     ProfScope prof(c, st, APPEND ? PROF_ROPE_APPEND : PROF_OTHER, (double)n_tokens * p->n_kv_heads * (8.0 * hd + p->row_bytes()));
     if (p->dtype == kKvQ4) {
@@ -286,7 +310,7 @@ int launch_kv_append(juno_ctx *c, const juno_kvpool *p, int layer, const CacheRo
 // ───────────────────────────── weights ────────────────────────────────────────────────────
 // w[row][kv_head][ld], the first positions of each row; STORE: into the pool.
 template <bool STORE>
-__global__ void __launch_bounds__(256) weights_kernel(const CacheRows rows, float *weights, int layer, int n_layers, int n_kv_heads, int track_tokens, float *w, int64_t ld) {
+__global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ CacheRows rows, float *weights, int layer, int n_layers, int n_kv_heads, int track_tokens, float *w, int64_t ld) {
     const int i = blockIdx.z, h = blockIdx.y, pos = blockIdx.x * 256 + threadIdx.x;
     const CacheRow r = cache_row(rows, i);
     if (pos >= r.upto) return;
@@ -319,102 +343,223 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kEvictThreads = 256, kEvictRows = 64;
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kSelectCached = 24576, kBins = 2048;
 
-// One CTA per (sequence, layer, head): the positions that stay, then their rows, in place and in order.  A row moves to the front or stays, so that what a
-// step of kEvictRows rows overwrites has been read by it or by an earlier one.
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const EvictParams p) {
+// Sum over the threads of the block before this one, in *all the sum over all of them.  `sums`: kSelectWarps words.
+__device__ __forceinline__ unsigned block_before(unsigned v, unsigned *sums, unsigned *all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned upto = v;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += y;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    unsigned s = sums[lane], w = s;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, w, x);
+        if (lane >= x) w += y;
+    }
+    *all = __shfl_sync(0xffffffffu, w, 31);
+    const unsigned before = __shfl_sync(0xffffffffu, w - s, warp);
+    __syncthreads();
+    return before + upto - v;
+}
+
+// One CTA per (sequence, layer, head): which positions stay, in order, and their weights.  The weight that decides (the need-th largest) is found digit by
+// digit, 11, 11 and 10 bits, with a count of every digit in shared memory: three passes over the weights, whatever they are.  Up to kSelectCached weights are
+// read from memory once.
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
     const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const EvictRow r = p.rows[i];
     float *w = p.weights + (((size_t)r.track * p.n_layers + layer) * p.n_kv_heads + h) * p.track_tokens;
     int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld;
-    for (int j = r.keep + tid; j < p.kept_ld; j += kEvictThreads) kept[j] = -1;
-    __shared__ unsigned hist[256];
-    __shared__ int sums[kEvictThreads / 32][2];
-    __shared__ unsigned sh_key, sh_need;
+    for (int j = r.keep + tid; j < p.kept_ld; j += kSelectThreads) kept[j] = -1;
     if (r.keep == r.len) {
-        for (int j = tid; j < r.keep; j += kEvictThreads) kept[j] = j;
+        for (int j = tid; j < r.keep; j += kSelectThreads) kept[j] = j;
         return;
     }
+    extern __shared__ float cached[];  // kSelectCached
+    __shared__ unsigned bins[kBins], sums[kSelectWarps], digit_s, left_s;
     const int old = r.len - r.recent;  // candidates
-    unsigned need = (unsigned)(r.keep - r.recent), key = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
+    const bool whole = r.len <= kSelectCached;
+    if (whole) {
+        for (int j = tid; j < r.len; j += kSelectThreads) cached[j] = w[j];
         __syncthreads();
-        for (int j = tid; j < old; j += kEvictThreads) {
-            const uint32_t u = weight_key(w[j]);
-            if ((u & mask) == key) atomicAdd(&hist[u >> shift & 255u], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            unsigned left = need;
-            int b = 255;
-            while (b > 0 && hist[b] < left) left -= hist[b--];
-            sh_key = key | (unsigned)b << shift;
-            sh_need = left;
-        }
-        __syncthreads();
-        key = sh_key;
-        need = sh_need;
-        mask |= 255u << shift;
     }
-    // positions above `key` stay, and the first `need` of those that equal it
-    int done = 0, equal = 0;
-    for (int base = 0; base < r.len; base += kEvictThreads) {
-        const int j = base + tid;
-        const uint32_t u = j < old ? weight_key(w[j]) : 0u;
-        const bool same = j < old && u == key;
-        const unsigned eq = __ballot_sync(0xffffffffu, same);
-        if (lane == 0) sums[warp][0] = __popc(eq);
+    unsigned need = (unsigned)(r.keep - r.recent), key = 0;
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const unsigned mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, digits = pass == 2 ? 1023u : 2047u;
+        bins[tid] = bins[tid + kSelectThreads] = 0;
         __syncthreads();
-        int before = equal, all = 0;
-        for (int k = 0; k < kEvictThreads / 32; k++) {
-            if (k < warp) before += sums[k][0];
-            all += sums[k][0];
+        for (int j = tid; j < old; j += kSelectThreads) {
+            const uint32_t u = weight_key(whole ? cached[j] : w[j]);
+            if ((u & mask) == key) atomicAdd(&bins[u >> shift & digits], 1u);
         }
-        const int rank = before + __popc(eq & ((1u << lane) - 1u));
-        const bool stays = j < r.len && (j >= old || u > key || (same && rank < (int)need));
-        const unsigned st = __ballot_sync(0xffffffffu, stays);
-        if (lane == 0) sums[warp][1] = __popc(st);
         __syncthreads();
-        int at = done, sum = 0;
-        for (int k = 0; k < kEvictThreads / 32; k++) {
-            if (k < warp) at += sums[k][1];
-            sum += sums[k][1];
+        // from the largest digit down: the one in which the need-th weight lies
+        const unsigned a = bins[kBins - 1 - 2 * tid], b = bins[kBins - 2 - 2 * tid];
+        unsigned all;
+        const unsigned before = block_before(a + b, sums, &all);
+        if (before < need && need <= before + a + b) {
+            const bool first = need <= before + a;
+            digit_s = kBins - 1 - 2 * tid - !first;
+            left_s = need - before - (first ? 0u : a);
         }
-        if (stays) kept[at + __popc(st & ((1u << lane) - 1u))] = j;
+        __syncthreads();
+        if (need > 0) {
+            key |= digit_s << shift;
+            need = left_s;
+        } else {
+            key = 0xffffffffu;  // no weight has this key
+            break;
+        }
+    }
+    // positions above `key` stay, and the first `need` of those that equal it.  A warp has a run of the positions; those of one stretch are all read before any
+    // weight moves, and weights move to the front.
+    unsigned done = 0, equal = 0;
+    for (int base = 0; base < r.len; base += kSelectCached) {
+        const int n = min(kSelectCached, r.len - base), run = (n + kSelectWarps * 32 - 1) / (kSelectWarps * 32) * 32, from = min(n, warp * run), to = min(n, from + run);
+        if (!whole) {
+            __syncthreads();
+            for (int j = tid; j < n; j += kSelectThreads) cached[j] = w[base + j];
+            __syncthreads();
+        }
+        unsigned same = 0, above = 0;  // of this warp, in lane 0
+        for (int j = from; j < to; j += 32) {
+            const int at = base + j + lane;
+            const uint32_t u = j + lane < to ? weight_key(cached[j + lane]) : 0u;
+            same += __popc(__ballot_sync(0xffffffffu, j + lane < to && at < old && u == key));
+            above += __popc(__ballot_sync(0xffffffffu, j + lane < to && (at >= old || u > key)));
+        }
+        unsigned all;
+        unsigned rank = equal + __shfl_sync(0xffffffffu, block_before(lane == 0 ? same : 0u, sums, &all), 0);
         equal += all;
-        done += sum;
-        __syncthreads();
+        const unsigned taken = rank < need ? min(same, need - rank) : 0u;
+        unsigned out = done + __shfl_sync(0xffffffffu, block_before(lane == 0 ? above + taken : 0u, sums, &all), 0);
+        done += all;
+        for (int j = from; j < to; j += 32) {
+            const int at = base + j + lane;
+            const bool on = j + lane < to;
+            const float v = on ? cached[j + lane] : 0.f;
+            const uint32_t u = weight_key(v);
+            const bool eq = on && at < old && u == key;
+            const unsigned eqs = __ballot_sync(0xffffffffu, eq);
+            const bool stays = on && (at >= old || u > key || (eq && rank + __popc(eqs & ((1u << lane) - 1u)) < need));
+            const unsigned st = __ballot_sync(0xffffffffu, stays);
+            if (stays) {
+                const unsigned to_j = out + __popc(st & ((1u << lane) - 1u));
+                kept[to_j] = at;
+                w[to_j] = v;
+            }
+            rank += __popc(eqs);
+            out += __popc(st);
+        }
     }
-    // the rows as half words: keys' numbers, values' numbers, and the four kinds of factors
-    extern __shared__ uint16_t rows_s[];  // [kEvictRows][hd * 5 / 8]
-    const int hd = p.hd, NG = hd / kQ4Group, halves = hd * 5 / 8;
-    __shared__ float w_s[kEvictRows];
-    auto block_of = [&](int list, int pos) {
-        return p.pool + (((size_t)layer * p.n_pages + p.pages[list + (pos >> 4)]) * p.n_kv_heads + h) * q4_block_bytes(hd);
-    };
-    auto at = [&](int pos, int i) {  // half word i of a row: where it lies in a block
-        const int pp = pos & 15, q = hd / 4;
-        if (i < q) return q4_k_code(hd, pp, 0, 0) + 2 * i;
-        if ((i -= q) < q) return q4_v_code(hd, pp, i / NG, i % NG);
-        i -= q;
-        const int kind = i / NG, g = i - kind * NG;
-        return kind == 0 ? q4_k_step(hd, pp, g) : kind == 1 ? q4_k_offset(hd, pp, g) : kind == 2 ? q4_v_step(hd, pp, g) : q4_v_offset(hd, pp, g);
-    };
-    for (int base = 0; base < r.keep; base += kEvictRows) {
-        const int n = min(kEvictRows, r.keep - base);
-        for (int idx = tid; idx < n * halves; idx += kEvictThreads) {
-            const int j = idx / halves, src = kept[base + j];
-            rows_s[idx] = *reinterpret_cast<const uint16_t *>(block_of(r.old_pages, src) + at(src, idx - j * halves));
+}
+
+// Copies between rows of two blocks in 16-, 8- and 2-byte pieces: PIECES of them in a row, this one is number `i`.
+template <int HD>
+struct Q4Row {
+    static constexpr int NG = HD / kQ4Group, CODES = HD / 32;                    // 16-byte pieces of a row's numbers, keys' or values'
+    static constexpr int FACTORS = 3, PIECES = 2 * CODES + FACTORS + NG;  // steps and offsets of keys, steps of values: NG half words each; values' offsets
+    uint4 data;
+    __device__ __forceinline__ void load(const uint8_t *b, int pp, int i) {
+        if (i < 2 * CODES) {
+            data = *reinterpret_cast<const uint4 *>(b + codes(pp, i));
+        } else if (i < 2 * CODES + FACTORS) {
+            const uint8_t *f = b + factors(pp, i - 2 * CODES);
+            if constexpr (NG == 4) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(f);
+                data.x = v.x;
+                data.y = v.y;
+            } else {
+                data.x = *reinterpret_cast<const uint32_t *>(f);
+            }
+        } else {
+            data.x = *reinterpret_cast<const uint16_t *>(b + q4_v_offset(HD, pp, i - 2 * CODES - FACTORS));
         }
-        if (tid < n) w_s[tid] = w[kept[base + tid]];
+    }
+    __device__ __forceinline__ void store(uint8_t *b, int pp, int i) const {
+        if (i < 2 * CODES) {
+            *reinterpret_cast<uint4 *>(b + codes(pp, i)) = data;
+        } else if (i < 2 * CODES + FACTORS) {
+            uint8_t *f = b + factors(pp, i - 2 * CODES);
+            if constexpr (NG == 4)
+                *reinterpret_cast<uint2 *>(f) = make_uint2(data.x, data.y);
+            else
+                *reinterpret_cast<uint32_t *>(f) = data.x;
+        } else {
+            *reinterpret_cast<uint16_t *>(b + q4_v_offset(HD, pp, i - 2 * CODES - FACTORS)) = (uint16_t)data.x;
+        }
+    }
+    static __device__ __forceinline__ int codes(int pp, int i) { return i < CODES ? q4_k_code(HD, pp, 0, 0) + 16 * i : q4_v_code(HD, pp, 0, i - CODES); }
+    static __device__ __forceinline__ int factors(int pp, int i) { return i == 0 ? q4_k_step(HD, pp, 0) : i == 1 ? q4_k_offset(HD, pp, 0) : q4_v_step(HD, pp, 0); }
+};
+
+__device__ __forceinline__ uint8_t *evict_block(const EvictParams &p, int layer, int h, int list, int pos) {
+    return p.pool + (((size_t)layer * p.n_pages + p.pages[list + (pos >> 4)]) * p.n_kv_heads + h) * (size_t)q4_block_bytes(p.hd);
+}
+
+// The rows that stay, into fresh pages: a warp has one page of one head.
+template <int HD>
+__global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) {
+    using Row = Q4Row<HD>;
+    const int i = blockIdx.z, layer = blockIdx.y, lane = threadIdx.x & 31;
+    const EvictRow r = p.rows[i];
+    if (r.keep == r.len) return;
+    const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), h = unit % p.n_kv_heads, base = unit / p.n_kv_heads * kPageTokens, n = min(kPageTokens, r.keep - base);
+    if (n <= 0) return;
+    const int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld + base;
+    const int src = lane < n ? kept[lane] : 0;
+    const uint8_t *from = evict_block(p, layer, h, r.old_pages, src);
+    uint8_t *to = evict_block(p, layer, h, r.new_pages, base);
+    constexpr int STEPS = (kPageTokens * Row::PIECES + 31) / 32;
+    Row row[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int x = k * 32 + lane, j = x / Row::PIECES;
+        const int at = __shfl_sync(0xffffffffu, src, j & 15);
+        const uint8_t *b = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, (unsigned long long)reinterpret_cast<uintptr_t>(from), j & 15));
+        if (j < n) row[k].load(b, at & 15, x - j * Row::PIECES);
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) {
+        const int x = k * 32 + lane, j = x / Row::PIECES;
+        if (j < n) row[k].store(to, j, x - j * Row::PIECES);
+    }
+}
+
+// The same in place, for a pool without enough free pages: one CTA per (sequence, layer, head) takes kMoveRows rows a step, in order.  A row moves to the
+// front or stays, so that what a step overwrites has been read by it or by an earlier one.
+constexpr int kMoveRows = 64, kMoveThreads = 512;
+template <int HD>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+    using Row = Q4Row<HD>;
+    const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, tid = threadIdx.x;
+    const EvictRow r = p.rows[i];
+    if (r.keep == r.len) return;
+    const int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld;
+    constexpr int STEPS = (kMoveRows * Row::PIECES + kMoveThreads - 1) / kMoveThreads;
+    for (int base = 0; base < r.keep; base += kMoveRows) {
+        const int n = min(kMoveRows, r.keep - base);
+        Row row[STEPS];
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const int x = k * kMoveThreads + tid, j = x / Row::PIECES;
+            if (j >= n) continue;
+            const int src = kept[base + j];
+            row[k].load(evict_block(p, layer, h, r.old_pages, src), src & 15, x - j * Row::PIECES);
+        }
         __syncthreads();
-        for (int idx = tid; idx < n * halves; idx += kEvictThreads) {
-            const int j = idx / halves, dst = base + j;
-            *reinterpret_cast<uint16_t *>(block_of(r.new_pages, dst) + at(dst, idx - j * halves)) = rows_s[idx];
+#pragma unroll
+        for (int k = 0; k < STEPS; k++) {
+            const int x = k * kMoveThreads + tid, j = x / Row::PIECES;
+            if (j < n) row[k].store(evict_block(p, layer, h, r.new_pages, base + j), (base + j) & 15, x - j * Row::PIECES);
         }
-        if (tid < n) w[base + tid] = w_s[tid];
         __syncthreads();
     }
 }
@@ -571,19 +716,23 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         JUNO_TRY(cache_call_distinct(p, n, seqs));
         for (int i = 0; i < n; i++) JUNO_REQUIRE(seqs[i]->track >= 0, "sequence %d keeps no weights (juno_seq_track)", i);
         if (kept_dev) JUNO_TRY(device_memory(c, kept_dev, "kept"));
-        // Pages of the front that another sequence holds too are left to it: their rows go to fresh pages.
-        std::vector<EvictRow> rows;
-        std::vector<int32_t> pages;
-        size_t fresh = 0;
+        // The rows go to fresh pages where the pool has enough of them, which all warps can fill side by side; else they move within their pages, but for pages
+        // that another sequence holds too: those are left to it, and their rows go to fresh ones.
+        const int np = (keep + kPageTokens - 1) / kPageTokens;
+        size_t shared = 0, cut = 0;
         for (int i = 0; i < n; i++) {
             const juno_seq *s = seqs[i];
             if (s->len <= keep) continue;
-            for (int j = 0; j < (keep + kPageTokens - 1) / kPageTokens; j++) fresh += p->page_refs[(size_t)s->pages[(size_t)j]] > 1;
+            cut++;
+            for (int j = 0; j < np; j++) shared += p->page_refs[(size_t)s->pages[(size_t)j]] > 1;
         }
-        if (fresh > p->free_pages.size()) {
-            set_error("KV pool exhausted: %zu pages free, %zu needed for rows of shared pages", p->free_pages.size(), fresh);
+        if (shared > p->free_pages.size()) {
+            set_error("KV pool exhausted: %zu pages free, %zu needed for rows of shared pages", p->free_pages.size(), shared);
             return JUNO_ERR_OOM;
         }
+        const bool fresh = cut * np <= p->free_pages.size();
+        std::vector<EvictRow> rows;
+        std::vector<int32_t> pages;
         size_t next = p->free_pages.size();
         for (int i = 0; i < n; i++) {
             const juno_seq *s = seqs[i];
@@ -591,9 +740,9 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
             if (s->len > keep) {
                 pages.insert(pages.end(), s->pages.begin(), s->pages.end());
                 r.new_pages = (int)pages.size();
-                for (int j = 0; j < (keep + kPageTokens - 1) / kPageTokens; j++) {
+                for (int j = 0; j < np; j++) {
                     const int pg = s->pages[(size_t)j];
-                    pages.push_back(p->page_refs[(size_t)pg] > 1 ? p->free_pages[--next] : pg);
+                    pages.push_back(fresh || p->page_refs[(size_t)pg] > 1 ? p->free_pages[--next] : pg);
                 }
             }
             rows.push_back(r);
@@ -620,18 +769,29 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         a.weights = p->weights;
         a.kept = kept_dev ? kept_dev : reinterpret_cast<int32_t *>(scratch + row_bytes + page_bytes);
         a.kept_ld = keep;
+        const dim3 heads((unsigned)p->n_kv_heads, (unsigned)p->n_layers, (unsigned)n), units((unsigned)((np * p->n_kv_heads + 7) / 8), (unsigned)p->n_layers, (unsigned)n);
+        const size_t cached = kSelectCached * sizeof(float);
+        static bool set[64] = {false};  // per device
+        if (!set[c->device & 63]) {
+            JUNO_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cached));
+            set[c->device & 63] = true;
+        }
         {
             ProfScope prof(c, st.st, PROF_OTHER, 0);
-            evict_kernel<<<dim3((unsigned)p->n_kv_heads, (unsigned)p->n_layers, (unsigned)n), kEvictThreads, (size_t)kEvictRows * p->head_dim * 5 / 4, st.st>>>(a);
+            evict_select_kernel<<<heads, kSelectThreads, cached, st.st>>>(a);
+            JUNO_CUDA_TRY(cudaGetLastError());
+            if (fresh)
+                p->head_dim == 128 ? evict_gather_kernel<128><<<units, 256, 0, st.st>>>(a) : evict_gather_kernel<64><<<units, 256, 0, st.st>>>(a);
+            else
+                p->head_dim == 128 ? evict_move_kernel<128><<<heads, kMoveThreads, 0, st.st>>>(a) : evict_move_kernel<64><<<heads, kMoveThreads, 0, st.st>>>(a);
         }
         JUNO_CUDA_TRY(cudaGetLastError());
-        c->kernel_launches++;
+        c->kernel_launches += 2;
         p->free_pages.resize(next);
         int rc = JUNO_OK;
         for (int i = 0; i < n; i++) {
             juno_seq *s = seqs[i];
             if (s->len <= keep) continue;
-            const int np = (keep + kPageTokens - 1) / kPageTokens;
             int32_t *row = p->h_table + (size_t)s->slot * p->max_pages_per_seq;
             int lo = np, hi = -1;
             for (int j = 0; j < (int)s->pages.size(); j++) {

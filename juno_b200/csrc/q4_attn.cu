@@ -76,6 +76,9 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t a) {
     else
         asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
 }
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
 // The steps of groups g and g + 1 (g even) lie in one word; a BF16 number is the upper half of an FP32 one.
 __device__ __forceinline__ float step_of(const uint32_t *words, int g) { return __uint_as_float(g & 1 ? words[g >> 1] & 0xffff0000u : words[g >> 1] << 16); }
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
@@ -140,6 +143,7 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
     const uint8_t *plane = p.pool + ((size_t)p.layer * p.n_pages * p.n_kv_heads + kvh) * BLOCK;
     const size_t page_bytes = (size_t)p.n_kv_heads * BLOCK;
     const uint64_t policy = l2_evict_first_policy();
+    const uint32_t v_piece = q4_v_code(HD, lane & 15, 0, lane >> 4);  // this lane's row of the four matrices of groups 0 and 1; two groups on: 32 bytes flipped
     const int share0 = share * p.share, share1 = min(p.total, share0 + p.share);
     unsigned issued = 0, used = 0;  // tiles through this warp's ring
     bool failed = false;
@@ -399,10 +403,9 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
             }
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++) {
-                const uint32_t base = tile + u * BLOCK + 10 * HD;
-                uint32_t v0[NG], v1[NG];
-                lds_words<NG>(v0, base + lane * NG * 4);
-                lds_words<NG>(v1, base + (32 + lane) * NG * 4);
+                uint32_t v0[NG], v1[NG];  // unit g8 of positions 2t, 2t + 1, and of those eight farther
+#pragma unroll
+                for (int g = 0; g < NG; g += 2) ldmatrix_x4_trans(v0[g], v1[g], v0[g + 1], v1[g + 1], tile + u * BLOCK + (g == 0 ? v_piece : v_piece ^ 32u));
                 float w[HPL][2], ws[HPL][2];
 #pragma unroll
                 for (int h = 0; h < HPL; h++) {

@@ -12,11 +12,12 @@
 //   keys    codes  word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group
 //           d      half word [position][group]
 //           m      half word [position][group]
-//   values  codes  half word [position / 8][u][position / 2 % 4][group][position % 2], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group
+//   values  codes  half word [position][group][u], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group; the 16-byte pieces of a position, one per
+//                  group, are permuted so that eight positions' pieces of one group lie on different banks
 //           d      half word [position][group]
 //           m      half word [group][position]
-// Every piece lies as the MMAs of decode attention want it: lane (g, t) of a warp finds the numbers of all groups of position g (keys), and of two positions of
-// unit g (values), at 16 * lane (8 * lane for heads of 64); the offsets are operands of an MMA as they are.
+// Every piece lies as the MMAs of decode attention want it: lane (g, t) of a warp finds the numbers of all groups of position g of the keys at 16 * lane
+// (8 * lane for heads of 64), those of the values come by ldmatrix, and the offsets are operands of an MMA as they are.
 #pragma once
 #include <stdint.h>
 #include <string.h>
@@ -32,16 +33,17 @@ JHD int q4_block_bytes(int hd) { return 20 * hd; }
 JHD int q4_k_code(int hd, int p, int t, int g) { return ((p * 4 + t) * (hd / kQ4Group) + g) * 4; }
 JHD int q4_k_step(int hd, int p, int g) { return 8 * hd + (p * (hd / kQ4Group) + g) * 2; }
 JHD int q4_k_offset(int hd, int p, int g) { return 9 * hd + (p * (hd / kQ4Group) + g) * 2; }
-JHD int q4_v_code(int hd, int p, int u, int g) { return 10 * hd + ((((p >> 3) * 8 + u) * 4 + (p >> 1 & 3)) * (hd / kQ4Group) + g) * 4 + (p & 1) * 2; }
+JHD int q4_v_piece(int hd, int p, int g) { return g ^ (hd == 128 ? p >> 1 & 3 : p >> 2 & 1); }
+JHD int q4_v_code(int hd, int p, int u, int g) { return 10 * hd + p * (hd / 2) + q4_v_piece(hd, p, g) * 16 + u * 2; }
 JHD int q4_v_step(int hd, int p, int g) { return 18 * hd + (p * (hd / kQ4Group) + g) * 2; }
 JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (g * 16 + p) * 2; }
 // Where number e of the eight of a key word lies: an AND with 0x000f000f leaves numbers 0 and 1 as the halves of an operand register, the
 // next ones follow at 4, 8 and 12 bits.
 JHD int q4_k_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }
 
-// The number of x in a group with offset m and step d (inv is about 1 / d).  s + r is x - m exactly; half-way points (q + 1/2) d have 13 bits and
-// are exact, so that the comparisons decide exactly what the estimate may have missed by one.
-JHD int q4_number(float x, float m, float d, float inv) {
+// The number of x in a group with offset m and step d, decided exactly (inv is about 1 / d).  s + r is x - m exactly; half-way points (q + 1/2) d have 13
+// bits and are exact, so that the comparisons decide what the estimate may have missed by one.
+JHD int q4_number_exact(float x, float m, float d, float inv) {
     if (!(d > 0.f)) return 0;
     const float s = x - m, a = s - x, r = (x - (s - a)) + (-m - a);
     const float guess = s * inv + 0.5f;
@@ -50,6 +52,17 @@ JHD int q4_number(float x, float m, float d, float inv) {
     if (s > above || (s == above && (r > 0.f || (r == 0.f && (q & 1))))) q++;
     else if (s < below || (s == below && (r < 0.f || (r == 0.f && (q & 1))))) q--;
     return q < 0 ? 0 : q > 15 ? 15 : q;
+}
+// The same where the estimate t = (x - m) inv is enough: t is off by less than 2^-18 (x - m, inv and the product are rounded once each, t <= 15.1), so a t
+// farther than 2^-16 from half-way between two numbers has the right one next to it.  inv is 0 for d = 0.
+JHD int q4_number(float x, float m, float d, float inv) {
+    float t = (x - m) * inv;
+    t = t < 0.f ? 0.f : t > 15.f ? 15.f : t;
+    const float near = t + 12582912.f, off = t - (near - 12582912.f);  // 1.5 * 2^23: the sum's last digit is 1
+    if (off > 0.49998474f || off < -0.49998474f) return q4_number_exact(x, m, d, inv);
+    uint32_t bits;
+    memcpy(&bits, &near, 4);
+    return (int)(bits & 15u);
 }
 constexpr float kQ4Most = 65504.f, kQ4Nothing = 8.271806125530277e-25f;  // 2^-80
 

@@ -3,7 +3,8 @@
 
 using namespace juno;
 
-extern "C" int q4_host_number(float x, float m, float d) { return q4_number(x, m, d, 1.f / d); }
+extern "C" int q4_host_number(float x, float m, float d) { return q4_number(x, m, d, d > 0.f ? 1.f / d : 0.f); }
+extern "C" int q4_host_number_exact(float x, float m, float d) { return q4_number_exact(x, m, d, d > 0.f ? 1.f / d : 0.f); }
 extern "C" int q4_host_block_bytes(int hd) { return q4_block_bytes(hd); }
 
 // Marks every half byte of a block that a number takes and every byte of its factors; returns how many were marked twice, or lie outside.

@@ -16,7 +16,7 @@ def host_library():
     if not os.path.exists(so) or os.path.getmtime(so) < max(os.path.getmtime(src), os.path.getmtime(header)):
         subprocess.check_call(["g++", "-O2", "-std=c++17", "-ffp-contract=off", "-shared", "-fPIC", "-o", so, src])
     L = C.CDLL(so)
-    L.q4_host_number.argtypes = [C.c_float] * 3
+    L.q4_host_number.argtypes = L.q4_host_number_exact.argtypes = [C.c_float] * 3
     return L
 
 

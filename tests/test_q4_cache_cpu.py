@@ -44,7 +44,8 @@ def test_numbers_are_decided_exactly(host):
     cases += [(np.float32(v), np.float32(m), np.float32(2.0)) for m in (-1.0, -3.0, -5.0) for v in (1e-30, 0.0, -1e-30)]
     for x, m, d in cases:
         assert host.q4_host_number(float(x), float(m), float(d)) == _nearest(x, m, d), (x, m, d)
-    assert host.q4_host_number(3.0, 1.0, 0.0) == 0
+        assert host.q4_host_number_exact(float(x), float(m), float(d)) == _nearest(x, m, d), (x, m, d)
+    assert host.q4_host_number(3.0, 1.0, 0.0) == host.q4_host_number_exact(3.0, 1.0, 0.0) == 0
 
 
 def test_oracle_numbers_agree_with_the_host_functions(host):

@@ -417,6 +417,62 @@ def test_eviction_keeps_what_the_oracle_keeps(ctx, kv, dim, keep, recent):
     cache.close()
 
 
+@pytest.mark.parametrize("n,keep,recent", [(24576, 9000, 100), (24577, 24576, 0), (60001, 777, 77)])
+def test_eviction_of_long_sequences(ctx, n, keep, recent):
+    """More weights than shared memory holds, and exactly as many."""
+    rng = np.random.default_rng(n)
+    kv, dim = 2, 64
+    cache = PagedKvCache(ctx, 1, kv, dim, (n + keep) // 16 + 2, "q4", track_seqs=1, track_tokens=n)
+    s = cache.new_sequence(n, track=True)
+    have = (rows(rng, n, kv, dim), rows(rng, n, kv, dim))
+    fill(cache, 0, [s], [0], [have])
+    w = some_weights(rng, (1, kv, n))
+    t, kept = dev(w), torch.full((1, 1, kv, keep), 99, dtype=torch.int32, device="cuda")
+    settle()
+    cache.weights_device(0, [s], [n], t, store=True)
+    cache.evict([s], keep, recent, kept=kept)
+    settle()
+    at, k, v, wl = expected([have], w, keep, recent)[0]
+    assert np.array_equal(kept.cpu().numpy()[0, 0], at)
+    got = read(cache, 0, [s], [0], [keep])
+    assert np.array_equal(got[0], f32(q4.held(k))) and np.array_equal(got[1], f32(q4.held(v)))
+    assert np.array_equal(weights(cache, 0, [s], [keep])[0], wl, equal_nan=True)
+    cache.close()
+
+
+@pytest.mark.parametrize("kv,dim", [(2, 64), (3, 128)])
+def test_eviction_in_a_full_pool_moves_rows_in_place(ctx, kv, dim):
+    """No page is free: sequences are cut down within their own pages, one of them shares its first pages with a shorter one and is refused."""
+    rng = np.random.default_rng(dim)
+    lens, keep, recent, layers = [333, 250, 90], 100, 20, 2
+    cache = PagedKvCache(ctx, layers, kv, dim, sum((n + 15) // 16 for n in lens), "q4", track_seqs=4, track_tokens=336)
+    seqs = [cache.new_sequence(336, track=True) for _ in lens]
+    have = [[(rows(rng, n, kv, dim), rows(rng, n, kv, dim)) for _ in range(layers)] for n in lens]
+    w = [some_weights(rng, (layers, kv, n)) for n in lens]
+    for l in range(layers):
+        fill(cache, l, seqs, [0] * 3, [h[l] for h in have])
+        buf = np.zeros((3, kv, max(lens)), np.float32)
+        for i, n in enumerate(lens):
+            buf[i, :, :n] = w[i][l]
+        t = dev(buf)
+        settle()
+        cache.weights_device(l, seqs, lens, t, store=True)
+        settle()
+    b = cache.fork(seqs[1], 30)
+    with pytest.raises(JunoError, match="pages free"):
+        cache.evict(seqs, keep, recent)
+    assert [cache.length(s) for s in seqs] == lens
+    cache.free_sequence(b)
+    cache.evict(seqs, keep, recent)
+    settle()
+    for i, s in enumerate(seqs):
+        for l, (_, k, v, wl) in enumerate(expected(have[i], w[i], keep, recent)):
+            got = read(cache, l, [s], [0], [len(k)])
+            assert np.array_equal(got[0], f32(q4.held(k))) and np.array_equal(got[1], f32(q4.held(v)))
+            assert np.array_equal(weights(cache, l, [s], [len(k)])[0], wl, equal_nan=True)
+    cache.close()
+
+
 def test_eviction_gives_pages_back_and_leaves_shared_ones(ctx):
     """A pool that a branch and its source fill but for the branch's new pages; without room nothing changes."""
     rng = np.random.default_rng(21)
