@@ -106,136 +106,196 @@ struct RowsParams {
     int track_tokens;
 };
 
-// One lane has eight neighbouring dimensions of a key or value, four lanes a group: what is stored of a position is contiguous but for the values' offsets.
-template <int HD>
+// Where the positions of a block's rows lie: found once per row, by one thread.
+struct RowPlace {
+    uint8_t *page;  // this layer's page, or null behind the last row
+    int pos, track;
+};
+template <int R>
+__device__ __forceinline__ void find_places(const RowsParams &p, int row0, size_t page_bytes, RowPlace (&places)[R]) {
+    if (threadIdx.x < R) {
+        const int row = row0 + threadIdx.x;
+        RowPlace at{nullptr, 0, -1};
+        if (row < p.n_tokens) {
+            const CacheRow r = cache_row(p.rows, cache_find(p.rows, row));
+            at.pos = r.upto + row - r.first;
+            at.track = r.track;
+            at.page = static_cast<uint8_t *>(p.kpool) + ((size_t)p.layer * p.n_pages + p.table[(size_t)r.slot * p.max_pages_per_seq + (at.pos >> 4)]) * page_bytes;
+        }
+        places[threadIdx.x] = at;
+    }
+    __syncthreads();
+}
+
+// The numbers of eight elements where an estimate was too close to call.
+__device__ __noinline__ uint32_t exact_numbers(float x0, float x1, float x2, float x3, float m, float d, float inv) {
+    return (uint32_t)q4_number_exact(x0, m, d, inv) | (uint32_t)q4_number_exact(x1, m, d, inv) << 8 | (uint32_t)q4_number_exact(x2, m, d, inv) << 16 |
+           (uint32_t)q4_number_exact(x3, m, d, inv) << 24;
+}
+
+// A CTA has R positions.  A lane has eight neighbouring dimensions of a key or value, four lanes a group: what is stored of a position is contiguous but for the
+// values' offsets.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate of q4_number (a
+// saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided exactly.
+template <int HD, int R>
 __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ RowsParams p) {
     constexpr int LPV = HD / 8;  // lanes per vector
-    const int H = p.n_kv_heads, sub = threadIdx.x % LPV;
-    const int64_t vec = (int64_t)blockIdx.x * (256 / LPV) + threadIdx.x / LPV, n_vec = (int64_t)p.n_tokens * 2 * H;
-    const bool on = vec < n_vec;
-    const int row = on ? (int)(vec / (2 * H)) : 0;
-    const int which = on ? (int)(vec - (int64_t)row * 2 * H) : 0, is_v = which >= H, h = which - is_v * H;
-    float x[8];
-    if (on) {
-        const float *src = (is_v ? p.v : p.k) + row * p.ld + h * HD + sub * 8;
-        if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-            const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
+    const int H = p.n_kv_heads, row0 = blockIdx.x * R, sub = threadIdx.x % LPV, g = sub >> 2;
+    __shared__ RowPlace places[R];
+    find_places<R>(p, row0, (size_t)H * q4_block_bytes(HD), places);
+    const int vectors = (2 * H + 31) / 32 * 32;  // whole warps take part in the sums of a group
+    for (int vec = threadIdx.x / LPV; vec < vectors; vec += blockDim.x / LPV) {
+        const bool is_v = vec >= H;
+        const int h = vec - (is_v ? H : 0);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = src[e];
+        for (int n = 0; n < R; n++) {
+            const RowPlace at = places[n];
+            const bool on = vec < 2 * H && at.page;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = 0.f;
+            if (on) {
+                const float *src = (is_v ? p.v : p.k) + (row0 + n) * p.ld + h * HD + sub * 8;
+                if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                    const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+                    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = src[e];
+                }
+            }
+            float lo = x[0], hi = x[0];
+            bool odd = x[0] != x[0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) {
+                odd |= x[e] != x[e];
+                lo = fminf(lo, x[e]);
+                hi = fmaxf(hi, x[e]);
+            }
+            if (odd || fmaxf(hi, -lo) > kQ4Most) {  // seldom: a NaN, or values beyond what FP16 holds
+                lo = kQ4Most;
+                hi = -kQ4Most;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e] = fminf(fmaxf(x[e], -kQ4Most), kQ4Most);
+                    lo = fminf(lo, x[e]);
+                    hi = fmaxf(hi, x[e]);
+                }
+                if (odd) hi = INFINITY;  // the group's mark of a NaN: no clamped value is infinite
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            const bool nan = hi == INFINITY;
+            const __half mh = nan ? __ushort_as_half(0x7e00) : __float2half_rn(lo);
+            const float reach = hi - lo;
+            // reach / 15 rounded to FP32, then to BF16.  The product with 1/15 is off by an FP32 step or two, which matters only next to the middle of two BF16 numbers.
+            float fifteenth = reach * (1.f / 15.f);
+            if ((__float_as_uint(fifteenth) + 0x7ffcu & 0xffffu) >= 0xfff8u) fifteenth = __fdiv_rn(reach, 15.f);
+            const __nv_bfloat16 dh = __float2bfloat16_rn(nan || reach < kQ4Nothing ? 0.f : fifteenth);
+            const float m = __half2float(mh), d = __bfloat162float(dh);
+            float inv;  // 1 / (15 d): 15 d has 12 bits
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d * 15.f));
+            inv = d > 0.f ? inv : 0.f;
+            uint32_t bits[8];
+            bool close = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float part = __saturatef((x[e] - m) * inv), near = fmaf(part, 15.f, 12582912.f);  // 1.5 * 2^23 and the number
+                bits[e] = __float_as_uint(near);
+                close |= fabsf(fmaf(part, 15.f, 12582912.f - near)) > 0.49998474f;  // as in q4_number
+            }
+            if (close) {
+                const uint32_t a = exact_numbers(x[0], x[1], x[2], x[3], m, d, inv * 15.f), b = exact_numbers(x[4], x[5], x[6], x[7], m, d, inv * 15.f);
+#pragma unroll
+                for (int e = 0; e < 8; e++) bits[e] = 0x4b400000u + ((e < 4 ? a : b) >> (8 * (e & 3)) & 15u);
+            }
+            if (!on) continue;
+            const int pp = at.pos & 15;
+            uint8_t *block = at.page + h * q4_block_bytes(HD);
+            uint32_t w = 0, ones = 0;  // the numbers come with the bits of 1.5 * 2^23, which are taken off the sum
+            if (is_v) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    w += bits[e] << (4 * e);
+                    ones += 0x4b400000u << (4 * e);
+                }
+                *reinterpret_cast<uint32_t *>(block + q4_v_code(HD, pp, 2 * (sub & 3), g)) = w - ones;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    w += bits[e] << q4_k_shift(e);
+                    ones += 0x4b400000u << q4_k_shift(e);
+                }
+                *reinterpret_cast<uint32_t *>(block + q4_k_code(HD, pp, sub & 3, g)) = w - ones;
+                if (sub == 0 && at.track >= 0) p.weights[(((size_t)at.track * p.n_layers + p.layer) * H + h) * p.track_tokens + at.pos] = 0.f;
+            }
+            if ((sub & 3) == 0) {
+                *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))) = __bfloat16_as_ushort(dh);
+                *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))) = __half_as_ushort(mh);
+            }
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = 0.f;
-    }
-    float lo = x[0], hi = x[0];
-    bool odd = x[0] != x[0];
-#pragma unroll
-    for (int e = 1; e < 8; e++) {
-        odd |= x[e] != x[e];
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-    }
-    if (odd || fmaxf(hi, -lo) > kQ4Most) {  // seldom: a NaN, or values beyond what FP16 holds
-        lo = kQ4Most;
-        hi = -kQ4Most;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[e] = fminf(fmaxf(x[e], -kQ4Most), kQ4Most);
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
-        }
-        if (odd) hi = INFINITY;  // the group's mark of a NaN: no clamped value is infinite
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const bool nan = hi == INFINITY;
-    const __half mh = nan ? __ushort_as_half(0x7e00) : __float2half_rn(lo);
-    const float reach = hi - lo;
-    const __nv_bfloat16 dh = __float2bfloat16_rn(nan || reach < kQ4Nothing ? 0.f : __fdiv_rn(reach, 15.f));
-    const float m = __half2float(mh), d = __bfloat162float(dh), inv = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
-    uint32_t q[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) q[e] = (uint32_t)q4_number(x[e], m, d, inv);
-    if (!on) return;
-    const CacheRow r = cache_row(p.rows, cache_find(p.rows, row));
-    const int pos = r.upto + row - r.first, pp = pos & 15, g = sub >> 2;
-    const int page = p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)];
-    uint8_t *block = static_cast<uint8_t *>(p.kpool) + (((size_t)p.layer * p.n_pages + page) * H + h) * q4_block_bytes(HD);
-    uint32_t w = 0;
-    if (is_v) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) w |= q[e] << (4 * e);
-        *reinterpret_cast<uint32_t *>(block + q4_v_code(HD, pp, 2 * (sub & 3), g)) = w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) w |= q[e] << q4_k_shift(e);
-        *reinterpret_cast<uint32_t *>(block + q4_k_code(HD, pp, sub & 3, g)) = w;
-        if (sub == 0 && r.track >= 0)
-            p.weights[(((size_t)r.track * p.n_layers + p.layer) * H + h) * p.track_tokens + pos] = 0.f;
-    }
-    if ((sub & 3) == 0) {
-        *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))) = __bfloat16_as_ushort(dh);
-        *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))) = __half_as_ushort(mh);
     }
 }
 
-// One lane has four neighbouring dimensions, so that a warp's stores are contiguous; kReadRows rows to a lane, whose loads are under way together.
-constexpr int kReadRows = 4;
+// A number that lies in bits of a word below 2^23, as FP32: without a conversion.
+__device__ __forceinline__ float bits_as_float(uint32_t w, uint32_t mask) { return __uint_as_float((w & mask) | 0x4b000000u) - 8388608.f; }
+
+// A CTA has kReadRows positions; a lane has four neighbouring dimensions, so that a warp's stores are contiguous.
+constexpr int kAppendRows = 4, kReadRows = 8, kReadAhead = 4;
 template <int HD>
 __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ RowsParams p) {
     constexpr int LPV = HD / 4;
-    const int H = p.n_kv_heads, sub = threadIdx.x % LPV, piece = sub & 7, g = sub >> 3;
-    const int64_t vec = (int64_t)blockIdx.x * (256 / LPV) + threadIdx.x / LPV;
-    const int row0 = (int)(vec / (2 * H)) * kReadRows;
-    if (row0 >= p.n_tokens) return;
-    const int which = (int)(vec % (2 * H)), is_v = which >= H, h = which - is_v * H;
-    int i = cache_find(p.rows, row0), next = i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : INT_MAX;
-    CacheRow r = cache_row(p.rows, i);
-    uint32_t w[kReadRows];
-    float m[kReadRows], d[kReadRows];
+    const int H = p.n_kv_heads, row0 = blockIdx.x * kReadRows, sub = threadIdx.x % LPV, piece = sub & 7, g = sub >> 3;
+    __shared__ RowPlace places[kReadRows];
+    find_places<kReadRows>(p, row0, (size_t)H * q4_block_bytes(HD), places);
+    for (int vec = threadIdx.x / LPV; vec < 2 * H; vec += 256 / LPV) {
+        const bool is_v = vec >= H;
+        const int h = vec - (is_v ? H : 0);
+        float *out = (is_v ? p.v : p.k) + row0 * p.ld + h * HD + sub * 4;
+        const bool vec4 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (p.ld & 3) == 0;
 #pragma unroll
-    for (int n = 0; n < kReadRows; n++) {
-        const int row = row0 + n;
-        if (row >= p.n_tokens) break;
-        if (row >= next) {
-            i = cache_find(p.rows, row);
-            r = cache_row(p.rows, i);
-            next = i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : INT_MAX;
-        }
-        const int pos = r.upto + row - r.first, pp = pos & 15;
-        const int page = p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)];
-        const uint8_t *block = static_cast<const uint8_t *>(p.kpool) + (((size_t)p.layer * p.n_pages + page) * H + h) * q4_block_bytes(HD);
-        m[n] = __half2float(*reinterpret_cast<const __half *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))));
-        d[n] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))));
-        // numbers 0..3 of a unit (values), or numbers 0..3 or 4..7 of a word (keys): brought to where a key word has numbers 0..3
-        if (is_v) {
-            const uint32_t u = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g));
-            w[n] = (u & 15u) | (u >> 4 & 15u) << 16 | (u >> 8 & 15u) << 4 | (u >> 12) << 20;
-        } else {
-            w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g)) >> (8 * (piece & 1));
-        }
-    }
-    float *out = (is_v ? p.v : p.k) + (int64_t)row0 * p.ld + h * HD + sub * 4;
-    const bool vec4 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (p.ld & 3) == 0;
+        for (int n0 = 0; n0 < kReadRows; n0 += kReadAhead) {
+            uint32_t w[kReadAhead];
+            float m[kReadAhead], d[kReadAhead];
 #pragma unroll
-    for (int n = 0; n < kReadRows; n++) {
-        if (row0 + n >= p.n_tokens) break;
-        const float4 x = make_float4(fmaf(d[n], (float)(w[n] & 15u), m[n]), fmaf(d[n], (float)(w[n] >> 16 & 15u), m[n]), fmaf(d[n], (float)(w[n] >> 4 & 15u), m[n]),
-                                     fmaf(d[n], (float)(w[n] >> 20 & 15u), m[n]));
-        float *to = out + n * p.ld;
-        if (vec4) {
-            *reinterpret_cast<float4 *>(to) = x;
-        } else {
-            to[0] = x.x;
-            to[1] = x.y;
-            to[2] = x.z;
-            to[3] = x.w;
+            for (int n = 0; n < kReadAhead; n++) {
+                const RowPlace at = places[n0 + n];
+                if (!at.page) continue;
+                const int pp = at.pos & 15;
+                const uint8_t *block = at.page + h * q4_block_bytes(HD);
+                if (is_v) {
+                    m[n] = __half2float(*reinterpret_cast<const __half *>(block + q4_v_offset(HD, pp, g)));
+                    d[n] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + q4_v_step(HD, pp, g)));
+                    w[n] = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g));
+                } else {
+                    m[n] = __half2float(*reinterpret_cast<const __half *>(block + q4_k_offset(HD, pp, g)));
+                    d[n] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + q4_k_step(HD, pp, g)));
+                    w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g)) >> (8 * (piece & 1));
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kReadAhead; n++) {
+                if (!places[n0 + n].page) continue;
+                float4 x;
+                if (is_v)
+                    x = make_float4(fmaf(d[n], bits_as_float(w[n], 0xfu), m[n]), fmaf(d[n] * 0x1p-4f, bits_as_float(w[n], 0xf0u), m[n]),
+                                    fmaf(d[n] * 0x1p-8f, bits_as_float(w[n], 0xf00u), m[n]), fmaf(d[n] * 0x1p-12f, bits_as_float(w[n], 0xf000u), m[n]));
+                else
+                    x = make_float4(fmaf(d[n], bits_as_float(w[n], 0xfu), m[n]), fmaf(d[n] * 0x1p-16f, bits_as_float(w[n], 0xf0000u), m[n]),
+                                    fmaf(d[n] * 0x1p-4f, bits_as_float(w[n], 0xf0u), m[n]), fmaf(d[n] * 0x1p-16f, bits_as_float(w[n] >> 4, 0xf0000u), m[n]));
+                float *to = out + (n0 + n) * p.ld;
+                if (vec4) {
+                    *reinterpret_cast<float4 *>(to) = x;
+                } else {
+                    to[0] = x.x;
+                    to[1] = x.y;
+                    to[2] = x.z;
+                    to[3] = x.w;
+                }
+            }
         }
     }
 }
@@ -283,19 +343,21 @@ static int launch_rows(juno_ctx *c, const juno_kvpool *p, int layer, const Cache
     a.weights = p->weights;
     a.track_tokens = p->track_tokens;
     const int hd = p->head_dim;
-    const int64_t lanes = p->dtype == kKvQ4 && !APPEND ? (int64_t)(n_tokens + kReadRows - 1) / kReadRows * 2 * p->n_kv_heads * (hd / 4)
-                                                       : (int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8);
-    const unsigned blocks = (unsigned)((lanes + 255) / 256);
     ProfScope prof(c, st, APPEND ? PROF_ROPE_APPEND : PROF_OTHER, (double)n_tokens * p->n_kv_heads * (8.0 * hd + p->row_bytes()));
-    if (p->dtype == kKvQ4) {
-        if (APPEND)
-            hd == 128 ? q4_append_kernel<128><<<blocks, 256, 0, st>>>(a) : q4_append_kernel<64><<<blocks, 256, 0, st>>>(a);
+    if (p->dtype == kKvQ4 && APPEND) {
+        // several positions to a CTA once there are CTAs for every SM several times over
+        const int each = n_tokens >= c->sm_count * 16 ? kAppendRows : 1;
+        const dim3 grid((unsigned)((n_tokens + each - 1) / each)), block((unsigned)std::min(256, (2 * p->n_kv_heads * (hd / 8) + 31) / 32 * 32));
+        if (each == 1)
+            hd == 128 ? q4_append_kernel<128, 1><<<grid, block, 0, st>>>(a) : q4_append_kernel<64, 1><<<grid, block, 0, st>>>(a);
         else
-            hd == 128 ? q4_read_kernel<128><<<blocks, 256, 0, st>>>(a) : q4_read_kernel<64><<<blocks, 256, 0, st>>>(a);
-    } else if (p->dtype == 0) {
-        rows_kernel<__half, APPEND><<<blocks, 256, 0, st>>>(a, hd);
+            hd == 128 ? q4_append_kernel<128, kAppendRows><<<grid, block, 0, st>>>(a) : q4_append_kernel<64, kAppendRows><<<grid, block, 0, st>>>(a);
+    } else if (p->dtype == kKvQ4) {
+        const unsigned grid = (unsigned)((n_tokens + kReadRows - 1) / kReadRows);
+        hd == 128 ? q4_read_kernel<128><<<grid, 256, 0, st>>>(a) : q4_read_kernel<64><<<grid, 256, 0, st>>>(a);
     } else {
-        rows_kernel<float, APPEND><<<blocks, 256, 0, st>>>(a, hd);
+        const unsigned grid = (unsigned)(((int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8) + 255) / 256);
+        p->dtype == 0 ? rows_kernel<__half, APPEND><<<grid, 256, 0, st>>>(a, hd) : rows_kernel<float, APPEND><<<grid, 256, 0, st>>>(a, hd);
     }
     JUNO_CUDA_TRY(cudaGetLastError());
     c->kernel_launches++;

@@ -172,15 +172,22 @@ class B200MatVec:
         return out
 
 
-def _device_ptr(x, name: str, rows: int, width: int, dtype: str = "float32"):
-    """(address, row stride) of a CUDA tensor (anything with data_ptr, dtype, shape and stride) that holds `rows` rows of `width` elements."""
-    if not hasattr(x, "data_ptr"):
-        raise ValueError(f"{name} is not a tensor in device memory")
-    if str(x.dtype).rsplit(".", 1)[-1] != dtype or not x.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor of {dtype} is wanted")
-    if x.dim() != 2 or x.shape[0] != rows or x.shape[1] != width or (width > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < width):
-        raise ValueError(f"{name}: shape [{rows}, {width}] with neighbouring elements in a row is wanted, not {list(x.shape)} with strides {list(x.stride())}")
-    return x.data_ptr(), (x.stride(0) if rows > 1 else width)
+_KINDS: dict = {}  # element type of a tensor -> its name, as far as seen
+
+
+def _device_ptr(x, name: str, rows: int, width: int, kind: str = "float32"):
+    """(address, row stride) of a CUDA tensor (anything with data_ptr, dtype, shape, stride and is_cuda) that holds `rows` rows of `width` elements."""
+    try:
+        shape, stride, dtype = x.shape, x.stride(), x.dtype
+    except (AttributeError, TypeError):
+        raise ValueError(f"{name} is not a tensor in device memory") from None
+    if dtype not in _KINDS:
+        _KINDS[dtype] = str(dtype).rsplit(".", 1)[-1]
+    if _KINDS[dtype] != kind or not x.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor of {kind} is wanted")
+    if shape != (rows, width) or (width > 1 and stride[1] != 1) or (rows > 1 and stride[0] < width):
+        raise ValueError(f"{name}: shape [{rows}, {width}] with neighbouring elements in a row is wanted, not {list(shape)} with strides {list(stride)}")
+    return x.data_ptr(), (stride[0] if rows > 1 else width)
 
 
 class SequenceBatch:
@@ -258,68 +265,78 @@ class PagedKvCache:
     @staticmethod
     def batch(seqs) -> SequenceBatch:
         """Sequences that several calls name together; every call takes one in the place of a list."""
-        return seqs if isinstance(seqs, SequenceBatch) else SequenceBatch(seqs)
+        return seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
 
     @staticmethod
-    def _ints(x, n: int, name: str) -> np.ndarray:
-        a = np.ascontiguousarray(x, dtype=np.int32)
+    def _ints(x, n: int, name: str):
+        """(array, address) of n whole numbers; the array has to outlive the use of the address."""
+        a = x if type(x) is np.ndarray and x.dtype == np.int32 and x.flags.c_contiguous else np.ascontiguousarray(x, dtype=np.int32)
         if a.shape != (n,):
             raise ValueError(f"{name}: {n} whole numbers are wanted, not shape {a.shape}")
-        return a
+        return a, a.__array_interface__["data"][0]
 
     @staticmethod
     def _stream(stream):
-        if stream is None:
-            return None
-        return int(getattr(stream, "cuda_stream", stream)) or 1  # cudaStreamLegacy
+        return None if stream is None else int(getattr(stream, "cuda_stream", stream)) or 1  # cudaStreamLegacy
 
-    def _rows(self, seqs, positions, counts, k, v):
-        b = self.batch(seqs)
-        positions, counts = self._ints(positions, b.n, "positions"), self._ints(counts, b.n, "counts")
-        rows, width = int(counts.sum()), self.n_kv_heads * self.head_dim
-        (kp, ld), (vp, ldv) = _device_ptr(k, "k", rows, width), _device_ptr(v, "v", rows, width)
+    def _move_rows(self, call, name, layer, seqs, positions, counts, k, v, stream) -> None:
+        b = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
+        positions, at = self._ints(positions, b.n, "positions")
+        counts, n = self._ints(counts, b.n, "counts")
+        rows, width = sum(counts.tolist()), self.n_kv_heads * self.head_dim
+        kp, ld = _device_ptr(k, "k", rows, width)
+        vp, ldv = _device_ptr(v, "v", rows, width)
         if ld != ldv:
             raise ValueError(f"the rows of k and v lie {ld} and {ldv} elements apart")
-        return b, positions, counts, kp, vp, ld
+        rc = call(self.ctx.handle, self.handle, layer, b.n, b.handles, at, n, kp, vp, ld, None if stream is None else self._stream(stream))
+        if rc:
+            check(rc, name)
 
     def append_device(self, layer: int, seqs, positions, counts, k, v, stream=None) -> None:
         """counts[i] new positions of sequence i, the first at positions[i]; k, v: [sum of counts, n_kv_heads * head_dim] (juno_kv_append_device)."""
-        b, positions, counts, kp, vp, ld = self._rows(seqs, positions, counts, k, v)
-        check(self._L.juno_kv_append_device(self.ctx.handle, self.handle, layer, b.n, b.handles, _ptr(positions), _ptr(counts), kp, vp, ld,
-                                            self._stream(stream)), "juno_kv_append_device")
+        self._move_rows(self._L.juno_kv_append_device, "juno_kv_append_device", layer, seqs, positions, counts, k, v, stream)
 
     def read_device(self, layer: int, seqs, positions, counts, k, v, stream=None) -> None:
         """What the pages hold for cached positions, into k and v (juno_kv_read_device)."""
-        b, positions, counts, kp, vp, ld = self._rows(seqs, positions, counts, k, v)
-        check(self._L.juno_kv_read_device(self.ctx.handle, self.handle, layer, b.n, b.handles, _ptr(positions), _ptr(counts), kp, vp, ld,
-                                          self._stream(stream)), "juno_kv_read_device")
+        self._move_rows(self._L.juno_kv_read_device, "juno_kv_read_device", layer, seqs, positions, counts, k, v, stream)
 
     def attention_device(self, layer: int, seqs, q, n_heads: int, out, lens=None, stream=None) -> None:
         """Decode attention over 4-bit pages; q, out: [sequences, n_heads * head_dim] (juno_attn_decode_device)."""
-        b = self.batch(seqs)
-        (qp, ldq), (op, ldo) = (_device_ptr(x, name, b.n, n_heads * self.head_dim) for x, name in ((q, "q"), (out, "out")))
-        check(self._L.juno_attn_decode_device(self.ctx.handle, self.handle, layer, b.n, b.handles, None if lens is None else _ptr(self._ints(lens, b.n, "lens")),
-                                              n_heads, qp, ldq, op, ldo, self._stream(stream)), "juno_attn_decode_device")
+        b = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
+        width = n_heads * self.head_dim
+        qp, ldq = _device_ptr(q, "q", b.n, width)
+        op, ldo = _device_ptr(out, "out", b.n, width)
+        lens, lp = (None, None) if lens is None else self._ints(lens, b.n, "lens")
+        rc = self._L.juno_attn_decode_device(self.ctx.handle, self.handle, layer, b.n, b.handles, lp, n_heads, qp, ldq, op, ldo,
+                                             None if stream is None else self._stream(stream))
+        if rc:
+            check(rc, "juno_attn_decode_device")
 
     def weights_device(self, layer: int, seqs, counts, w, store: bool = False, stream=None) -> None:
         """The weights of the first counts[i] positions of each sequence into w [sequences, n_kv_heads, at least most counts], or from it
         (juno_kv_weights_device)."""
-        b = self.batch(seqs)
-        if not (hasattr(w, "data_ptr") and w.dim() == 3 and tuple(w.shape[:2]) == (b.n, self.n_kv_heads) and w.is_contiguous()):
+        b = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
+        if not (hasattr(w, "data_ptr") and w.dim() == 3 and w.shape[:2] == (b.n, self.n_kv_heads) and w.is_contiguous()):
             raise ValueError(f"w: a contiguous tensor [{b.n}, {self.n_kv_heads}, positions] is wanted")
-        wp, ld = _device_ptr(w.view(b.n * self.n_kv_heads, w.shape[2]), "w", b.n * self.n_kv_heads, w.shape[2])
-        check(self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, _ptr(self._ints(counts, b.n, "counts")), wp, ld,
-                                             1 if store else 0, self._stream(stream)), "juno_kv_weights_device")
+        ld = w.shape[2]
+        wp, _ = _device_ptr(w.view(-1, ld), "w", b.n * self.n_kv_heads, ld)
+        counts, n = self._ints(counts, b.n, "counts")
+        rc = self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, n, wp, ld, 1 if store else 0,
+                                            None if stream is None else self._stream(stream))
+        if rc:
+            check(rc, "juno_kv_weights_device")
 
     def evict(self, seqs, keep: int, recent: int = 0, kept=None, stream=None) -> None:
         """Cuts sequences down to the `keep` positions of most weight, the newest `recent` among them, in every layer and key/value head; kept:
         int32 [n_layers, sequences, n_kv_heads, keep] gets their places (juno_kv_evict)."""
-        b, kp = self.batch(seqs), None
+        b, kp = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs), None
         if kept is not None:
-            if not (hasattr(kept, "data_ptr") and tuple(kept.shape) == (self.n_layers, b.n, self.n_kv_heads, keep) and kept.is_contiguous()):
+            if not (hasattr(kept, "data_ptr") and kept.shape == (self.n_layers, b.n, self.n_kv_heads, keep) and kept.is_contiguous()):
                 raise ValueError(f"kept: a contiguous tensor [{self.n_layers}, {b.n}, {self.n_kv_heads}, {keep}] is wanted")
             kp = _device_ptr(kept.view(-1, keep), "kept", self.n_layers * b.n * self.n_kv_heads, keep, "int32")[0]
-        check(self._L.juno_kv_evict(self.ctx.handle, self.handle, b.n, b.handles, keep, recent, kp, self._stream(stream)), "juno_kv_evict")
+        rc = self._L.juno_kv_evict(self.ctx.handle, self.handle, b.n, b.handles, keep, recent, kp, None if stream is None else self._stream(stream))
+        if rc:
+            check(rc, "juno_kv_evict")
 
     def close(self) -> None:
         if self.handle is not None:
