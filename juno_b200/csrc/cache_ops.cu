@@ -127,52 +127,55 @@ __device__ __forceinline__ void find_places(const RowsParams &p, int row0, size_
     __syncthreads();
 }
 
-// The numbers of eight elements where an estimate was too close to call.
-__device__ __noinline__ uint32_t exact_numbers(float x0, float x1, float x2, float x3, float m, float d, float inv) {
-    return (uint32_t)q4_number_exact(x0, m, d, inv) | (uint32_t)q4_number_exact(x1, m, d, inv) << 8 | (uint32_t)q4_number_exact(x2, m, d, inv) << 16 |
-           (uint32_t)q4_number_exact(x3, m, d, inv) << 24;
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-// A CTA has R positions.  A lane has eight neighbouring dimensions of a key or value, four lanes a group: what is stored of a position is contiguous but for the
-// values' offsets.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate of q4_number (a
-// saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided exactly.
-template <int HD, int R>
-__global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ RowsParams p) {
+// A CTA has R positions, of keys (blockIdx.y = 0) or values.  A lane has eight neighbouring dimensions, four lanes a group: what is stored of a position is
+// contiguous but for the values' offsets.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate
+// of q4_number (a saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided
+// exactly.
+template <int HD, int R, bool V>
+__device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace (&places)[R], int row0) {
     constexpr int LPV = HD / 8;  // lanes per vector
-    const int H = p.n_kv_heads, row0 = blockIdx.x * R, sub = threadIdx.x % LPV, g = sub >> 2;
-    __shared__ RowPlace places[R];
-    find_places<R>(p, row0, (size_t)H * q4_block_bytes(HD), places);
-    const int vectors = (2 * H + 31) / 32 * 32;  // whole warps take part in the sums of a group
-    for (int vec = threadIdx.x / LPV; vec < vectors; vec += blockDim.x / LPV) {
-        const bool is_v = vec >= H;
-        const int h = vec - (is_v ? H : 0);
+    const int H = p.n_kv_heads, sub = threadIdx.x % LPV, g = sub >> 2;
+    for (int vec = threadIdx.x / LPV; vec < (H + 3) / 4 * 4; vec += blockDim.x / LPV) {  // whole warps take part in the sums of a group
+        const int h = min(vec, H - 1);
+        float rows[R][8];  // of all positions: their loads are under way together
+        const float *src = (V ? p.v : p.k) + row0 * p.ld + h * HD + sub * 8;
+        const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && (p.ld & 3) == 0;
+#pragma unroll
+        for (int n = 0; n < R; n++) {
+            float(&x)[8] = rows[n];
+            if (aligned) {
+                const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+                x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = src[e];
+            }
+            if (row0 + n + 1 < p.n_tokens) src += p.ld;  // behind the last row: that one again
+        }
 #pragma unroll
         for (int n = 0; n < R; n++) {
             const RowPlace at = places[n];
-            const bool on = vec < 2 * H && at.page;
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = 0.f;
-            if (on) {
-                const float *src = (is_v ? p.v : p.k) + (row0 + n) * p.ld + h * HD + sub * 8;
-                if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                    const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = src[e];
-                }
-            }
+            float(&x)[8] = rows[n];
             float lo = x[0], hi = x[0];
-            bool odd = x[0] != x[0];
 #pragma unroll
             for (int e = 1; e < 8; e++) {
-                odd |= x[e] != x[e];
-                lo = fminf(lo, x[e]);
-                hi = fmaxf(hi, x[e]);
+                lo = min_nan(lo, x[e]);
+                hi = max_nan(hi, x[e]);
             }
-            if (odd || fmaxf(hi, -lo) > kQ4Most) {  // seldom: a NaN, or values beyond what FP16 holds
+            if (!(fmaxf(hi, -lo) <= kQ4Most && lo == lo)) {  // seldom: a NaN, or values beyond what FP16 holds
+                const bool nan = lo != lo;
                 lo = kQ4Most;
                 hi = -kQ4Most;
 #pragma unroll
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ 
                     lo = fminf(lo, x[e]);
                     hi = fmaxf(hi, x[e]);
                 }
-                if (odd) hi = INFINITY;  // the group's mark of a NaN: no clamped value is infinite
+                if (nan) hi = INFINITY;  // the group's mark of a NaN: no clamped value is infinite
             }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
@@ -199,105 +202,111 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ 
             float inv;  // 1 / (15 d): 15 d has 12 bits
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d * 15.f));
             inv = d > 0.f ? inv : 0.f;
-            uint32_t bits[8];
-            bool close = false;
+            uint32_t w = 0, ones = 0;  // the numbers come with the bits of 1.5 * 2^23, which are taken off the sum
+            float worst = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float part = __saturatef((x[e] - m) * inv), near = fmaf(part, 15.f, 12582912.f);  // 1.5 * 2^23 and the number
-                bits[e] = __float_as_uint(near);
-                close |= fabsf(fmaf(part, 15.f, 12582912.f - near)) > 0.49998474f;  // as in q4_number
+                const float part = __saturatef((x[e] - m) * inv), near = fmaf(part, 15.f, 12582912.f);
+                const int shift = V ? 4 * e : q4_k_shift(e);
+                w += __float_as_uint(near) << shift;
+                ones += 0x4b400000u << shift;
+                worst = fmaxf(worst, fabsf(fmaf(part, 15.f, 12582912.f - near)));
             }
-            if (close) {
-                const uint32_t a = exact_numbers(x[0], x[1], x[2], x[3], m, d, inv * 15.f), b = exact_numbers(x[4], x[5], x[6], x[7], m, d, inv * 15.f);
+            w -= ones;
+            if (worst > 0.49998474f) {  // as in q4_number
+                w = 0;
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                    float v = x[0];
 #pragma unroll
-                for (int e = 0; e < 8; e++) bits[e] = 0x4b400000u + ((e < 4 ? a : b) >> (8 * (e & 3)) & 15u);
+                    for (int k = 1; k < 8; k++) v = e == k ? x[k] : v;
+                    w |= (uint32_t)q4_number_exact(v, m, d, inv * 15.f) << (V ? 4 * e : q4_k_shift(e));
+                }
             }
-            if (!on) continue;
+            if (vec >= H || !at.page) continue;
             const int pp = at.pos & 15;
             uint8_t *block = at.page + h * q4_block_bytes(HD);
-            uint32_t w = 0, ones = 0;  // the numbers come with the bits of 1.5 * 2^23, which are taken off the sum
-            if (is_v) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    w += bits[e] << (4 * e);
-                    ones += 0x4b400000u << (4 * e);
-                }
-                *reinterpret_cast<uint32_t *>(block + q4_v_code(HD, pp, 2 * (sub & 3), g)) = w - ones;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    w += bits[e] << q4_k_shift(e);
-                    ones += 0x4b400000u << q4_k_shift(e);
-                }
-                *reinterpret_cast<uint32_t *>(block + q4_k_code(HD, pp, sub & 3, g)) = w - ones;
-                if (sub == 0 && at.track >= 0) p.weights[(((size_t)at.track * p.n_layers + p.layer) * H + h) * p.track_tokens + at.pos] = 0.f;
-            }
+            *reinterpret_cast<uint32_t *>(block + (V ? q4_v_code(HD, pp, 2 * (sub & 3), g) : q4_k_code(HD, pp, sub & 3, g))) = w;
+            if (!V && sub == 0 && at.track >= 0) p.weights[(((size_t)at.track * p.n_layers + p.layer) * H + h) * p.track_tokens + at.pos] = 0.f;
             if ((sub & 3) == 0) {
-                *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))) = __bfloat16_as_ushort(dh);
-                *reinterpret_cast<uint16_t *>(block + (is_v ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))) = __half_as_ushort(mh);
+                *reinterpret_cast<uint16_t *>(block + (V ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g))) = __bfloat16_as_ushort(dh);
+                *reinterpret_cast<uint16_t *>(block + (V ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g))) = __half_as_ushort(mh);
             }
         }
     }
+}
+template <int HD, int R>
+__global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ RowsParams p) {
+    __shared__ RowPlace places[R];
+    const int row0 = blockIdx.x * R;
+    find_places<R>(p, row0, (size_t)p.n_kv_heads * q4_block_bytes(HD), places);
+    if (blockIdx.y == 0)
+        append_rows<HD, R, false>(p, places, row0);
+    else
+        append_rows<HD, R, true>(p, places, row0);
 }
 
 // A number that lies in bits of a word below 2^23, as FP32: without a conversion.
 __device__ __forceinline__ float bits_as_float(uint32_t w, uint32_t mask) { return __uint_as_float((w & mask) | 0x4b000000u) - 8388608.f; }
 
-// A CTA has kReadRows positions; a lane has four neighbouring dimensions, so that a warp's stores are contiguous.
-constexpr int kAppendRows = 4, kReadRows = 8, kReadAhead = 4;
-template <int HD>
-__global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ RowsParams p) {
+// A CTA has kReadRows positions, of keys (blockIdx.y = 0) or values; a lane has four neighbouring dimensions, so that a warp's stores are contiguous.
+constexpr int kAppendRows = 4, kReadRows = 8;
+template <int HD, bool V>
+__device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&places)[kReadRows], int row0) {
     constexpr int LPV = HD / 4;
-    const int H = p.n_kv_heads, row0 = blockIdx.x * kReadRows, sub = threadIdx.x % LPV, piece = sub & 7, g = sub >> 3;
-    __shared__ RowPlace places[kReadRows];
-    find_places<kReadRows>(p, row0, (size_t)H * q4_block_bytes(HD), places);
-    for (int vec = threadIdx.x / LPV; vec < 2 * H; vec += 256 / LPV) {
-        const bool is_v = vec >= H;
-        const int h = vec - (is_v ? H : 0);
-        float *out = (is_v ? p.v : p.k) + row0 * p.ld + h * HD + sub * 4;
-        const bool vec4 = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (p.ld & 3) == 0;
+    const int H = p.n_kv_heads, sub = threadIdx.x % LPV, piece = sub & 7, g = sub >> 3, n_rows = min(kReadRows, p.n_tokens - row0);
+    for (int h = threadIdx.x / LPV; h < H; h += blockDim.x / LPV) {
+        float *to = (V ? p.v : p.k) + row0 * p.ld + h * HD + sub * 4;
+        const bool vec4 = (reinterpret_cast<uintptr_t>(to) & 15) == 0 && (p.ld & 3) == 0;
+        uint32_t w[kReadRows];
+        __half m[kReadRows];
+        __nv_bfloat16 d[kReadRows];
 #pragma unroll
-        for (int n0 = 0; n0 < kReadRows; n0 += kReadAhead) {
-            uint32_t w[kReadAhead];
-            float m[kReadAhead], d[kReadAhead];
+        for (int n = 0; n < kReadRows; n++) {
+            const RowPlace at = places[min(n, n_rows - 1)];
+            const int pp = at.pos & 15;
+            const uint8_t *block = at.page + h * q4_block_bytes(HD);
+            m[n] = *reinterpret_cast<const __half *>(block + (V ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g)));
+            d[n] = *reinterpret_cast<const __nv_bfloat16 *>(block + (V ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g)));
+            if constexpr (V)
+                w[n] = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g));
+            else
+                w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g));
+        }
 #pragma unroll
-            for (int n = 0; n < kReadAhead; n++) {
-                const RowPlace at = places[n0 + n];
-                if (!at.page) continue;
-                const int pp = at.pos & 15;
-                const uint8_t *block = at.page + h * q4_block_bytes(HD);
-                if (is_v) {
-                    m[n] = __half2float(*reinterpret_cast<const __half *>(block + q4_v_offset(HD, pp, g)));
-                    d[n] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + q4_v_step(HD, pp, g)));
-                    w[n] = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g));
-                } else {
-                    m[n] = __half2float(*reinterpret_cast<const __half *>(block + q4_k_offset(HD, pp, g)));
-                    d[n] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(block + q4_k_step(HD, pp, g)));
-                    w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g)) >> (8 * (piece & 1));
-                }
+        for (int n = 0; n < kReadRows; n++) {
+            if (n >= n_rows) break;
+            const float mf = __half2float(m[n]), df = __bfloat162float(d[n]);
+            float4 x;
+            if constexpr (V) {
+                x = make_float4(fmaf(df, bits_as_float(w[n], 0xfu), mf), fmaf(df * 0x1p-4f, bits_as_float(w[n], 0xf0u), mf),
+                                fmaf(df * 0x1p-8f, bits_as_float(w[n], 0xf00u), mf), fmaf(df * 0x1p-12f, bits_as_float(w[n], 0xf000u), mf));
+            } else {
+                const uint32_t y = w[n] >> (8 * (piece & 1));
+                x = make_float4(fmaf(df, bits_as_float(y, 0xfu), mf), fmaf(df * 0x1p-16f, bits_as_float(y, 0xf0000u), mf),
+                                fmaf(df * 0x1p-4f, bits_as_float(y, 0xf0u), mf), fmaf(df * 0x1p-16f, bits_as_float(y >> 4, 0xf0000u), mf));
             }
-#pragma unroll
-            for (int n = 0; n < kReadAhead; n++) {
-                if (!places[n0 + n].page) continue;
-                float4 x;
-                if (is_v)
-                    x = make_float4(fmaf(d[n], bits_as_float(w[n], 0xfu), m[n]), fmaf(d[n] * 0x1p-4f, bits_as_float(w[n], 0xf0u), m[n]),
-                                    fmaf(d[n] * 0x1p-8f, bits_as_float(w[n], 0xf00u), m[n]), fmaf(d[n] * 0x1p-12f, bits_as_float(w[n], 0xf000u), m[n]));
-                else
-                    x = make_float4(fmaf(d[n], bits_as_float(w[n], 0xfu), m[n]), fmaf(d[n] * 0x1p-16f, bits_as_float(w[n], 0xf0000u), m[n]),
-                                    fmaf(d[n] * 0x1p-4f, bits_as_float(w[n], 0xf0u), m[n]), fmaf(d[n] * 0x1p-16f, bits_as_float(w[n] >> 4, 0xf0000u), m[n]));
-                float *to = out + (n0 + n) * p.ld;
-                if (vec4) {
-                    *reinterpret_cast<float4 *>(to) = x;
-                } else {
-                    to[0] = x.x;
-                    to[1] = x.y;
-                    to[2] = x.z;
-                    to[3] = x.w;
-                }
+            if (vec4) {
+                *reinterpret_cast<float4 *>(to) = x;
+            } else {
+                to[0] = x.x;
+                to[1] = x.y;
+                to[2] = x.z;
+                to[3] = x.w;
             }
+            to += p.ld;
         }
     }
+}
+template <int HD>
+__global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ RowsParams p) {
+    __shared__ RowPlace places[kReadRows];
+    const int row0 = blockIdx.x * kReadRows;
+    find_places<kReadRows>(p, row0, (size_t)p.n_kv_heads * q4_block_bytes(HD), places);
+    if (blockIdx.y == 0)
+        read_rows<HD, false>(p, places, row0);
+    else
+        read_rows<HD, true>(p, places, row0);
 }
 
 // FP16 and FP32 pages: eight elements a thread, both directions.
@@ -347,14 +356,14 @@ static int launch_rows(juno_ctx *c, const juno_kvpool *p, int layer, const Cache
     if (p->dtype == kKvQ4 && APPEND) {
         // several positions to a CTA once there are CTAs for every SM several times over
         const int each = n_tokens >= c->sm_count * 16 ? kAppendRows : 1;
-        const dim3 grid((unsigned)((n_tokens + each - 1) / each)), block((unsigned)std::min(256, (2 * p->n_kv_heads * (hd / 8) + 31) / 32 * 32));
+        const dim3 grid((unsigned)((n_tokens + each - 1) / each), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 8) + 31) / 32 * 32));
         if (each == 1)
             hd == 128 ? q4_append_kernel<128, 1><<<grid, block, 0, st>>>(a) : q4_append_kernel<64, 1><<<grid, block, 0, st>>>(a);
         else
             hd == 128 ? q4_append_kernel<128, kAppendRows><<<grid, block, 0, st>>>(a) : q4_append_kernel<64, kAppendRows><<<grid, block, 0, st>>>(a);
     } else if (p->dtype == kKvQ4) {
-        const unsigned grid = (unsigned)((n_tokens + kReadRows - 1) / kReadRows);
-        hd == 128 ? q4_read_kernel<128><<<grid, 256, 0, st>>>(a) : q4_read_kernel<64><<<grid, 256, 0, st>>>(a);
+        const dim3 grid((unsigned)((n_tokens + kReadRows - 1) / kReadRows), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 4) + 31) / 32 * 32));
+        hd == 128 ? q4_read_kernel<128><<<grid, block, 0, st>>>(a) : q4_read_kernel<64><<<grid, block, 0, st>>>(a);
     } else {
         const unsigned grid = (unsigned)(((int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8) + 255) / 256);
         p->dtype == 0 ? rows_kernel<__half, APPEND><<<grid, 256, 0, st>>>(a, hd) : rows_kernel<float, APPEND><<<grid, 256, 0, st>>>(a, hd);
