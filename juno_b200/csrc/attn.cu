@@ -1061,9 +1061,9 @@ int seq_create(juno_kvpool *p, int max_tokens, juno_seq **out) {
 // Entries [lo, hi] of the sequence's row of the page table, from the mirror to the device.  The calls on a pool of its own return before the device
 // is done with them, and the mirror may have changed again by then: the entries travel with the launch.  A model's calls wait for their work.
 struct TableWords {
-    int32_t v[480];
+    int32_t v[2000];  // 8 KB of parameters
 };
-static __global__ void table_store_kernel(int32_t *dst, const TableWords w, int n) {
+static __global__ void table_store_kernel(int32_t *dst, const __grid_constant__ TableWords w, int n) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = w.v[i];
 }
 int table_store(const juno_kvpool *p, int slot, int lo, int hi, cudaStream_t st) {
@@ -1077,7 +1077,23 @@ int table_store(const juno_kvpool *p, int slot, int lo, int hi, cudaStream_t st)
         TableWords w;
         const int n = std::min(kWords, hi - lo + 1);
         memcpy(w.v, p->h_table + at + lo, (size_t)n * sizeof(int32_t));
-        table_store_kernel<<<1, 128, 0, st>>>(p->d_table + at + lo, w, n);
+        table_store_kernel<<<1, 256, 0, st>>>(p->d_table + at + lo, w, n);
+        JUNO_CUDA_TRY(cudaGetLastError());
+        p->ctx->kernel_launches++;
+    }
+    return JUNO_OK;
+}
+
+static __global__ void table_pairs_kernel(int32_t *table, const __grid_constant__ TableWords w, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) table[w.v[2 * i]] = w.v[2 * i + 1];
+}
+int table_store_pairs(const juno_kvpool *p, const std::vector<int32_t> &pairs, cudaStream_t st) {
+    constexpr size_t kWords = sizeof(TableWords) / sizeof(int32_t);
+    for (size_t at = 0; at < pairs.size(); at += kWords) {
+        TableWords w;
+        const size_t n = std::min(kWords, pairs.size() - at);
+        memcpy(w.v, pairs.data() + at, n * sizeof(int32_t));
+        table_pairs_kernel<<<1, 256, 0, st>>>(p->d_table, w, (int)(n / 2));
         JUNO_CUDA_TRY(cudaGetLastError());
         p->ctx->kernel_launches++;
     }
@@ -1103,7 +1119,7 @@ static int page_copy(juno_kvpool *p, int dst, int src, cudaStream_t st) {
     return JUNO_OK;
 }
 
-int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st) {
+int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<int32_t> *later) {
     juno_kvpool *p = s->pool;
     JUNO_REQUIRE(upto <= s->max_tokens, "position %d is beyond this sequence's limit of %d", upto - 1, s->max_tokens);
     const int need = (upto + kPageTokens - 1) / kPageTokens;
@@ -1141,6 +1157,13 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st) {
         row[i] = pg;
         lo = std::min(lo, i);
         hi = std::max(hi, i);
+    }
+    if (later) {
+        for (int i = lo; i <= hi; i++) {
+            later->push_back(s->slot * p->max_pages_per_seq + i);
+            later->push_back(row[i]);
+        }
+        return JUNO_OK;
     }
     return table_store(p, s->slot, lo, hi, st);
 }

@@ -109,9 +109,11 @@ int seq_create(juno_kvpool *p, int max_tokens, juno_seq **out);
 // Makes sure pages exist for positions [0, upto) and that the device page table row is current (stream-ordered).
 // Makes the positions [from, upto) of the sequence writable: allocates missing pages and gives the sequence a private
 // copy of every page of the range that it shares with another sequence (copy-on-write, ordered on `st`).
-int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st);
+// later: the changed entries of the page table are left to the caller, as pairs (place in the table, page), for table_store_pairs.
+int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<int32_t> *later = nullptr);
 // Entries [lo, hi] of a row of the page table, from the mirror to the device, ordered on `st`.
 int table_store(const juno_kvpool *p, int slot, int lo, int hi, cudaStream_t st);
+int table_store_pairs(const juno_kvpool *p, const std::vector<int32_t> &pairs, cudaStream_t st);  // pools outside models
 int seq_check(const juno_seq *s);  // JUNO_ERR_CLOSED for a handle that was freed
 
 }  // namespace juno

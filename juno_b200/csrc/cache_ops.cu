@@ -64,9 +64,9 @@ int cache_scratch(juno_ctx *c, size_t bytes, uint8_t **out) {
 
 // By value: neither the caller's memory nor a staging buffer has to outlive the call.
 struct WordsByValue {
-    int32_t v[960];
+    int32_t v[2000];  // 8 KB of parameters
 };
-static __global__ void words_kernel(int32_t *dst, const WordsByValue w, int n) {
+static __global__ void words_kernel(int32_t *dst, const __grid_constant__ WordsByValue w, int n) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = w.v[i];
 }
 int cache_words(juno_ctx *c, const int32_t *words, size_t n, int32_t *dst, cudaStream_t st) {
@@ -707,8 +707,12 @@ int juno_kv_append_device(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n,
         JUNO_TRY(device_memory(c, v_dev, "v"));
         CacheStream s(c, stream);
         JUNO_TRY(s.status);
-        for (int i = 0; i < n; i++)
-            if (counts[i]) JUNO_TRY(seq_reserve(seqs[i], positions[i], positions[i] + counts[i], s.st));
+        std::vector<int32_t> table;
+        int rc = JUNO_OK;
+        for (int i = 0; rc == JUNO_OK && i < n; i++)
+            if (counts[i]) rc = seq_reserve(seqs[i], positions[i], positions[i] + counts[i], s.st, &table);
+        JUNO_TRY(table_store_pairs(p, table, s.st));  // of those that have their pages, too, when others do not
+        JUNO_TRY(rc);
         JUNO_TRY(launch_kv_append(c, p, layer, rows.data(), (int)rows.size(), total, k_dev, v_dev, ld, s.st));
         for (int i = 0; i < n; i++) seqs[i]->len = std::max(seqs[i]->len, positions[i] + counts[i]);
         return JUNO_OK;
@@ -821,15 +825,18 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         CacheStream st(c, stream);
         JUNO_TRY(st.status);
         auto padded = [](size_t b) { return (b + 255) & ~(size_t)255; };
-        const size_t row_bytes = padded(rows.size() * sizeof(EvictRow)), page_bytes = padded(pages.size() * 4),
-                     kept_bytes = kept_dev ? 0 : (size_t)p->n_layers * n * p->n_kv_heads * keep * 4;
+        // rows, then pages, by value
+        constexpr size_t kRowWords = sizeof(EvictRow) / sizeof(int32_t);
+        std::vector<int32_t> words(rows.size() * kRowWords + pages.size());
+        memcpy(words.data(), rows.data(), rows.size() * sizeof(EvictRow));
+        if (!pages.empty()) memcpy(words.data() + rows.size() * kRowWords, pages.data(), pages.size() * sizeof(int32_t));
+        const size_t word_bytes = padded(words.size() * sizeof(int32_t)), kept_bytes = kept_dev ? 0 : (size_t)p->n_layers * n * p->n_kv_heads * keep * sizeof(int32_t);
         uint8_t *scratch = nullptr;
-        JUNO_TRY(cache_scratch(c, row_bytes + page_bytes + kept_bytes, &scratch));
-        JUNO_TRY(cache_words(c, reinterpret_cast<const int32_t *>(rows.data()), rows.size() * sizeof(EvictRow) / 4, reinterpret_cast<int32_t *>(scratch), st.st));
-        JUNO_TRY(cache_words(c, pages.data(), pages.size(), reinterpret_cast<int32_t *>(scratch + row_bytes), st.st));
+        JUNO_TRY(cache_scratch(c, word_bytes + kept_bytes, &scratch));
+        JUNO_TRY(cache_words(c, words.data(), words.size(), reinterpret_cast<int32_t *>(scratch), st.st));
         EvictParams a;
         a.rows = reinterpret_cast<const EvictRow *>(scratch);
-        a.pages = reinterpret_cast<const int32_t *>(scratch + row_bytes);
+        a.pages = reinterpret_cast<const int32_t *>(scratch) + rows.size() * kRowWords;
         a.pool = static_cast<uint8_t *>(p->k);
         a.n = n;
         a.n_pages = p->n_pages;
@@ -838,7 +845,7 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         a.track_tokens = p->track_tokens;
         a.hd = p->head_dim;
         a.weights = p->weights;
-        a.kept = kept_dev ? kept_dev : reinterpret_cast<int32_t *>(scratch + row_bytes + page_bytes);
+        a.kept = kept_dev ? kept_dev : reinterpret_cast<int32_t *>(scratch + word_bytes);
         a.kept_ld = keep;
         const dim3 heads((unsigned)p->n_kv_heads, (unsigned)p->n_layers, (unsigned)n), units((unsigned)((np * p->n_kv_heads + 7) / 8), (unsigned)p->n_layers, (unsigned)n);
         const size_t cached = kSelectCached * sizeof(float);
@@ -859,12 +866,11 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         JUNO_CUDA_TRY(cudaGetLastError());
         c->kernel_launches += 2;
         p->free_pages.resize(next);
-        int rc = JUNO_OK;
+        std::vector<int32_t> table;
         for (int i = 0; i < n; i++) {
             juno_seq *s = seqs[i];
             if (s->len <= keep) continue;
             int32_t *row = p->h_table + (size_t)s->slot * p->max_pages_per_seq;
-            int lo = np, hi = -1;
             for (int j = 0; j < (int)s->pages.size(); j++) {
                 const int old = s->pages[(size_t)j], now = j < np ? pages[(size_t)rows[(size_t)i].new_pages + j] : -1;
                 if (now == old) continue;
@@ -872,14 +878,13 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
                 if (now < 0) continue;
                 p->page_refs[(size_t)now] = 1;
                 s->pages[(size_t)j] = row[j] = now;
-                lo = std::min(lo, j);
-                hi = j;
+                table.push_back(s->slot * p->max_pages_per_seq + j);
+                table.push_back(now);
             }
             s->pages.resize((size_t)np);
             s->len = keep;
-            if (hi >= 0 && rc == JUNO_OK) rc = table_store(p, s->slot, lo, hi, st.st);
         }
-        return rc;
+        return table_store_pairs(p, table, st.st);
     });
 }
 

@@ -24,6 +24,7 @@ struct Q4AttnParams {
     int64_t ldq, ldo;
     float *out;
     float *part_o, *part_ml;  // [part][head][hd], [part][head][max, sum]
+    float2 *sums;             // sequences that keep weights: [row][head] largest score of all, 1 / sum
     unsigned *arrived;        // [row][kv_head]: parts that are done, zero between launches
     float *scores;            // sequences that keep weights: [kv_head][position of all pages][G], log2 domain
     float *weights;
@@ -101,21 +102,6 @@ struct Q4Smem {  // bytes
                          kQuery = kMerge + kQ4Warps<HPL> * 4 * HPL * (HD + 2) * 4, kQueryRow = HD + 8,  // halves; the pad keeps the rows on different banks
         kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kBack = kSums + 2 * 4 * HPL * 4 * 2, kAll = kBack + 4 * HPL * 4;
 };
-
-// The largest score of a (row, head) and the sum of its weights over the row's parts, by all threads of a warp.
-__device__ __forceinline__ float2 row_sums(const Q4AttnParams &p, int i, int share0, int parts, int h, int lane) {
-    float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < parts; s += 32) M = fmaxf(M, __ldcg(p.part_ml + ((size_t)(i + share0 + s) * p.n_heads + h) * 2));
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    for (int s = lane; s < parts; s += 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml + ((size_t)(i + share0 + s) * p.n_heads + h) * 2));
-        L = fmaf(ml.y, exp2_fast(ml.x - M), L);
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-    return make_float2(M, L);
-}
 
 template <int HD, int HPL, bool TRACK>
 __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
@@ -515,7 +501,8 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
             } else {
                 *reinterpret_cast<float2 *>(p.part_o + part * HD + d) = make_float2(ax, ay);
             }
-            if (d == 0 && (parts > 1 || track)) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(M, L);
+            if (d == 0 && parts > 1) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(M, L);
+            if (TRACK && d == 0 && parts == 1) p.sums[(size_t)i * p.n_heads + h0 + g] = make_float2(M, 1.f / L);
         }
         // The rows that this share has with others are its first and its last.  Whoever of a row is last puts its parts together, at the end.
         if (parts > 1) {
@@ -600,35 +587,40 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
             float *to_o = p.out + (size_t)i * p.ldo + (h0 + g) * HD + d;
             to_o[0] = ax / L;
             to_o[1] = ay / L;
+            if (TRACK && d == 0) p.sums[(size_t)i * p.n_heads + h0 + g] = make_float2(M, 1.f / L);
         }
     }
 }
 
-// One block per kQ4WeightPages pages of all rows and key/value head: the weight that their positions have received.
-constexpr int kQ4WeightThreads = 128, kQ4WeightPages = kQ4WeightThreads / kPageTokens;
+// The weight that positions have received: a thread has one position of all rows' pages and one key/value head.
+constexpr int kQ4WeightThreads = 256;
+template <int G>
+__device__ __forceinline__ float weight_of(const float *scores, const float2 *sums, int g_max) {
+    float s[G], sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++) s[g] = g < g_max ? scores[g] : 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+        if (g < g_max) sum = fmaf(exp2_fast(s[g] - sums[g].x), sums[g].y, sum);
+    return sum;
+}
 __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __grid_constant__ Q4AttnParams p) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    __shared__ float2 sums[kQ4MaxGroup];
-    const int kvh = blockIdx.x % p.n_kv_heads, page0 = blockIdx.x / p.n_kv_heads * kQ4WeightPages, page1 = min(p.total, page0 + kQ4WeightPages);
-    const int G = p.n_heads / p.n_kv_heads;
     pdl_wait();
-    for (int i = cache_find(p.rows, page0); i < p.rows.n; i++) {
-        const CacheRow r = cache_row(p.rows, i);
-        if (r.first >= page1) break;
-        if (r.track < 0 || r.upto == 0) continue;
-        const int share0 = r.first / p.share, parts = (row_end(p, i) - 1) / p.share - share0 + 1;
-        __syncthreads();
-        for (int g = warp; g < G; g += kQ4WeightThreads / 32) {
-            const float2 ml = row_sums(p, i, share0, parts, kvh * G + g, lane);
-            if (lane == 0) sums[g] = make_float2(ml.x, 1.f / ml.y);
-        }
-        __syncthreads();
-        const int pos = (page0 - r.first) * kPageTokens + tid;
-        if (pos < 0 || pos >= r.upto) continue;
-        const float *s = p.scores + (((size_t)kvh * p.total + page0) * kPageTokens + tid) * G;
-        float sum = 0.f;
-        for (int g = 0; g < G; g++) sum = fmaf(exp2_fast(s[g] - sums[g].x), sums[g].y, sum);
-        p.weights[(((size_t)r.track * p.n_layers + p.layer) * p.n_kv_heads + kvh) * p.track_tokens + pos] += sum;
+    const int kvh = blockIdx.y, at = blockIdx.x * kQ4WeightThreads + threadIdx.x, G = p.n_heads / p.n_kv_heads;
+    if (at >= p.total * kPageTokens) return;
+    const int i = cache_find(p.rows, at >> 4);
+    const CacheRow r = cache_row(p.rows, i);
+    const int pos = at - r.first * kPageTokens;
+    if (r.track < 0 || pos >= r.upto) return;
+    const float *scores = p.scores + ((size_t)kvh * p.total * kPageTokens + at) * G;
+    const float2 *sums = p.sums + (size_t)i * p.n_heads + kvh * G;
+    float *w = p.weights + (((size_t)r.track * p.n_layers + p.layer) * p.n_kv_heads + kvh) * p.track_tokens + pos;
+    const float old = *w;
+    if (G == 4) {
+        const float4 s = *reinterpret_cast<const float4 *>(scores);  // 16-byte multiples: four heads a position
+        *w = old + fmaf(exp2_fast(s.w - sums[3].x), sums[3].y, fmaf(exp2_fast(s.z - sums[2].x), sums[2].y, fmaf(exp2_fast(s.y - sums[1].x), sums[1].y, exp2_fast(s.x - sums[0].x) * sums[0].y)));
+    } else {
+        *w = old + weight_of<kQ4MaxGroup>(scores, sums, G);
     }
 }
 
@@ -689,9 +681,9 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     Q4AttnParams a;
     auto padded = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t parts = (size_t)(n + shares), far_b = cache_rows_bytes(n), ml_b = padded(parts * n_heads * 8), o_b = whole ? 0 : padded(parts * n_heads * hd * 4),
-                 s_b = track ? (size_t)pages * kPageTokens * n_heads * 4 : 0;
+                 s_b = track ? padded((size_t)pages * kPageTokens * n_heads * 4) : 0, sum_b = track ? (size_t)n * n_heads * sizeof(float2) : 0;
     uint8_t *scratch = nullptr;
-    JUNO_TRY(cache_scratch(c, far_b + ml_b + o_b + s_b, &scratch));
+    JUNO_TRY(cache_scratch(c, far_b + ml_b + o_b + s_b + sum_b, &scratch));
     JUNO_TRY(cache_rows(c, rows.data(), n, reinterpret_cast<CacheRow *>(scratch), &a.rows, st));
     a.pool = static_cast<const uint8_t *>(p->k);
     a.table = p->d_table;
@@ -710,6 +702,7 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     a.part_ml = reinterpret_cast<float *>(scratch + far_b);
     a.part_o = reinterpret_cast<float *>(scratch + far_b + ml_b);
     a.scores = track ? reinterpret_cast<float *>(scratch + far_b + ml_b + o_b) : nullptr;
+    a.sums = track ? reinterpret_cast<float2 *>(scratch + far_b + ml_b + o_b + s_b) : nullptr;
     a.weights = p->weights;
     a.track_tokens = p->track_tokens;
     a.arrived = c->cache_arrived;
@@ -721,7 +714,7 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
         JUNO_TRY((track ? launch_q4_attn<64, true>(a, G, shares, st) : launch_q4_attn<64, false>(a, G, shares, st)));
     c->kernel_launches++;
     if (!track) return JUNO_OK;
-    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages + kQ4WeightPages - 1) / kQ4WeightPages * H)), dim3(kQ4WeightThreads), 0, st, a));
+    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages * kPageTokens + kQ4WeightThreads - 1) / kQ4WeightThreads), (unsigned)H), dim3(kQ4WeightThreads), 0, st, a));
     c->kernel_launches++;
     return JUNO_OK;
 }
