@@ -1168,6 +1168,20 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<in
     return table_store(p, s->slot, lo, hi, st);
 }
 
+// A sequence's weights, one plane of `room` (a multiple of 16) positions for each layer and head: the first `len` of another one's, zeros behind.
+static __global__ void track_kernel(float *own, const float *from, int room, int len) {
+    const int pos = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (pos >= room) return;
+    const size_t at = (size_t)blockIdx.y * room + pos;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (pos < len) {
+        v = *reinterpret_cast<const float4 *>(from + at);
+        if (pos + 1 >= len) v.y = 0.f;
+        if (pos + 2 >= len) v.z = 0.f;
+        if (pos + 3 >= len) v.w = 0.f;
+    }
+    *reinterpret_cast<float4 *>(own + at) = v;
+}
 // Gives the sequence one of the pool's weight planes: zeros, or what `src` holds for the positions that both have.
 static int seq_track(juno_seq *s, const juno_seq *src) {
     juno_kvpool *p = s->pool;
@@ -1178,12 +1192,12 @@ static int seq_track(juno_seq *s, const juno_seq *src) {
         return JUNO_ERR_OOM;
     }
     const int track = p->free_tracks.back();
-    const size_t pitch = (size_t)p->track_tokens * sizeof(float), planes = (size_t)p->n_layers * p->n_kv_heads;
+    const size_t planes = (size_t)p->n_layers * p->n_kv_heads;
     float *own = p->weights + track * p->track_stride();
-    JUNO_CUDA_TRY(cudaMemsetAsync(own, 0, pitch * planes, p->ctx->stream));
-    if (src && s->len)
-        JUNO_CUDA_TRY(cudaMemcpy2DAsync(own, pitch, p->weights + src->track * p->track_stride(), pitch, (size_t)s->len * sizeof(float), planes,
-                                        cudaMemcpyDeviceToDevice, p->ctx->stream));
+    const dim3 grid((unsigned)((p->track_tokens / 4 + 255) / 256), (unsigned)planes);
+    track_kernel<<<grid, 256, 0, p->ctx->stream>>>(own, src ? p->weights + src->track * p->track_stride() : nullptr, p->track_tokens, src ? s->len : 0);
+    JUNO_CUDA_TRY(cudaGetLastError());
+    p->ctx->kernel_launches++;
     p->free_tracks.pop_back();
     s->track = track;
     return JUNO_OK;

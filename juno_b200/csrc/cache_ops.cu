@@ -413,8 +413,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     const uint32_t u = __float_as_uint(w + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float key_weight(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }  // 0 becomes a NaN again
 
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kSelectCached = 24576, kBins = 2048;
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kSelectCached = 24576, kBins = 2048;
 
 // Sum over the threads of the block before this one, in *all the sum over all of them.  `sums`: kSelectWarps words.
 __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *sums, unsigned *all) {
@@ -427,7 +428,7 @@ __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *sums, uns
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    unsigned s = sums[lane], w = s;
+    unsigned s = lane < kSelectWarps ? sums[lane] : 0u, w = s;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, w, x);
@@ -452,33 +453,47 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         for (int j = tid; j < r.keep; j += kSelectThreads) kept[j] = j;
         return;
     }
-    extern __shared__ float cached[];  // kSelectCached
+    extern __shared__ uint32_t keys[];  // kSelectCached
     __shared__ unsigned bins[kBins], sums[kSelectWarps], digit_s, left_s;
     const int old = r.len - r.recent;  // candidates
     const bool whole = r.len <= kSelectCached;
     if (whole) {
-        for (int j = tid; j < r.len; j += kSelectThreads) cached[j] = w[j];
+        for (int j = tid; j < r.len; j += kSelectThreads) keys[j] = weight_key(w[j]);
         __syncthreads();
     }
     unsigned need = (unsigned)(r.keep - r.recent), key = 0;
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const unsigned mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, digits = pass == 2 ? 1023u : 2047u;
-        bins[tid] = bins[tid + kSelectThreads] = 0;
+        for (int j = tid; j < kBins; j += kSelectThreads) bins[j] = 0;
         __syncthreads();
-        for (int j = tid; j < old; j += kSelectThreads) {
-            const uint32_t u = weight_key(whole ? cached[j] : w[j]);
-            if ((u & mask) == key) atomicAdd(&bins[u >> shift & digits], 1u);
+        if (whole) {
+            for (int j = tid; j < old; j += kSelectThreads) {
+                const uint32_t u = keys[j];
+                if ((u & mask) == key) atomicAdd(&bins[u >> shift & digits], 1u);
+            }
+        } else {
+            for (int j = tid; j < old; j += kSelectThreads) {
+                const uint32_t u = weight_key(w[j]);
+                if ((u & mask) == key) atomicAdd(&bins[u >> shift & digits], 1u);
+            }
         }
         __syncthreads();
         // from the largest digit down: the one in which the need-th weight lies
-        const unsigned a = bins[kBins - 1 - 2 * tid], b = bins[kBins - 2 - 2 * tid];
-        unsigned all;
-        const unsigned before = block_before(a + b, sums, &all);
-        if (before < need && need <= before + a + b) {
-            const bool first = need <= before + a;
-            digit_s = kBins - 1 - 2 * tid - !first;
-            left_s = need - before - (first ? 0u : a);
+        constexpr int EACH = kBins / kSelectThreads;
+        unsigned mine = 0, count[EACH], all;
+#pragma unroll
+        for (int k = 0; k < EACH; k++) mine += count[k] = bins[kBins - 1 - EACH * tid - k];
+        unsigned before = block_before(mine, sums, &all);
+        if (before < need && need <= before + mine) {
+#pragma unroll
+            for (int k = 0; k < EACH; k++) {
+                if (before < need && need <= before + count[k]) {
+                    digit_s = kBins - 1 - EACH * tid - k;
+                    left_s = need - before;
+                }
+                before += count[k];
+            }
         }
         __syncthreads();
         if (need > 0) {
@@ -496,15 +511,14 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         const int n = min(kSelectCached, r.len - base), run = (n + kSelectWarps * 32 - 1) / (kSelectWarps * 32) * 32, from = min(n, warp * run), to = min(n, from + run);
         if (!whole) {
             __syncthreads();
-            for (int j = tid; j < n; j += kSelectThreads) cached[j] = w[base + j];
+            for (int j = tid; j < n; j += kSelectThreads) keys[j] = weight_key(w[base + j]);
             __syncthreads();
         }
-        unsigned same = 0, above = 0;  // of this warp, in lane 0
-        for (int j = from; j < to; j += 32) {
-            const int at = base + j + lane;
-            const uint32_t u = j + lane < to ? weight_key(cached[j + lane]) : 0u;
-            same += __popc(__ballot_sync(0xffffffffu, j + lane < to && at < old && u == key));
-            above += __popc(__ballot_sync(0xffffffffu, j + lane < to && (at >= old || u > key)));
+        unsigned same = 0, above = 0;  // of this warp
+        for (int j = from + lane; j - lane < to; j += 32) {
+            const uint32_t u = j < to ? keys[j] : 0u;
+            same += __popc(__ballot_sync(0xffffffffu, u == key && j < to && base + j < old));
+            above += __popc(__ballot_sync(0xffffffffu, j < to && (u > key || base + j >= old)));
         }
         unsigned all;
         unsigned rank = equal + __shfl_sync(0xffffffffu, block_before(lane == 0 ? same : 0u, sums, &all), 0);
@@ -512,19 +526,17 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         const unsigned taken = rank < need ? min(same, need - rank) : 0u;
         unsigned out = done + __shfl_sync(0xffffffffu, block_before(lane == 0 ? above + taken : 0u, sums, &all), 0);
         done += all;
-        for (int j = from; j < to; j += 32) {
-            const int at = base + j + lane;
-            const bool on = j + lane < to;
-            const float v = on ? cached[j + lane] : 0.f;
-            const uint32_t u = weight_key(v);
-            const bool eq = on && at < old && u == key;
+        for (int j = from + lane; j - lane < to; j += 32) {
+            const int at = base + j;
+            const uint32_t u = j < to ? keys[j] : 0u;
+            const bool eq = u == key && j < to && at < old;
             const unsigned eqs = __ballot_sync(0xffffffffu, eq);
-            const bool stays = on && (at >= old || u > key || (eq && rank + __popc(eqs & ((1u << lane) - 1u)) < need));
+            const bool stays = j < to && (u > key || at >= old || (eq && rank + __popc(eqs & ((1u << lane) - 1u)) < need));
             const unsigned st = __ballot_sync(0xffffffffu, stays);
             if (stays) {
                 const unsigned to_j = out + __popc(st & ((1u << lane) - 1u));
                 kept[to_j] = at;
-                w[to_j] = v;
+                w[to_j] = key_weight(u);
             }
             rank += __popc(eqs);
             out += __popc(st);
@@ -532,104 +544,107 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     }
 }
 
-// Copies between rows of two blocks in 16-, 8- and 2-byte pieces: PIECES of them in a row, this one is number `i`.
+// A row in pieces, one to a lane of sixteen: the numbers of keys and values in 16 bytes, the keys' steps and offsets and the values' steps in 2 NG, the values'
+// offsets in 2.  Where piece i of position pp lies: at + pp * stride, but for the values' numbers, whose pieces are permuted.
 template <int HD>
-struct Q4Row {
-    static constexpr int NG = HD / kQ4Group, CODES = HD / 32;                    // 16-byte pieces of a row's numbers, keys' or values'
-    static constexpr int FACTORS = 3, PIECES = 2 * CODES + FACTORS + NG;  // steps and offsets of keys, steps of values: NG half words each; values' offsets
-    uint4 data;
-    __device__ __forceinline__ void load(const uint8_t *b, int pp, int i) {
-        if (i < 2 * CODES) {
-            data = *reinterpret_cast<const uint4 *>(b + codes(pp, i));
-        } else if (i < 2 * CODES + FACTORS) {
-            const uint8_t *f = b + factors(pp, i - 2 * CODES);
-            if constexpr (NG == 4) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(f);
-                data.x = v.x;
-                data.y = v.y;
-            } else {
-                data.x = *reinterpret_cast<const uint32_t *>(f);
-            }
-        } else {
-            data.x = *reinterpret_cast<const uint16_t *>(b + q4_v_offset(HD, pp, i - 2 * CODES - FACTORS));
+struct Q4Piece {
+    static constexpr int NG = HD / kQ4Group, CODES = HD / 32, PIECES = 2 * CODES + 3 + NG;
+    int kind, at, stride, group;  // 0: 16 bytes, 1: values' 16 bytes, 2: NG half words, 3: one, 4: none
+    __device__ __forceinline__ explicit Q4Piece(int i) : kind(4), at(0), stride(0), group(0) {
+        if (i < CODES) {
+            kind = 0, at = q4_k_code(HD, 0, 0, 0) + 16 * i, stride = HD / 2;
+        } else if (i < 2 * CODES) {
+            kind = 1, at = 10 * HD, stride = HD / 2, group = i - CODES;
+        } else if (i < 2 * CODES + 3) {
+            const int k = i - 2 * CODES;
+            kind = 2, at = k == 0 ? q4_k_step(HD, 0, 0) : k == 1 ? q4_k_offset(HD, 0, 0) : q4_v_step(HD, 0, 0), stride = 2 * NG;
+        } else if (i < PIECES) {
+            kind = 3, at = q4_v_offset(HD, 0, i - 2 * CODES - 3), stride = 2;
         }
     }
-    __device__ __forceinline__ void store(uint8_t *b, int pp, int i) const {
-        if (i < 2 * CODES) {
-            *reinterpret_cast<uint4 *>(b + codes(pp, i)) = data;
-        } else if (i < 2 * CODES + FACTORS) {
-            uint8_t *f = b + factors(pp, i - 2 * CODES);
-            if constexpr (NG == 4)
-                *reinterpret_cast<uint2 *>(f) = make_uint2(data.x, data.y);
-            else
-                *reinterpret_cast<uint32_t *>(f) = data.x;
-        } else {
-            *reinterpret_cast<uint16_t *>(b + q4_v_offset(HD, pp, i - 2 * CODES - FACTORS)) = (uint16_t)data.x;
-        }
+    __device__ __forceinline__ int place(int pp) const { return at + pp * stride + (kind == 1 ? 16 * q4_v_piece(HD, pp, group) : 0); }
+    __device__ __forceinline__ uint4 load(const uint8_t *block, int pp) const {
+        const uint8_t *b = block + place(pp);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (kind <= 1)
+            v = *reinterpret_cast<const uint4 *>(b);
+        else if (kind == 2 && NG == 4) {
+            const uint2 y = *reinterpret_cast<const uint2 *>(b);
+            v.x = y.x;
+            v.y = y.y;
+        } else if (kind == 2)
+            v.x = *reinterpret_cast<const uint32_t *>(b);
+        else if (kind == 3)
+            v.x = *reinterpret_cast<const uint16_t *>(b);
+        return v;
     }
-    static __device__ __forceinline__ int codes(int pp, int i) { return i < CODES ? q4_k_code(HD, pp, 0, 0) + 16 * i : q4_v_code(HD, pp, 0, i - CODES); }
-    static __device__ __forceinline__ int factors(int pp, int i) { return i == 0 ? q4_k_step(HD, pp, 0) : i == 1 ? q4_k_offset(HD, pp, 0) : q4_v_step(HD, pp, 0); }
+    __device__ __forceinline__ void store(uint8_t *block, int pp, uint4 v) const {
+        uint8_t *b = block + place(pp);
+        if (kind <= 1)
+            *reinterpret_cast<uint4 *>(b) = v;
+        else if (kind == 2 && NG == 4)
+            *reinterpret_cast<uint2 *>(b) = make_uint2(v.x, v.y);
+        else if (kind == 2)
+            *reinterpret_cast<uint32_t *>(b) = v.x;
+        else if (kind == 3)
+            *reinterpret_cast<uint16_t *>(b) = (uint16_t)v.x;
+    }
 };
 
 __device__ __forceinline__ uint8_t *evict_block(const EvictParams &p, int layer, int h, int list, int pos) {
     return p.pool + (((size_t)layer * p.n_pages + p.pages[list + (pos >> 4)]) * p.n_kv_heads + h) * (size_t)q4_block_bytes(p.hd);
 }
 
-// The rows that stay, into fresh pages: a warp has one page of one head.
+// The rows that stay, into fresh pages: a warp has one page of one head, two rows a step.
 template <int HD>
 __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) {
-    using Row = Q4Row<HD>;
+    static_assert(Q4Piece<HD>::PIECES <= 16, "a piece to a lane");
     const int i = blockIdx.z, layer = blockIdx.y, lane = threadIdx.x & 31;
     const EvictRow r = p.rows[i];
     if (r.keep == r.len) return;
     const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), h = unit % p.n_kv_heads, base = unit / p.n_kv_heads * kPageTokens, n = min(kPageTokens, r.keep - base);
     if (n <= 0) return;
     const int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld + base;
-    const int src = lane < n ? kept[lane] : 0;
-    const uint8_t *from = evict_block(p, layer, h, r.old_pages, src);
-    uint8_t *to = evict_block(p, layer, h, r.new_pages, base);
-    constexpr int STEPS = (kPageTokens * Row::PIECES + 31) / 32;
-    Row row[STEPS];
+    const int src = kept[min(lane, n - 1)], src_page = p.pages[r.old_pages + (src >> 4)];
+    const size_t page_bytes = (size_t)p.n_kv_heads * q4_block_bytes(HD);
+    uint8_t *plane = p.pool + (size_t)layer * p.n_pages * page_bytes + h * q4_block_bytes(HD);
+    uint8_t *to = plane + p.pages[r.new_pages + (base >> 4)] * page_bytes;
+    const Q4Piece<HD> piece(lane & 15);
+    uint4 v[kPageTokens / 2];
 #pragma unroll
-    for (int k = 0; k < STEPS; k++) {
-        const int x = k * 32 + lane, j = x / Row::PIECES;
-        const int at = __shfl_sync(0xffffffffu, src, j & 15);
-        const uint8_t *b = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, (unsigned long long)reinterpret_cast<uintptr_t>(from), j & 15));
-        if (j < n) row[k].load(b, at & 15, x - j * Row::PIECES);
+    for (int k = 0; k < kPageTokens / 2; k++) {  // rows behind the last one: that one again
+        const int j = min(2 * k + (lane >> 4), n - 1), at = __shfl_sync(0xffffffffu, src, j), page = __shfl_sync(0xffffffffu, src_page, j);
+        v[k] = piece.load(plane + page * page_bytes, at & 15);
     }
 #pragma unroll
-    for (int k = 0; k < STEPS; k++) {
-        const int x = k * 32 + lane, j = x / Row::PIECES;
-        if (j < n) row[k].store(to, j, x - j * Row::PIECES);
-    }
+    for (int k = 0; k < kPageTokens / 2; k++)
+        if (2 * k + (lane >> 4) < n) piece.store(to, 2 * k + (lane >> 4), v[k]);
 }
 
 // The same in place, for a pool without enough free pages: one CTA per (sequence, layer, head) takes kMoveRows rows a step, in order.  A row moves to the
 // front or stays, so that what a step overwrites has been read by it or by an earlier one.
-constexpr int kMoveRows = 64, kMoveThreads = 512;
+constexpr int kMoveThreads = 512, kMoveRows = kMoveThreads / 16 * 2;
 template <int HD>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
-    using Row = Q4Row<HD>;
-    const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, tid = threadIdx.x;
+    const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, sub = threadIdx.x >> 4;
     const EvictRow r = p.rows[i];
     if (r.keep == r.len) return;
     const int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld;
-    constexpr int STEPS = (kMoveRows * Row::PIECES + kMoveThreads - 1) / kMoveThreads;
+    const size_t page_bytes = (size_t)p.n_kv_heads * q4_block_bytes(HD);
+    uint8_t *plane = p.pool + (size_t)layer * p.n_pages * page_bytes + h * q4_block_bytes(HD);
+    const Q4Piece<HD> piece(threadIdx.x & 15);
     for (int base = 0; base < r.keep; base += kMoveRows) {
-        const int n = min(kMoveRows, r.keep - base);
-        Row row[STEPS];
+        uint4 v[2];
 #pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            const int x = k * kMoveThreads + tid, j = x / Row::PIECES;
-            if (j >= n) continue;
-            const int src = kept[base + j];
-            row[k].load(evict_block(p, layer, h, r.old_pages, src), src & 15, x - j * Row::PIECES);
+        for (int k = 0; k < 2; k++) {
+            const int j = base + sub + k * (kMoveThreads / 16), src = j < r.keep ? kept[j] : 0;
+            if (j < r.keep) v[k] = piece.load(plane + p.pages[r.old_pages + (src >> 4)] * page_bytes, src & 15);
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < STEPS; k++) {
-            const int x = k * kMoveThreads + tid, j = x / Row::PIECES;
-            if (j < n) row[k].store(evict_block(p, layer, h, r.new_pages, base + j), (base + j) & 15, x - j * Row::PIECES);
+        for (int k = 0; k < 2; k++) {
+            const int j = base + sub + k * (kMoveThreads / 16);
+            if (j < r.keep) piece.store(plane + p.pages[r.new_pages + (j >> 4)] * page_bytes, j & 15, v[k]);
         }
         __syncthreads();
     }

@@ -175,19 +175,35 @@ class B200MatVec:
 _KINDS: dict = {}  # element type of a tensor -> its name, as far as seen
 
 
-def _device_ptr(x, name: str, rows: int, width: int, kind: str = "float32"):
-    """(address, row stride) of a CUDA tensor (anything with data_ptr, dtype, shape, stride and is_cuda) that holds `rows` rows of `width` elements."""
-    try:
-        shape, stride, dtype = x.shape, x.stride(), x.dtype
-    except (AttributeError, TypeError):
-        raise ValueError(f"{name} is not a tensor in device memory") from None
+def _is_cuda(x, kind: str) -> bool:
+    dtype = x.dtype
     if dtype not in _KINDS:
         _KINDS[dtype] = str(dtype).rsplit(".", 1)[-1]
-    if _KINDS[dtype] != kind or not x.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor of {kind} is wanted")
+    return _KINDS[dtype] == kind and x.is_cuda
+
+
+def _device_ptr(x, name: str, rows: int, width: int):
+    """(address, row stride) of a CUDA tensor of float32 (anything with data_ptr, dtype, shape, stride and is_cuda) that holds `rows` rows of `width` elements."""
+    try:
+        shape, stride, fits = x.shape, x.stride(), _is_cuda(x, "float32")
+    except (AttributeError, TypeError):
+        raise ValueError(f"{name} is not a tensor in device memory") from None
+    if not fits:
+        raise ValueError(f"{name}: a CUDA tensor of float32 is wanted")
     if shape != (rows, width) or (width > 1 and stride[1] != 1) or (rows > 1 and stride[0] < width):
         raise ValueError(f"{name}: shape [{rows}, {width}] with neighbouring elements in a row is wanted, not {list(shape)} with strides {list(stride)}")
     return x.data_ptr(), (stride[0] if rows > 1 else width)
+
+
+def _whole_ptr(x, name: str, kind: str, lead: tuple):
+    """Address of a contiguous CUDA tensor whose shape is `lead` and one more dimension of any length."""
+    try:
+        fits = _is_cuda(x, kind) and x.is_contiguous() and x.shape[:-1] == lead
+    except (AttributeError, TypeError):
+        fits = False
+    if not fits:
+        raise ValueError(f"{name}: a contiguous CUDA tensor of {kind} with shape {[*lead, 'n']} is wanted")
+    return x.data_ptr()
 
 
 class SequenceBatch:
@@ -316,10 +332,8 @@ class PagedKvCache:
         """The weights of the first counts[i] positions of each sequence into w [sequences, n_kv_heads, at least most counts], or from it
         (juno_kv_weights_device)."""
         b = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
-        if not (hasattr(w, "data_ptr") and w.dim() == 3 and w.shape[:2] == (b.n, self.n_kv_heads) and w.is_contiguous()):
-            raise ValueError(f"w: a contiguous tensor [{b.n}, {self.n_kv_heads}, positions] is wanted")
+        wp = _whole_ptr(w, "w", "float32", (b.n, self.n_kv_heads))
         ld = w.shape[2]
-        wp, _ = _device_ptr(w.view(-1, ld), "w", b.n * self.n_kv_heads, ld)
         counts, n = self._ints(counts, b.n, "counts")
         rc = self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, n, wp, ld, 1 if store else 0,
                                             None if stream is None else self._stream(stream))
@@ -331,9 +345,9 @@ class PagedKvCache:
         int32 [n_layers, sequences, n_kv_heads, keep] gets their places (juno_kv_evict)."""
         b, kp = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs), None
         if kept is not None:
-            if not (hasattr(kept, "data_ptr") and kept.shape == (self.n_layers, b.n, self.n_kv_heads, keep) and kept.is_contiguous()):
-                raise ValueError(f"kept: a contiguous tensor [{self.n_layers}, {b.n}, {self.n_kv_heads}, {keep}] is wanted")
-            kp = _device_ptr(kept.view(-1, keep), "kept", self.n_layers * b.n * self.n_kv_heads, keep, "int32")[0]
+            kp = _whole_ptr(kept, "kept", "int32", (self.n_layers, b.n, self.n_kv_heads))
+            if kept.shape[3] != keep:
+                raise ValueError(f"kept: {keep} places for each head are wanted, not {kept.shape[3]}")
         rc = self._L.juno_kv_evict(self.ctx.handle, self.handle, b.n, b.handles, keep, recent, kp, None if stream is None else self._stream(stream))
         if rc:
             check(rc, "juno_kv_evict")
