@@ -35,11 +35,11 @@ struct Q4AttnParams {
 __device__ __forceinline__ int row_end(const Q4AttnParams &p, int i) { return i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : p.total; }
 
 constexpr int kQ4MaxGroup = 8, kQ4Slots = 2, kQ4Tile = 2;  // pages of a tile: a warp's step
-// Warps of a CTA and CTAs on an SM: 16 warps of 128 registers, 12 of 168.
-template <int HPL>
-constexpr int kQ4Warps = HPL == 1 ? 8 : 4;
-template <int HPL>
-constexpr int kQ4Ctas = HPL == 1 ? 2 : 3;
+// Warps of a CTA and CTAs on an SM: 16 warps of 128 registers, 12 of 168 for more than four heads of 128.
+template <int HD, int HPL>
+constexpr int kQ4Warps = HPL == 1 || HD == 64 ? 8 : 4;
+template <int HD, int HPL>
+constexpr int kQ4Ctas = HPL == 1 || HD == 64 ? 2 : 3;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -98,34 +98,33 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
 template <int HD, int HPL>
 struct Q4Smem {  // bytes
-    static constexpr int kRing = kQ4Warps<HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HPL> * kQ4Slots * 8,
-                         kQuery = kMerge + kQ4Warps<HPL> * 4 * HPL * (HD + 2) * 4, kQueryRow = HD + 8,  // halves; the pad keeps the rows on different banks
+    static constexpr int kRing = kQ4Warps<HD, HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HD, HPL> * kQ4Slots * 8, kMergeRow = HD + 8,  // floats; the pads keep rows on different banks
+                         kQuery = kMerge + kQ4Warps<HD, HPL> * 4 * HPL * (kMergeRow + 2) * 4, kQueryRow = HD + 8,  // halves
         kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kBack = kSums + 2 * 4 * HPL * 4 * 2, kAll = kBack + 4 * HPL * 4;
 };
 
 template <int HD, int HPL, bool TRACK>
-__global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
-    constexpr int NG = HD / kQ4Group, NW = NG / 2, BLOCK = 20 * HD, TILE = kQ4Tile * BLOCK, W = kQ4Warps<HPL>, HEADS = 4 * HPL;
+__global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
+    constexpr int NG = HD / kQ4Group, NW = NG / 2, BLOCK = 20 * HD, TILE = kQ4Tile * BLOCK, W = kQ4Warps<HD, HPL>, HEADS = 4 * HPL;
     using Smem = Q4Smem<HD, HPL>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t = lane & 3;
     const int kvh = blockIdx.x % p.n_kv_heads, share = blockIdx.x / p.n_kv_heads, G = p.n_heads / p.n_kv_heads, h0 = kvh * G;
     const uint32_t ring = smem_u32(smem) + warp * kQ4Slots * TILE, bars = smem_u32(smem) + Smem::kBars + warp * kQ4Slots * 8;
-    float *mg_o = reinterpret_cast<float *>(smem + Smem::kMerge);  // where the warps meet: [warp][head][HD], [warp][head], [warp][head]
-    float *mg_m = mg_o + W * G * HD, *mg_l = mg_m + W * G;
+    float *mg_o = reinterpret_cast<float *>(smem + Smem::kMerge);  // where the warps meet: [warp][head][kMergeRow], [warp][head], [warp][head]
+    float *mg_m = mg_o + W * G * Smem::kMergeRow, *mg_l = mg_m + W * G;
     __half *q_s = reinterpret_cast<__half *>(smem + Smem::kQuery);    // [limb][head][kQueryRow]
     __half *sums_s = reinterpret_cast<__half *>(smem + Smem::kSums);  // [limb][head][4]: the query's sums over groups, scaled
     float *back_s = reinterpret_cast<float *>(smem + Smem::kBack);    // [head]: what takes the scale of the scores back
     int row_a = -1, row_b = -1;             // rows that other shares have parts of, too: the first, the last
     unsigned before_a = 0u, before_b = 0u;  // thread 0: their parts that were done before
     if (lane == 0) {
-        for (int s = 0; s < kQ4Slots; s++) mbar_init(bars + s * 8, 1);
+        for (int s = 0; s < kQ4Slots; s++) mbar_init(bars + s * 8, kQ4Tile);  // an arrival for each page of a tile
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
     }
     __syncwarp();
     pdl_launch_dependents();
-    pdl_wait();
     const uint8_t *plane = p.pool + ((size_t)p.layer * p.n_pages * p.n_kv_heads + kvh) * BLOCK;
     const size_t page_bytes = (size_t)p.n_kv_heads * BLOCK;
     const uint64_t policy = l2_evict_first_policy();
@@ -134,25 +133,23 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
     unsigned issued = 0, used = 0;  // tiles through this warp's ring
     bool failed = false;
 
-    // The part that is copied: its pages in the row's table, and how many of its tiles are this warp's and under way.  The places of 16 tiles' pages wait in the
-    // lanes, the next 16 are asked for ahead.
-    int row, part_tiles = 0, part_issued = 0, places = 0, places_next = 0, part_pages = 0;
+    // The part that is copied: its pages in the row's table, and how many of its tiles are this warp's and under way.  The places of 16 tiles' pages (in 16 bytes
+    // from `plane`) wait in the lanes, which copy them when it is their turn; the next 16 are asked for ahead.
+    constexpr uint32_t kNone = 0xffffffffu;
+    int row, part_tiles = 0, part_issued = 0, part_pages = 0;
+    uint32_t places = kNone, places_next = kNone;
     CacheRow r;
     const int32_t *table = nullptr;
     int page0 = 0;
     auto place = [&](int tile) {  // of this lane's page among the 16 tiles from `tile`
         const int pg = kQ4Tile * (warp + W * (tile + (lane >> 1))) + (lane & 1);
-        return pg < part_pages ? table[pg] : 0;
+        return pg < part_pages ? (uint32_t)table[pg] * (uint32_t)(page_bytes >> 4) : kNone;
     };
     auto issue = [&] {
-        const int at = (part_issued & 15) * 2;
-        const int a = __shfl_sync(0xffffffffu, places, at), b = __shfl_sync(0xffffffffu, places, at + 1);
-        if (lane == 0) {
-            const uint32_t slot = issued % kQ4Slots, bar = bars + slot * 8, to = ring + slot * TILE;
-            const bool two = kQ4Tile * (warp + W * part_issued) + 1 < part_pages;
-            mbar_expect_tx(bar, two ? TILE : BLOCK);
-            bulk_g2s(to, plane + a * page_bytes, BLOCK, bar, policy);
-            if (two) bulk_g2s(to + BLOCK, plane + b * page_bytes, BLOCK, bar, policy);
+        if ((lane >> 1) == (part_issued & 15)) {
+            const uint32_t slot = issued % kQ4Slots, bar = bars + slot * 8;
+            mbar_expect_tx(bar, places == kNone ? 0 : BLOCK);  // a part that ends within a tile: no copy
+            if (places != kNone) bulk_g2s(ring + slot * TILE + (lane & 1) * BLOCK, plane + (uint64_t)places * 16, BLOCK, bar, policy);
         }
         issued++;
         if ((++part_issued & 15) == 0) {
@@ -182,7 +179,11 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
         places_next = place(16);
         while (part_issued < min(part_tiles, kQ4Slots)) issue();
     };
-    if (share0 < share1) begin(cache_find(p.rows, share0), share0);
+    // Rows that came with the launch are there before the kernels ahead are done; nothing else is.
+    if (p.rows.far) pdl_wait();
+    const int row_first = cache_find(p.rows, min(share0, p.total - 1));
+    pdl_wait();
+    if (share0 < share1) begin(row_first, share0);
 
     int from = share0;
     while (from < share1) {
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
                     const float *c = &o[g][x >> 1][2 * (x & 1)];
                     v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], x & 1 ? unscale * 0.0625f : unscale, offset[h][g]);
                 }
-                *reinterpret_cast<float4 *>(mg_o + ((size_t)warp * G + head) * HD + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(mg_o + (warp * G + head) * Smem::kMergeRow + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
             }
             if (g8 == 0) {
                 mg_m[warp * G + head] = m_run[h];
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kQ4Warps<HPL> * 32, kQ4Ctas<HPL>) q4_attn_kern
 #pragma unroll
             for (int w = 0; w < W; w++) {
                 const float f = __shfl_sync(0xffffffffu, fw, w);
-                const float2 v = *reinterpret_cast<const float2 *>(mg_o + ((size_t)w * G + g) * HD + d);
+                const float2 v = *reinterpret_cast<const float2 *>(mg_o + (w * G + g) * Smem::kMergeRow + d);
                 if (f != 0.f) {
                     ax = fmaf(v.x, f, ax);
                     ay = fmaf(v.y, f, ay);
@@ -633,7 +634,7 @@ static int launch_q4_attn(const Q4AttnParams &a, int shares, cudaStream_t st) {
         JUNO_CUDA_TRY(cudaFuncSetAttribute(q4_attn_kernel<HD, HPL, TRACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD, HPL>::kAll));
         set[dev & 63] = true;
     }
-    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL, TRACK>, dim3((unsigned)(shares * a.n_kv_heads)), dim3(kQ4Warps<HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
+    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL, TRACK>, dim3((unsigned)(shares * a.n_kv_heads)), dim3(kQ4Warps<HD, HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
     return JUNO_OK;
 }
 
@@ -671,7 +672,8 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
         JUNO_REQUIRE(pages < (1 << 27), "attention over %lld pages in one call", (long long)pages);
     }
     // One share for every CTA that the GPU holds at a time, so that all end together; none below a tile for each warp.
-    const int warps = G <= 4 ? kQ4Warps<1> : kQ4Warps<2>, ctas = G <= 4 ? kQ4Ctas<1> : kQ4Ctas<2>;
+    const bool wide = G > 4 && hd == 128;
+    const int warps = wide ? kQ4Warps<128, 2> : kQ4Warps<64, 2>, ctas = wide ? kQ4Ctas<128, 2> : kQ4Ctas<64, 2>;
     const int64_t slots = std::max(1, c->sm_count * ctas / H);
     const int share = (int)std::max<int64_t>(warps * kQ4Tile, (pages + slots - 1) / slots);
     const int shares = (int)((pages + share - 1) / share);
