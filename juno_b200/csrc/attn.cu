@@ -1389,7 +1389,7 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     const unsigned blocks = (unsigned)((total + 255) / 256);
     const int32_t *row = p->d_table + (size_t)s->slot * p->max_pages_per_seq;
     if (p->dtype == kKvQ4) {
-        const CacheRow r{s->slot, pos, 0, s->track};
+        const CacheRow r{s->slot, pos, 0, s->track, 0};
         JUNO_TRY(launch_kv_append(c, p, layer, &r, 1, n_tokens, c->stage_x, c->stage_y, kvdim, c->stream));
     } else if (p->dtype == 0)
         kv_scatter_kernel<__half><<<blocks, 256, 0, c->stream>>>(p->k, p->v, row, p->n_pages, p->n_kv_heads, p->head_dim,

@@ -90,8 +90,8 @@ int cache_rows(juno_ctx *c, const CacheRow *rows, int n, CacheRow *far, CacheRow
         return JUNO_OK;
     }
     out->far = far;
-    static_assert(sizeof(CacheRow) == 4 * sizeof(int32_t), "rows travel as words");
-    return cache_words(c, reinterpret_cast<const int32_t *>(rows), (size_t)n * 4, reinterpret_cast<int32_t *>(far), st);
+    constexpr size_t kWords = sizeof(CacheRow) / sizeof(int32_t);
+    return cache_words(c, reinterpret_cast<const int32_t *>(rows), (size_t)n * kWords, reinterpret_cast<int32_t *>(far), st);
 }
 
 // ───────────────────────────── append and read ────────────────────────────────────────────
@@ -685,7 +685,7 @@ static int token_rows(int n, juno_seq *const *seqs, const int32_t *positions, co
     for (int i = 0; i < n; i++) {
         JUNO_REQUIRE(positions[i] >= 0 && counts[i] >= 0, "bad position range of sequence %d", i);
         if (counts[i] == 0) continue;
-        rows->push_back({seqs[i]->slot, positions[i], (int)sum, seqs[i]->track});
+        rows->push_back({seqs[i]->slot, positions[i], (int)sum, seqs[i]->track, 0});
         sum += counts[i];
     }
     JUNO_REQUIRE(sum <= (1 << 24), "%lld positions in one call", (long long)sum);
@@ -772,7 +772,7 @@ int juno_kv_weights_device(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n
         for (int i = 0; i < n; i++) {
             JUNO_REQUIRE(seqs[i]->track >= 0, "sequence %d keeps no weights (juno_seq_track)", i);
             JUNO_REQUIRE(counts[i] >= 0 && counts[i] <= seqs[i]->len, "sequence %d has %d cached positions, not %d", i, seqs[i]->len, counts[i]);
-            rows.push_back({seqs[i]->slot, counts[i], i, seqs[i]->track});
+            rows.push_back({seqs[i]->slot, counts[i], i, seqs[i]->track, 0});
             most = std::max(most, counts[i]);
         }
         JUNO_REQUIRE(ld >= most, "rows of %lld weights hold no %d", (long long)ld, most);

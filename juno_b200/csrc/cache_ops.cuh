@@ -14,6 +14,7 @@ struct CacheRow {
     int upto;   // append, read: first position; attention: positions to attend
     int first;  // the row's first unit of work among those of all rows (cached position of the call, context split): ascending
     int track;  // weight plane, -1 = none
+    int share;  // attention: the share of the work that has the row's first page
 };
 constexpr int kInlineRows = 64;
 struct CacheRows {

@@ -11,32 +11,37 @@
 
 namespace juno {
 
-// A row's pages are cut into parts of about equal length, a CTA for each part and key/value head; whoever of a row is done last puts its parts together.
+// The pages of all rows follow one another (a row without positions counts as one page) and are cut into shares; a CTA takes one share of one key/value
+// head, which may hold the end of a row, whole ones and the beginning of another.  What a share has of a row is a part: its number, row + share, is different
+// for each (along the cut, each part has a later row or share than the one before), and a row's parts follow one another.
+constexpr int kInlineCuts = 160;
 struct Q4AttnParams {
-    CacheRows rows;  // first: the row's first part among those of all rows
+    CacheRows rows;  // first: the row's first page among those of all rows; share: the share that has it
+    const int32_t *far_cuts;  // null: `cuts`
+    int cuts[kInlineCuts];    // share w has the pages [cuts[w], cuts[w + 1])
     const uint8_t *pool;
     const int32_t *table;
     int max_pages_per_seq, n_pages, n_kv_heads, n_heads, layer, n_layers;
-    int n_parts, longest;  // parts of all rows, most pages of one
+    int total, shares;  // pages of all rows
     const float *q;
     int64_t ldq, ldo;
     float *out;
     float *part_o, *part_ml;  // [part][head][hd], [part][head][max, sum]
     float2 *sums;             // sequences that keep weights: [row][head] largest score of all, 1 / sum
     unsigned *arrived;        // [row][kv_head]: parts that are done, zero between launches
-    float *scores;            // sequences that keep weights: [kv_head][part][longest * 16][G], log2 domain
+    float *scores;            // sequences that keep weights: [kv_head][position of all rows' pages][G], log2 domain
     float *weights;
     int track_tokens;
     unsigned *err;
 };
 
-// Part `id` of row `i`: how many the row has, and which pages of the row it is.
-struct Q4Part {
-    int parts, page0, page1;
-};
-__device__ __forceinline__ Q4Part part_of(const Q4AttnParams &p, const CacheRow &r, int i, int id) {
-    const int parts = (i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : p.n_parts) - r.first, k = id - r.first, pages = (r.upto + kPageTokens - 1) / kPageTokens;
-    return {parts, k * pages / parts, (k + 1) * pages / parts};
+__device__ __forceinline__ int row_end(const Q4AttnParams &p, int i) { return i + 1 < p.rows.n ? cache_row(p.rows, i + 1).first : p.total; }
+__device__ __forceinline__ int cut_at(const Q4AttnParams &p, int w) { return p.far_cuts ? p.far_cuts[w] : p.cuts[w]; }
+// How many parts row i has: up to the share that the next row begins in, which has some of this one unless it begins with that one.
+__device__ __forceinline__ int row_parts(const Q4AttnParams &p, int i, const CacheRow &r) {
+    if (i + 1 >= p.rows.n) return p.shares - r.share;
+    const CacheRow next = cache_row(p.rows, i + 1);
+    return next.share - r.share + (cut_at(p, next.share) < next.first);
 }
 
 constexpr int kQ4MaxGroup = 8, kQ4Slots = 2, kQ4Tile = 2;  // pages of a tile: a warp's step
@@ -90,7 +95,8 @@ __device__ __forceinline__ float step_of(const uint32_t *words, int g) { return 
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
 __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
-// A part's pages are tiles of two, spread over the warps; each warp has a ring of kQ4Slots tiles that bulk copies fill.  Per page
+// A share's pages of one row are tiles of two pages, spread over four warps; each warp has a ring of kQ4Slots tiles that bulk copies fill, the next row's first
+// tiles already while this one's results are put together.  Per page
 //   S = K Q   m16n8k16: the 16 positions are the rows, a group's 32 dimensions the k of two MMAs, the columns query heads.  The numbers are not converted: in
 //             the low bits of a half they are the subnormal q 2^-24, in the next four 16 q 2^-24, which the query's side takes back; two ANDs
 //             and half a shift make a register.  A group's result is multiplied by its step d in FP32 and the offset's part, m times the sum of the query
@@ -113,389 +119,446 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
     using Smem = Q4Smem<HD, HPL>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t = lane & 3;
-    const int kvh = blockIdx.x % p.n_kv_heads, id = blockIdx.x / p.n_kv_heads, G = p.n_heads / p.n_kv_heads, h0 = kvh * G;
+    const int kvh = blockIdx.x % p.n_kv_heads, share = blockIdx.x / p.n_kv_heads, G = p.n_heads / p.n_kv_heads, h0 = kvh * G;
     const uint32_t ring = smem_u32(smem) + warp * kQ4Slots * TILE, bars = smem_u32(smem) + Smem::kBars + warp * kQ4Slots * 8;
     float *mg_o = reinterpret_cast<float *>(smem + Smem::kMerge);  // where the warps meet: [warp][head][kMergeRow], [warp][head], [warp][head]
     float *mg_m = mg_o + W * G * Smem::kMergeRow, *mg_l = mg_m + W * G;
     __half *q_s = reinterpret_cast<__half *>(smem + Smem::kQuery);    // [limb][head][kQueryRow]
     __half *sums_s = reinterpret_cast<__half *>(smem + Smem::kSums);  // [limb][head][4]: the query's sums over groups, scaled
     float *back_s = reinterpret_cast<float *>(smem + Smem::kBack);    // [head]: what takes the scale of the scores back
+    int row_a = -1, row_b = -1;             // rows that other shares have parts of, too: the first, the last
+    unsigned before_a = 0u, before_b = 0u;  // thread 0: their parts that were done before
     if (lane == 0) {
         for (int s = 0; s < kQ4Slots; s++) mbar_init(bars + s * 8, kQ4Tile);  // an arrival for each page of a tile
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async;" ::: "memory");
     }
     __syncwarp();
+    pdl_launch_dependents();
+    // What came with the launch is there before the kernels ahead are done; nothing else is.
+    if (p.rows.far || p.far_cuts) pdl_wait();
+    const int share0 = cut_at(p, share), share1 = cut_at(p, share + 1), row_first = cache_find(p.rows, share0);
     const uint8_t *plane = p.pool + ((size_t)p.layer * p.n_pages * p.n_kv_heads + kvh) * BLOCK;
     const size_t page_bytes = (size_t)p.n_kv_heads * BLOCK;
     const uint64_t policy = l2_evict_first_policy();
     const uint32_t v_piece = q4_v_code(HD, lane & 15, 0, lane >> 4);  // this lane's row of the four matrices of groups 0 and 1; two groups on: 32 bytes flipped
-    pdl_launch_dependents();
-    // Rows that came with the launch are there before the kernels ahead are done; nothing else is.
-    if (p.rows.far) pdl_wait();
-    const int i = cache_find(p.rows, id);
-    const CacheRow r = cache_row(p.rows, i);
-    const Q4Part part = part_of(p, r, i, id);
-    const int pos_end = min(r.upto, part.page1 << 4), part_pages = part.page1 - part.page0, tiles = (part_pages + kQ4Tile - 1) / kQ4Tile;
-    const int n_tiles = tiles > warp ? (tiles - warp + W - 1) / W : 0;  // of this warp
-    const bool track = TRACK && r.track >= 0;
-    pdl_wait();
-    // The places of 16 tiles' pages (in 16 bytes from `plane`) wait in the lanes, which copy them when it is their turn; the next 16 are asked for ahead.
+    unsigned issued = 0, used = 0;  // tiles through this warp's ring
+    bool failed = false;
+
+    // The part that is copied: its pages in the row's table, and how many of its tiles are this warp's and under way.  The places of 16 tiles' pages (in 16 bytes
+    // from `plane`) wait in the lanes, which copy them when it is their turn; the next 16 are asked for ahead.
     constexpr uint32_t kNone = 0xffffffffu;
-    const int32_t *table = p.table + (size_t)r.slot * p.max_pages_per_seq + part.page0;
+    int row, part_tiles = 0, part_issued = 0, part_pages = 0;
+    uint32_t places = kNone, places_next = kNone;
+    CacheRow r;
+    const int32_t *table = nullptr;
+    int page0 = 0;
     auto place = [&](int tile) {  // of this lane's page among the 16 tiles from `tile`
         const int pg = kQ4Tile * (warp + W * (tile + (lane >> 1))) + (lane & 1);
         return pg < part_pages ? (uint32_t)table[pg] * (uint32_t)(page_bytes >> 4) : kNone;
     };
-    uint32_t places = place(0), places_next = place(16);
-    int issued = 0, used = 0;
-    bool failed = false;
     auto issue = [&] {
-        if ((lane >> 1) == (issued & 15)) {
+        if ((lane >> 1) == (part_issued & 15)) {
             const uint32_t slot = issued % kQ4Slots, bar = bars + slot * 8;
             mbar_expect_tx(bar, places == kNone ? 0 : BLOCK);  // a part that ends within a tile: no copy
             if (places != kNone) bulk_g2s(ring + slot * TILE + (lane & 1) * BLOCK, plane + (uint64_t)places * 16, BLOCK, bar, policy);
         }
-        if ((++issued & 15) == 0) {
+        issued++;
+        if ((++part_issued & 15) == 0) {
             places = places_next;
-            places_next = place(issued + 16);
+            places_next = place(part_issued + 16);
         }
     };
-    while (issued < min(n_tiles, kQ4Slots)) issue();
+    constexpr int E = HD / 32, QUERIES = (HEADS + W - 1) / W;  // elements of a lane, heads of a warp
+    float query[QUERIES][E];
+    auto begin = [&](int i, int from) {  // row i from page `from` of all pages
+        row = i;
+#pragma unroll
+        for (int n = 0; n < QUERIES; n++) {
+            const int head = warp + n * W;
+            const float *src = p.q + (size_t)i * p.ldq + (size_t)(h0 + head) * HD + E * lane;
+#pragma unroll
+            for (int e = 0; e < E; e++) query[n][e] = head < G ? src[e] : 0.f;
+        }
+        r = cache_row(p.rows, i);
+        page0 = from - r.first;
+        part_pages = r.upto > 0 ? min(share1, row_end(p, i)) - from : 0;
+        table = p.table + (size_t)r.slot * p.max_pages_per_seq + page0;
+        const int tiles = (part_pages + kQ4Tile - 1) / kQ4Tile;
+        part_tiles = tiles > warp ? (tiles - warp + W - 1) / W : 0;
+        part_issued = 0;
+        places = place(0);
+        places_next = place(16);
+        while (part_issued < min(part_tiles, kQ4Slots)) issue();
+    };
+    pdl_wait();
+    begin(row_first, share0);
 
-    // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
-    // largest element), in two FP16 limbs.  Elements 2, 3, 6, 7 of eight meet 16 q.
-    constexpr int E = HD / 32;  // elements of a lane
-    for (int head = warp; head < HEADS; head += W) {
-        const float scale = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
-        const float *src = p.q + (size_t)i * p.ldq + (size_t)(h0 + head) * HD + E * lane;
-        float y[E], top = 0.f, sum = 0.f;
+    int from = share0;
+    while (from < share1) {
+        const int i = row, to = min(share1, row_end(p, i)), n_tiles = part_tiles, pos_first = page0 << 4;
+        const int pos_end = min(r.upto, (to - r.first) << 4);  // of this part, in the row
+        const bool track = TRACK && r.track >= 0;
+        // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
+        // largest element), in two FP16 limbs.  Elements 2, 3, 6, 7 of eight meet 16 q.
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            y[e] = head < G ? src[e] * scale : 0.f;
-            sum += y[e];
-            top = fmaxf(top, fabsf(y[e]));
-        }
+        for (int n = 0; n < QUERIES; n++) {
+            const int head = warp + n * W;
+            if (head >= HEADS) break;
+            const float scale = (float)(1.0 / sqrt((double)HD)) * 1.4426950408889634f;
+            float y[E], top = 0.f, sum = 0.f;
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            if (x < kQ4Group / E) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        }
-        const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127)), up = 13 - e2;
-        const float shift = __uint_as_float((uint32_t)(127 + up) << 23);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float s = (E * lane + e) & 2 ? shift * 0.0625f : shift, y0 = y[e] * s, y1 = y[e + 1] * s;
-            const uint32_t hi = pack_h2(y0, y1);
-            const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-            uint32_t *to_q = reinterpret_cast<uint32_t *>(q_s + head * Smem::kQueryRow + E * lane + e);
-            to_q[0] = hi;
-            to_q[HEADS * Smem::kQueryRow / 2] = pack_h2(y0 - hf.x, y1 - hf.y);
-        }
-        if (lane % (kQ4Group / E) == 0) {  // 32 elements of up to 2^14: five powers of two less
-            const float whole = sum * (shift * 0.03125f);
-            const __half hi = __float2half_rn(whole);
-            sums_s[head * 4 + lane / (kQ4Group / E)] = hi;
-            sums_s[(HEADS + head) * 4 + lane / (kQ4Group / E)] = __float2half_rn(whole - __half2float(hi));
-        }
-        if (lane == 0) back_s[head] = __uint_as_float((uint32_t)(127 + 5 - up) << 23);
-    }
-    __syncthreads();
-    // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8, as the B operand wants them
-    uint32_t qh[NG][4], ql[HPL == 2 ? NG : 1][4];
-    uint32_t qsum[HPL];  // k: the groups
-    float back[HPL];     // of this lane's own heads
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const __half *from_q = q_s + (HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : g8) * Smem::kQueryRow + g * kQ4Group + 8 * t;
-        lds_words<4>(qh[g], smem_u32(from_q));
-        if constexpr (HPL == 2) lds_words<4>(ql[g], smem_u32(from_q + HEADS * Smem::kQueryRow));
-    }
-#pragma unroll
-    for (int h = 0; h < HPL; h++) {
-        const int column = HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : h * HEADS + g8;  // HPL = 2: h is the limb
-        qsum[h] = t < NW ? *reinterpret_cast<const uint32_t *>(sums_s + column * 4 + 2 * t) : 0u;
-        back[h] = back_s[HPL * t + h];
-    }
-    float o[NG][2][4], oo[4] = {0.f, 0.f, 0.f, 0.f}, m_run[HPL], l_run[HPL], vscale = 0.f;  // oo: the offsets' part, row g8 = group
-    uint32_t limit = 0;  // largest step in the scale's range, in both halves
-#pragma unroll
-    for (int g = 0; g < NG; g++)
-#pragma unroll
-        for (int x = 0; x < 4; x++) o[g][0][x] = o[g][1][x] = 0.f;
-#pragma unroll
-    for (int h = 0; h < HPL; h++) {
-        m_run[h] = -INFINITY;
-        l_run[h] = 0.f;
-    }
-    constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    int pos0 = (part.page0 + warp * kQ4Tile) << 4;
-    for (int j = 0; j < n_tiles; j++, pos0 += W * kQ4Tile * kPageTokens) {
-        mbar_wait_bounded(bars + j % kQ4Slots * 8, ring_parity(j, kQ4Slots), 0, p.err, failed, kErrCacheWait);
-        if (__any_sync(0xffffffffu, failed)) {
-            failed = true;
-            break;
-        }
-        const uint32_t tile = ring + j % kQ4Slots * TILE;
-        used = j + 1;
-        float s[HPL][kQ4Tile][2];  // rows g8 and g8 + 8 of each page
-#pragma unroll
-        for (int u = 0; u < kQ4Tile; u++) {
-            const uint32_t base = tile + u * BLOCK;
-            uint32_t k0[NG], k1[NG], d0[NW], d1[NW], m0[1], m1[1];
-            lds_words<NG>(k0, base + lane * NG * 4);
-            lds_words<NG>(k1, base + (32 + lane) * NG * 4);
-            lds_words<NW>(d0, base + 8 * HD + g8 * NG * 2);
-            lds_words<NW>(d1, base + 8 * HD + (g8 + 8) * NG * 2);
-            lds_words<1>(m0, base + 9 * HD + g8 * NG * 2 + (t % NW) * 4);  // k beyond the groups: once more, times the zeros of qsum
-            lds_words<1>(m1, base + 9 * HD + (g8 + 8) * NG * 2 + (t % NW) * 4);
-            float off[4], sum[HPL][2];
-            mma_f16_first(off, m0[0], m1[0], 0u, 0u, qsum[0], 0u);
-            if constexpr (HPL == 1) {
-                off[0] += off[1];
-                off[1] = off[2] + off[3];
-            } else {
-                mma_f16(off, m0[0], m1[0], 0u, 0u, qsum[1], 0u);
+            for (int e = 0; e < E; e++) {
+                y[e] = query[n][e] * scale;
+                sum += y[e];
+                top = fmaxf(top, fabsf(y[e]));
             }
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                float c[4];
-                const uint32_t x0 = k0[g] >> 8, x1 = k1[g] >> 8;
-                mma_f16_first(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, qh[g][0], qh[g][1]);
-                mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, qh[g][2], qh[g][3]);
+            for (int x = 1; x < 32; x <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                if (x < kQ4Group / E) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            }
+            const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127)), up = 13 - e2;
+            const float shift = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float s = (E * lane + e) & 2 ? shift * 0.0625f : shift, y0 = y[e] * s, y1 = y[e + 1] * s;
+                const uint32_t hi = pack_h2(y0, y1);
+                const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                uint32_t *to_q = reinterpret_cast<uint32_t *>(q_s + head * Smem::kQueryRow + E * lane + e);
+                to_q[0] = hi;
+                to_q[HEADS * Smem::kQueryRow / 2] = pack_h2(y0 - hf.x, y1 - hf.y);
+            }
+            if (lane % (kQ4Group / E) == 0) {  // 32 elements of up to 2^14: five powers of two less
+                const float whole = sum * (shift * 0.03125f);
+                const __half hi = __float2half_rn(whole);
+                sums_s[head * 4 + lane / (kQ4Group / E)] = hi;
+                sums_s[(HEADS + head) * 4 + lane / (kQ4Group / E)] = __float2half_rn(whole - __half2float(hi));
+            }
+            if (lane == 0) back_s[head] = __uint_as_float((uint32_t)(127 + 5 - up) << 23);
+        }
+        __syncthreads();
+        // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8, as the B operand wants them
+        uint32_t qh[NG][4], ql[HPL == 2 ? NG : 1][4];
+        uint32_t qsum[HPL];  // k: the groups
+        float back[HPL];     // of this lane's own heads
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const __half *from_q = q_s + (HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : g8) * Smem::kQueryRow + g * kQ4Group + 8 * t;
+            lds_words<4>(qh[g], smem_u32(from_q));
+            if constexpr (HPL == 2) lds_words<4>(ql[g], smem_u32(from_q + HEADS * Smem::kQueryRow));
+        }
+#pragma unroll
+        for (int h = 0; h < HPL; h++) {
+            const int column = HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : h * HEADS + g8;  // HPL = 2: h is the limb
+            qsum[h] = t < NW ? *reinterpret_cast<const uint32_t *>(sums_s + column * 4 + 2 * t) : 0u;
+            back[h] = back_s[HPL * t + h];
+        }
+        float o[NG][2][4], oo[4] = {0.f, 0.f, 0.f, 0.f}, m_run[HPL], l_run[HPL], vscale = 0.f;  // oo: the offsets' part, row g8 = group
+        uint32_t limit = 0;  // largest step in the scale's range, in both halves
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[g][0][x] = o[g][1][x] = 0.f;
+#pragma unroll
+        for (int h = 0; h < HPL; h++) {
+            m_run[h] = -INFINITY;
+            l_run[h] = 0.f;
+        }
+        constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+        int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
+        for (int j = 0; j < n_tiles; j++, pos0 += W * kQ4Tile * kPageTokens) {
+            mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
+            if (__any_sync(0xffffffffu, failed)) {
+                failed = true;
+                break;
+            }
+            const uint32_t tile = ring + used % kQ4Slots * TILE;
+            used++;
+            float s[HPL][kQ4Tile][2];  // rows g8 and g8 + 8 of each page
+#pragma unroll
+            for (int u = 0; u < kQ4Tile; u++) {
+                const uint32_t base = tile + u * BLOCK;
+                uint32_t k0[NG], k1[NG], d0[NW], d1[NW], m0[1], m1[1];
+                lds_words<NG>(k0, base + lane * NG * 4);
+                lds_words<NG>(k1, base + (32 + lane) * NG * 4);
+                lds_words<NW>(d0, base + 8 * HD + g8 * NG * 2);
+                lds_words<NW>(d1, base + 8 * HD + (g8 + 8) * NG * 2);
+                lds_words<1>(m0, base + 9 * HD + g8 * NG * 2 + (t % NW) * 4);  // k beyond the groups: once more, times the zeros of qsum
+                lds_words<1>(m1, base + 9 * HD + (g8 + 8) * NG * 2 + (t % NW) * 4);
+                float off[4], sum[HPL][2];
+                mma_f16_first(off, m0[0], m1[0], 0u, 0u, qsum[0], 0u);
                 if constexpr (HPL == 1) {
-                    c[0] += c[1];
-                    c[1] = c[2] + c[3];
+                    off[0] += off[1];
+                    off[1] = off[2] + off[3];
                 } else {
-                    mma_f16(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, ql[g][0], ql[g][1]);
-                    mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, ql[g][2], ql[g][3]);
+                    mma_f16(off, m0[0], m1[0], 0u, 0u, qsum[1], 0u);
                 }
 #pragma unroll
-                for (int h = 0; h < HPL; h++) {
-                    sum[h][0] = g ? fmaf(step_of(d0, g), c[h], sum[h][0]) : step_of(d0, g) * c[h];
-                    sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
+                for (int g = 0; g < NG; g++) {
+                    float c[4];
+                    const uint32_t x0 = k0[g] >> 8, x1 = k1[g] >> 8;
+                    mma_f16_first(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, qh[g][0], qh[g][1]);
+                    mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, qh[g][2], qh[g][3]);
+                    if constexpr (HPL == 1) {
+                        c[0] += c[1];
+                        c[1] = c[2] + c[3];
+                    } else {
+                        mma_f16(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, ql[g][0], ql[g][1]);
+                        mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, ql[g][2], ql[g][3]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < HPL; h++) {
+                        sum[h][0] = g ? fmaf(step_of(d0, g), c[h], sum[h][0]) : step_of(d0, g) * c[h];
+                        sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
+                    }
                 }
+                // 2^24 of the numbers, 2^-up; the sums' 2^5 2^-up
+#pragma unroll
+                for (int h = 0; h < HPL; h++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 524288.f, off[x * HPL + h]) * back[h];
             }
-            // 2^24 of the numbers, 2^-up; the sums' 2^5 2^-up
+            if (track) {
+                float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
 #pragma unroll
-            for (int h = 0; h < HPL; h++)
+                for (int h = 0; h < HPL; h++)
 #pragma unroll
-                for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 524288.f, off[x * HPL + h]) * back[h];
-        }
-        if (track) {
-            float *to_s = p.scores + (((size_t)kvh * p.n_parts + id) * p.longest * kPageTokens + pos0 - part.page0 * kPageTokens + g8) * G;
+                    for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
-            for (int h = 0; h < HPL; h++)
-#pragma unroll
-                for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-                        if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
-        }
-        uint32_t d[kQ4Tile][2][NW], m[kQ4Tile][2], steps = limit;
-#pragma unroll
-        for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
-                uint32_t one[1];
-                lds_words<1>(one, tile + u * BLOCK + 19 * HD + (g8 % NG) * 32 + x * 16 + t * 4);  // rows beyond the groups: again, and not looked at
-                m[u][x] = one[0];
+                        for (int x = 0; x < 2; x++)
+                            if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
             }
-        if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
+            uint32_t d[kQ4Tile][2][NW], m[kQ4Tile][2], steps = limit;
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const int at = pos0 + 16 * u + 8 * x;
-                    const bool on = at + g8 < pos_end;
-#pragma unroll
-                    for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
-#pragma unroll
-                    for (int g = 0; g < NW; g++) d[u][x][g] = on ? d[u][x][g] : 0u;
-                    m[u][x] &= (at + 2 * t < pos_end ? 0xffffu : 0u) | (at + 2 * t + 1 < pos_end ? 0xffff0000u : 0u);
+                    lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
+                    uint32_t one[1];
+                    lds_words<1>(one, tile + u * BLOCK + 19 * HD + (g8 % NG) * 32 + x * 16 + t * 4);  // rows beyond the groups: again, and not looked at
+                    m[u][x] = one[0];
                 }
-        }
+            if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
 #pragma unroll
-        for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-            for (int g = 0; g < NW; g++) steps = __vmaxu2(steps, __vmaxu2(d[u][0][g], d[u][1][g]));
-        // a score far above the reference, or a step beyond the scale's range: seldom after the first tile
-        float top[HPL];
-        bool grown = steps != limit;
-#pragma unroll
-        for (int h = 0; h < HPL; h++) {
-            top[h] = s[h][0][0];
-#pragma unroll
-            for (int u = 0; u < kQ4Tile; u++) top[h] = fmaxf(fmaxf(top[h], s[h][u][0]), s[h][u][1]);
-            grown |= top[h] > m_run[h] + 8.f;
-        }
-        if (__any_sync(0xffffffffu, grown)) {
-            float fix[HPL], vfix = 1.f;
-            steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
-            if (steps > (limit & 0xffffu)) {  // the largest step to 2^2 .. 2^3, up to 2^7 in range: times weights of up to 2^8
-                const int e = max((int)(steps >> 7) - 127, -100);
-                const float next = __uint_as_float((uint32_t)(127 + 2 - e) << 23);
-                vfix = vscale == 0.f ? 0.f : next / vscale;
-                vscale = next;
-                limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
-            }
-#pragma unroll
-            for (int h = 0; h < HPL; h++) {
-                float mx = fmaxf(m_run[h], top[h]);
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
-                m_run[h] = mx;
-                l_run[h] *= fix[h];
-            }
-#pragma unroll
-            for (int x = 0; x < 4; x++) oo[x] *= fix[HPL == 1 ? 0 : x & 1];
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const float y = fix[HPL == 1 ? 0 : x & 1] * vfix;
-                    o[g][0][x] *= y;
-                    o[g][1][x] *= y;
-                }
-        }
-#pragma unroll
-        for (int u = 0; u < kQ4Tile; u++) {
-            uint32_t v0[NG], v1[NG];  // unit g8 of positions 2t, 2t + 1, and of those eight farther
-#pragma unroll
-            for (int g = 0; g < NG; g += 2) ldmatrix_x4_trans(v0[g], v1[g], v0[g + 1], v1[g + 1], tile + u * BLOCK + (g == 0 ? v_piece : v_piece ^ 32u));
-            float w[HPL][2], ws[HPL][2];
-#pragma unroll
-            for (int h = 0; h < HPL; h++) {
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
-                    ws[h][x] = w[h][x] * vscale;
-                }
-                l_run[h] += w[h][0] + w[h][1];
-            }
-            // group -1: the weights alone, for the offsets
-#pragma unroll
-            for (int g = -1; g < NG; g++) {
-                float hi[HPL][2], lo[HPL][2];
-#pragma unroll
-                for (int h = 0; h < HPL; h++)
+                for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const float y = g < 0 ? w[h][x] : ws[h][x] * step_of(d[u][x], g < 0 ? 0 : g);
-                        hi[h][x] = upper_limb(y);
-                        lo[h][x] = y - hi[h][x];
-                    }
+                        const int at = pos0 + 16 * u + 8 * x;
+                        const bool on = at + g8 < pos_end;
 #pragma unroll
-                for (int limb = 0; limb < HPL; limb++) {
-                    uint32_t b0, b1;
-                    if constexpr (HPL == 1) {
-                        b0 = transpose8(pack_h2(hi[0][0], lo[0][0]));
-                        b1 = transpose8(pack_h2(hi[0][1], lo[0][1]));
-                    } else {
-                        b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
-                        b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
+                        for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
+#pragma unroll
+                        for (int g = 0; g < NW; g++) d[u][x][g] = on ? d[u][x][g] : 0u;
+                        m[u][x] &= (at + 2 * t < pos_end ? 0xffffu : 0u) | (at + 2 * t + 1 < pos_end ? 0xffff0000u : 0u);
                     }
-                    if (g < 0) {
-                        mma_f16(oo, m[u][0], m[u][0], m[u][1], m[u][1], b0, b1);
-                    } else {
-                        const uint32_t a0 = v0[g < 0 ? 0 : g], a1 = v1[g < 0 ? 0 : g], x0 = a0 >> 8, x1 = a1 >> 8;
-                        mma_f16(o[g < 0 ? 0 : g][0], a0 & kLow, a0 & kHigh, a1 & kLow, a1 & kHigh, b0, b1);
-                        mma_f16(o[g < 0 ? 0 : g][1], x0 & kLow, x0 & kHigh, x1 & kLow, x1 & kHigh, b0, b1);
+            }
+#pragma unroll
+            for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                for (int g = 0; g < NW; g++) steps = __vmaxu2(steps, __vmaxu2(d[u][0][g], d[u][1][g]));
+            // a score far above the reference, or a step beyond the scale's range: seldom after the first tile
+            float top[HPL];
+            bool grown = steps != limit;
+#pragma unroll
+            for (int h = 0; h < HPL; h++) {
+                top[h] = s[h][0][0];
+#pragma unroll
+                for (int u = 0; u < kQ4Tile; u++) top[h] = fmaxf(fmaxf(top[h], s[h][u][0]), s[h][u][1]);
+                grown |= top[h] > m_run[h] + 8.f;
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+                float fix[HPL], vfix = 1.f;
+                steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
+                if (steps > (limit & 0xffffu)) {  // the largest step to 2^2 .. 2^3, up to 2^7 in range: times weights of up to 2^8
+                    const int e = max((int)(steps >> 7) - 127, -100);
+                    const float next = __uint_as_float((uint32_t)(127 + 2 - e) << 23);
+                    vfix = vscale == 0.f ? 0.f : next / vscale;
+                    vscale = next;
+                    limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
+                }
+#pragma unroll
+                for (int h = 0; h < HPL; h++) {
+                    float mx = fmaxf(m_run[h], top[h]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
+                    m_run[h] = mx;
+                    l_run[h] *= fix[h];
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++) oo[x] *= fix[HPL == 1 ? 0 : x & 1];
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const float y = fix[HPL == 1 ? 0 : x & 1] * vfix;
+                        o[g][0][x] *= y;
+                        o[g][1][x] *= y;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < kQ4Tile; u++) {
+                uint32_t v0[NG], v1[NG];  // unit g8 of positions 2t, 2t + 1, and of those eight farther
+#pragma unroll
+                for (int g = 0; g < NG; g += 2) ldmatrix_x4_trans(v0[g], v1[g], v0[g + 1], v1[g + 1], tile + u * BLOCK + (g == 0 ? v_piece : v_piece ^ 32u));
+                float w[HPL][2], ws[HPL][2];
+#pragma unroll
+                for (int h = 0; h < HPL; h++) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
+                        ws[h][x] = w[h][x] * vscale;
+                    }
+                    l_run[h] += w[h][0] + w[h][1];
+                }
+                // group -1: the weights alone, for the offsets
+#pragma unroll
+                for (int g = -1; g < NG; g++) {
+                    float hi[HPL][2], lo[HPL][2];
+#pragma unroll
+                    for (int h = 0; h < HPL; h++)
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const float y = g < 0 ? w[h][x] : ws[h][x] * step_of(d[u][x], g < 0 ? 0 : g);
+                            hi[h][x] = upper_limb(y);
+                            lo[h][x] = y - hi[h][x];
+                        }
+#pragma unroll
+                    for (int limb = 0; limb < HPL; limb++) {
+                        uint32_t b0, b1;
+                        if constexpr (HPL == 1) {
+                            b0 = transpose8(pack_h2(hi[0][0], lo[0][0]));
+                            b1 = transpose8(pack_h2(hi[0][1], lo[0][1]));
+                        } else {
+                            b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
+                            b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
+                        }
+                        if (g < 0) {
+                            mma_f16(oo, m[u][0], m[u][0], m[u][1], m[u][1], b0, b1);
+                        } else {
+                            const uint32_t a0 = v0[g < 0 ? 0 : g], a1 = v1[g < 0 ? 0 : g], x0 = a0 >> 8, x1 = a1 >> 8;
+                            mma_f16(o[g < 0 ? 0 : g][0], a0 & kLow, a0 & kHigh, a1 & kLow, a1 & kHigh, b0, b1);
+                            mma_f16(o[g < 0 ? 0 : g][1], x0 & kLow, x0 & kHigh, x1 & kLow, x1 & kHigh, b0, b1);
+                        }
                     }
                 }
             }
+            __syncwarp();  // all lanes have read the tile before it is filled again
+            if (part_issued < part_tiles) issue();
         }
-        __syncwarp();  // all lanes have read the tile before it is filled again
-        if (issued < n_tiles) issue();
-    }
-    // sums over the lanes that share a head, then over the warps
+        const CacheRow now = r;
+        from = to;
+        if (from < share1 && !failed) begin(i + 1, from);  // the next row's pages are on their way from here on
+        // sums over the lanes that share a head, then over the warps
 #pragma unroll
-    for (int h = 0; h < HPL; h++) {
+        for (int h = 0; h < HPL; h++) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
-    }
-    float offset[HPL][NG];  // row g of the offsets' part: lanes 4 g + t
+            for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
+        }
+        float offset[HPL][NG];  // row g of the offsets' part: lanes 4 g + t
 #pragma unroll
-    for (int h = 0; h < HPL; h++)
+        for (int h = 0; h < HPL; h++)
 #pragma unroll
-        for (int g = 0; g < NG; g++) offset[h][g] = __shfl_sync(0xffffffffu, HPL == 1 ? oo[0] + oo[1] : oo[h], 4 * g + t);
-    const float unscale = vscale == 0.f ? 0.f : 16777216.f / vscale;
+            for (int g = 0; g < NG; g++) offset[h][g] = __shfl_sync(0xffffffffu, HPL == 1 ? oo[0] + oo[1] : oo[h], 4 * g + t);
+        const float unscale = vscale == 0.f ? 0.f : 16777216.f / vscale;
 #pragma unroll
-    for (int h = 0; h < HPL; h++) {
-        const int head = HPL * t + h;
-        if (head >= G) continue;
+        for (int h = 0; h < HPL; h++) {
+            const int head = HPL * t + h;
+            if (head >= G) continue;
 #pragma unroll
-        for (int g = 0; g < NG; g++) {
-            float v[4];  // dimensions 4 g8 .. 4 g8 + 3 of the group
+            for (int g = 0; g < NG; g++) {
+                float v[4];  // dimensions 4 g8 .. 4 g8 + 3 of the group
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float *c = &o[g][x >> 1][2 * (x & 1)];
-                v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], x & 1 ? unscale * 0.0625f : unscale, offset[h][g]);
+                for (int x = 0; x < 4; x++) {
+                    const float *c = &o[g][x >> 1][2 * (x & 1)];
+                    v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], x & 1 ? unscale * 0.0625f : unscale, offset[h][g]);
+                }
+                *reinterpret_cast<float4 *>(mg_o + (warp * G + head) * Smem::kMergeRow + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
             }
-            *reinterpret_cast<float4 *>(mg_o + (warp * G + head) * Smem::kMergeRow + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-        if (g8 == 0) {
-            mg_m[warp * G + head] = m_run[h];
-            mg_l[warp * G + head] = l_run[h];
-        }
-    }
-    __syncthreads();
-    for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {  // two dimensions of a head; a head to a warp, whose first lanes have the warps' shares of it
-        const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
-        float mw = lane < W ? mg_m[lane * G + g] : -INFINITY, lw = lane < W ? mg_l[lane * G + g] : 0.f, M = mw;
-#pragma unroll
-        for (int x = 1; x < W; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-        M = __shfl_sync(0xffffffffu, M, 0);
-        const float fw = lw == 0.f ? 0.f : exp2_fast(mw - M);  // a warp without pages has no share
-        float L = lw * fw, ax = 0.f, ay = 0.f;
-#pragma unroll
-        for (int x = 1; x < W; x <<= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-        L = __shfl_sync(0xffffffffu, L, 0);
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float f = __shfl_sync(0xffffffffu, fw, w);
-            const float2 v = *reinterpret_cast<const float2 *>(mg_o + (w * G + g) * Smem::kMergeRow + d);
-            if (f != 0.f) {
-                ax = fmaf(v.x, f, ax);
-                ay = fmaf(v.y, f, ay);
+            if (g8 == 0) {
+                mg_m[warp * G + head] = m_run[h];
+                mg_l[warp * G + head] = l_run[h];
             }
         }
-        const size_t at = (size_t)id * p.n_heads + h0 + g;
-        if (part.parts == 1) {
-            float *to_o = p.out + (size_t)i * p.ldo + (h0 + g) * HD + d;
-            to_o[0] = pos_end > 0 ? ax / L : 0.f;
-            to_o[1] = pos_end > 0 ? ay / L : 0.f;
-        } else {
-            *reinterpret_cast<float2 *>(p.part_o + at * HD + d) = make_float2(ax, ay);
+        __syncthreads();
+        const int parts = row_parts(p, i, now);
+        for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {  // two dimensions of a head; a head to a warp, whose first lanes have the warps' shares of it
+            const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
+            float mw = lane < W ? mg_m[lane * G + g] : -INFINITY, lw = lane < W ? mg_l[lane * G + g] : 0.f, M = mw;
+#pragma unroll
+            for (int x = 1; x < W; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+            M = __shfl_sync(0xffffffffu, M, 0);
+            const float fw = lw == 0.f ? 0.f : exp2_fast(mw - M);  // a warp without pages has no share
+            float L = lw * fw, ax = 0.f, ay = 0.f;
+#pragma unroll
+            for (int x = 1; x < W; x <<= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+            L = __shfl_sync(0xffffffffu, L, 0);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float f = __shfl_sync(0xffffffffu, fw, w);
+                const float2 v = *reinterpret_cast<const float2 *>(mg_o + (w * G + g) * Smem::kMergeRow + d);
+                if (f != 0.f) {
+                    ax = fmaf(v.x, f, ax);
+                    ay = fmaf(v.y, f, ay);
+                }
+            }
+            const size_t part = (size_t)(i + share) * p.n_heads + h0 + g;
+            if (parts == 1) {
+                float *to_o = p.out + (size_t)i * p.ldo + (h0 + g) * HD + d;
+                to_o[0] = pos_end > 0 ? ax / L : 0.f;
+                to_o[1] = pos_end > 0 ? ay / L : 0.f;
+            } else {
+                *reinterpret_cast<float2 *>(p.part_o + part * HD + d) = make_float2(ax, ay);
+            }
+            if (d == 0 && parts > 1) *reinterpret_cast<float2 *>(p.part_ml + part * 2) = make_float2(M, L);
+            if (TRACK && d == 0 && parts == 1) p.sums[(size_t)i * p.n_heads + h0 + g] = make_float2(M, 1.f / L);
         }
-        if (d == 0 && part.parts > 1) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(M, L);
-        if (TRACK && d == 0 && part.parts == 1) p.sums[(size_t)i * p.n_heads + h0 + g] = make_float2(M, 1.f / L);
+        // The rows that this share has with others are its first and its last.  Whoever of a row is last puts its parts together, at the end.
+        if (parts > 1) {
+            __syncthreads();
+            unsigned before = 0u;
+            if (tid == 0) {
+                __threadfence();
+                before = atomicAdd(p.arrived + (size_t)i * p.n_kv_heads + kvh, 1u);
+            }
+            if (now.first < share0)
+                row_a = i, before_a = before;
+            else
+                row_b = i, before_b = before;
+        }
+        __syncthreads();  // the warps' results have been read
+        if (__syncthreads_or(failed)) {
+            failed = true;
+            break;
+        }
     }
-    if (failed)
-        for (int j = ring_open(issued, used, kQ4Slots); j < issued; j++)
-            mbar_wait_bounded(bars + j % kQ4Slots * 8, ring_parity(j, kQ4Slots), 0, p.err, failed, kErrCacheWait);
-    if (part.parts == 1) return;
-    __syncthreads();
-    bool last = false;
-    if (tid == 0) {
-        unsigned *arrived = p.arrived + (size_t)i * p.n_kv_heads + kvh;
-        __threadfence();
-        last = atomicAdd(arrived, 1u) == (unsigned)part.parts - 1;
-        if (last) {
-            *arrived = 0;
+    if (failed) {  // the parts that are left count as done, so that the next launch finds zeros
+        for (unsigned j = ring_open((int)issued, (int)used, kQ4Slots); j < issued; j++)
+            mbar_wait_bounded(bars + j % kQ4Slots * 8, j / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
+        if (tid == 0)
+            for (int i = cache_find(p.rows, min(p.total - 1, from)); from < share1; from = row_end(p, i++)) {
+                const int parts = row_parts(p, i, cache_row(p.rows, i));
+                unsigned *arrived = p.arrived + (size_t)i * p.n_kv_heads + kvh;
+                if (parts > 1 && atomicAdd(arrived, 1u) == (unsigned)parts - 1) *arrived = 0;
+            }
+    }
+    for (int which = 0; which < 2; which++) {
+        const int i = which ? row_b : row_a;
+        if (i < 0) continue;
+        const CacheRow whole = cache_row(p.rows, i);
+        const int share_a = whole.share, parts = row_parts(p, i, whole);
+        if (!__syncthreads_or(tid == 0 && (which ? before_b : before_a) == (unsigned)parts - 1)) continue;
+        // two dimensions of a head to a thread, a head to a warp, a part's largest score and sum to a lane
+        if (tid == 0) {
             __threadfence();
+            p.arrived[(size_t)i * p.n_kv_heads + kvh] = 0;
         }
-    }
-    // two dimensions of a head to a thread, a head to a warp, a part's largest score and sum to a lane
-    if (__syncthreads_or(last)) {
-        const int parts = part.parts;
         const size_t stride = (size_t)p.n_heads * HD;
         for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {
             const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
-            const float2 *from_ml = reinterpret_cast<const float2 *>(p.part_ml) + (size_t)r.first * p.n_heads + h0 + g;
-            const float *from_o = p.part_o + (size_t)r.first * stride + (size_t)(h0 + g) * HD + d;
+            const float2 *from_ml = reinterpret_cast<const float2 *>(p.part_ml) + (size_t)(i + share_a) * p.n_heads + h0 + g;
+            const float *from_o = p.part_o + (size_t)(i + share_a) * stride + (size_t)(h0 + g) * HD + d;
             constexpr int AHEAD = 8;  // parts asked for before their weights are known
             float2 v[AHEAD], ml = make_float2(-INFINITY, 0.f);
             if (lane < parts) ml = __ldcg(from_ml + (size_t)lane * p.n_heads);
@@ -540,7 +603,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
     }
 }
 
-// The weight that positions have received: a thread has one position of a part and one key/value head.
+// The weight that positions have received: a thread has one position of all rows' pages and one key/value head.
 constexpr int kQ4WeightThreads = 256;
 template <int G>
 __device__ __forceinline__ float weight_of(const float *scores, const float2 *sums, int g_max) {
@@ -554,13 +617,13 @@ __device__ __forceinline__ float weight_of(const float *scores, const float2 *su
 }
 __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __grid_constant__ Q4AttnParams p) {
     pdl_wait();
-    const int kvh = blockIdx.y, blocks = (p.longest * kPageTokens + kQ4WeightThreads - 1) / kQ4WeightThreads, id = blockIdx.x / blocks, G = p.n_heads / p.n_kv_heads;
-    const int i = cache_find(p.rows, id), at = (blockIdx.x - id * blocks) * kQ4WeightThreads + threadIdx.x;
+    const int kvh = blockIdx.y, at = blockIdx.x * kQ4WeightThreads + threadIdx.x, G = p.n_heads / p.n_kv_heads;
+    if (at >= p.total * kPageTokens) return;
+    const int i = cache_find(p.rows, at >> 4);
     const CacheRow r = cache_row(p.rows, i);
-    const Q4Part part = part_of(p, r, i, id);
-    const int pos = part.page0 * kPageTokens + at;
-    if (r.track < 0 || pos >= min(r.upto, part.page1 * kPageTokens)) return;
-    const float *scores = p.scores + (((size_t)kvh * p.n_parts + id) * p.longest * kPageTokens + at) * G;
+    const int pos = at - r.first * kPageTokens;
+    if (r.track < 0 || pos >= r.upto) return;
+    const float *scores = p.scores + ((size_t)kvh * p.total * kPageTokens + at) * G;
     const float2 *sums = p.sums + (size_t)i * p.n_heads + kvh * G;
     float *w = p.weights + (((size_t)r.track * p.n_layers + p.layer) * p.n_kv_heads + kvh) * p.track_tokens + pos;
     const float old = *w;
@@ -573,7 +636,7 @@ __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __gr
 }
 
 template <int HD, int HPL, bool TRACK>
-static int launch_q4_attn(const Q4AttnParams &a, cudaStream_t st) {
+static int launch_q4_attn(const Q4AttnParams &a, int shares, cudaStream_t st) {
     static bool set[64] = {false};  // per device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -581,49 +644,49 @@ static int launch_q4_attn(const Q4AttnParams &a, cudaStream_t st) {
         JUNO_CUDA_TRY(cudaFuncSetAttribute(q4_attn_kernel<HD, HPL, TRACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<HD, HPL>::kAll));
         set[dev & 63] = true;
     }
-    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL, TRACK>, dim3((unsigned)(a.n_parts * a.n_kv_heads)), dim3(kQ4Warps<HD, HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
+    JUNO_CUDA_TRY(launch_pdl(q4_attn_kernel<HD, HPL, TRACK>, dim3((unsigned)(shares * a.n_kv_heads)), dim3(kQ4Warps<HD, HPL> * 32), Q4Smem<HD, HPL>::kAll, st, a));
     return JUNO_OK;
 }
 
 template <int HD, bool TRACK>
-static int launch_q4_attn(const Q4AttnParams &a, int G, cudaStream_t st) {
-    return G <= 4 ? launch_q4_attn<HD, 1, TRACK>(a, st) : launch_q4_attn<HD, 2, TRACK>(a, st);
+static int launch_q4_attn(const Q4AttnParams &a, int G, int shares, cudaStream_t st) {
+    return G <= 4 ? launch_q4_attn<HD, 1, TRACK>(a, shares, st) : launch_q4_attn<HD, 2, TRACK>(a, shares, st);
 }
 
-// How the rows are cut: at most `slots` parts for each key/value head run at a time.  A part costs its rounds (of `round` pages, a tile for every warp) and
-// about kQ4PartCost more; parts run in waves, and what is cut has to be put together.  Sets `first` of the rows, returns the number of parts.
-constexpr int kQ4PartCost = 2, kQ4MergeCost = 1;
-static int q4_cut(std::vector<CacheRow> &rows, int64_t pages, int most, int slots, int round, int *longest) {
-    const int n = (int)rows.size();
-    auto count = [](const CacheRow &r, int len) { return std::max(1, ((r.upto + kPageTokens - 1) / kPageTokens + len - 1) / len); };
-    int best_len = most;
-    double best = 1e30;
-    for (int waves = 1; waves <= 4; waves++) {
-        // the shortest parts, in whole rounds, that are no more than these waves hold
-        int len = (int)((pages + (int64_t)waves * slots - 1) / ((int64_t)waves * slots));
-        len = std::max(1, (len + round - 1) / round) * round;
-        int64_t parts = 0;
-        for (;; len += std::max(1, len / (8 * round)) * round) {
-            parts = 0;
-            for (const CacheRow &r : rows) parts += count(r, len);
-            if (parts <= (int64_t)waves * slots || len >= most) break;
+// How the pages are cut for `slots` CTAs per key/value head that run at a time.  Either each row into parts of about equal length, no more than `slots` of them:
+// then a CTA begins once, and the longest part is waited for; or all pages into equal shares across the rows: no CTA waits for another, but most begin
+// a second row (kQ4BeginCost rounds).  A round is `round` pages, a tile for every warp of a CTA.
+constexpr int kQ4BeginCost = 4;
+static void q4_cut(std::vector<CacheRow> &rows, int pages, int slots, int round, std::vector<int32_t> *cuts) {
+    const int n = (int)rows.size(), share = std::max(round, (pages + slots - 1) / slots);
+    auto end_of = [&](int i) { return i + 1 < n ? rows[(size_t)i + 1].first : pages; };
+    int len = 0;
+    if (n <= slots) {  // the shortest parts, in whole rounds, that the slots hold
+        for (len = (share + round - 1) / round * round;; len += std::max(1, len / (8 * round)) * round) {
+            int parts = 0;
+            for (int i = 0; i < n; i++) parts += (end_of(i) - rows[(size_t)i].first + len - 1) / len;
+            if (parts <= slots) break;
         }
-        const double rounds = (std::min(len, most) + round - 1) / round, cost = (double)((parts + slots - 1) / slots) * (rounds + kQ4PartCost) + (parts > n ? kQ4MergeCost : 0);
-        if (cost < best) {
-            best = cost;
-            best_len = len;
+        if (n > 1 && len > share + kQ4BeginCost * round) len = 0;
+    }
+    for (int i = 0; i < n; i++) {
+        const int from = rows[(size_t)i].first, size = end_of(i) - from;
+        if (len) {
+            const int k = (size + len - 1) / len;
+            rows[(size_t)i].share = (int)cuts->size();
+            for (int j = 0; j < k; j++) cuts->push_back(from + (int)((int64_t)size * j / k));
+        } else {
+            rows[(size_t)i].share = from / share;
+            while ((int64_t)cuts->size() * share < end_of(i)) cuts->push_back((int32_t)cuts->size() * share);
         }
-        if (len >= most) break;
     }
-    int64_t parts = 0;
-    *longest = 1;
-    for (CacheRow &r : rows) {
-        const int k = count(r, best_len), pg = (r.upto + kPageTokens - 1) / kPageTokens;
-        r.first = (int)parts;
-        parts += k;
-        *longest = std::max(*longest, (pg + k - 1) / k);
-    }
-    return (int)parts;
+    cuts->push_back(pages);
+}
+// Whether every row lies in one share.
+static bool q4_whole(const std::vector<CacheRow> &rows, const std::vector<int32_t> &cuts) {
+    for (size_t i = 0; i < rows.size(); i++)
+        if (cuts[(size_t)rows[i].share + 1] < (i + 1 < rows.size() ? rows[i + 1].first : cuts.back())) return false;
+    return true;
 }
 
 // Zeros, once; every launch leaves them so.
@@ -645,28 +708,35 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     }
     std::vector<CacheRow> rows((size_t)n);
     int64_t pages = 0, bytes = 0;
-    int most = 1;
     bool track = false;
     for (int i = 0; i < n; i++) {
-        const int len = lens ? lens[i] : seqs[i]->len, pg = std::max(1, (len + kPageTokens - 1) / kPageTokens);
-        rows[(size_t)i] = {seqs[i]->slot, len, 0, seqs[i]->track};
-        pages += pg;
-        most = std::max(most, pg);
+        const int len = lens ? lens[i] : seqs[i]->len;
+        rows[(size_t)i] = {seqs[i]->slot, len, (int)pages, seqs[i]->track, 0};
+        pages += std::max(1, (len + kPageTokens - 1) / kPageTokens);
         track |= seqs[i]->track >= 0;
         bytes += len;
+        JUNO_REQUIRE(pages < (1 << 27), "attention over %lld pages in one call", (long long)pages);
     }
     const bool wide = G > 4 && hd == 128;
     const int warps = wide ? kQ4Warps<128, 2> : kQ4Warps<64, 2>, ctas = wide ? kQ4Ctas<128, 2> : kQ4Ctas<64, 2>;
-    int longest = 0;
-    const int n_parts = q4_cut(rows, pages, most, std::max(1, c->sm_count * ctas / H), warps * kQ4Tile, &longest);
-    if (n_parts > n) JUNO_TRY(arrival_words(c, (size_t)n * H, st));
+    std::vector<int32_t> cuts;
+    q4_cut(rows, (int)pages, std::max(1, c->sm_count * ctas / H), warps * kQ4Tile, &cuts);
+    const int shares = (int)cuts.size() - 1;
+    const bool whole = shares == 1 || q4_whole(rows, cuts);
+    if (!whole) JUNO_TRY(arrival_words(c, (size_t)n * H, st));
     Q4AttnParams a;
     auto padded = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    const size_t parts = n_parts > n ? (size_t)n_parts : 0, far_b = cache_rows_bytes(n), ml_b = padded(parts * n_heads * 8), o_b = padded(parts * n_heads * hd * 4),
-                 s_b = track ? padded((size_t)n_parts * longest * kPageTokens * n_heads * 4) : 0, sum_b = track ? (size_t)n * n_heads * sizeof(float2) : 0;
+    const size_t parts = whole ? 0 : (size_t)(n + shares), row_b = cache_rows_bytes(n), cut_b = shares + 1 > kInlineCuts ? padded(cuts.size() * sizeof(int32_t)) : 0,
+                 far_b = row_b + cut_b, ml_b = padded(parts * n_heads * 8), o_b = padded(parts * n_heads * hd * 4),
+                 s_b = track ? padded((size_t)pages * kPageTokens * n_heads * 4) : 0, sum_b = track ? (size_t)n * n_heads * sizeof(float2) : 0;
     uint8_t *scratch = nullptr;
     JUNO_TRY(cache_scratch(c, far_b + ml_b + o_b + s_b + sum_b, &scratch));
     JUNO_TRY(cache_rows(c, rows.data(), n, reinterpret_cast<CacheRow *>(scratch), &a.rows, st));
+    a.far_cuts = cut_b ? reinterpret_cast<const int32_t *>(scratch + row_b) : nullptr;
+    if (cut_b)
+        JUNO_TRY(cache_words(c, cuts.data(), cuts.size(), reinterpret_cast<int32_t *>(scratch + row_b), st));
+    else
+        std::copy(cuts.begin(), cuts.end(), a.cuts);
     a.pool = static_cast<const uint8_t *>(p->k);
     a.table = p->d_table;
     a.max_pages_per_seq = p->max_pages_per_seq;
@@ -675,8 +745,8 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     a.n_heads = n_heads;
     a.layer = layer;
     a.n_layers = p->n_layers;
-    a.n_parts = n_parts;
-    a.longest = longest;
+    a.total = (int)pages;
+    a.shares = shares;
     a.q = q;
     a.ldq = ldq;
     a.out = out;
@@ -691,12 +761,12 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     a.err = c->gemv_scratch.qerr + word;
     ProfScope prof(c, st, PROF_ATTN, (double)bytes * H * p->row_bytes());
     if (hd == 128)
-        JUNO_TRY((track ? launch_q4_attn<128, true>(a, G, st) : launch_q4_attn<128, false>(a, G, st)));
+        JUNO_TRY((track ? launch_q4_attn<128, true>(a, G, shares, st) : launch_q4_attn<128, false>(a, G, shares, st)));
     else
-        JUNO_TRY((track ? launch_q4_attn<64, true>(a, G, st) : launch_q4_attn<64, false>(a, G, st)));
+        JUNO_TRY((track ? launch_q4_attn<64, true>(a, G, shares, st) : launch_q4_attn<64, false>(a, G, shares, st)));
     c->kernel_launches++;
     if (!track) return JUNO_OK;
-    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)(n_parts * ((longest * kPageTokens + kQ4WeightThreads - 1) / kQ4WeightThreads)), (unsigned)H), dim3(kQ4WeightThreads), 0, st, a));
+    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages * kPageTokens + kQ4WeightThreads - 1) / kQ4WeightThreads), (unsigned)H), dim3(kQ4WeightThreads), 0, st, a));
     c->kernel_launches++;
     return JUNO_OK;
 }
