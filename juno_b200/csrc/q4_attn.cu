@@ -527,8 +527,8 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             else
                 row_b = i, before_b = before;
         }
-        __syncthreads();  // the warps' results have been read
-        if (__syncthreads_or(failed)) {
+        if (from >= share1) break;
+        if (__syncthreads_or(failed)) {  // the warps' results have been read
             failed = true;
             break;
         }
