@@ -284,12 +284,11 @@ class PagedKvCache:
         return seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
 
     @staticmethod
-    def _ints(x, n: int, name: str):
-        """(array, address) of n whole numbers; the array has to outlive the use of the address."""
-        a = x if type(x) is np.ndarray and x.dtype == np.int32 and x.flags.c_contiguous else np.ascontiguousarray(x, dtype=np.int32)
+    def _ints(x, n: int, name: str) -> np.ndarray:
+        a = np.asarray(x, dtype=np.int32)
         if a.shape != (n,):
             raise ValueError(f"{name}: {n} whole numbers are wanted, not shape {a.shape}")
-        return a, a.__array_interface__["data"][0]
+        return a
 
     @staticmethod
     def _stream(stream):
@@ -297,14 +296,13 @@ class PagedKvCache:
 
     def _move_rows(self, call, name, layer, seqs, positions, counts, k, v, stream) -> None:
         b = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
-        positions, at = self._ints(positions, b.n, "positions")
-        counts, n = self._ints(counts, b.n, "counts")
+        positions, counts = self._ints(positions, b.n, "positions"), self._ints(counts, b.n, "counts")
         rows, width = sum(counts.tolist()), self.n_kv_heads * self.head_dim
         kp, ld = _device_ptr(k, "k", rows, width)
         vp, ldv = _device_ptr(v, "v", rows, width)
         if ld != ldv:
             raise ValueError(f"the rows of k and v lie {ld} and {ldv} elements apart")
-        rc = call(self.ctx.handle, self.handle, layer, b.n, b.handles, at, n, kp, vp, ld, None if stream is None else self._stream(stream))
+        rc = call(self.ctx.handle, self.handle, layer, b.n, b.handles, positions.tobytes(), counts.tobytes(), kp, vp, ld, None if stream is None else self._stream(stream))
         if rc:
             check(rc, name)
 
@@ -322,8 +320,8 @@ class PagedKvCache:
         width = n_heads * self.head_dim
         qp, ldq = _device_ptr(q, "q", b.n, width)
         op, ldo = _device_ptr(out, "out", b.n, width)
-        lens, lp = (None, None) if lens is None else self._ints(lens, b.n, "lens")
-        rc = self._L.juno_attn_decode_device(self.ctx.handle, self.handle, layer, b.n, b.handles, lp, n_heads, qp, ldq, op, ldo,
+        lens = None if lens is None else self._ints(lens, b.n, "lens").tobytes()
+        rc = self._L.juno_attn_decode_device(self.ctx.handle, self.handle, layer, b.n, b.handles, lens, n_heads, qp, ldq, op, ldo,
                                              None if stream is None else self._stream(stream))
         if rc:
             check(rc, "juno_attn_decode_device")
@@ -334,8 +332,8 @@ class PagedKvCache:
         b = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs)
         wp = _whole_ptr(w, "w", "float32", (b.n, self.n_kv_heads))
         ld = w.shape[2]
-        counts, n = self._ints(counts, b.n, "counts")
-        rc = self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, n, wp, ld, 1 if store else 0,
+        counts = self._ints(counts, b.n, "counts").tobytes()
+        rc = self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, counts, wp, ld, 1 if store else 0,
                                             None if stream is None else self._stream(stream))
         if rc:
             check(rc, "juno_kv_weights_device")
