@@ -64,7 +64,7 @@ int juno_device_total_mem(int32_t device, int64_t *bytes);
 int juno_ctx_create(int32_t device, juno_ctx **out);
 int juno_ctx_destroy(juno_ctx *ctx); /* idempotent on a closed handle: returns JUNO_ERR_CLOSED */
 int juno_ctx_device(juno_ctx *ctx, int32_t *device);
-/* Waits for the context's stream.  JUNO_ERR_TIMEOUT, once, when a product of juno_gemv_device gave up a wait (its result is
+/* Waits for the context's stream.  JUNO_ERR_TIMEOUT, once, when a product of juno_gemv_device or a call of juno_attn_decode_device gave up a wait (its result is
  * not valid); one on a stream of the caller's has to have finished before the call. */
 int juno_ctx_synchronize(juno_ctx *ctx);
 /* The cudaStream_t all work of this context is enqueued on (replaces the per-thread stream of

@@ -907,6 +907,7 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
                  "bad KV pool geometry");
     JUNO_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim %d is not supported (64, 128)", head_dim);
     JUNO_REQUIRE(dtype == 0 || dtype == 1 || dtype == kKvQ4, "kv_dtype %d (0 = f16, 1 = f32, 3 = 4 bits)", dtype);
+    JUNO_REQUIRE(dtype != kKvQ4 || (int64_t)n_pages * n_kv_heads * q4_block_bytes(head_dim) < (1ll << 36), "a layer of 4-bit pages has up to 64 GB");
     juno_kvpool *p = new juno_kvpool();
     p->magic = kMagicPool;
     p->ctx = ctx;
@@ -1275,9 +1276,9 @@ int juno_seq_free(juno_seq *s) {
 int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
     JUNO_TRY(seq_check(src));
     JUNO_REQUIRE(out, "out is null");
-    JUNO_REQUIRE(n_tokens >= 0 && n_tokens <= src->len, "cannot share %d positions of a sequence that holds %d", n_tokens, src->len);
     juno_kvpool *p = src->pool;
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
+    JUNO_REQUIRE(n_tokens >= 0 && n_tokens <= src->len, "cannot share %d positions of a sequence that holds %d", n_tokens, src->len);
     DeviceGuard g(p->ctx->device);
     JUNO_TRY(seq_resume_check(p, src->len, n_tokens));
     juno_seq *s = nullptr;

@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     const EvictRow r = p.rows[i];
     float *w = p.weights + (((size_t)r.track * p.n_layers + layer) * p.n_kv_heads + h) * p.track_tokens;
     int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld;
-    for (int j = r.keep + tid; j < p.kept_ld; j += kSelectThreads) kept[j] = -1;
+    for (int64_t j = r.keep + tid; j < p.kept_ld; j += kSelectThreads) kept[j] = -1;
     if (r.keep == r.len) {
         for (int j = tid; j < r.keep; j += kSelectThreads) kept[j] = j;
         return;
@@ -806,6 +806,11 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         JUNO_TRY(cache_call_distinct(p, n, seqs));
         for (int i = 0; i < n; i++) JUNO_REQUIRE(seqs[i]->track >= 0, "sequence %d keeps no weights (juno_seq_track)", i);
         if (kept_dev) JUNO_TRY(device_memory(c, kept_dev, "kept"));
+        int most = 1;
+        for (int i = 0; i < n; i++) most = std::max(most, seqs[i]->len);
+        const int kept_ld = keep;
+        keep = std::min(keep, most);  // where no sequence is longer nothing is cut
+        recent = std::min(recent, keep);
         // The rows go to fresh pages where the pool has enough of them, which all warps can fill side by side; else they move within their pages, but for pages
         // that another sequence holds too: those are left to it, and their rows go to fresh ones.
         const int np = (keep + kPageTokens - 1) / kPageTokens;
@@ -861,7 +866,7 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         a.hd = p->head_dim;
         a.weights = p->weights;
         a.kept = kept_dev ? kept_dev : reinterpret_cast<int32_t *>(scratch + word_bytes);
-        a.kept_ld = keep;
+        a.kept_ld = kept_dev ? kept_ld : keep;
         const dim3 heads((unsigned)p->n_kv_heads, (unsigned)p->n_layers, (unsigned)n), units((unsigned)((np * p->n_kv_heads + 7) / 8), (unsigned)p->n_layers, (unsigned)n);
         const size_t cached = kSelectCached * sizeof(float);
         static bool set[64] = {false};  // per device

@@ -715,7 +715,7 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
         pages += std::max(1, (len + kPageTokens - 1) / kPageTokens);
         track |= seqs[i]->track >= 0;
         bytes += len;
-        JUNO_REQUIRE(pages < (1 << 27), "attention over %lld pages in one call", (long long)pages);
+        JUNO_REQUIRE(pages < (1 << 26), "attention over %lld pages in one call", (long long)pages);
     }
     const bool wide = G > 4 && hd == 128;
     const int warps = wide ? kQ4Warps<128, 2> : kQ4Warps<64, 2>, ctas = wide ? kQ4Ctas<128, 2> : kQ4Ctas<64, 2>;

@@ -706,6 +706,141 @@ def test_a_graph_is_refused_and_goes_on(ctx):
     cache.close()
 
 
+def test_a_wait_that_was_given_up_is_reported_once(ctx, wait_words):
+    rng = np.random.default_rng(31)
+    cache = PagedKvCache(ctx, 1, 2, 64, 8, "q4")
+    s = cache.new_sequence(100)
+    k = rows(rng, 100, 2, 64)
+    fill(cache, 0, [s], [0], [(k, k)])
+    q = f32(rng.standard_normal((1, 8, 64)))
+    want = attend(cache, 0, [s], q)
+    page = 9 | 2 << 8 | 5 << 16  # a page that warp 2 of block 5 waited for
+    wait_words[0] = page
+    with pytest.raises(JunoError, match="page of the cache .warp 2 of block 5") as e:
+        cache.attention(0, [s], q.reshape(1, -1), 8)
+    assert e.value.rc == _lib.ERR_TIMEOUT and wait_words[0] == 0
+    wait_words[1] = page
+    assert np.array_equal(attend(cache, 0, [s], q), want)  # enqueued work is answered for by the synchronisation
+    with pytest.raises(JunoError, match="page of the cache"):
+        ctx.synchronize()
+    ctx.synchronize()
+    assert np.array_equal(cache.attention(0, [s], q.reshape(1, -1), 8).reshape(want.shape), want)
+    cache.close()
+
+
+def test_eviction_of_sequences_that_are_short_enough(ctx):
+    """Whatever the budget is: nothing moves, and no room is asked for that the sequences do not have."""
+    rng = np.random.default_rng(32)
+    cache = PagedKvCache(ctx, 2, 2, 64, 8, "q4", track_seqs=2, track_tokens=64)
+    a, b = cache.new_sequence(64, track=True), cache.new_sequence(64, track=True)  # b is empty
+    k = rows(rng, 50, 2, 64)
+    for l in range(2):
+        fill(cache, l, [a], [0], [(k, k)])
+    for keep, recent in ((50, 0), (51, 51), (2 ** 31 - 1, 7), (2 ** 31 - 1, 2 ** 31 - 1)):
+        cache.evict([a, b], keep, recent)
+    kept = torch.full((2, 2, 2, 60), 9, dtype=torch.int32, device="cuda")
+    settle()
+    cache.evict([b, a], 60, 60, kept=kept)
+    settle()
+    kept = kept.cpu().numpy()
+    assert (kept[:, 0] == -1).all() and (kept[:, 1, :, :50] == np.arange(50)).all() and (kept[:, 1, :, 50:] == -1).all()
+    assert cache.length(a) == 50 and cache.length(b) == 0
+    assert np.array_equal(read(cache, 1, [a], [0], [50])[0], f32(q4.held(k)))
+    cache.close()
+
+
+def test_two_threads_share_a_pool(ctx):
+    """Calls from two threads, each with sequences of its own: as if one had made them."""
+    import threading
+    rng = np.random.default_rng(33)
+    cache = PagedKvCache(ctx, 1, 4, 64, 300, "q4", track_seqs=8, track_tokens=400)
+    q = f32(rng.standard_normal((1, 16, 64)))
+    qd = dev(q.reshape(1, -1))
+    parts = [rows(rng, 390, 4, 64) for _ in range(2)]
+    data = [dev(p.reshape(390, -1)) for p in parts]
+    outs = [[torch.zeros((1, 1024), device="cuda") for _ in range(25)] for _ in range(2)]
+    settle()
+    errors = []
+
+    def work(t):
+        try:
+            for r in range(25):
+                s = cache.new_sequence(400, track=True)
+                cache.append_device(0, [s], [0], [300], data[t][:300], data[t][:300])
+                f = cache.fork(s, 290)
+                cache.append_device(0, [f], [290], [90], data[t][290:380], data[t][290:380])
+                cache.attention_device(0, [f], qd, 16, outs[t][r])
+                cache.evict([f], 100, 10)
+                cache.free_sequence(s)
+                cache.free_sequence(f)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    settle()
+    assert not errors, errors
+    for t in range(2):
+        h = q4.held(parts[t][:380])
+        for o in outs[t]:
+            check_attention(o.cpu().numpy().reshape(16, 64), q[0], h, h)
+    cache.close()
+
+
+def test_results_may_take_the_place_of_the_queries(ctx):
+    rng = np.random.default_rng(34)
+    cache = PagedKvCache(ctx, 1, 2, 128, 300, "q4")
+    seqs, parts = [cache.new_sequence(2500) for _ in range(2)], [(rows(rng, n, 2, 128), rows(rng, n, 2, 128)) for n in (2500, 40)]
+    fill(cache, 0, seqs, [0, 0], parts)
+    q = f32(rng.standard_normal((2, 16, 128)))
+    x = dev(q.reshape(2, -1))
+    settle()
+    cache.attention_device(0, seqs, x, 16, x)
+    settle()
+    for i, p in enumerate(parts):
+        check_attention(x[i].cpu().numpy().reshape(16, 128), q[i], q4.held(p[0]), q4.held(p[1]))
+    cache.close()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 64), (8, 1, 128), (64, 64, 64), (5, 1, 128)])
+def test_attention_of_few_and_of_many_heads(ctx, heads, kv, dim):
+    """One key/value head, whose parts are more than travel with a launch; more heads than CTAs of a wave; batches cut across their rows."""
+    rng = np.random.default_rng(heads * dim)
+    lens = [9000, 1, 4000, 700] if kv == 1 else [300, 1, 77, 640]
+    cache = PagedKvCache(ctx, 1, kv, dim, sum((n + 15) // 16 for n in lens), "q4", track_seqs=4, track_tokens=max(lens))
+    seqs = [cache.new_sequence(max(lens), track=i % 2 == 0) for i in range(4)]
+    parts = [(rows(rng, n, kv, dim), rows(rng, n, kv, dim)) for n in lens]
+    fill(cache, 0, seqs, [0] * 4, parts)
+    q = f32(rng.standard_normal((4, heads, dim)))
+    out = attend(cache, 0, seqs, q)
+    for i, p in enumerate(parts):
+        w = check_attention(out[i], q[i], q4.held(p[0]), q4.held(p[1]))
+        if i % 2 == 0:
+            check_weights(weights(cache, 0, [seqs[i]], [lens[i]])[0], w, q[i], p[0])
+    cache.close()
+
+
+def test_rows_of_unequal_lengths_share_the_work(ctx):
+    """Rows that are cut across: one very long, one in the middle, many short, empty ones between; and each again in another order."""
+    rng = np.random.default_rng(35)
+    kv, dim, heads = 8, 128, 64
+    lens = [3000, 0, 17, 6000, 1, 333, 0, 2900, 16] + [int(n) for n in rng.integers(1, 900, 30)]
+    cache = PagedKvCache(ctx, 1, kv, dim, sum((n + 15) // 16 for n in lens), "q4")
+    seqs = [cache.new_sequence(max(n, 1)) for n in lens]
+    parts = [(rows(rng, n, kv, dim), rows(rng, n, kv, dim)) for n in lens]
+    fill(cache, 0, seqs, [0] * len(lens), parts)
+    q = f32(rng.standard_normal((len(lens), heads, dim)))
+    for order in (np.arange(len(lens)), np.argsort(lens), np.argsort(lens)[::-1]):
+        out = attend(cache, 0, [seqs[i] for i in order], q[order], lens=[lens[i] for i in order])
+        for j, i in enumerate(order):
+            if lens[i] == 0:
+                assert (out[j] == 0).all()
+            else:
+                check_attention(out[j], q[i], q4.held(parts[i][0]), q4.held(parts[i][1]))
+    cache.close()
+
+
 def test_closing_a_context_gives_its_working_memory_back(ctx):
     own = GpuContext(0)
     cache = PagedKvCache(own, 1, 2, 64, 8, "q4")
