@@ -139,7 +139,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // A CTA has R positions, of keys (blockIdx.y = 0) or values.  A lane has eight neighbouring dimensions, four lanes a group: what is stored of a position is
-// contiguous but for the values' offsets.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate
+// contiguous.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate
 // of q4_number (a saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided
 // exactly.
 template <int HD, int R, bool V>
@@ -544,22 +544,20 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     }
 }
 
-// A row in pieces, one to a lane of sixteen: the numbers of keys and values in 16 bytes, the keys' steps and offsets and the values' steps in 2 NG, the values'
-// offsets in 2.  Where piece i of position pp lies: at + pp * stride, but for the values' numbers, whose pieces are permuted.
+// A row in pieces, one to a lane of sixteen: the numbers of keys and values in 16 bytes, steps and offsets of both in 2 NG.  Where piece i of position pp
+// lies: at + pp * stride, but for the values' numbers, whose pieces are permuted.
 template <int HD>
 struct Q4Piece {
-    static constexpr int NG = HD / kQ4Group, CODES = HD / 32, PIECES = 2 * CODES + 3 + NG;
-    int kind, at, stride, group;  // 0: 16 bytes, 1: values' 16 bytes, 2: NG half words, 3: one, 4: none
-    __device__ __forceinline__ explicit Q4Piece(int i) : kind(4), at(0), stride(0), group(0) {
+    static constexpr int NG = HD / kQ4Group, CODES = HD / 32, PIECES = 2 * CODES + 4;
+    int kind, at, stride, group;  // 0: 16 bytes, 1: values' 16 bytes, 2: NG half words, 3: none
+    __device__ __forceinline__ explicit Q4Piece(int i) : kind(3), at(0), stride(0), group(0) {
         if (i < CODES) {
             kind = 0, at = q4_k_code(HD, 0, 0, 0) + 16 * i, stride = HD / 2;
         } else if (i < 2 * CODES) {
             kind = 1, at = 10 * HD, stride = HD / 2, group = i - CODES;
-        } else if (i < 2 * CODES + 3) {
-            const int k = i - 2 * CODES;
-            kind = 2, at = k == 0 ? q4_k_step(HD, 0, 0) : k == 1 ? q4_k_offset(HD, 0, 0) : q4_v_step(HD, 0, 0), stride = 2 * NG;
         } else if (i < PIECES) {
-            kind = 3, at = q4_v_offset(HD, 0, i - 2 * CODES - 3), stride = 2;
+            const int k = i - 2 * CODES;
+            kind = 2, at = k == 0 ? q4_k_step(HD, 0, 0) : k == 1 ? q4_k_offset(HD, 0, 0) : k == 2 ? q4_v_step(HD, 0, 0) : q4_v_offset(HD, 0, 0), stride = 2 * NG;
         }
     }
     __device__ __forceinline__ int place(int pp) const { return at + pp * stride + (kind == 1 ? 16 * q4_v_piece(HD, pp, group) : 0); }
@@ -586,8 +584,6 @@ struct Q4Piece {
             *reinterpret_cast<uint2 *>(b) = make_uint2(v.x, v.y);
         else if (kind == 2)
             *reinterpret_cast<uint32_t *>(b) = v.x;
-        else if (kind == 3)
-            *reinterpret_cast<uint16_t *>(b) = (uint16_t)v.x;
     }
 };
 

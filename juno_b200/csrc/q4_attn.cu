@@ -92,6 +92,13 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t &r0, uint32_t &r1, ui
 }
 // The steps of groups g and g + 1 (g even) lie in one word; a BF16 number is the upper half of an FP32 one.
 __device__ __forceinline__ float step_of(const uint32_t *words, int g) { return __uint_as_float(g & 1 ? words[g >> 1] & 0xffff0000u : words[g >> 1] << 16); }
+// Numbers in bits 0..3 (SHIFT = 0) or 4..7 of both halves as FP16: with the exponent put before them they are 1024 + q, or 64 + q.
+template <int SHIFT>
+__device__ __forceinline__ uint32_t numbers_f16(uint32_t w) {
+    const uint32_t with = SHIFT ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u, off = SHIFT ? 0x54005400u : 0x64006400u;
+    const __half2 q = __hsub2(*reinterpret_cast<const __half2 *>(&with), *reinterpret_cast<const __half2 *>(&off));
+    return *reinterpret_cast<const uint32_t *>(&q);
+}
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
 __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             qsum[h] = t < NW ? *reinterpret_cast<const uint32_t *>(sums_s + column * 4 + 2 * t) : 0u;
             back[h] = back_s[HPL * t + h];
         }
-        float o[NG][2][4], oo[4] = {0.f, 0.f, 0.f, 0.f}, m_run[HPL], l_run[HPL], vscale = 0.f;  // oo: the offsets' part, row g8 = group
+        float o[NG][2][4], offset[HPL][NG], m_run[HPL], l_run[HPL], vscale = 0.f;  // offset: the offsets' part, of this lane's positions
         uint32_t limit = 0;  // largest step in the scale's range, in both halves
 #pragma unroll
         for (int g = 0; g < NG; g++)
@@ -264,6 +271,8 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         for (int h = 0; h < HPL; h++) {
             m_run[h] = -INFINITY;
             l_run[h] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; g++) offset[h][g] = 0.f;
         }
         constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
@@ -329,28 +338,23 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                         for (int x = 0; x < 2; x++)
                             if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
             }
-            uint32_t d[kQ4Tile][2][NW], m[kQ4Tile][2], steps = limit;
+            uint32_t d[kQ4Tile][2][NW], steps = limit;
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
-                    uint32_t one[1];
-                    lds_words<1>(one, tile + u * BLOCK + 19 * HD + (g8 % NG) * 32 + x * 16 + t * 4);  // rows beyond the groups: again, and not looked at
-                    m[u][x] = one[0];
                 }
             if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
 #pragma unroll
                 for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const int at = pos0 + 16 * u + 8 * x;
-                        const bool on = at + g8 < pos_end;
+                        const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
 #pragma unroll
                         for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
 #pragma unroll
                         for (int g = 0; g < NW; g++) d[u][x][g] = on ? d[u][x][g] : 0u;
-                        m[u][x] &= (at + 2 * t < pos_end ? 0xffffu : 0u) | (at + 2 * t + 1 < pos_end ? 0xffff0000u : 0u);
                     }
             }
 #pragma unroll
@@ -365,29 +369,32 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 top[h] = s[h][0][0];
 #pragma unroll
                 for (int u = 0; u < kQ4Tile; u++) top[h] = fmaxf(fmaxf(top[h], s[h][u][0]), s[h][u][1]);
-                grown |= top[h] > m_run[h] + 8.f;
+                grown |= top[h] > m_run[h] + 15.f;
             }
             if (__any_sync(0xffffffffu, grown)) {
                 float fix[HPL], vfix = 1.f;
                 steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
-                if (steps > (limit & 0xffffu)) {  // the largest step to 2^2 .. 2^3, up to 2^7 in range: times weights of up to 2^8
+                if (steps > (limit & 0xffffu)) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
                     const int e = max((int)(steps >> 7) - 127, -100);
-                    const float next = __uint_as_float((uint32_t)(127 + 2 - e) << 23);
+                    const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23);
                     vfix = vscale == 0.f ? 0.f : next / vscale;
                     vscale = next;
                     limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
                 }
 #pragma unroll
                 for (int h = 0; h < HPL; h++) {
-                    float mx = fmaxf(m_run[h], top[h]);
+                    float mx = fmaxf(m_run[h] + 11.f, top[h]);
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                    mx -= 11.f;
                     fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
                     m_run[h] = mx;
                     l_run[h] *= fix[h];
                 }
 #pragma unroll
-                for (int x = 0; x < 4; x++) oo[x] *= fix[HPL == 1 ? 0 : x & 1];
+                for (int h = 0; h < HPL; h++)
+#pragma unroll
+                    for (int g = 0; g < NG; g++) offset[h][g] *= fix[h];
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -412,15 +419,32 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                     }
                     l_run[h] += w[h][0] + w[h][1];
                 }
-                // group -1: the weights alone, for the offsets
+                // the offsets' part, in FP32: an MMA cuts off what its sum of 22-bit products has below 24 bits, always towards zero, and this part and the
+                // numbers' are often large and of opposite sign
 #pragma unroll
-                for (int g = -1; g < NG; g++) {
+                for (int x = 0; x < 2; x++) {
+                    uint32_t m[NW];
+                    lds_words<NW>(m, tile + u * BLOCK + 19 * HD + (g8 + 8 * x) * NG * 2);
+                    const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
+#pragma unroll
+                    for (int g = 0; g < NG; g += 2) {
+                        const uint32_t pair = on ? m[g >> 1] : 0u;
+                        const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&pair));
+#pragma unroll
+                        for (int h = 0; h < HPL; h++) {
+                            offset[h][g] = fmaf(w[h][x], two.x, offset[h][g]);
+                            offset[h][g + 1] = fmaf(w[h][x], two.y, offset[h][g + 1]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
                     float hi[HPL][2], lo[HPL][2];
 #pragma unroll
                     for (int h = 0; h < HPL; h++)
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            const float y = g < 0 ? w[h][x] : ws[h][x] * step_of(d[u][x], g < 0 ? 0 : g);
+                            const float y = ws[h][x] * step_of(d[u][x], g);
                             hi[h][x] = upper_limb(y);
                             lo[h][x] = y - hi[h][x];
                         }
@@ -434,13 +458,9 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
                             b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
                         }
-                        if (g < 0) {
-                            mma_f16(oo, m[u][0], m[u][0], m[u][1], m[u][1], b0, b1);
-                        } else {
-                            const uint32_t a0 = v0[g < 0 ? 0 : g], a1 = v1[g < 0 ? 0 : g], x0 = a0 >> 8, x1 = a1 >> 8;
-                            mma_f16(o[g < 0 ? 0 : g][0], a0 & kLow, a0 & kHigh, a1 & kLow, a1 & kHigh, b0, b1);
-                            mma_f16(o[g < 0 ? 0 : g][1], x0 & kLow, x0 & kHigh, x1 & kLow, x1 & kHigh, b0, b1);
-                        }
+                        const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
+                        mma_f16(o[g][0], numbers_f16<0>(v0[g]), numbers_f16<4>(v0[g]), numbers_f16<0>(v1[g]), numbers_f16<4>(v1[g]), b0, b1);
+                        mma_f16(o[g][1], numbers_f16<0>(x0), numbers_f16<4>(x0), numbers_f16<0>(x1), numbers_f16<4>(x1), b0, b1);
                     }
                 }
             }
@@ -454,14 +474,13 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
+            for (int x = 4; x < 32; x <<= 1) {
+                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
+#pragma unroll
+                for (int g = 0; g < NG; g++) offset[h][g] += __shfl_xor_sync(0xffffffffu, offset[h][g], x);
+            }
         }
-        float offset[HPL][NG];  // row g of the offsets' part: lanes 4 g + t
-#pragma unroll
-        for (int h = 0; h < HPL; h++)
-#pragma unroll
-            for (int g = 0; g < NG; g++) offset[h][g] = __shfl_sync(0xffffffffu, HPL == 1 ? oo[0] + oo[1] : oo[h], 4 * g + t);
-        const float unscale = vscale == 0.f ? 0.f : 16777216.f / vscale;
+        const float unscale = vscale == 0.f ? 0.f : 1.f / vscale;
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
             const int head = HPL * t + h;
@@ -472,7 +491,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const float *c = &o[g][x >> 1][2 * (x & 1)];
-                    v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], x & 1 ? unscale * 0.0625f : unscale, offset[h][g]);
+                    v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], unscale, offset[h][g]);
                 }
                 *reinterpret_cast<float4 *>(mg_o + (warp * G + head) * Smem::kMergeRow + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
             }

@@ -15,9 +15,9 @@
 //   values  codes  half word [position][group][u], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group; the 16-byte pieces of a position, one per
 //                  group, are permuted so that eight positions' pieces of one group lie on different banks
 //           d      half word [position][group]
-//           m      half word [group][position]
+//           m      half word [position][group]
 // Every piece lies as the MMAs of decode attention want it: lane (g, t) of a warp finds the numbers of all groups of position g of the keys at 16 * lane
-// (8 * lane for heads of 64), those of the values come by ldmatrix, and the offsets are operands of an MMA as they are.
+// (8 * lane for heads of 64), those of the values come by ldmatrix, and the keys' offsets are operands of an MMA as they are.
 #pragma once
 #include <stdint.h>
 #include <string.h>
@@ -36,7 +36,7 @@ JHD int q4_k_offset(int hd, int p, int g) { return 9 * hd + (p * (hd / kQ4Group)
 JHD int q4_v_piece(int hd, int p, int g) { return g ^ (hd == 128 ? p >> 1 & 3 : p >> 2 & 1); }
 JHD int q4_v_code(int hd, int p, int u, int g) { return 10 * hd + p * (hd / 2) + q4_v_piece(hd, p, g) * 16 + u * 2; }
 JHD int q4_v_step(int hd, int p, int g) { return 18 * hd + (p * (hd / kQ4Group) + g) * 2; }
-JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (g * 16 + p) * 2; }
+JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (p * (hd / kQ4Group) + g) * 2; }
 // Where number e of the eight of a key word lies: an AND with 0x000f000f leaves numbers 0 and 1 as the halves of an operand register, the
 // next ones follow at 4, 8 and 12 bits.
 JHD int q4_k_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }
