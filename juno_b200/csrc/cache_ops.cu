@@ -202,26 +202,27 @@ __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace 
             float inv;  // 1 / (15 d): 15 d has 12 bits
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d * 15.f));
             inv = d > 0.f ? inv : 0.f;
-            uint32_t w = 0, ones = 0;  // the numbers come with the bits of 1.5 * 2^23, which are taken off the sum
+            uint32_t bits[8];
             float worst = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float part = __saturatef((x[e] - m) * inv), near = fmaf(part, 15.f, 12582912.f);
-                const int shift = V ? 4 * e : q4_k_shift(e);
-                w += __float_as_uint(near) << shift;
-                ones += 0x4b400000u << shift;
+                bits[e] = __float_as_uint(near) - 0x4b400000u;
                 worst = fmaxf(worst, fabsf(fmaf(part, 15.f, 12582912.f - near)));
             }
-            w -= ones;
-            if (worst > 0.49998474f) {  // as in q4_number
-                w = 0;
-#pragma unroll 1
-                for (int e = 0; e < 8; e++) {
-                    float v = x[0];
+            auto word = [](const uint32_t (&q)[8]) {
+                if (V) return q4_v_pack(q[0], q[1], q[2], q[3]) | q4_v_pack(q[4], q[5], q[6], q[7]) << 16;
+                uint32_t w = 0;
 #pragma unroll
-                    for (int k = 1; k < 8; k++) v = e == k ? x[k] : v;
-                    w |= (uint32_t)q4_number_exact(v, m, d, inv * 15.f) << (V ? 4 * e : q4_k_shift(e));
-                }
+                for (int e = 0; e < 8; e++) w |= q[e] << q4_k_shift(e);
+                return w;
+            };
+            uint32_t w = word(bits);
+            if (worst > 0.49998474f) {  // as in q4_number
+                uint32_t q[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) q[e] = (uint32_t)q4_number_exact(x[e], m, d, inv * 15.f);
+                w = word(q);
             }
             if (vec >= H || !at.page) continue;
             const int pp = at.pos & 15;
@@ -279,8 +280,9 @@ __device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&
             const float mf = __half2float(m[n]), df = __bfloat162float(d[n]);
             float4 x;
             if constexpr (V) {
-                x = make_float4(fmaf(df, bits_as_float(w[n], 0xfu), mf), fmaf(df * 0x1p-4f, bits_as_float(w[n], 0xf0u), mf),
-                                fmaf(df * 0x1p-8f, bits_as_float(w[n], 0xf00u), mf), fmaf(df * 0x1p-12f, bits_as_float(w[n], 0xf000u), mf));
+                const uint32_t turned = w[n] >> 8 | w[n] << 8;
+                x = make_float4(fmaf(df * 0x1p-6f, bits_as_float(w[n], 0x3c0u), mf), fmaf(df * 0x1p-10f, bits_as_float(w[n], 0x3c00u), mf),
+                                fmaf(df * 0x1p-2f, bits_as_float(w[n], 0x3cu), mf), fmaf(df * 0x1p-6f, bits_as_float(turned, 0x3c0u), mf));
             } else {
                 const uint32_t y = w[n] >> (8 * (piece & 1));
                 x = make_float4(fmaf(df, bits_as_float(y, 0xfu), mf), fmaf(df * 0x1p-16f, bits_as_float(y, 0xf0000u), mf),

@@ -92,13 +92,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t &r0, uint32_t &r1, ui
 }
 // The steps of groups g and g + 1 (g even) lie in one word; a BF16 number is the upper half of an FP32 one.
 __device__ __forceinline__ float step_of(const uint32_t *words, int g) { return __uint_as_float(g & 1 ? words[g >> 1] & 0xffff0000u : words[g >> 1] << 16); }
-// Numbers in bits 0..3 (SHIFT = 0) or 4..7 of both halves as FP16: with the exponent put before them they are 1024 + q, or 64 + q.
-template <int SHIFT>
-__device__ __forceinline__ uint32_t numbers_f16(uint32_t w) {
-    const uint32_t with = SHIFT ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u, off = SHIFT ? 0x54005400u : 0x64006400u;
-    const __half2 q = __hsub2(*reinterpret_cast<const __half2 *>(&with), *reinterpret_cast<const __half2 *>(&off));
-    return *reinterpret_cast<const uint32_t *>(&q);
-}
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
 __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
@@ -458,9 +451,9 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
                             b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
                         }
-                        const uint32_t x0 = v0[g] >> 8, x1 = v1[g] >> 8;
-                        mma_f16(o[g][0], numbers_f16<0>(v0[g]), numbers_f16<4>(v0[g]), numbers_f16<0>(v1[g]), numbers_f16<4>(v1[g]), b0, b1);
-                        mma_f16(o[g][1], numbers_f16<0>(x0), numbers_f16<4>(x0), numbers_f16<0>(x1), numbers_f16<4>(x1), b0, b1);
+                        constexpr uint32_t kTop = 0x03c003c0u;
+                        mma_f16(o[g][0], v0[g] & kTop, v0[g] >> 4 & kTop, v1[g] & kTop, v1[g] >> 4 & kTop, b0, b1);
+                        mma_f16(o[g][1], v0[g] << 4 & kTop, __byte_perm(v0[g], 0, 0x2301) & kTop, v1[g] << 4 & kTop, __byte_perm(v1[g], 0, 0x2301) & kTop, b0, b1);
                     }
                 }
             }
@@ -480,7 +473,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 for (int g = 0; g < NG; g++) offset[h][g] += __shfl_xor_sync(0xffffffffu, offset[h][g], x);
             }
         }
-        const float unscale = vscale == 0.f ? 0.f : 1.f / vscale;
+        const float unscale = vscale == 0.f ? 0.f : 262144.f / vscale;  // 2^18
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
             const int head = HPL * t + h;

@@ -25,6 +25,14 @@ def test_a_block_holds_every_number_and_factor_once(host, hd):
     assert (nibbles == 1).all()
 
 
+def test_the_numbers_of_a_unit(host):
+    out = (C.c_int * 4)()
+    for n in range(1 << 16):
+        want = [n >> 4 * i & 15 for i in range(4)]
+        host.q4_host_unit(*want, out)
+        assert list(out) == want
+
+
 def _nearest(x, m, d):
     """In rational numbers: the whole number nearest to (x - m) / d, ties to even, within [0, 15]."""
     return max(0, min(15, round((Fraction(float(x)) - Fraction(float(m))) / Fraction(float(d)))))
