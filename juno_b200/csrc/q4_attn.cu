@@ -331,12 +331,13 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                         for (int x = 0; x < 2; x++)
                             if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
             }
-            uint32_t d[kQ4Tile][2][NW], steps = limit;
+            uint32_t d[kQ4Tile][2][NW], vm[kQ4Tile][2][NW], steps = limit;
 #pragma unroll
             for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
+                    lds_words<NW>(vm[u][x], tile + u * BLOCK + 19 * HD + (g8 + 8 * x) * NG * 2);
                 }
             if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
 #pragma unroll
@@ -347,7 +348,10 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                         for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
 #pragma unroll
-                        for (int g = 0; g < NW; g++) d[u][x][g] = on ? d[u][x][g] : 0u;
+                        for (int g = 0; g < NW; g++) {
+                            d[u][x][g] = on ? d[u][x][g] : 0u;
+                            vm[u][x][g] = on ? vm[u][x][g] : 0u;
+                        }
                     }
             }
 #pragma unroll
@@ -416,13 +420,9 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 // numbers' are often large and of opposite sign
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    uint32_t m[NW];
-                    lds_words<NW>(m, tile + u * BLOCK + 19 * HD + (g8 + 8 * x) * NG * 2);
-                    const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
 #pragma unroll
                     for (int g = 0; g < NG; g += 2) {
-                        const uint32_t pair = on ? m[g >> 1] : 0u;
-                        const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&pair));
+                        const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&vm[u][x][g >> 1]));
 #pragma unroll
                         for (int h = 0; h < HPL; h++) {
                             offset[h][g] = fmaf(w[h][x], two.x, offset[h][g]);
