@@ -226,6 +226,7 @@ __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace 
             }
             if (vec >= H || !at.page) continue;
             const int pp = at.pos & 15;
+            if (V) w ^= q4_v_flip(pp);
             uint8_t *block = at.page + h * q4_block_bytes(HD);
             *reinterpret_cast<uint32_t *>(block + (V ? q4_v_code(HD, pp, 2 * (sub & 3), g) : q4_k_code(HD, pp, sub & 3, g))) = w;
             if (!V && sub == 0 && at.track >= 0) p.weights[(((size_t)at.track * p.n_layers + p.layer) * H + h) * p.track_tokens + at.pos] = 0.f;
@@ -270,7 +271,7 @@ __device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&
             m[n] = *reinterpret_cast<const __half *>(block + (V ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g)));
             d[n] = *reinterpret_cast<const __nv_bfloat16 *>(block + (V ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g)));
             if constexpr (V)
-                w[n] = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g));
+                w[n] = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g)) ^ (q4_v_flip(pp) & 0xffffu);
             else
                 w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g));
         }
@@ -563,23 +564,27 @@ struct Q4Piece {
         }
     }
     __device__ __forceinline__ int place(int pp) const { return at + pp * stride + (kind == 1 ? 16 * q4_v_piece(HD, pp, group) : 0); }
+    static __device__ __forceinline__ void flip(uint4 &v, int pp) {
+        const uint32_t f = q4_v_flip(pp);
+        v = make_uint4(v.x ^ f, v.y ^ f, v.z ^ f, v.w ^ f);
+    }
     __device__ __forceinline__ uint4 load(const uint8_t *block, int pp) const {
         const uint8_t *b = block + place(pp);
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (kind <= 1)
+        if (kind <= 1) {
             v = *reinterpret_cast<const uint4 *>(b);
-        else if (kind == 2 && NG == 4) {
+            if (kind == 1) flip(v, pp);
+        } else if (kind == 2 && NG == 4) {
             const uint2 y = *reinterpret_cast<const uint2 *>(b);
             v.x = y.x;
             v.y = y.y;
         } else if (kind == 2)
             v.x = *reinterpret_cast<const uint32_t *>(b);
-        else if (kind == 3)
-            v.x = *reinterpret_cast<const uint16_t *>(b);
         return v;
     }
     __device__ __forceinline__ void store(uint8_t *block, int pp, uint4 v) const {
         uint8_t *b = block + place(pp);
+        if (kind == 1) flip(v, pp);
         if (kind <= 1)
             *reinterpret_cast<uint4 *>(b) = v;
         else if (kind == 2 && NG == 4)

@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
             for (int g = 0; g < NG; g++) offset[h][g] = 0.f;
         }
+        const float fifteen = g8 & 1 ? 15.f : 0.f;
         constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
         for (int j = 0; j < n_tiles; j++, pos0 += W * kQ4Tile * kPageTokens) {
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
-                        ws[h][x] = w[h][x] * vscale;
+                        ws[h][x] = w[h][x] * (g8 & 1 ? -vscale : vscale);  // odd positions: 15 - q
                     }
                     l_run[h] += w[h][0] + w[h][1];
                 }
@@ -423,10 +424,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                     for (int g = 0; g < NG; g += 2) {
                         const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&vm[u][x][g >> 1]));
+                        const float m0 = fmaf(step_of(d[u][x], g), fifteen, two.x), m1 = fmaf(step_of(d[u][x], g + 1), fifteen, two.y);
 #pragma unroll
                         for (int h = 0; h < HPL; h++) {
-                            offset[h][g] = fmaf(w[h][x], two.x, offset[h][g]);
-                            offset[h][g + 1] = fmaf(w[h][x], two.y, offset[h][g + 1]);
+                            offset[h][g] = fmaf(w[h][x], m0, offset[h][g]);
+                            offset[h][g + 1] = fmaf(w[h][x], m1, offset[h][g + 1]);
                         }
                     }
                 }

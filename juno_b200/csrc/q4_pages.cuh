@@ -12,7 +12,8 @@
 //   keys    codes  word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group
 //           d      half word [position][group]
 //           m      half word [position][group]
-//   values  codes  half word [position][group][u], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group (q4_v_pack); the 16-byte pieces of a position, one per
+//   values  codes  half word [position][group][u], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group (q4_v_pack), in odd positions as
+//                  15 - q: decode attention adds up (m + 15 d) - d (15 - q) there, so that its sums of numbers do not grow all one way; the 16-byte pieces of a position, one per
 //                  group, are permuted so that eight positions' pieces of one group lie on different banks
 //           d      half word [position][group]
 //           m      half word [position][group]
@@ -40,6 +41,8 @@ JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (p * (hd / kQ4Group
 // Four numbers of a unit: the first in bits 6..9, the second and third four bits higher and lower, the fourth's lower half in bits 14 and 15, its upper half in
 // bits 0 and 1.  Shifted by 4 either way, or with its bytes changed round, the half word has each of them in bits 6..9.
 JHD uint32_t q4_v_pack(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a << 6 | b << 10 | c << 2 | (d & 3u) << 14 | d >> 2; }
+// 15 - q for q, all numbers of a word: what an XOR with this does.
+JHD uint32_t q4_v_flip(int p) { return p & 1 ? 0xffffffffu : 0u; }
 // Where number e of the eight of a key word lies: an AND with 0x000f000f leaves numbers 0 and 1 as the halves of an operand register, the
 // next ones follow at 4, 8 and 12 bits.
 JHD int q4_k_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }

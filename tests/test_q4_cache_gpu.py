@@ -216,6 +216,38 @@ def test_attention_of_long_contexts(ctx, n, heads, kv, dim):
     cache.close()
 
 
+# Zero-mean values in a long context: the result is smaller than the sum of the weighted magnitudes by the root of the number of positions that count, so an error
+# that goes one way (sums cut off instead of rounded) shows.  In 64 bits from the rows that the pages hold.  What the kernel rounds: a score's 5 to 9 sums and products
+# in FP32, each to 2^-24 of terms up to 30 in size, together about 2e-6 of a weight, at random over the positions; weights in limbs, 2^-22.  So about 2e-6 of the
+# result's length; 1e-5 leaves a factor of five.  Sums cut off at 2^-24 give 1e-4 here.
+@pytest.mark.parametrize("n,batch,heads,kv,dim", [(65536, 1, 32, 8, 128), (16384, 7, 32, 4, 128), (9001, 16, 16, 4, 64), (30000, 5, 24, 4, 64), (12000, 40, 2, 1, 64)])
+def test_long_sums_are_not_biased(ctx, n, batch, heads, kv, dim):
+    g = torch.Generator("cuda")
+    g.manual_seed(n)
+    draw = lambda *shape: torch.randn(shape, generator=g, device="cuda")  # noqa: E731
+    cache = PagedKvCache(ctx, 1, kv, dim, batch * (n // 16 + 1), "q4")
+    try:
+        seqs = [cache.new_sequence(n) for _ in range(batch)]
+        k = draw(batch * n, kv, dim) * (0.5 * draw(kv, dim)).exp() + 0.5 * draw(kv, dim)
+        v, q = 0.5 * draw(batch * n, kv * dim), 1.5 * draw(batch, heads * dim)
+        held_k, held_v, out = torch.empty_like(v), torch.empty_like(v), torch.empty_like(q)
+        settle()
+        cache.append_device(0, seqs, [0] * batch, [n] * batch, k.flatten(1), v)
+        cache.read_device(0, seqs, [0] * batch, [n] * batch, held_k, held_v)
+        cache.attention_device(0, seqs, q, heads, out)
+        ctx.synchronize()
+        for i in range(batch):
+            for h in range(kv):
+                of = lambda x: x[i * n:(i + 1) * n, h * dim:(h + 1) * dim].double()  # noqa: E731
+                mine = slice(h * heads // kv * dim, (h + 1) * heads // kv * dim)
+                x = q[i, mine].double().view(-1, dim) @ of(held_k).T / dim ** 0.5
+                ref = torch.softmax(x, -1) @ of(held_v)
+                error = (out[i, mine].double().view(-1, dim) - ref).norm(dim=-1) / ref.norm(dim=-1)
+                assert error.max() <= 1e-5, (i, h, error)
+    finally:
+        cache.close()
+
+
 def test_attention_of_many_short_sequences_and_of_parts(ctx):
     """More sequences than travel with a launch; a prompt's rows: one sequence many times, each time one position more, none at first."""
     rng = np.random.default_rng(11)
