@@ -210,13 +210,7 @@ __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace 
                 bits[e] = __float_as_uint(near) - 0x4b400000u;
                 worst = fmaxf(worst, fabsf(fmaf(part, 15.f, 12582912.f - near)));
             }
-            auto word = [](const uint32_t (&q)[8]) {
-                if (V) return q4_v_pack(q[0], q[1], q[2], q[3]) | q4_v_pack(q[4], q[5], q[6], q[7]) << 16;
-                uint32_t w = 0;
-#pragma unroll
-                for (int e = 0; e < 8; e++) w |= q[e] << q4_k_shift(e);
-                return w;
-            };
+            auto word = [](const uint32_t (&q)[8]) { return q4_unit(q[0], q[1], q[2], q[3]) | q4_unit(q[4], q[5], q[6], q[7]) << 16; };
             uint32_t w = word(bits);
             if (worst > 0.49998474f) {  // as in q4_number
                 uint32_t q[8];
@@ -270,25 +264,16 @@ __device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&
             const uint8_t *block = at.page + h * q4_block_bytes(HD);
             m[n] = *reinterpret_cast<const __half *>(block + (V ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g)));
             d[n] = *reinterpret_cast<const __nv_bfloat16 *>(block + (V ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g)));
-            if constexpr (V)
-                w[n] = *reinterpret_cast<const uint16_t *>(block + q4_v_code(HD, pp, piece, g)) ^ (q4_v_flip(pp) & 0xffffu);
-            else
-                w[n] = *reinterpret_cast<const uint32_t *>(block + q4_k_code(HD, pp, piece >> 1, g));
+            w[n] = *reinterpret_cast<const uint16_t *>(block + (V ? q4_v_code(HD, pp, piece, g) : q4_k_code(HD, pp, piece >> 1, g) + 2 * (piece & 1)));
+            if (V) w[n] ^= q4_v_flip(pp) & 0xffffu;
         }
 #pragma unroll
         for (int n = 0; n < kReadRows; n++) {
             if (n >= n_rows) break;
             const float mf = __half2float(m[n]), df = __bfloat162float(d[n]);
-            float4 x;
-            if constexpr (V) {
-                const uint32_t turned = w[n] >> 8 | w[n] << 8;
-                x = make_float4(fmaf(df * 0x1p-6f, bits_as_float(w[n], 0x3c0u), mf), fmaf(df * 0x1p-10f, bits_as_float(w[n], 0x3c00u), mf),
-                                fmaf(df * 0x1p-2f, bits_as_float(w[n], 0x3cu), mf), fmaf(df * 0x1p-6f, bits_as_float(turned, 0x3c0u), mf));
-            } else {
-                const uint32_t y = w[n] >> (8 * (piece & 1));
-                x = make_float4(fmaf(df, bits_as_float(y, 0xfu), mf), fmaf(df * 0x1p-16f, bits_as_float(y, 0xf0000u), mf),
-                                fmaf(df * 0x1p-4f, bits_as_float(y, 0xf0u), mf), fmaf(df * 0x1p-16f, bits_as_float(y >> 4, 0xf0000u), mf));
-            }
+            const uint32_t turned = w[n] >> 8 | w[n] << 8;
+            const float4 x = make_float4(fmaf(df * 0x1p-6f, bits_as_float(w[n], 0x3c0u), mf), fmaf(df * 0x1p-10f, bits_as_float(w[n], 0x3c00u), mf),
+                                         fmaf(df * 0x1p-2f, bits_as_float(w[n], 0x3cu), mf), fmaf(df * 0x1p-6f, bits_as_float(turned, 0x3c0u), mf));
             if (vec4) {
                 *reinterpret_cast<float4 *>(to) = x;
             } else {

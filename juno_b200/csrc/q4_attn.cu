@@ -51,6 +51,11 @@ constexpr int kQ4Warps = HPL == 1 || HD == 64 ? 8 : 4;
 template <int HD, int HPL>
 constexpr int kQ4Ctas = HPL == 1 || HD == 64 ? 2 : 3;
 
+// Tiles whose products are added up in an MMA's sums: an MMA cuts off what lies more than 24 bits below the sum, so that a long chain of them falls behind by
+// 2^-25 of it a time.  After 32 the sums go to FP32 ones in shared memory.
+template <int HPL>
+constexpr int kQ4Chain = HPL == 1 ? 16 : 8;
+
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -92,6 +97,14 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t &r0, uint32_t &r1, ui
 }
 // The steps of groups g and g + 1 (g even) lie in one word; a BF16 number is the upper half of an FP32 one.
 __device__ __forceinline__ float step_of(const uint32_t *words, int g) { return __uint_as_float(g & 1 ? words[g >> 1] & 0xffff0000u : words[g >> 1] << 16); }
+// Two units' numbers, each pair as two halves: q 2^-18.
+__device__ __forceinline__ void numbers_of(uint32_t units, uint32_t (&x)[4]) {
+    constexpr uint32_t kTop = 0x03c003c0u;
+    x[0] = units & kTop;
+    x[1] = units >> 4 & kTop;
+    x[2] = units << 4 & kTop;
+    x[3] = __byte_perm(units, 0, 0x2301) & kTop;
+}
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
 __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
@@ -122,7 +135,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
     const int kvh = blockIdx.x % p.n_kv_heads, share = blockIdx.x / p.n_kv_heads, G = p.n_heads / p.n_kv_heads, h0 = kvh * G;
     const uint32_t ring = smem_u32(smem) + warp * kQ4Slots * TILE, bars = smem_u32(smem) + Smem::kBars + warp * kQ4Slots * 8;
     float *mg_o = reinterpret_cast<float *>(smem + Smem::kMerge);  // where the warps meet: [warp][head][kMergeRow], [warp][head], [warp][head]
-    float *mg_m = mg_o + W * G * Smem::kMergeRow, *mg_l = mg_m + W * G;
+    float *mg_m = mg_o + W * HEADS * Smem::kMergeRow, *mg_l = mg_m + W * HEADS;
     __half *q_s = reinterpret_cast<__half *>(smem + Smem::kQuery);    // [limb][head][kQueryRow]
     __half *sums_s = reinterpret_cast<__half *>(smem + Smem::kSums);  // [limb][head][4]: the query's sums over groups, scaled
     float *back_s = reinterpret_cast<float *>(smem + Smem::kBack);    // [head]: what takes the scale of the scores back
@@ -200,7 +213,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         const int pos_end = min(r.upto, (to - r.first) << 4);  // of this part, in the row
         const bool track = TRACK && r.track >= 0;
         // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
-        // largest element), in two FP16 limbs.  Elements 2, 3, 6, 7 of eight meet 16 q.
+        // largest element), in two FP16 limbs; number i of the first unit of eight is next to that of the second.
 #pragma unroll
         for (int n = 0; n < QUERIES; n++) {
             const int head = warp + n * W;
@@ -221,13 +234,13 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127)), up = 13 - e2;
             const float shift = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float s = (E * lane + e) & 2 ? shift * 0.0625f : shift, y0 = y[e] * s, y1 = y[e + 1] * s;
-                const uint32_t hi = pack_h2(y0, y1);
-                const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                uint32_t *to_q = reinterpret_cast<uint32_t *>(q_s + head * Smem::kQueryRow + E * lane + e);
+            for (int e = 0; e < E; e++) {
+                const int dim = E * lane + e;
+                const float whole = y[e] * shift;
+                const __half hi = __float2half_rn(whole);
+                __half *to_q = q_s + head * Smem::kQueryRow + (dim & ~7) + (dim & 3) * 2 + (dim >> 2 & 1);
                 to_q[0] = hi;
-                to_q[HEADS * Smem::kQueryRow / 2] = pack_h2(y0 - hf.x, y1 - hf.y);
+                to_q[HEADS * Smem::kQueryRow] = __float2half_rn(whole - __half2float(hi));
             }
             if (lane % (kQ4Group / E) == 0) {  // 32 elements of up to 2^14: five powers of two less
                 const float whole = sum * (shift * 0.03125f);
@@ -238,7 +251,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             if (lane == 0) back_s[head] = __uint_as_float((uint32_t)(127 + 5 - up) << 23);
         }
         __syncthreads();
-        // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8, as the B operand wants them
+        // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8
         uint32_t qh[NG][4], ql[HPL == 2 ? NG : 1][4];
         uint32_t qsum[HPL];  // k: the groups
         float back[HPL];     // of this lane's own heads
@@ -268,8 +281,37 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             for (int g = 0; g < NG; g++) offset[h][g] = 0.f;
         }
         const float fifteen = g8 & 1 ? 15.f : 0.f;
-        constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
+        // The sums so far to where the warps meet, in FP32, the offsets' part with them at the end.
+        bool put = false;
+        auto put_by = [&](bool end) {
+            const float unscale = vscale == 0.f ? 0.f : 262144.f / vscale;  // 2^18
+#pragma unroll
+            for (int h = 0; h < HPL; h++)
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    float4 *to = reinterpret_cast<float4 *>(mg_o + (warp * HEADS + HPL * t + h) * Smem::kMergeRow + g * kQ4Group + 4 * g8);  // dimensions 4 g8 .. 4 g8 + 3 of the group
+                    float v[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const float *c = &o[g][x >> 1][2 * (x & 1)];
+                        v[x] = (HPL == 1 ? c[0] + c[1] : c[h]) * unscale + (end ? offset[h][g] : 0.f);
+                    }
+                    if (put) {
+                        const float4 before = *to;
+                        v[0] += before.x;
+                        v[1] += before.y;
+                        v[2] += before.z;
+                        v[3] += before.w;
+                    }
+                    *to = make_float4(v[0], v[1], v[2], v[3]);
+                }
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[g][0][x] = o[g][1][x] = 0.f;
+            put = true;
+        };
         for (int j = 0; j < n_tiles; j++, pos0 += W * kQ4Tile * kPageTokens) {
             mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
             if (__any_sync(0xffffffffu, failed)) {
@@ -300,15 +342,17 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
                     float c[4];
-                    const uint32_t x0 = k0[g] >> 8, x1 = k1[g] >> 8;
-                    mma_f16_first(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, qh[g][0], qh[g][1]);
-                    mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, qh[g][2], qh[g][3]);
+                    uint32_t x0[4], x1[4];
+                    numbers_of(k0[g], x0);
+                    numbers_of(k1[g], x1);
+                    mma_f16_first(c, x0[0], x1[0], x0[1], x1[1], qh[g][0], qh[g][1]);
+                    mma_f16(c, x0[2], x1[2], x0[3], x1[3], qh[g][2], qh[g][3]);
                     if constexpr (HPL == 1) {
                         c[0] += c[1];
                         c[1] = c[2] + c[3];
                     } else {
-                        mma_f16(c, k0[g] & kLow, k1[g] & kLow, k0[g] & kHigh, k1[g] & kHigh, ql[g][0], ql[g][1]);
-                        mma_f16(c, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, ql[g][2], ql[g][3]);
+                        mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[g][0], ql[g][1]);
+                        mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[g][2], ql[g][3]);
                     }
 #pragma unroll
                     for (int h = 0; h < HPL; h++) {
@@ -316,11 +360,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                         sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
                     }
                 }
-                // 2^24 of the numbers, 2^-up; the sums' 2^5 2^-up
+                // 2^18 of the numbers, 2^-up; the sums' 2^5 2^-up
 #pragma unroll
                 for (int h = 0; h < HPL; h++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 524288.f, off[x * HPL + h]) * back[h];
+                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 8192.f, off[x * HPL + h]) * back[h];
             }
             if (track) {
                 float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
@@ -393,6 +437,16 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 for (int h = 0; h < HPL; h++)
 #pragma unroll
                     for (int g = 0; g < NG; g++) offset[h][g] *= fix[h];
+                if (put) {
+#pragma unroll
+                    for (int h = 0; h < HPL; h++)
+#pragma unroll
+                        for (int g = 0; g < NG; g++) {
+                            float4 *at = reinterpret_cast<float4 *>(mg_o + (warp * HEADS + HPL * t + h) * Smem::kMergeRow + g * kQ4Group + 4 * g8);
+                            const float4 y = *at;
+                            *at = make_float4(y.x * fix[h], y.y * fix[h], y.z * fix[h], y.w * fix[h]);
+                        }
+                }
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -453,14 +507,17 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
                             b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
                         }
-                        constexpr uint32_t kTop = 0x03c003c0u;
-                        mma_f16(o[g][0], v0[g] & kTop, v0[g] >> 4 & kTop, v1[g] & kTop, v1[g] >> 4 & kTop, b0, b1);
-                        mma_f16(o[g][1], v0[g] << 4 & kTop, __byte_perm(v0[g], 0, 0x2301) & kTop, v1[g] << 4 & kTop, __byte_perm(v1[g], 0, 0x2301) & kTop, b0, b1);
+                        uint32_t x0[4], x1[4];
+                        numbers_of(v0[g], x0);
+                        numbers_of(v1[g], x1);
+                        mma_f16(o[g][0], x0[0], x0[1], x1[0], x1[1], b0, b1);
+                        mma_f16(o[g][1], x0[2], x0[3], x1[2], x1[3], b0, b1);
                     }
                 }
             }
             __syncwarp();  // all lanes have read the tile before it is filled again
             if (part_issued < part_tiles) issue();
+            if (j % kQ4Chain<HPL> == kQ4Chain<HPL> - 1) put_by(false);
         }
         const CacheRow now = r;
         from = to;
@@ -475,31 +532,20 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 for (int g = 0; g < NG; g++) offset[h][g] += __shfl_xor_sync(0xffffffffu, offset[h][g], x);
             }
         }
-        const float unscale = vscale == 0.f ? 0.f : 262144.f / vscale;  // 2^18
+        put_by(true);
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
             const int head = HPL * t + h;
-            if (head >= G) continue;
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                float v[4];  // dimensions 4 g8 .. 4 g8 + 3 of the group
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const float *c = &o[g][x >> 1][2 * (x & 1)];
-                    v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], unscale, offset[h][g]);
-                }
-                *reinterpret_cast<float4 *>(mg_o + (warp * G + head) * Smem::kMergeRow + g * kQ4Group + 4 * g8) = make_float4(v[0], v[1], v[2], v[3]);
-            }
             if (g8 == 0) {
-                mg_m[warp * G + head] = m_run[h];
-                mg_l[warp * G + head] = l_run[h];
+                mg_m[warp * HEADS + head] = m_run[h];
+                mg_l[warp * HEADS + head] = l_run[h];
             }
         }
         __syncthreads();
         const int parts = row_parts(p, i, now);
         for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {  // two dimensions of a head; a head to a warp, whose first lanes have the warps' shares of it
             const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
-            float mw = lane < W ? mg_m[lane * G + g] : -INFINITY, lw = lane < W ? mg_l[lane * G + g] : 0.f, M = mw;
+            float mw = lane < W ? mg_m[lane * HEADS + g] : -INFINITY, lw = lane < W ? mg_l[lane * HEADS + g] : 0.f, M = mw;
 #pragma unroll
             for (int x = 1; x < W; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
             M = __shfl_sync(0xffffffffu, M, 0);
@@ -511,7 +557,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
             for (int w = 0; w < W; w++) {
                 const float f = __shfl_sync(0xffffffffu, fw, w);
-                const float2 v = *reinterpret_cast<const float2 *>(mg_o + (w * G + g) * Smem::kMergeRow + d);
+                const float2 v = *reinterpret_cast<const float2 *>(mg_o + (w * HEADS + g) * Smem::kMergeRow + d);
                 if (f != 0.f) {
                     ax = fmaf(v.x, f, ax);
                     ay = fmaf(v.y, f, ay);

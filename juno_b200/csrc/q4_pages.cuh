@@ -9,12 +9,12 @@
 // A NaN makes its group NaN (m is NaN, d 0).
 //
 // The pages of a head (16 positions) are one block of 20 * hd bytes, [layer][page][kv_head] in the pool:
-//   keys    codes  word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group
+//   keys    codes  word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group, a unit of four to a half word
 //           d      half word [position][group]
 //           m      half word [position][group]
-//   values  codes  half word [position][group][u], u = 0..7: the numbers of dimensions 4u .. 4u + 3 of the group (q4_v_pack), in odd positions as
-//                  15 - q: decode attention adds up (m + 15 d) - d (15 - q) there, so that its sums of numbers do not grow all one way; the 16-byte pieces of a position, one per
-//                  group, are permuted so that eight positions' pieces of one group lie on different banks
+//   values  codes  half word [position][group][u], u = 0..7: the unit of dimensions 4u .. 4u + 3 of the group, in odd positions of 15 - q: decode attention adds
+//                  up (m + 15 d) - d (15 - q) there, so that its sums of numbers do not grow all one way; the 16-byte pieces of a position, one per group, are
+//                  permuted so that eight positions' pieces of one group lie on different banks
 //           d      half word [position][group]
 //           m      half word [position][group]
 // Every piece lies as the MMAs of decode attention want it: lane (g, t) of a warp finds the numbers of all groups of position g of the keys at 16 * lane
@@ -38,14 +38,12 @@ JHD int q4_v_piece(int hd, int p, int g) { return g ^ (hd == 128 ? p >> 1 & 3 : 
 JHD int q4_v_code(int hd, int p, int u, int g) { return 10 * hd + p * (hd / 2) + q4_v_piece(hd, p, g) * 16 + u * 2; }
 JHD int q4_v_step(int hd, int p, int g) { return 18 * hd + (p * (hd / kQ4Group) + g) * 2; }
 JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (p * (hd / kQ4Group) + g) * 2; }
-// Four numbers of a unit: the first in bits 6..9, the second and third four bits higher and lower, the fourth's lower half in bits 14 and 15, its upper half in
-// bits 0 and 1.  Shifted by 4 either way, or with its bytes changed round, the half word has each of them in bits 6..9.
-JHD uint32_t q4_v_pack(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a << 6 | b << 10 | c << 2 | (d & 3u) << 14 | d >> 2; }
+// A unit: the first number in bits 6..9, the second and third four bits higher and lower, the fourth's lower half in bits 14 and 15, its upper half in bits 0
+// and 1.  Shifted by 4 either way, or with its bytes changed round, the half word has each of them in bits 6..9, the upper bits of an FP16 number's
+// fraction: with an AND it is the FP16 number q 2^-18.
+JHD uint32_t q4_unit(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a << 6 | b << 10 | c << 2 | (d & 3u) << 14 | d >> 2; }
 // 15 - q for q, all numbers of a word: what an XOR with this does.
 JHD uint32_t q4_v_flip(int p) { return p & 1 ? 0xffffffffu : 0u; }
-// Where number e of the eight of a key word lies: an AND with 0x000f000f leaves numbers 0 and 1 as the halves of an operand register, the
-// next ones follow at 4, 8 and 12 bits.
-JHD int q4_k_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }
 
 // The number of x in a group with offset m and step d, decided exactly (inv is about 1 / d).  s + r is x - m exactly; half-way points (q + 1/2) d have 13
 // bits and are exact, so that the comparisons decide what the estimate may have missed by one.

@@ -17,9 +17,9 @@ extern "C" int q4_host_cover(int hd, unsigned char *nibbles) {
     for (int p = 0; p < 16; p++)
         for (int g = 0; g < hd / kQ4Group; g++) {
             for (int t = 0; t < 4; t++)
-                for (int e = 0; e < 8; e++) mark(2 * q4_k_code(hd, p, t, g) + q4_k_shift(e) / 4);
+                for (int e = 0; e < 8; e++) mark(2 * q4_k_code(hd, p, t, g) + e);
             for (int u = 0; u < 8; u++)
-                for (int i = 0; i < 4; i++) mark(2 * q4_v_code(hd, p, u, g) + i);  // all 16 bits
+                for (int i = 0; i < 4; i++) mark(2 * q4_v_code(hd, p, u, g) + i);
             for (int b = 0; b < 4; b++) {
                 mark(2 * q4_k_step(hd, p, g) + b);
                 mark(2 * q4_k_offset(hd, p, g) + b);
@@ -32,7 +32,7 @@ extern "C" int q4_host_cover(int hd, unsigned char *nibbles) {
 
 // The four numbers of a packed unit, each from bits 6..9 of the half word as it is shifted or turned for it.
 extern "C" void q4_host_unit(int a, int b, int c, int d, int *out) {
-    const uint32_t u = q4_v_pack((uint32_t)a, (uint32_t)b, (uint32_t)c, (uint32_t)d), turned = (u >> 8 | u << 8) & 0xffffu;
+    const uint32_t u = q4_unit((uint32_t)a, (uint32_t)b, (uint32_t)c, (uint32_t)d), turned = (u >> 8 | u << 8) & 0xffffu;
     out[0] = (int)(u >> 6 & 15u);
     out[1] = (int)(u >> 4 >> 6 & 15u);
     out[2] = (int)(u << 4 >> 6 & 15u);
