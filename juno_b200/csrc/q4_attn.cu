@@ -97,12 +97,14 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t &r0, uint32_t &r1, ui
 }
 // The steps of groups g and g + 1 (g even) lie in one word; a BF16 number is the upper half of an FP32 one.
 __device__ __forceinline__ float step_of(const uint32_t *words, int g) { return __uint_as_float(g & 1 ? words[g >> 1] & 0xffff0000u : words[g >> 1] << 16); }
-// Two units' numbers, each pair as two halves: q 2^-18.
+// Two units' numbers, each pair as two halves: q 2^-18.  The third pair of the keys stays where it lies, q 2^-22, and the query's side takes the 16 back: an MMA
+// aligns subnormal operands as if they were 2^-14, so that four bits of a score's 24 or more are lost, and two instructions of 300 a page saved.
+template <bool KEYS>
 __device__ __forceinline__ void numbers_of(uint32_t units, uint32_t (&x)[4]) {
     constexpr uint32_t kTop = 0x03c003c0u;
     x[0] = units & kTop;
     x[1] = units >> 4 & kTop;
-    x[2] = units << 4 & kTop;
+    x[2] = KEYS ? units & kTop >> 4 : units << 4 & kTop;
     x[3] = __byte_perm(units, 0, 0x2301) & kTop;
 }
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
@@ -212,8 +214,8 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         const int i = row, to = min(share1, row_end(p, i)), n_tiles = part_tiles, pos_first = page0 << 4;
         const int pos_end = min(r.upto, (to - r.first) << 4);  // of this part, in the row
         const bool track = TRACK && r.track >= 0;
-        // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two (the second limb then ends 38 bits below the
-        // largest element), in two FP16 limbs; number i of the first unit of eight is next to that of the second.
+        // The query, a head to a warp: times the scale of the scores, brought to 2^13 .. 2^14 by a power of two, those of numbers that stay where they lie; a sixteenth of it the
+        // others (the second limb then ends 34 bits below the largest element), in two FP16 limbs; number i of the first unit of eight is next to that of the second.
 #pragma unroll
         for (int n = 0; n < QUERIES; n++) {
             const int head = warp + n * W;
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const int dim = E * lane + e;
-                const float whole = y[e] * shift;
+                const float whole = y[e] * ((dim & 3) == 2 ? shift : shift * 0.0625f);
                 const __half hi = __float2half_rn(whole);
                 __half *to_q = q_s + head * Smem::kQueryRow + (dim & ~7) + (dim & 3) * 2 + (dim >> 2 & 1);
                 to_q[0] = hi;
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         // The sums so far to where the warps meet, in FP32, the offsets' part with them at the end.
         bool put = false;
         auto put_by = [&](bool end) {
-            const float unscale = vscale == 0.f ? 0.f : 262144.f / vscale;  // 2^18
+            const float unscale = vscale == 0.f ? 0.f : 262144.f / fabsf(vscale);  // 2^18
 #pragma unroll
             for (int h = 0; h < HPL; h++)
 #pragma unroll
@@ -343,8 +345,8 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 for (int g = 0; g < NG; g++) {
                     float c[4];
                     uint32_t x0[4], x1[4];
-                    numbers_of(k0[g], x0);
-                    numbers_of(k1[g], x1);
+                    numbers_of<true>(k0[g], x0);
+                    numbers_of<true>(k1[g], x1);
                     mma_f16_first(c, x0[0], x1[0], x0[1], x1[1], qh[g][0], qh[g][1]);
                     mma_f16(c, x0[2], x1[2], x0[3], x1[3], qh[g][2], qh[g][3]);
                     if constexpr (HPL == 1) {
@@ -360,11 +362,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                         sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
                     }
                 }
-                // 2^18 of the numbers, 2^-up; the sums' 2^5 2^-up
+                // 2^22 of the numbers, 2^-up; the sums' 2^5 2^-up
 #pragma unroll
                 for (int h = 0; h < HPL; h++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 8192.f, off[x * HPL + h]) * back[h];
+                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 131072.f, off[x * HPL + h]) * back[h];
             }
             if (track) {
                 float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
                 if (steps > (limit & 0xffffu)) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
                     const int e = max((int)(steps >> 7) - 127, -100);
-                    const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23);
+                    const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23 | (uint32_t)(g8 & 1) << 31);  // odd positions have 15 - q
                     vfix = vscale == 0.f ? 0.f : next / vscale;
                     vscale = next;
                     limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
-                        ws[h][x] = w[h][x] * (g8 & 1 ? -vscale : vscale);  // odd positions: 15 - q
+                        ws[h][x] = w[h][x] * vscale;
                     }
                     l_run[h] += w[h][0] + w[h][1];
                 }
@@ -508,8 +510,8 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
                         }
                         uint32_t x0[4], x1[4];
-                        numbers_of(v0[g], x0);
-                        numbers_of(v1[g], x1);
+                        numbers_of<false>(v0[g], x0);
+                        numbers_of<false>(v1[g], x1);
                         mma_f16(o[g][0], x0[0], x0[1], x1[0], x1[1], b0, b1);
                         mma_f16(o[g][1], x0[2], x0[3], x1[2], x1[3], b0, b1);
                     }
