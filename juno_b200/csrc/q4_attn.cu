@@ -269,274 +269,260 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             qsum[h] = t < NW ? *reinterpret_cast<const uint32_t *>(sums_s + column * 4 + 2 * t) : 0u;
             back[h] = back_s[HPL * t + h];
         }
-        float o[NG][2][4], offset[HPL][NG], m_run[HPL], l_run[HPL], vscale = 0.f;  // offset: the offsets' part, of this lane's positions
+        float m_run[HPL], l_run[HPL], vscale = 0.f;
         uint32_t limit = 0;  // largest step in the scale's range, in both halves
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) o[g][0][x] = o[g][1][x] = 0.f;
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
             m_run[h] = -INFINITY;
             l_run[h] = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; g++) offset[h][g] = 0.f;
         }
         const float fifteen = g8 & 1 ? 15.f : 0.f;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
-        // The sums so far to where the warps meet, in FP32, the offsets' part with them at the end.
-        bool put = false;
-        auto put_by = [&](bool end) {
+        float *own_row = mg_o + (warp * HEADS + HPL * t) * Smem::kMergeRow + 4 * g8;  // of head HPL * t: dimensions 4 g8 .. 4 g8 + 3 of a group
+        int j = 0;
+        do {
+            float o[NG][2][4], offset[HPL][NG];  // offset: the offsets' part, of this lane's positions
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[g][0][x] = o[g][1][x] = 0.f;
+#pragma unroll
+                for (int h = 0; h < HPL; h++) offset[h][g] = 0.f;
+            }
+            const int first = j, chain_end = min(n_tiles, j + kQ4Chain<HPL>);
+            for (; j < chain_end; j++, pos0 += W * kQ4Tile * kPageTokens) {
+                mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
+                if (__any_sync(0xffffffffu, failed)) {
+                    failed = true;
+                    break;
+                }
+                const uint32_t tile = ring + used % kQ4Slots * TILE;
+                used++;
+                float s[HPL][kQ4Tile][2];  // rows g8 and g8 + 8 of each page
+#pragma unroll
+                for (int u = 0; u < kQ4Tile; u++) {
+                    const uint32_t base = tile + u * BLOCK;
+                    uint32_t k0[NG], k1[NG], d0[NW], d1[NW], m0[1], m1[1];
+                    lds_words<NG>(k0, base + lane * NG * 4);
+                    lds_words<NG>(k1, base + (32 + lane) * NG * 4);
+                    lds_words<NW>(d0, base + 8 * HD + g8 * NG * 2);
+                    lds_words<NW>(d1, base + 8 * HD + (g8 + 8) * NG * 2);
+                    lds_words<1>(m0, base + 9 * HD + g8 * NG * 2 + (t % NW) * 4);  // k beyond the groups: once more, times the zeros of qsum
+                    lds_words<1>(m1, base + 9 * HD + (g8 + 8) * NG * 2 + (t % NW) * 4);
+                    float off[4], sum[HPL][2];
+                    mma_f16_first(off, m0[0], m1[0], 0u, 0u, qsum[0], 0u);
+                    if constexpr (HPL == 1) {
+                        off[0] += off[1];
+                        off[1] = off[2] + off[3];
+                    } else {
+                        mma_f16(off, m0[0], m1[0], 0u, 0u, qsum[1], 0u);
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        float c[4];
+                        uint32_t x0[4], x1[4];
+                        numbers_of<true>(k0[g], x0);
+                        numbers_of<true>(k1[g], x1);
+                        mma_f16_first(c, x0[0], x1[0], x0[1], x1[1], qh[g][0], qh[g][1]);
+                        mma_f16(c, x0[2], x1[2], x0[3], x1[3], qh[g][2], qh[g][3]);
+                        if constexpr (HPL == 1) {
+                            c[0] += c[1];
+                            c[1] = c[2] + c[3];
+                        } else {
+                            mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[g][0], ql[g][1]);
+                            mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[g][2], ql[g][3]);
+                        }
+#pragma unroll
+                        for (int h = 0; h < HPL; h++) {
+                            sum[h][0] = g ? fmaf(step_of(d0, g), c[h], sum[h][0]) : step_of(d0, g) * c[h];
+                            sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
+                        }
+                    }
+                    // 2^22 of the numbers, 2^-up; the sums' 2^5 2^-up
+#pragma unroll
+                    for (int h = 0; h < HPL; h++)
+#pragma unroll
+                        for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 131072.f, off[x * HPL + h]) * back[h];
+                }
+                if (track) {
+                    float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
+#pragma unroll
+                    for (int h = 0; h < HPL; h++)
+#pragma unroll
+                        for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                            for (int x = 0; x < 2; x++)
+                                if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
+                }
+                uint32_t d[kQ4Tile][2][NW], vm[kQ4Tile][2][NW], steps = limit;
+#pragma unroll
+                for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
+                        lds_words<NW>(vm[u][x], tile + u * BLOCK + 19 * HD + (g8 + 8 * x) * NG * 2);
+                    }
+                if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
+#pragma unroll
+                    for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
+#pragma unroll
+                            for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < NW; g++) {
+                                d[u][x][g] = on ? d[u][x][g] : 0u;
+                                vm[u][x][g] = on ? vm[u][x][g] : 0u;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < kQ4Tile; u++)
+#pragma unroll
+                    for (int g = 0; g < NW; g++) steps = __vmaxu2(steps, __vmaxu2(d[u][0][g], d[u][1][g]));
+                // a score far above the reference, or a step beyond the scale's range: seldom after the first tile
+                float top[HPL];
+                bool grown = steps != limit;
+#pragma unroll
+                for (int h = 0; h < HPL; h++) {
+                    top[h] = s[h][0][0];
+#pragma unroll
+                    for (int u = 0; u < kQ4Tile; u++) top[h] = fmaxf(fmaxf(top[h], s[h][u][0]), s[h][u][1]);
+                    grown |= top[h] > m_run[h] + 15.f;
+                }
+                if (__any_sync(0xffffffffu, grown)) {
+                    float fix[HPL], vfix = 1.f;
+                    steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
+                    if (steps > (limit & 0xffffu)) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
+                        const int e = max((int)(steps >> 7) - 127, -100);
+                        const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23 | (uint32_t)(g8 & 1) << 31);  // odd positions have 15 - q
+                        vfix = vscale == 0.f ? 0.f : next / vscale;
+                        vscale = next;
+                        limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
+                    }
+#pragma unroll
+                    for (int h = 0; h < HPL; h++) {
+                        float mx = fmaxf(m_run[h] + 11.f, top[h]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        mx -= 11.f;
+                        fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
+                        m_run[h] = mx;
+                        l_run[h] *= fix[h];
+                    }
+#pragma unroll
+                    for (int h = 0; h < HPL; h++)
+#pragma unroll
+                        for (int g = 0; g < NG; g++) offset[h][g] *= fix[h];
+                    if (first > 0) {
+#pragma unroll
+                        for (int h = 0; h < HPL; h++)
+#pragma unroll
+                            for (int g = 0; g < NG; g++) {
+                                float4 *at = reinterpret_cast<float4 *>(own_row + h * Smem::kMergeRow + g * kQ4Group);
+                                const float4 y = *at;
+                                *at = make_float4(y.x * fix[h], y.y * fix[h], y.z * fix[h], y.w * fix[h]);
+                            }
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; g++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const float y = fix[HPL == 1 ? 0 : x & 1] * vfix;
+                            o[g][0][x] *= y;
+                            o[g][1][x] *= y;
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < kQ4Tile; u++) {
+                    uint32_t v0[NG], v1[NG];  // unit g8 of positions 2t, 2t + 1, and of those eight farther
+#pragma unroll
+                    for (int g = 0; g < NG; g += 2) ldmatrix_x4_trans(v0[g], v1[g], v0[g + 1], v1[g + 1], tile + u * BLOCK + (g == 0 ? v_piece : v_piece ^ 32u));
+                    float w[HPL][2], ws[HPL][2];
+#pragma unroll
+                    for (int h = 0; h < HPL; h++) {
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
+                            ws[h][x] = w[h][x] * vscale;
+                        }
+                        l_run[h] += w[h][0] + w[h][1];
+                    }
+                    // the offsets' part, in FP32: an MMA cuts off what its sum of 22-bit products has below 24 bits, always towards zero, and this part and the
+                    // numbers' are often large and of opposite sign
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+#pragma unroll
+                        for (int g = 0; g < NG; g += 2) {
+                            const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&vm[u][x][g >> 1]));
+                            const float m0 = fmaf(step_of(d[u][x], g), fifteen, two.x), m1 = fmaf(step_of(d[u][x], g + 1), fifteen, two.y);
+#pragma unroll
+                            for (int h = 0; h < HPL; h++) {
+                                offset[h][g] = fmaf(w[h][x], m0, offset[h][g]);
+                                offset[h][g + 1] = fmaf(w[h][x], m1, offset[h][g + 1]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        float hi[HPL][2], lo[HPL][2];
+#pragma unroll
+                        for (int h = 0; h < HPL; h++)
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                const float y = ws[h][x] * step_of(d[u][x], g);
+                                hi[h][x] = upper_limb(y);
+                                lo[h][x] = y - hi[h][x];
+                            }
+#pragma unroll
+                        for (int limb = 0; limb < HPL; limb++) {
+                            uint32_t b0, b1;
+                            if constexpr (HPL == 1) {
+                                b0 = transpose8(pack_h2(hi[0][0], lo[0][0]));
+                                b1 = transpose8(pack_h2(hi[0][1], lo[0][1]));
+                            } else {
+                                b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
+                                b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
+                            }
+                            uint32_t x0[4], x1[4];
+                            numbers_of<false>(v0[g], x0);
+                            numbers_of<false>(v1[g], x1);
+                            mma_f16(o[g][0], x0[0], x0[1], x1[0], x1[1], b0, b1);
+                            mma_f16(o[g][1], x0[2], x0[3], x1[2], x1[3], b0, b1);
+                        }
+                    }
+                }
+                __syncwarp();  // all lanes have read the tile before it is filled again
+                if (part_issued < part_tiles) issue();
+            }
+            // a chain's sums, over the lanes that share a head for the offsets' part, to where the warps meet
             const float unscale = vscale == 0.f ? 0.f : 262144.f / fabsf(vscale);  // 2^18
 #pragma unroll
             for (int h = 0; h < HPL; h++)
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    float4 *to = reinterpret_cast<float4 *>(mg_o + (warp * HEADS + HPL * t + h) * Smem::kMergeRow + g * kQ4Group + 4 * g8);  // dimensions 4 g8 .. 4 g8 + 3 of the group
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) offset[h][g] += __shfl_xor_sync(0xffffffffu, offset[h][g], x);
                     float v[4];
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
                         const float *c = &o[g][x >> 1][2 * (x & 1)];
-                        v[x] = (HPL == 1 ? c[0] + c[1] : c[h]) * unscale + (end ? offset[h][g] : 0.f);
+                        v[x] = fmaf(HPL == 1 ? c[0] + c[1] : c[h], unscale, offset[h][g]);
                     }
-                    if (put) {
-                        const float4 before = *to;
-                        v[0] += before.x;
-                        v[1] += before.y;
-                        v[2] += before.z;
-                        v[3] += before.w;
-                    }
-                    *to = make_float4(v[0], v[1], v[2], v[3]);
+                    float4 *at = reinterpret_cast<float4 *>(own_row + h * Smem::kMergeRow + g * kQ4Group);
+                    const float4 before = first > 0 ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                    *at = make_float4(v[0] + before.x, v[1] + before.y, v[2] + before.z, v[3] + before.w);
                 }
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) o[g][0][x] = o[g][1][x] = 0.f;
-            put = true;
-        };
-        for (int j = 0; j < n_tiles; j++, pos0 += W * kQ4Tile * kPageTokens) {
-            mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
-            if (__any_sync(0xffffffffu, failed)) {
-                failed = true;
-                break;
-            }
-            const uint32_t tile = ring + used % kQ4Slots * TILE;
-            used++;
-            float s[HPL][kQ4Tile][2];  // rows g8 and g8 + 8 of each page
-#pragma unroll
-            for (int u = 0; u < kQ4Tile; u++) {
-                const uint32_t base = tile + u * BLOCK;
-                uint32_t k0[NG], k1[NG], d0[NW], d1[NW], m0[1], m1[1];
-                lds_words<NG>(k0, base + lane * NG * 4);
-                lds_words<NG>(k1, base + (32 + lane) * NG * 4);
-                lds_words<NW>(d0, base + 8 * HD + g8 * NG * 2);
-                lds_words<NW>(d1, base + 8 * HD + (g8 + 8) * NG * 2);
-                lds_words<1>(m0, base + 9 * HD + g8 * NG * 2 + (t % NW) * 4);  // k beyond the groups: once more, times the zeros of qsum
-                lds_words<1>(m1, base + 9 * HD + (g8 + 8) * NG * 2 + (t % NW) * 4);
-                float off[4], sum[HPL][2];
-                mma_f16_first(off, m0[0], m1[0], 0u, 0u, qsum[0], 0u);
-                if constexpr (HPL == 1) {
-                    off[0] += off[1];
-                    off[1] = off[2] + off[3];
-                } else {
-                    mma_f16(off, m0[0], m1[0], 0u, 0u, qsum[1], 0u);
-                }
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    float c[4];
-                    uint32_t x0[4], x1[4];
-                    numbers_of<true>(k0[g], x0);
-                    numbers_of<true>(k1[g], x1);
-                    mma_f16_first(c, x0[0], x1[0], x0[1], x1[1], qh[g][0], qh[g][1]);
-                    mma_f16(c, x0[2], x1[2], x0[3], x1[3], qh[g][2], qh[g][3]);
-                    if constexpr (HPL == 1) {
-                        c[0] += c[1];
-                        c[1] = c[2] + c[3];
-                    } else {
-                        mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[g][0], ql[g][1]);
-                        mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[g][2], ql[g][3]);
-                    }
-#pragma unroll
-                    for (int h = 0; h < HPL; h++) {
-                        sum[h][0] = g ? fmaf(step_of(d0, g), c[h], sum[h][0]) : step_of(d0, g) * c[h];
-                        sum[h][1] = g ? fmaf(step_of(d1, g), c[HPL + h], sum[h][1]) : step_of(d1, g) * c[HPL + h];
-                    }
-                }
-                // 2^22 of the numbers, 2^-up; the sums' 2^5 2^-up
-#pragma unroll
-                for (int h = 0; h < HPL; h++)
-#pragma unroll
-                    for (int x = 0; x < 2; x++) s[h][u][x] = fmaf(sum[h][x], 131072.f, off[x * HPL + h]) * back[h];
-            }
-            if (track) {
-                float *to_s = p.scores + (((size_t)kvh * p.total + r.first) * kPageTokens + pos0 + g8) * G;
-#pragma unroll
-                for (int h = 0; h < HPL; h++)
-#pragma unroll
-                    for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-                        for (int x = 0; x < 2; x++)
-                            if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
-            }
-            uint32_t d[kQ4Tile][2][NW], vm[kQ4Tile][2][NW], steps = limit;
-#pragma unroll
-            for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    lds_words<NW>(d[u][x], tile + u * BLOCK + 18 * HD + (g8 + 8 * x) * NG * 2);
-                    lds_words<NW>(vm[u][x], tile + u * BLOCK + 19 * HD + (g8 + 8 * x) * NG * 2);
-                }
-            if (pos0 + kQ4Tile * kPageTokens > pos_end) {  // positions behind the end: whatever their place holds
-#pragma unroll
-                for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const bool on = pos0 + 16 * u + 8 * x + g8 < pos_end;
-#pragma unroll
-                        for (int h = 0; h < HPL; h++) s[h][u][x] = on ? s[h][u][x] : -INFINITY;
-#pragma unroll
-                        for (int g = 0; g < NW; g++) {
-                            d[u][x][g] = on ? d[u][x][g] : 0u;
-                            vm[u][x][g] = on ? vm[u][x][g] : 0u;
-                        }
-                    }
-            }
-#pragma unroll
-            for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-                for (int g = 0; g < NW; g++) steps = __vmaxu2(steps, __vmaxu2(d[u][0][g], d[u][1][g]));
-            // a score far above the reference, or a step beyond the scale's range: seldom after the first tile
-            float top[HPL];
-            bool grown = steps != limit;
-#pragma unroll
-            for (int h = 0; h < HPL; h++) {
-                top[h] = s[h][0][0];
-#pragma unroll
-                for (int u = 0; u < kQ4Tile; u++) top[h] = fmaxf(fmaxf(top[h], s[h][u][0]), s[h][u][1]);
-                grown |= top[h] > m_run[h] + 15.f;
-            }
-            if (__any_sync(0xffffffffu, grown)) {
-                float fix[HPL], vfix = 1.f;
-                steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
-                if (steps > (limit & 0xffffu)) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
-                    const int e = max((int)(steps >> 7) - 127, -100);
-                    const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23 | (uint32_t)(g8 & 1) << 31);  // odd positions have 15 - q
-                    vfix = vscale == 0.f ? 0.f : next / vscale;
-                    vscale = next;
-                    limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
-                }
-#pragma unroll
-                for (int h = 0; h < HPL; h++) {
-                    float mx = fmaxf(m_run[h] + 11.f, top[h]);
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                    mx -= 11.f;
-                    fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
-                    m_run[h] = mx;
-                    l_run[h] *= fix[h];
-                }
-#pragma unroll
-                for (int h = 0; h < HPL; h++)
-#pragma unroll
-                    for (int g = 0; g < NG; g++) offset[h][g] *= fix[h];
-                if (put) {
-#pragma unroll
-                    for (int h = 0; h < HPL; h++)
-#pragma unroll
-                        for (int g = 0; g < NG; g++) {
-                            float4 *at = reinterpret_cast<float4 *>(mg_o + (warp * HEADS + HPL * t + h) * Smem::kMergeRow + g * kQ4Group + 4 * g8);
-                            const float4 y = *at;
-                            *at = make_float4(y.x * fix[h], y.y * fix[h], y.z * fix[h], y.w * fix[h]);
-                        }
-                }
-#pragma unroll
-                for (int g = 0; g < NG; g++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const float y = fix[HPL == 1 ? 0 : x & 1] * vfix;
-                        o[g][0][x] *= y;
-                        o[g][1][x] *= y;
-                    }
-            }
-#pragma unroll
-            for (int u = 0; u < kQ4Tile; u++) {
-                uint32_t v0[NG], v1[NG];  // unit g8 of positions 2t, 2t + 1, and of those eight farther
-#pragma unroll
-                for (int g = 0; g < NG; g += 2) ldmatrix_x4_trans(v0[g], v1[g], v0[g + 1], v1[g + 1], tile + u * BLOCK + (g == 0 ? v_piece : v_piece ^ 32u));
-                float w[HPL][2], ws[HPL][2];
-#pragma unroll
-                for (int h = 0; h < HPL; h++) {
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
-                        ws[h][x] = w[h][x] * vscale;
-                    }
-                    l_run[h] += w[h][0] + w[h][1];
-                }
-                // the offsets' part, in FP32: an MMA cuts off what its sum of 22-bit products has below 24 bits, always towards zero, and this part and the
-                // numbers' are often large and of opposite sign
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-#pragma unroll
-                    for (int g = 0; g < NG; g += 2) {
-                        const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&vm[u][x][g >> 1]));
-                        const float m0 = fmaf(step_of(d[u][x], g), fifteen, two.x), m1 = fmaf(step_of(d[u][x], g + 1), fifteen, two.y);
-#pragma unroll
-                        for (int h = 0; h < HPL; h++) {
-                            offset[h][g] = fmaf(w[h][x], m0, offset[h][g]);
-                            offset[h][g + 1] = fmaf(w[h][x], m1, offset[h][g + 1]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    float hi[HPL][2], lo[HPL][2];
-#pragma unroll
-                    for (int h = 0; h < HPL; h++)
-#pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            const float y = ws[h][x] * step_of(d[u][x], g);
-                            hi[h][x] = upper_limb(y);
-                            lo[h][x] = y - hi[h][x];
-                        }
-#pragma unroll
-                    for (int limb = 0; limb < HPL; limb++) {
-                        uint32_t b0, b1;
-                        if constexpr (HPL == 1) {
-                            b0 = transpose8(pack_h2(hi[0][0], lo[0][0]));
-                            b1 = transpose8(pack_h2(hi[0][1], lo[0][1]));
-                        } else {
-                            b0 = transpose8(limb ? pack_h2(lo[0][0], lo[1][0]) : pack_h2(hi[0][0], hi[1][0]));
-                            b1 = transpose8(limb ? pack_h2(lo[0][1], lo[1][1]) : pack_h2(hi[0][1], hi[1][1]));
-                        }
-                        uint32_t x0[4], x1[4];
-                        numbers_of<false>(v0[g], x0);
-                        numbers_of<false>(v1[g], x1);
-                        mma_f16(o[g][0], x0[0], x0[1], x1[0], x1[1], b0, b1);
-                        mma_f16(o[g][1], x0[2], x0[3], x1[2], x1[3], b0, b1);
-                    }
-                }
-            }
-            __syncwarp();  // all lanes have read the tile before it is filled again
-            if (part_issued < part_tiles) issue();
-            if (j % kQ4Chain<HPL> == kQ4Chain<HPL> - 1) put_by(false);
-        }
+        } while (j < n_tiles && !failed);
         const CacheRow now = r;
         from = to;
         if (from < share1 && !failed) begin(i + 1, from);  // the next row's pages are on their way from here on
-        // sums over the lanes that share a head, then over the warps
+        // sums over the lanes that share a head; those over the warps follow
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
-#pragma unroll
-                for (int g = 0; g < NG; g++) offset[h][g] += __shfl_xor_sync(0xffffffffu, offset[h][g], x);
-            }
-        }
-        put_by(true);
-#pragma unroll
-        for (int h = 0; h < HPL; h++) {
+            for (int x = 4; x < 32; x <<= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], x);
             const int head = HPL * t + h;
             if (g8 == 0) {
                 mg_m[warp * HEADS + head] = m_run[h];
