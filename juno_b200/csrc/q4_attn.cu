@@ -124,7 +124,7 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 template <int HD, int HPL>
 struct Q4Smem {  // bytes
     static constexpr int kRing = kQ4Warps<HD, HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HD, HPL> * kQ4Slots * 8, kMergeRow = HD + 8,  // floats; the pads keep rows on different banks
-                         kQuery = kMerge + kQ4Warps<HD, HPL> * 4 * HPL * (kMergeRow + 2) * 4, kQueryRow = HD + 8,  // halves
+                         kQuery = kMerge + kQ4Warps<HD, HPL> * 4 * HPL * (kMergeRow + 2) * 4, kQueryRow = HD + 32,  // halves
         kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kBack = kSums + 2 * 4 * HPL * 4 * 2, kAll = kBack + 4 * HPL * 4;
 };
 
@@ -254,14 +254,13 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         }
         __syncthreads();
         // lane (g8, t) has dimensions 8t .. 8t + 7 of every group of the head of column g8
-        uint32_t qh[NG][4], ql[HPL == 2 ? NG : 1][4];
+        uint32_t qh[NG][4];
         uint32_t qsum[HPL];  // k: the groups
         float back[HPL];     // of this lane's own heads
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const __half *from_q = q_s + (HPL == 1 ? (g8 & 1) * HEADS + (g8 >> 1) : g8) * Smem::kQueryRow + g * kQ4Group + 8 * t;
             lds_words<4>(qh[g], smem_u32(from_q));
-            if constexpr (HPL == 2) lds_words<4>(ql[g], smem_u32(from_q + HEADS * Smem::kQueryRow));
         }
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
@@ -329,8 +328,10 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             c[0] += c[1];
                             c[1] = c[2] + c[3];
                         } else {
-                            mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[g][0], ql[g][1]);
-                            mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[g][2], ql[g][3]);
+                            uint32_t ql[4];  // from shared memory each time: in registers they would push others out (121 us instead of 118, 48 rows of 8192)
+                            lds_words<4>(ql, smem_u32(q_s + (HEADS + g8) * Smem::kQueryRow + g * kQ4Group + 8 * t));
+                            mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[0], ql[1]);
+                            mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[2], ql[3]);
                         }
 #pragma unroll
                         for (int h = 0; h < HPL; h++) {
