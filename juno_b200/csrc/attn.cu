@@ -1170,7 +1170,9 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<in
 }
 
 // A sequence's weights, one plane of `room` (a multiple of 16) positions for each layer and head: the first `len` of another one's, zeros behind.
-static __global__ void track_kernel(float *own, const float *from, int room, int len) {
+static __global__ void track_kernel(float *own, const float *from, int room, int len, int32_t *table, const __grid_constant__ TableWords w, int n) {
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = threadIdx.x; i < n; i += blockDim.x) table[i] = w.v[i];
     const int pos = (blockIdx.x * 256 + threadIdx.x) * 4;
     if (pos >= room) return;
     const size_t at = (size_t)blockIdx.y * room + pos;
@@ -1183,7 +1185,7 @@ static __global__ void track_kernel(float *own, const float *from, int room, int
     }
     *reinterpret_cast<float4 *>(own + at) = v;
 }
-// Gives the sequence one of the pool's weight planes: zeros, or what `src` holds for the positions that both have.
+// Gives the sequence one of the pool's weight planes: zeros, or what `src` holds for the positions that both have.  A branch's page table goes with the launch.
 static int seq_track(juno_seq *s, const juno_seq *src) {
     juno_kvpool *p = s->pool;
     JUNO_REQUIRE(s->max_tokens <= p->track_tokens, "a sequence of up to %d positions does not fit the pool's weights (juno_kvpool_track: %d)", s->max_tokens,
@@ -1196,7 +1198,13 @@ static int seq_track(juno_seq *s, const juno_seq *src) {
     const size_t planes = (size_t)p->n_layers * p->n_kv_heads;
     float *own = p->weights + track * p->track_stride();
     const dim3 grid((unsigned)((p->track_tokens / 4 + 255) / 256), (unsigned)planes);
-    track_kernel<<<grid, 256, 0, p->ctx->stream>>>(own, src ? p->weights + src->track * p->track_stride() : nullptr, p->track_tokens, src ? s->len : 0);
+    constexpr size_t kWords = sizeof(TableWords) / sizeof(int32_t);
+    const size_t at = (size_t)s->slot * p->max_pages_per_seq, n = src ? std::min(s->pages.size(), kWords) : 0;
+    if (src && s->pages.size() > kWords) JUNO_TRY(table_store(p, s->slot, (int)kWords, (int)s->pages.size() - 1, p->ctx->stream));
+    TableWords w;
+    memcpy(w.v, p->h_table + at, n * sizeof(int32_t));
+    track_kernel<<<grid, 256, 0, p->ctx->stream>>>(own, src ? p->weights + src->track * p->track_stride() : nullptr, p->track_tokens, src ? s->len : 0, p->d_table + at, w,
+                                                   (int)n);
     JUNO_CUDA_TRY(cudaGetLastError());
     p->ctx->kernel_launches++;
     p->free_tracks.pop_back();
@@ -1303,8 +1311,7 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
         row[i] = pg;
     }
     s->len = n_tokens;
-    int rc = n_pg ? table_store(p, s->slot, 0, n_pg - 1, p->ctx->stream) : JUNO_OK;
-    if (rc == JUNO_OK && src->track >= 0) rc = seq_track(s, src);
+    const int rc = src->track >= 0 ? seq_track(s, src) : n_pg ? table_store(p, s->slot, 0, n_pg - 1, p->ctx->stream) : JUNO_OK;
     if (rc != JUNO_OK) {
         for (int pg : s->pages) p->page_refs[(size_t)pg]--;
         p->free_slots.push_back(s->slot);

@@ -113,6 +113,8 @@ struct RowPlace {
 };
 template <int R>
 __device__ __forceinline__ void find_places(const RowsParams &p, int row0, size_t page_bytes, RowPlace (&places)[R]) {
+    pdl_launch_dependents();
+    pdl_wait();
     if (threadIdx.x < R) {
         const int row = row0 + threadIdx.x;
         RowPlace at{nullptr, 0, -1};
@@ -346,12 +348,12 @@ static int launch_rows(juno_ctx *c, const juno_kvpool *p, int layer, const Cache
         const int each = n_tokens >= c->sm_count * 16 ? kAppendRows : 1;
         const dim3 grid((unsigned)((n_tokens + each - 1) / each), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 8) + 31) / 32 * 32));
         if (each == 1)
-            hd == 128 ? q4_append_kernel<128, 1><<<grid, block, 0, st>>>(a) : q4_append_kernel<64, 1><<<grid, block, 0, st>>>(a);
+            JUNO_CUDA_TRY(launch_pdl(hd == 128 ? q4_append_kernel<128, 1> : q4_append_kernel<64, 1>, grid, block, 0, st, a));
         else
-            hd == 128 ? q4_append_kernel<128, kAppendRows><<<grid, block, 0, st>>>(a) : q4_append_kernel<64, kAppendRows><<<grid, block, 0, st>>>(a);
+            JUNO_CUDA_TRY(launch_pdl(hd == 128 ? q4_append_kernel<128, kAppendRows> : q4_append_kernel<64, kAppendRows>, grid, block, 0, st, a));
     } else if (p->dtype == kKvQ4) {
         const dim3 grid((unsigned)((n_tokens + kReadRows - 1) / kReadRows), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 4) + 31) / 32 * 32));
-        hd == 128 ? q4_read_kernel<128><<<grid, block, 0, st>>>(a) : q4_read_kernel<64><<<grid, block, 0, st>>>(a);
+        JUNO_CUDA_TRY(launch_pdl(hd == 128 ? q4_read_kernel<128> : q4_read_kernel<64>, grid, block, 0, st, a));
     } else {
         const unsigned grid = (unsigned)(((int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8) + 255) / 256);
         p->dtype == 0 ? rows_kernel<__half, APPEND><<<grid, 256, 0, st>>>(a, hd) : rows_kernel<float, APPEND><<<grid, 256, 0, st>>>(a, hd);
@@ -371,6 +373,8 @@ int launch_kv_append(juno_ctx *c, const juno_kvpool *p, int layer, const CacheRo
 template <bool STORE>
 __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ CacheRows rows, float *weights, int layer, int n_layers, int n_kv_heads, int track_tokens, float *w, int64_t ld) {
     const int i = blockIdx.z, h = blockIdx.y, pos = blockIdx.x * 256 + threadIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
     const CacheRow r = cache_row(rows, i);
     if (pos >= r.upto) return;
     float *own = weights + (((size_t)r.track * n_layers + layer) * n_kv_heads + h) * track_tokens + pos;
@@ -383,17 +387,26 @@ __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ Ca
 
 // ───────────────────────────── eviction ───────────────────────────────────────────────────
 struct EvictRow {
-    int len, keep, recent, track, old_pages, new_pages;  // the last two: offsets into `pages`
+    int len, keep, recent, track, slot, new_pages;  // new_pages: the first of the row's new pages among those of all rows
 };
+constexpr int kRowWords = sizeof(EvictRow) / sizeof(int32_t), kEvictWords = 900;
 struct EvictParams {
-    const EvictRow *rows;
-    const int32_t *pages;
+    int32_t in[kEvictWords];  // the rows, then new pages of all of them: in the launch where they fit, else in `far`
+    const int32_t *far;
+    const int32_t *table;  // as it was before: the rows' old pages
     uint8_t *pool;
-    int n, n_pages, n_kv_heads, n_layers, track_tokens, hd;
+    int n, n_pages, n_kv_heads, n_layers, track_tokens, max_pages_per_seq;
     float *weights;
     int32_t *kept;  // [layer][row][kv_head][kept_ld]
     int kept_ld;
 };
+__device__ __forceinline__ int evict_word(const EvictParams &p, int k) { return p.far ? p.far[k] : p.in[k]; }
+__device__ __forceinline__ EvictRow evict_row(const EvictParams &p, int i) {
+    const int k = i * kRowWords;
+    return {evict_word(p, k), evict_word(p, k + 1), evict_word(p, k + 2), evict_word(p, k + 3), evict_word(p, k + 4), evict_word(p, k + 5)};
+}
+__device__ __forceinline__ int old_page(const EvictParams &p, const EvictRow &r, int pos) { return p.table[(size_t)r.slot * p.max_pages_per_seq + (pos >> 4)]; }
+__device__ __forceinline__ int new_page(const EvictParams &p, const EvictRow &r, int pos) { return evict_word(p, p.n * kRowWords + r.new_pages + (pos >> 4)); }
 
 // Order of weights as whole numbers: larger weight, larger key; both zeros alike, a NaN below everything.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -431,9 +444,11 @@ __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *sums, uns
 // One CTA per (sequence, layer, head): which positions stay, in order, and their weights.  The weight that decides (the need-th largest) is found digit by
 // digit, 11, 11 and 10 bits, with a count of every digit in shared memory: three passes over the weights, whatever they are.  Up to kSelectCached weights are
 // read from memory once.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
     const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const EvictRow r = p.rows[i];
+    pdl_launch_dependents();
+    pdl_wait();
+    const EvictRow r = evict_row(p, i);
     float *w = p.weights + (((size_t)r.track * p.n_layers + layer) * p.n_kv_heads + h) * p.track_tokens;
     int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld;
     for (int64_t j = r.keep + tid; j < p.kept_ld; j += kSelectThreads) kept[j] = -1;
@@ -579,24 +594,22 @@ struct Q4Piece {
     }
 };
 
-__device__ __forceinline__ uint8_t *evict_block(const EvictParams &p, int layer, int h, int list, int pos) {
-    return p.pool + (((size_t)layer * p.n_pages + p.pages[list + (pos >> 4)]) * p.n_kv_heads + h) * (size_t)q4_block_bytes(p.hd);
-}
-
 // The rows that stay, into fresh pages: a warp has one page of one head, two rows a step.
 template <int HD>
-__global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(256) evict_gather_kernel(const __grid_constant__ EvictParams p) {
     static_assert(Q4Piece<HD>::PIECES <= 16, "a piece to a lane");
     const int i = blockIdx.z, layer = blockIdx.y, lane = threadIdx.x & 31;
-    const EvictRow r = p.rows[i];
+    pdl_launch_dependents();
+    pdl_wait();
+    const EvictRow r = evict_row(p, i);
     if (r.keep == r.len) return;
     const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), h = unit % p.n_kv_heads, base = unit / p.n_kv_heads * kPageTokens, n = min(kPageTokens, r.keep - base);
     if (n <= 0) return;
     const int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld + base;
-    const int src = kept[min(lane, n - 1)], src_page = p.pages[r.old_pages + (src >> 4)];
+    const int src = kept[min(lane, n - 1)], src_page = old_page(p, r, src);
     const size_t page_bytes = (size_t)p.n_kv_heads * q4_block_bytes(HD);
     uint8_t *plane = p.pool + (size_t)layer * p.n_pages * page_bytes + h * q4_block_bytes(HD);
-    uint8_t *to = plane + p.pages[r.new_pages + (base >> 4)] * page_bytes;
+    uint8_t *to = plane + new_page(p, r, base) * page_bytes;
     const Q4Piece<HD> piece(lane & 15);
     uint4 v[kPageTokens / 2];
 #pragma unroll
@@ -613,9 +626,11 @@ __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) 
 // front or stays, so that what a step overwrites has been read by it or by an earlier one.
 constexpr int kMoveThreads = 512, kMoveRows = kMoveThreads / 16 * 2;
 template <int HD>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
     const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, sub = threadIdx.x >> 4;
-    const EvictRow r = p.rows[i];
+    pdl_launch_dependents();
+    pdl_wait();
+    const EvictRow r = evict_row(p, i);
     if (r.keep == r.len) return;
     const int32_t *kept = p.kept + (((size_t)layer * p.n + i) * p.n_kv_heads + h) * p.kept_ld;
     const size_t page_bytes = (size_t)p.n_kv_heads * q4_block_bytes(HD);
@@ -626,13 +641,13 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int j = base + sub + k * (kMoveThreads / 16), src = j < r.keep ? kept[j] : 0;
-            if (j < r.keep) v[k] = piece.load(plane + p.pages[r.old_pages + (src >> 4)] * page_bytes, src & 15);
+            if (j < r.keep) v[k] = piece.load(plane + old_page(p, r, src) * page_bytes, src & 15);
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int j = base + sub + k * (kMoveThreads / 16);
-            if (j < r.keep) piece.store(plane + p.pages[r.new_pages + (j >> 4)] * page_bytes, j & 15, v[k]);
+            if (j < r.keep) piece.store(plane + new_page(p, r, j) * page_bytes, j & 15, v[k]);
         }
         __syncthreads();
     }
@@ -775,9 +790,9 @@ int juno_kv_weights_device(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n
         const dim3 grid((unsigned)((most + 255) / 256), (unsigned)p->n_kv_heads, (unsigned)n);
         ProfScope prof(c, s.st, PROF_OTHER, 0);
         if (store)
-            weights_kernel<true><<<grid, 256, 0, s.st>>>(r, p->weights, layer, p->n_layers, p->n_kv_heads, p->track_tokens, w_dev, ld);
+            JUNO_CUDA_TRY(launch_pdl(weights_kernel<true>, grid, dim3(256), 0, s.st, r, p->weights, layer, p->n_layers, p->n_kv_heads, p->track_tokens, w_dev, ld));
         else
-            weights_kernel<false><<<grid, 256, 0, s.st>>>(r, p->weights, layer, p->n_layers, p->n_kv_heads, p->track_tokens, w_dev, ld);
+            JUNO_CUDA_TRY(launch_pdl(weights_kernel<false>, grid, dim3(256), 0, s.st, r, p->weights, layer, p->n_layers, p->n_kv_heads, p->track_tokens, w_dev, ld));
         JUNO_CUDA_TRY(cudaGetLastError());
         c->kernel_launches++;
         return JUNO_OK;
@@ -819,39 +834,43 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         size_t next = p->free_pages.size();
         for (int i = 0; i < n; i++) {
             const juno_seq *s = seqs[i];
-            EvictRow r{s->len, std::min(s->len, keep), std::min(s->len, recent), s->track, (int)pages.size(), 0};
-            if (s->len > keep) {
-                pages.insert(pages.end(), s->pages.begin(), s->pages.end());
-                r.new_pages = (int)pages.size();
+            EvictRow r{s->len, std::min(s->len, keep), std::min(s->len, recent), s->track, s->slot, (int)pages.size()};
+            if (s->len > keep)
                 for (int j = 0; j < np; j++) {
                     const int pg = s->pages[(size_t)j];
                     pages.push_back(fresh || p->page_refs[(size_t)pg] > 1 ? p->free_pages[--next] : pg);
                 }
-            }
             rows.push_back(r);
         }
+        std::vector<int32_t> table;
+        table.reserve(2 * pages.size());
         CacheStream st(c, stream);
         JUNO_TRY(st.status);
-        auto padded = [](size_t b) { return (b + 255) & ~(size_t)255; };
-        // rows, then pages, by value
-        constexpr size_t kRowWords = sizeof(EvictRow) / sizeof(int32_t);
-        std::vector<int32_t> words(rows.size() * kRowWords + pages.size());
-        memcpy(words.data(), rows.data(), rows.size() * sizeof(EvictRow));
-        if (!pages.empty()) memcpy(words.data() + rows.size() * kRowWords, pages.data(), pages.size() * sizeof(int32_t));
-        const size_t word_bytes = padded(words.size() * sizeof(int32_t)), kept_bytes = kept_dev ? 0 : (size_t)p->n_layers * n * p->n_kv_heads * keep * sizeof(int32_t);
+        const size_t row_words = rows.size() * kRowWords, words = row_words + pages.size();
+        const size_t word_bytes = words <= kEvictWords ? 0 : (words * sizeof(int32_t) + 255) & ~(size_t)255;
+        const size_t kept_bytes = kept_dev ? 0 : (size_t)p->n_layers * n * p->n_kv_heads * keep * sizeof(int32_t);
         uint8_t *scratch = nullptr;
-        JUNO_TRY(cache_scratch(c, word_bytes + kept_bytes, &scratch));
-        JUNO_TRY(cache_words(c, words.data(), words.size(), reinterpret_cast<int32_t *>(scratch), st.st));
+        if (word_bytes + kept_bytes) JUNO_TRY(cache_scratch(c, word_bytes + kept_bytes, &scratch));
         EvictParams a;
-        a.rows = reinterpret_cast<const EvictRow *>(scratch);
-        a.pages = reinterpret_cast<const int32_t *>(scratch) + rows.size() * kRowWords;
+        a.far = nullptr;
+        if (word_bytes) {
+            std::vector<int32_t> all(words);
+            memcpy(all.data(), rows.data(), row_words * sizeof(int32_t));
+            memcpy(all.data() + row_words, pages.data(), pages.size() * sizeof(int32_t));
+            JUNO_TRY(cache_words(c, all.data(), words, reinterpret_cast<int32_t *>(scratch), st.st));
+            a.far = reinterpret_cast<const int32_t *>(scratch);
+        } else {
+            memcpy(a.in, rows.data(), row_words * sizeof(int32_t));
+            if (!pages.empty()) memcpy(a.in + row_words, pages.data(), pages.size() * sizeof(int32_t));
+        }
+        a.table = p->d_table;
+        a.max_pages_per_seq = p->max_pages_per_seq;
         a.pool = static_cast<uint8_t *>(p->k);
         a.n = n;
         a.n_pages = p->n_pages;
         a.n_kv_heads = p->n_kv_heads;
         a.n_layers = p->n_layers;
         a.track_tokens = p->track_tokens;
-        a.hd = p->head_dim;
         a.weights = p->weights;
         a.kept = kept_dev ? kept_dev : reinterpret_cast<int32_t *>(scratch + word_bytes);
         a.kept_ld = kept_dev ? kept_ld : keep;
@@ -864,17 +883,14 @@ int juno_kv_evict(juno_ctx *c, juno_kvpool *p, int32_t n, juno_seq *const *seqs,
         }
         {
             ProfScope prof(c, st.st, PROF_OTHER, 0);
-            evict_select_kernel<<<heads, kSelectThreads, cached, st.st>>>(a);
-            JUNO_CUDA_TRY(cudaGetLastError());
+            JUNO_CUDA_TRY(launch_pdl(evict_select_kernel, heads, dim3(kSelectThreads), cached, st.st, a));
             if (fresh)
-                p->head_dim == 128 ? evict_gather_kernel<128><<<units, 256, 0, st.st>>>(a) : evict_gather_kernel<64><<<units, 256, 0, st.st>>>(a);
+                JUNO_CUDA_TRY(launch_pdl(p->head_dim == 128 ? evict_gather_kernel<128> : evict_gather_kernel<64>, units, dim3(256), 0, st.st, a));
             else
-                p->head_dim == 128 ? evict_move_kernel<128><<<heads, kMoveThreads, 0, st.st>>>(a) : evict_move_kernel<64><<<heads, kMoveThreads, 0, st.st>>>(a);
+                JUNO_CUDA_TRY(launch_pdl(p->head_dim == 128 ? evict_move_kernel<128> : evict_move_kernel<64>, heads, dim3(kMoveThreads), 0, st.st, a));
         }
-        JUNO_CUDA_TRY(cudaGetLastError());
         c->kernel_launches += 2;
         p->free_pages.resize(next);
-        std::vector<int32_t> table;
         for (int i = 0; i < n; i++) {
             juno_seq *s = seqs[i];
             if (s->len <= keep) continue;

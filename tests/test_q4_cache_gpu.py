@@ -472,6 +472,38 @@ def test_eviction_of_long_sequences(ctx, n, keep, recent):
     cache.close()
 
 
+@pytest.mark.parametrize("n,branches", [(40000, 1), (500, 60)])
+def test_branches_are_cut_down_alone(ctx, n, branches):
+    """A long branch, whose page table takes several launches, and many at once, whose rows and pages do not fit into one; the sequence they come from stays."""
+    rng = np.random.default_rng(branches)
+    kv, dim, keep, recent = 2, 64, 300, 40
+    cache = PagedKvCache(ctx, 1, kv, dim, (n + 15) // 16 + branches * ((keep + 15) // 16), "q4", track_seqs=branches + 1, track_tokens=n)
+    s = cache.new_sequence(n, track=True)
+    have = (rows(rng, n, kv, dim), rows(rng, n, kv, dim))
+    fill(cache, 0, [s], [0], [have])
+    w = some_weights(rng, (1, kv, n))
+    t = dev(w)
+    settle()
+    cache.weights_device(0, [s], [n], t, store=True)
+    of = [n - i for i in range(branches)]
+    cut = [cache.fork(s, m) for m in of]
+    kept = torch.full((1, branches, kv, keep), 99, dtype=torch.int32, device="cuda")
+    settle()
+    cache.evict(cut, keep, recent, kept=kept)
+    settle()
+    got, got_w = read(cache, 0, cut, [0] * branches, [keep] * branches), weights(cache, 0, cut, [keep] * branches)
+    for i, m in enumerate(of):
+        at, k, v, wl = expected([(have[0][:m], have[1][:m])], w[..., :m], keep, recent)[0]
+        assert np.array_equal(kept.cpu().numpy()[0, i], at)
+        mine = slice(i * keep, (i + 1) * keep)
+        assert np.array_equal(got[0][mine], f32(q4.held(k))) and np.array_equal(got[1][mine], f32(q4.held(v)))
+        assert np.array_equal(got_w[i], wl, equal_nan=True)
+    whole = read(cache, 0, [s], [0], [n])
+    assert np.array_equal(whole[0], f32(q4.held(have[0]))) and np.array_equal(whole[1], f32(q4.held(have[1])))
+    assert np.array_equal(weights(cache, 0, [s], [n])[0], w[0], equal_nan=True)
+    cache.close()
+
+
 @pytest.mark.parametrize("kv,dim", [(2, 64), (3, 128)])
 def test_eviction_in_a_full_pool_moves_rows_in_place(ctx, kv, dim):
     """No page is free: sequences are cut down within their own pages, one of them shares its first pages with a shorter one and is refused."""
