@@ -275,7 +275,6 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             m_run[h] = -INFINITY;
             l_run[h] = 0.f;
         }
-        const float fifteen = g8 & 1 ? 15.f : 0.f;
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
         float *own_row = mg_o + (warp * HEADS + HPL * t) * Smem::kMergeRow + 4 * g8;  // of head HPL * t: dimensions 4 g8 .. 4 g8 + 3 of a group
         int j = 0;
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                     steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
                     if (steps > (limit & 0xffffu)) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
                         const int e = max((int)(steps >> 7) - 127, -100);
-                        const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23 | (uint32_t)(g8 & 1) << 31);  // odd positions have 15 - q
+                        const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23);
                         vfix = vscale == 0.f ? 0.f : next / vscale;
                         vscale = next;
                         limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
@@ -446,7 +445,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
                             w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
-                            ws[h][x] = w[h][x] * vscale;
+                            ws[h][x] = w[h][x] * (x ? -vscale : vscale);  // positions 8..15: 15 - q
                         }
                         l_run[h] += w[h][0] + w[h][1];
                     }
@@ -457,7 +456,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                         for (int g = 0; g < NG; g += 2) {
                             const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&vm[u][x][g >> 1]));
-                            const float m0 = fmaf(step_of(d[u][x], g), fifteen, two.x), m1 = fmaf(step_of(d[u][x], g + 1), fifteen, two.y);
+                            const float m0 = x ? fmaf(step_of(d[u][x], g), 15.f, two.x) : two.x, m1 = x ? fmaf(step_of(d[u][x], g + 1), 15.f, two.y) : two.y;
 #pragma unroll
                             for (int h = 0; h < HPL; h++) {
                                 offset[h][g] = fmaf(w[h][x], m0, offset[h][g]);
@@ -498,7 +497,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 if (part_issued < part_tiles) issue();
             }
             // a chain's sums, over the lanes that share a head for the offsets' part, to where the warps meet
-            const float unscale = vscale == 0.f ? 0.f : 262144.f / fabsf(vscale);  // 2^18
+            const float unscale = vscale == 0.f ? 0.f : 262144.f / vscale;  // 2^18
 #pragma unroll
             for (int h = 0; h < HPL; h++)
 #pragma unroll

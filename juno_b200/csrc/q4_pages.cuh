@@ -12,7 +12,7 @@
 //   keys    codes  word [position][t][group], t = 0..3: the numbers of dimensions 8t .. 8t + 7 of the group, a unit of four to a half word
 //           d      half word [position][group]
 //           m      half word [position][group]
-//   values  codes  half word [position][group][u], u = 0..7: the unit of dimensions 4u .. 4u + 3 of the group, in odd positions of 15 - q: decode attention adds
+//   values  codes  half word [position][group][u], u = 0..7: the unit of dimensions 4u .. 4u + 3 of the group, in positions 8..15 of 15 - q: decode attention adds
 //                  up (m + 15 d) - d (15 - q) there, so that its sums of numbers do not grow all one way; the 16-byte pieces of a position, one per group, are
 //                  permuted so that eight positions' pieces of one group lie on different banks
 //           d      half word [position][group]
@@ -43,7 +43,7 @@ JHD int q4_v_offset(int hd, int p, int g) { return 19 * hd + (p * (hd / kQ4Group
 // fraction: with an AND it is the FP16 number q 2^-18.
 JHD uint32_t q4_unit(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return a << 6 | b << 10 | c << 2 | (d & 3u) << 14 | d >> 2; }
 // 15 - q for q, all numbers of a word: what an XOR with this does.
-JHD uint32_t q4_v_flip(int p) { return p & 1 ? 0xffffffffu : 0u; }
+JHD uint32_t q4_v_flip(int p) { return p & 8 ? 0xffffffffu : 0u; }
 
 // The number of x in a group with offset m and step d, decided exactly (inv is about 1 / d).  s + r is x - m exactly; half-way points (q + 1/2) d have 13
 // bits and are exact, so that the comparisons decide what the estimate may have missed by one.
