@@ -344,8 +344,9 @@ static int launch_rows(juno_ctx *c, const juno_kvpool *p, int layer, const Cache
     const int hd = p->head_dim;
     ProfScope prof(c, st, APPEND ? PROF_ROPE_APPEND : PROF_OTHER, (double)n_tokens * p->n_kv_heads * (8.0 * hd + p->row_bytes()));
     if (p->dtype == kKvQ4 && APPEND) {
-        // several positions to a CTA once there are CTAs for every SM several times over
-        const int each = n_tokens >= c->sm_count * 16 ? kAppendRows : 1;
+        // Several positions to a CTA hide the loads once there are CTAs for every SM many times over, one gives few positions more SMs (eight heads of 128, one
+        // and four: 592 positions 6.2 and 12.0 us, 2368 10.6 and 12.8, 4736 both 16.5, 8156 26 and 24).
+        const int each = n_tokens >= c->sm_count * 32 ? kAppendRows : 1;
         const dim3 grid((unsigned)((n_tokens + each - 1) / each), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 8) + 31) / 32 * 32));
         if (each == 1)
             JUNO_CUDA_TRY(launch_pdl(hd == 128 ? q4_append_kernel<128, 1> : q4_append_kernel<64, 1>, grid, block, 0, st, a));

@@ -45,14 +45,16 @@ __device__ __forceinline__ int row_parts(const Q4AttnParams &p, int i, const Cac
 }
 
 constexpr int kQ4MaxGroup = 8, kQ4Slots = 2, kQ4Tile = 2;  // pages of a tile: a warp's step
-// Warps of a CTA and CTAs on an SM: 16 warps of 128 registers, 12 of 168 for more than four heads of 128.
+// Warps of a CTA and CTAs on an SM: 16 warps of 128 registers, 12 of 168 for more than four heads of 128, whose sums need them (48 requests of 8192 positions with
+// eight heads a key/value head: 118 us; 16 warps with tiles of one page, so that they fit into 128 registers, 138, 12 with such tiles 131).
 template <int HD, int HPL>
 constexpr int kQ4Warps = HPL == 1 || HD == 64 ? 8 : 4;
 template <int HD, int HPL>
 constexpr int kQ4Ctas = HPL == 1 || HD == 64 ? 2 : 3;
 
-// Tiles whose products are added up in an MMA's sums: an MMA cuts off what lies more than 24 bits below the sum, so that a long chain of them falls behind by
-// 2^-25 of it a time.  After 32 the sums go to FP32 ones in shared memory.
+// Tiles whose products are added up in an MMA's sums.  An MMA cuts off what lies more than 24 bits below its largest term or sum, always towards zero, so
+// that a long chain of them falls behind by some 2^-25 of the sum a time: 48 requests of 8192 positions were 5.8e-6 of the result off without a limit, where one
+// request of 2048 is 6e-7 off; they are 1.7e-6 off with chains of 32 MMAs, whose sums then go to FP32 ones in shared memory.  That costs 1 % of the time.
 template <int HPL>
 constexpr int kQ4Chain = HPL == 1 ? 16 : 8;
 
@@ -110,23 +112,100 @@ __device__ __forceinline__ void numbers_of(uint32_t units, uint32_t (&x)[4]) {
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
 __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
-// A share's pages of one row are tiles of two pages, spread over four warps; each warp has a ring of kQ4Slots tiles that bulk copies fill, the next row's first
+// A share's pages of one row are tiles of two pages, spread over the CTA's warps; each warp has a ring of kQ4Slots tiles that bulk copies fill, the next row's first
 // tiles already while this one's results are put together.  Per page
-//   S = K Q   m16n8k16: the 16 positions are the rows, a group's 32 dimensions the k of two MMAs, the columns query heads.  The numbers are not converted: in
-//             the low bits of a half they are the subnormal q 2^-24, in the next four 16 q 2^-24, which the query's side takes back; two ANDs
-//             and half a shift make a register.  A group's result is multiplied by its step d in FP32 and the offset's part, m times the sum of the query
-//             over the group, added.
+//   S = K Q   m16n8k16: the 16 positions are the rows, a group's 32 dimensions the k of two MMAs, the columns query heads.  The numbers are FP16 numbers as they lie
+//             (q4_unit), after an AND.  A group's result is multiplied by its step d in FP32, and the offsets' part, m times the sum of the query over the group,
+//             comes from one more MMA, whose operand m is as it lies in the page.
 //   O += V P  rows are dimensions, k the positions, columns heads; a weight is multiplied by the step of its position and group first, and the offsets' part
-//             is a sum of their own per lane.  The product is scaled by a power of two that follows the largest step, so that it keeps its digits in FP16.
+//             is a sum of its own per lane, in FP32.  The product is scaled by a power of two that follows the largest step, so that it keeps its digits in FP16.
+//             The numbers of half the positions count from the other end (q4_v_flip), those positions' products have a minus: the sums stay as small as
+//             the result, where sums of numbers that are all positive would be larger than it by the root of the number of positions that count.
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
 // eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
+// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and 350 of them (four heads of 128, of which 33
+// MMAs) or 440 (eight) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
+// over 8 of 128: 42 us for 168 MB, 4.0 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 15.6, of which 10 begin and end
+// parts; 48 of up to 8192 with eight heads to a key/value head 116 us for 384 MB.
 template <int HD, int HPL>
 struct Q4Smem {  // bytes
     static constexpr int kRing = kQ4Warps<HD, HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HD, HPL> * kQ4Slots * 8, kMergeRow = HD + 8,  // floats; the pads keep rows on different banks
                          kQuery = kMerge + kQ4Warps<HD, HPL> * 4 * HPL * (kMergeRow + 2) * 4, kQueryRow = HD + 32,  // halves
         kSums = kQuery + 2 * 4 * HPL * kQueryRow * 2, kBack = kSums + 2 * 4 * HPL * 4 * 2, kAll = kBack + 4 * HPL * 4;
 };
+
+// A row's parts put together, by the CTA that was last: two dimensions of a head to a thread, a head to a warp, a part's largest score and sum to a lane.
+template <int HD, int HPL, bool TRACK>
+__device__ __forceinline__ void q4_merge_parts(const Q4AttnParams &p, int i, int share_a, int parts, int kvh) {
+    constexpr int W = kQ4Warps<HD, HPL>, HEADS = 4 * HPL;
+    const int tid = threadIdx.x, lane = tid & 31, G = p.n_heads / p.n_kv_heads, h0 = kvh * G;
+    // The results of 16 parts are asked for at once, or of 8 where a thread has four places: one CTA reads them, and what it waits for is their latency
+    // (one row of 16384 positions with eight heads a key/value head, 43 parts: 22 us; 36 with eight parts at a time and one place after the other).
+    constexpr int ITEMS = (HEADS * (HD / 2) + W * 32 - 1) / (W * 32), AHEAD = ITEMS == 1 ? 16 : 8;
+    const size_t stride = (size_t)p.n_heads * HD;
+    const float2 *from_ml = reinterpret_cast<const float2 *>(p.part_ml) + (size_t)(i + share_a) * p.n_heads + h0;
+    const float *from_o = p.part_o + (size_t)(i + share_a) * stride + (size_t)h0 * HD;
+    float2 v[ITEMS][AHEAD], ml[ITEMS];
+    auto ask = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++) {
+            const int idx = tid + k * W * 32;
+            if (idx >= G * (HD / 2)) continue;
+#pragma unroll
+            for (int s = 0; s < AHEAD; s++)
+                if (base + s < parts) v[k][s] = __ldcg(reinterpret_cast<const float2 *>(from_o + (base + s) * stride) + idx);
+        }
+    };
+    auto largest = [&](int k, int s) {
+        const int g = min((tid + k * W * 32) / (HD / 2), G - 1);
+        return s < parts ? __ldcg(from_ml + (size_t)s * p.n_heads + g) : make_float2(-INFINITY, 0.f);
+    };
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) ml[k] = largest(k, lane);
+    ask(0);
+    float M[ITEMS], L[ITEMS], f[ITEMS], ax[ITEMS], ay[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+        M[k] = ml[k].x;
+        for (int s = lane + 32; s < parts; s += 32) M[k] = fmaxf(M[k], largest(k, s).x);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x));
+        L[k] = ax[k] = ay[k] = 0.f;
+    }
+    for (int base = 0; base < parts; base += AHEAD) {
+        if (base > 0) ask(base);
+        if ((base & 31) == 0) {
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++) {
+                if (base > 0) ml[k] = largest(k, base + lane);
+                f[k] = exp2_fast(ml[k].x - M[k]);
+                L[k] = fmaf(ml[k].y, f[k], L[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++)
+#pragma unroll
+            for (int s = 0; s < AHEAD; s++) {
+                const float fs = __shfl_sync(0xffffffffu, f[k], (base + s) & 31);
+                if (base + s < parts) {
+                    ax[k] = fmaf(v[k][s].x, fs, ax[k]);
+                    ay[k] = fmaf(v[k][s].y, fs, ay[k]);
+                }
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x);
+        const int idx = tid + k * W * 32, g = idx / (HD / 2);
+        if (g >= G) continue;
+        float *to_o = p.out + (size_t)i * p.ldo + h0 * HD + 2 * idx;
+        to_o[0] = ax[k] / L[k];
+        to_o[1] = ay[k] / L[k];
+        if (TRACK && idx == g * (HD / 2)) p.sums[(size_t)i * p.n_heads + h0 + g] = make_float2(M[k], 1.f / L[k]);
+    }
+}
 
 template <int HD, int HPL, bool TRACK>
 __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
@@ -597,61 +676,16 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         const CacheRow whole = cache_row(p.rows, i);
         const int share_a = whole.share, parts = row_parts(p, i, whole);
         if (!__syncthreads_or(tid == 0 && (which ? before_b : before_a) == (unsigned)parts - 1)) continue;
-        // two dimensions of a head to a thread, a head to a warp, a part's largest score and sum to a lane
         if (tid == 0) {
             __threadfence();
             p.arrived[(size_t)i * p.n_kv_heads + kvh] = 0;
         }
-        const size_t stride = (size_t)p.n_heads * HD;
-        for (int idx = tid; idx < G * (HD / 2); idx += W * 32) {
-            const int g = idx / (HD / 2), d = 2 * (idx - g * (HD / 2));
-            const float2 *from_ml = reinterpret_cast<const float2 *>(p.part_ml) + (size_t)(i + share_a) * p.n_heads + h0 + g;
-            const float *from_o = p.part_o + (size_t)(i + share_a) * stride + (size_t)(h0 + g) * HD + d;
-            constexpr int AHEAD = 8;  // parts asked for before their weights are known
-            float2 v[AHEAD], ml = make_float2(-INFINITY, 0.f);
-            if (lane < parts) ml = __ldcg(from_ml + (size_t)lane * p.n_heads);
-#pragma unroll
-            for (int s = 0; s < AHEAD; s++)
-                if (s < parts) v[s] = __ldcg(reinterpret_cast<const float2 *>(from_o + s * stride));
-            float M = ml.x;
-            for (int s = lane + 32; s < parts; s += 32) M = fmaxf(M, __ldcg(from_ml + (size_t)s * p.n_heads).x);
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-            float L = 0.f, ax = 0.f, ay = 0.f;
-            for (int base = 0; base < parts; base += 32) {
-                if (base > 0) ml = base + lane < parts ? __ldcg(from_ml + (size_t)(base + lane) * p.n_heads) : make_float2(-INFINITY, 0.f);
-                const float f = base + lane < parts ? exp2_fast(ml.x - M) : 0.f;
-                L = fmaf(ml.y, f, L);
-                const int n = min(32, parts - base);
-                if (base == 0) {
-#pragma unroll
-                    for (int s = 0; s < AHEAD; s++) {
-                        const float fs = __shfl_sync(0xffffffffu, f, s);
-                        if (s < parts) {
-                            ax = fmaf(v[s].x, fs, ax);
-                            ay = fmaf(v[s].y, fs, ay);
-                        }
-                    }
-                }
-#pragma unroll 12
-                for (int s = base ? 0 : AHEAD; s < n; s++) {
-                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(from_o + (base + s) * stride));
-                    const float fs = __shfl_sync(0xffffffffu, f, s);
-                    ax = fmaf(y.x, fs, ax);
-                    ay = fmaf(y.y, fs, ay);
-                }
-            }
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-            float *to_o = p.out + (size_t)i * p.ldo + (h0 + g) * HD + d;
-            to_o[0] = ax / L;
-            to_o[1] = ay / L;
-            if (TRACK && d == 0) p.sums[(size_t)i * p.n_heads + h0 + g] = make_float2(M, 1.f / L);
-        }
+        q4_merge_parts<HD, HPL, TRACK>(p, i, share_a, parts, kvh);
     }
 }
 
-// The weight that positions have received: a thread has one position of all rows' pages and one key/value head.
+// The weight that positions have received: a thread has one position of all rows' pages and one key/value head.  Bound by the scores, which come out of L2:
+// 10 us of the 51 that attention and weights of 16 sequences of up to 8192 positions take.
 constexpr int kQ4WeightThreads = 256;
 template <int G>
 __device__ __forceinline__ float weight_of(const float *scores, const float2 *sums, int g_max) {
