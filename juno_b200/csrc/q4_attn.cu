@@ -122,12 +122,12 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 //             The numbers of half the positions count from the other end (q4_v_flip), those positions' products have a minus: the sums stay as small as
 //             the result, where sums of numbers that are all positive would be larger than it by the root of the number of positions that count.
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
-// eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.
+// eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.  Four heads of 131072 positions take 41 us as the former, 60 as the latter.
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
 // What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and 350 of them (four heads of 128, of which 33
 // MMAs) or 440 (eight) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
-// over 8 of 128: 42 us for 168 MB, 4.0 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 15.6, of which 10 begin and end
-// parts; 48 of up to 8192 with eight heads to a key/value head 116 us for 384 MB.
+// over 8 of 128: 41 us for 168 MB, 4.1 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 15.7, of which 10 begin and end
+// parts; 48 of up to 8192 with eight heads to a key/value head 117 us for 384 MB.
 template <int HD, int HPL>
 struct Q4Smem {  // bytes
     static constexpr int kRing = kQ4Warps<HD, HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HD, HPL> * kQ4Slots * 8, kMergeRow = HD + 8,  // floats; the pads keep rows on different banks
@@ -675,11 +675,12 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         if (i < 0) continue;
         const CacheRow whole = cache_row(p.rows, i);
         const int share_a = whole.share, parts = row_parts(p, i, whole);
-        if (!__syncthreads_or(tid == 0 && (which ? before_b : before_a) == (unsigned)parts - 1)) continue;
-        if (tid == 0) {
+        const bool last = tid == 0 && (which ? before_b : before_a) == (unsigned)parts - 1;
+        if (last) {
             __threadfence();
             p.arrived[(size_t)i * p.n_kv_heads + kvh] = 0;
         }
+        if (!__syncthreads_or(last)) continue;
         q4_merge_parts<HD, HPL, TRACK>(p, i, share_a, parts, kvh);
     }
 }
@@ -737,7 +738,8 @@ static int launch_q4_attn(const Q4AttnParams &a, int G, int shares, cudaStream_t
 
 // How the pages are cut for `slots` CTAs per key/value head that run at a time.  Either each row into parts of about equal length, no more than `slots` of them:
 // then a CTA begins once, and the longest part is waited for; or all pages into equal shares across the rows: no CTA waits for another, but most begin
-// a second row (kQ4BeginCost rounds).  A round is `round` pages, a tile for every warp of a CTA.
+// a second row (kQ4BeginCost rounds).  A round is `round` pages, a tile for every warp of a CTA.  Parts and shares, 32 heads over 8 of 128: 4 rows of 4096 positions
+// 12.5 and 15.8 us, 16 of 8192 35.9 and 37.0, 24 of 8192 63.4 and 49.0, which the rule tells apart; 32 of 4096 38.1 and 39.5, which it does not.
 constexpr int kQ4BeginCost = 4;
 static void q4_cut(std::vector<CacheRow> &rows, int pages, int slots, int round, std::vector<int32_t> *cuts) {
     const int n = (int)rows.size(), share = std::max(round, (pages + slots - 1) / slots);
