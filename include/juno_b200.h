@@ -205,8 +205,8 @@ int juno_kv_weights_device(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t
                            const int32_t *counts, float *w_dev, int64_t ld, int32_t store, void *stream);
 /* Cuts sequences that keep weights down to `keep` positions: in every layer and key/value head the newest `recent` (at most keep) stay, and
  * of the older ones those of most weight, the earlier of two equal ones (a NaN counts least).  They move to the front in order, with
- * their weights, and the sequence's length is `keep`; pages behind return to the pool.  Pages shared with a fork are left to it, which takes fresh ones
- * (JUNO_ERR_OOM, and nothing has changed, when there are not enough).  Shorter sequences stay as they are.  From then on the cached
+ * their weights, and the sequence's length is `keep`; pages behind return to the pool.  Pages that another sequence shares are left to it, and the rows go to
+ * fresh ones (JUNO_ERR_OOM, and nothing has changed, when there are not enough).  Shorter sequences stay as they are.  From then on the cached
  * positions of different heads are different tokens, in order: keys carry their rotation, so attention and further appends go on.
  * kept_dev (or NULL): int32 [n_layers][n][n_kv_heads][keep], the places before, ascending, -1 behind a shorter sequence's. */
 int juno_kv_evict(juno_ctx *ctx, juno_kvpool *p, int32_t n, juno_seq *const *seqs, int32_t keep, int32_t recent,

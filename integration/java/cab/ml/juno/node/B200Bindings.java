@@ -81,6 +81,14 @@ final class B200Bindings {
 	static final MethodHandle seqFree = h("juno_seq_free", fn(ADDRESS));
 	static final MethodHandle seqLength = h("juno_seq_length", fn(ADDRESS, ADDRESS));
 	static final MethodHandle seqFork = h("juno_seq_fork", fn(ADDRESS, JAVA_INT, ADDRESS));
+	/** JUNO_KV_Q4 pools: device pointers, a cudaStream_t (NULL = the context's stream); the calls return before their work is done. */
+	static final MethodHandle kvAppendDevice = h("juno_kv_append_device", fn(ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS));
+	static final MethodHandle kvReadDevice = h("juno_kv_read_device", fn(ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS));
+	static final MethodHandle attnDecodeDevice = h("juno_attn_decode_device", fn(ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_LONG, ADDRESS, JAVA_LONG, ADDRESS));
+	static final MethodHandle kvpoolTrack = h("juno_kvpool_track", fn(ADDRESS, JAVA_INT, JAVA_INT));
+	static final MethodHandle seqTrack = h("juno_seq_track", fn(ADDRESS));
+	static final MethodHandle kvWeightsDevice = h("juno_kv_weights_device", fn(ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, JAVA_INT, ADDRESS));
+	static final MethodHandle kvEvict = h("juno_kv_evict", fn(ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS));
 	static final MethodHandle forward = h("juno_forward", fn(ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS));
 	static final MethodHandle prefill = h("juno_prefill", fn(ADDRESS, ADDRESS, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS));
 	static final MethodHandle decodeGreedy = h("juno_decode_greedy", fn(ADDRESS, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, JAVA_INT, ADDRESS));

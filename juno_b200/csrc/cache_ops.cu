@@ -143,7 +143,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // A CTA has R positions, of keys (blockIdx.y = 0) or values.  A lane has eight neighbouring dimensions, four lanes a group: what is stored of a position is
 // contiguous.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate
 // of q4_number (a saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided
-// exactly.  131072 positions of eight heads of 128: 1.24 GB in 250 us, 5.0 TB/s; 8156 of them 77 MB in 20 us.
+// exactly.  131072 positions of eight heads of 128: 1.24 GB in 250 us, 5.0 TB/s; 8156 of them 77 MB in 24 us.
 template <int HD, int R, bool V>
 __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace (&places)[R], int row0) {
     constexpr int LPV = HD / 8;  // lanes per vector
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ 
 __device__ __forceinline__ float bits_as_float(uint32_t w, uint32_t mask) { return __uint_as_float((w & mask) | 0x4b000000u) - 8388608.f; }
 
 // A CTA has kReadRows positions, of keys (blockIdx.y = 0) or values; a lane has four neighbouring dimensions, so that a warp's stores are contiguous, and the loads of
-// all positions are under way together.  8156 positions of eight heads of 128: 77 MB in 15 us, 5.1 TB/s.
+// all positions are under way together.  8156 positions of eight heads of 128: 77 MB in 17 us, 4.6 TB/s.
 constexpr int kAppendRows = 4, kReadRows = 8;
 template <int HD, bool V>
 __device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&places)[kReadRows], int row0) {
@@ -445,8 +445,8 @@ __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *sums, uns
 
 // One CTA per (sequence, layer, head): which positions stay, in order, and their weights.  The weight that decides (the need-th largest) is found digit by
 // digit, 11, 11 and 10 bits, with a count of every digit in shared memory: three passes over the weights, whatever they are.  Up to kSelectCached weights are
-// read from memory once.  Six sequences of up to 8192 positions, four layers, eight heads: 20 us, a chain of barriers and passes over shared memory (11 of the 15 are
-// counts and scans; 1024 threads instead of 512 take as long).
+// read from memory once.  Six sequences of up to 8192 positions, four layers, eight heads: 20 us, a chain of barriers and passes over shared memory (1024 threads
+// instead of 512 take as long).
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
     const int h = blockIdx.x, layer = blockIdx.y, i = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_launch_dependents();
