@@ -1340,6 +1340,10 @@ int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens) {
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
     JUNO_REQUIRE(!p->weights, "this pool keeps weights already");
     DeviceGuard g(p->ctx->device);
+    JUNO_TRY(guarded([&]() -> int {
+        p->free_tracks.reserve((size_t)n_seqs);
+        return JUNO_OK;
+    }));
     const int room = (max_tokens + kPageTokens - 1) / kPageTokens * kPageTokens;
     const size_t bytes = (size_t)n_seqs * p->n_layers * p->n_kv_heads * room * sizeof(float);
     const cudaError_t e = cudaMalloc((void **)&p->weights, bytes);
@@ -1379,9 +1383,9 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     JUNO_REQUIRE(!p->latent, "this sequence belongs to a model with latent pages: it has no K and V to append");
     JUNO_REQUIRE(layer >= 0 && layer < p->n_layers, "layer %d out of range", layer);
     JUNO_REQUIRE(pos >= 0 && n_tokens >= 0, "bad position range");
-    JUNO_REQUIRE(p->dtype != kKvQ4 || pos <= s->len, "position %d is not behind the %d cached ones", pos, s->len);
     if (n_tokens == 0) return JUNO_OK;
     std::lock_guard<std::recursive_mutex> lk(c->mu);
+    JUNO_REQUIRE(p->dtype != kKvQ4 || pos <= s->len, "position %d is not behind the %d cached ones", pos, s->len);
     DeviceGuard g(c->device);
     JUNO_TRY(seq_reserve(s, pos, pos + n_tokens, c->stream));
     const int kvdim = p->n_kv_heads * p->head_dim;
@@ -1447,7 +1451,7 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
         JUNO_TRY(ensure_device(&py, &c->stage_y_bytes, qbytes));
         c->stage_y = (float *)py;
         JUNO_CUDA_TRY(cudaMemcpyAsync(c->stage_x, q_host, qbytes, cudaMemcpyHostToDevice, c->stream));
-        JUNO_TRY(q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, WAIT_BLOCKING, c->stream));
+        JUNO_TRY(guarded([&] { return q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, WAIT_BLOCKING, c->stream); }));
         JUNO_CUDA_TRY(cudaMemcpyAsync(out_host, c->stage_y, qbytes, cudaMemcpyDeviceToHost, c->stream));
         JUNO_CUDA_TRY(cudaStreamSynchronize(c->stream));
         JUNO_TRY(wait_status(c, WAIT_BLOCKING));

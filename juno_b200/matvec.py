@@ -221,7 +221,8 @@ class PagedKvCache:
     the attention weights of that many sequences of up to track_tokens positions; `evict` cuts such sequences down by them.
 
     The *_device calls take CUDA tensors and return before the work is done; `stream` is a cudaStream_t as an integer or an object with
-    `cuda_stream`, None the context's stream.  The legacy default stream, whose handle is 0, is meant by 0."""
+    `cuda_stream`, None the context's stream.  The legacy default stream, whose handle is 0, is meant by 0.  The caller's own work on the tensors is
+    ordered by that stream and no other: name the stream that made them (torch.cuda.current_stream()), and keep them until the work is done."""
 
     def __init__(self, ctx: GpuContext, n_layers: int, n_kv_heads: int, head_dim: int, n_pages: int, kv_dtype: str = "f16",
                  track_seqs: int = 0, track_tokens: int = 0):
@@ -285,7 +286,12 @@ class PagedKvCache:
 
     @staticmethod
     def _ints(x, n: int, name: str) -> np.ndarray:
-        a = np.asarray(x, dtype=np.int32)
+        a = np.asarray(x)
+        if a.dtype != np.int32:
+            whole = a.astype(np.int32) if a.dtype.kind in "iu" else None
+            if whole is None or (whole != a).any():
+                raise ValueError(f"{name}: whole numbers of 32 bits are wanted")
+            a = whole
         if a.shape != (n,):
             raise ValueError(f"{name}: {n} whole numbers are wanted, not shape {a.shape}")
         return a
@@ -342,6 +348,8 @@ class PagedKvCache:
         """Cuts sequences down to the `keep` positions of most weight, the newest `recent` among them, in every layer and key/value head; kept:
         int32 [n_layers, sequences, n_kv_heads, keep] gets their places (juno_kv_evict)."""
         b, kp = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs), None
+        if keep >= 1 << 31 or recent >= 1 << 31:
+            raise ValueError(f"keep {keep}, recent {recent}: whole numbers of 32 bits are wanted")
         if kept is not None:
             kp = _whole_ptr(kept, "kept", "int32", (self.n_layers, b.n, self.n_kv_heads))
             if kept.shape[3] != keep:

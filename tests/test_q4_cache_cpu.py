@@ -129,3 +129,14 @@ def test_binding_refuses_what_is_not_a_tensor():
     with pytest.raises(ValueError, match="whole numbers"):
         PagedKvCache._ints([1, 2], 3, "counts")
     assert PagedKvCache._stream(None) is None and PagedKvCache._stream(0) == 1 and PagedKvCache._stream(77) == 77
+
+
+def test_lengths_are_whole_numbers_of_32_bits():
+    from juno_b200.matvec import PagedKvCache
+    ints = PagedKvCache._ints
+    for x in ([1, 2], (1, 2), np.array([1, 2]), np.array([1, 2], dtype=np.uint8), np.array([1, 9, 2], dtype=np.int32)[::2]):
+        a = ints(x, 2, "lens")
+        assert a.dtype == np.int32 and a.tolist() == [1, 2]
+    for x in ([1.0, 2.0], [1], [[1, 2]], [True, False], [1, 2 ** 32 + 1], np.array([1, 2 ** 31]), ["1", "2"]):
+        with pytest.raises(ValueError):
+            ints(x, 2, "lens")

@@ -703,6 +703,8 @@ def test_refusals(ctx):
         ("keeps no weights", lambda: cache.evict([a, b], 1)),
         ("there twice", lambda: cache.evict([a, a], 1)),
         ("keep 0", lambda: cache.evict([a], 0)),
+        ("32 bits", lambda: cache.evict([a], 2 ** 32 + 1)),
+        ("32 bits", lambda: cache.attention_device(0, [a], q, 8, out, lens=[1.5])),
         ("recent 3", lambda: cache.evict([a], 2, 3)),
         ("recent -1", lambda: cache.evict([a], 2, -1)),
         ("cached positions", lambda: cache.weights_device(0, [a], [3], torch.zeros((1, 2, 3), device="cuda"))),
