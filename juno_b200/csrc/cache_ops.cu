@@ -247,16 +247,28 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ 
 // A number that lies in bits of a word below 2^23, as FP32: without a conversion.
 __device__ __forceinline__ float bits_as_float(uint32_t w, uint32_t mask) { return __uint_as_float((w & mask) | 0x4b000000u) - 8388608.f; }
 
-// A CTA has kReadRows positions, of keys (blockIdx.y = 0) or values; a lane has four neighbouring dimensions, so that a warp's stores are contiguous, and the loads of
-// all positions are under way together.  8156 positions of eight heads of 128: 77 MB in 17 us, 4.6 TB/s.
-constexpr int kAppendRows = 4, kReadRows = 8;
+// A CTA has kReadRows positions, of keys (blockIdx.y = 0) or values; a lane has eight neighbouring dimensions, which it writes at once where they are aligned, and
+// the loads of all positions are under way together.  8156 positions of eight heads of 128, 77 MB, with their append: 33.7 us (four dimensions of two groups a lane
+// 34.2, of one group 34.9).
+constexpr int kAppendRows = 4, kReadRows = 4;
+__device__ __forceinline__ void store8(float *to, const float (&x)[8], int wide) {
+    if (wide == 2) {
+        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]) : "memory");
+    } else if (wide == 1) {
+        *reinterpret_cast<float4 *>(to) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) to[e] = x[e];
+    }
+}
 template <int HD, bool V>
 __device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&places)[kReadRows], int row0) {
-    constexpr int LPV = HD / 4;
-    const int H = p.n_kv_heads, sub = threadIdx.x % LPV, piece = sub & 7, g = sub >> 3, n_rows = min(kReadRows, p.n_tokens - row0);
+    constexpr int LPV = HD / 8;
+    const int H = p.n_kv_heads, sub = threadIdx.x % LPV, t = sub & 3, g = sub >> 2, n_rows = min(kReadRows, p.n_tokens - row0);
     for (int h = threadIdx.x / LPV; h < H; h += blockDim.x / LPV) {
-        float *to = (V ? p.v : p.k) + row0 * p.ld + h * HD + sub * 4;
-        const bool vec4 = (reinterpret_cast<uintptr_t>(to) & 15) == 0 && (p.ld & 3) == 0;
+        float *to = (V ? p.v : p.k) + row0 * p.ld + h * HD + sub * 8;
+        const int wide = (reinterpret_cast<uintptr_t>(to) & 31) == 0 && (p.ld & 7) == 0 ? 2 : (reinterpret_cast<uintptr_t>(to) & 15) == 0 && (p.ld & 3) == 0 ? 1 : 0;
         uint32_t w[kReadRows];
         __half m[kReadRows];
         __nv_bfloat16 d[kReadRows];
@@ -267,24 +279,23 @@ __device__ __forceinline__ void read_rows(const RowsParams &p, const RowPlace (&
             const uint8_t *block = at.page + h * q4_block_bytes(HD);
             m[n] = *reinterpret_cast<const __half *>(block + (V ? q4_v_offset(HD, pp, g) : q4_k_offset(HD, pp, g)));
             d[n] = *reinterpret_cast<const __nv_bfloat16 *>(block + (V ? q4_v_step(HD, pp, g) : q4_k_step(HD, pp, g)));
-            w[n] = *reinterpret_cast<const uint16_t *>(block + (V ? q4_v_code(HD, pp, piece, g) : q4_k_code(HD, pp, piece >> 1, g) + 2 * (piece & 1)));
-            if (V) w[n] ^= q4_v_flip(pp) & 0xffffu;
+            w[n] = *reinterpret_cast<const uint32_t *>(block + (V ? q4_v_code(HD, pp, 2 * t, g) : q4_k_code(HD, pp, t, g)));
+            if (V) w[n] ^= q4_v_flip(pp);
         }
 #pragma unroll
         for (int n = 0; n < kReadRows; n++) {
             if (n >= n_rows) break;
-            const float mf = __half2float(m[n]), df = __bfloat162float(d[n]);
-            const uint32_t turned = w[n] >> 8 | w[n] << 8;
-            const float4 x = make_float4(fmaf(df * 0x1p-6f, bits_as_float(w[n], 0x3c0u), mf), fmaf(df * 0x1p-10f, bits_as_float(w[n], 0x3c00u), mf),
-                                         fmaf(df * 0x1p-2f, bits_as_float(w[n], 0x3cu), mf), fmaf(df * 0x1p-6f, bits_as_float(turned, 0x3c0u), mf));
-            if (vec4) {
-                *reinterpret_cast<float4 *>(to) = x;
-            } else {
-                to[0] = x.x;
-                to[1] = x.y;
-                to[2] = x.z;
-                to[3] = x.w;
+            const float off = __half2float(m[n]), df = __bfloat162float(d[n]);
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t u = k ? w[n] >> 16 : w[n], turned = __byte_perm(w[n], 0, k ? 0x0023 : 0x0001);
+                x[4 * k] = fmaf(df * 0x1p-6f, bits_as_float(u, 0x3c0u), off);
+                x[4 * k + 1] = fmaf(df * 0x1p-10f, bits_as_float(u, 0x3c00u), off);
+                x[4 * k + 2] = fmaf(df * 0x1p-2f, bits_as_float(u, 0x3cu), off);
+                x[4 * k + 3] = fmaf(df * 0x1p-6f, bits_as_float(turned, 0x3c0u), off);
             }
+            store8(to, x, wide);
             to += p.ld;
         }
     }
@@ -354,7 +365,7 @@ static int launch_rows(juno_ctx *c, const juno_kvpool *p, int layer, const Cache
         else
             JUNO_CUDA_TRY(launch_pdl(hd == 128 ? q4_append_kernel<128, kAppendRows> : q4_append_kernel<64, kAppendRows>, grid, block, 0, st, a));
     } else if (p->dtype == kKvQ4) {
-        const dim3 grid((unsigned)((n_tokens + kReadRows - 1) / kReadRows), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 4) + 31) / 32 * 32));
+        const dim3 grid((unsigned)((n_tokens + kReadRows - 1) / kReadRows), 2), block((unsigned)std::min(256, (p->n_kv_heads * (hd / 8) + 31) / 32 * 32));
         JUNO_CUDA_TRY(launch_pdl(hd == 128 ? q4_read_kernel<128> : q4_read_kernel<64>, grid, block, 0, st, a));
     } else {
         const unsigned grid = (unsigned)(((int64_t)n_tokens * 2 * p->n_kv_heads * (hd / 8) + 255) / 256);
