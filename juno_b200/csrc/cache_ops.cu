@@ -106,7 +106,7 @@ struct RowsParams {
     int track_tokens;
 };
 
-// Where the positions of a block's rows lie: found once per row, by one thread.
+// Where the positions of a block's rows lie: found once per row, by one thread.  A barrier has to follow.
 struct RowPlace {
     uint8_t *page;  // this layer's page, or null behind the last row
     int pos, track;
@@ -126,7 +126,6 @@ __device__ __forceinline__ void find_places(const RowsParams &p, int row0, size_
         }
         places[threadIdx.x] = at;
     }
-    __syncthreads();
 }
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -148,6 +147,7 @@ template <int HD, int R, bool V>
 __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace (&places)[R], int row0) {
     constexpr int LPV = HD / 8;  // lanes per vector
     const int H = p.n_kv_heads, sub = threadIdx.x % LPV, g = sub >> 2;
+    bool found = false;  // the places, by all threads: each of them has a vector
     for (int vec = threadIdx.x / LPV; vec < (H + 3) / 4 * 4; vec += blockDim.x / LPV) {  // whole warps take part in the sums of a group
         const int h = min(vec, H - 1);
         float rows[R][8];  // of all positions: their loads are under way together
@@ -166,6 +166,8 @@ __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace 
             }
             if (row0 + n + 1 < p.n_tokens) src += p.ld;  // behind the last row: that one again
         }
+        if (!found) __syncthreads();  // the rows are on their way meanwhile
+        found = true;
 #pragma unroll
         for (int n = 0; n < R; n++) {
             const RowPlace at = places[n];
@@ -305,6 +307,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Ro
     __shared__ RowPlace places[kReadRows];
     const int row0 = blockIdx.x * kReadRows;
     find_places<kReadRows>(p, row0, (size_t)p.n_kv_heads * q4_block_bytes(HD), places);
+    __syncthreads();
     if (blockIdx.y == 0)
         read_rows<HD, false>(p, places, row0);
     else
