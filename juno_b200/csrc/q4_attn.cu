@@ -54,9 +54,10 @@ constexpr int kQ4Ctas = HPL == 1 || HD == 64 ? 2 : 3;
 
 // Tiles whose products are added up in an MMA's sums.  An MMA cuts off what lies more than 24 bits below its largest term or sum, always towards zero, so
 // that a long chain of them falls behind by some 2^-25 of the sum a time: 48 requests of 8192 positions were 5.8e-6 of the result off without a limit, where one
-// request of 2048 is 6e-7 off; they are 1.7e-6 off with chains of 32 MMAs, whose sums then go to FP32 ones in shared memory.  That costs 1 % of the time.
-template <int HPL>
-constexpr int kQ4Chain = HPL == 1 ? 16 : 8;
+// request of 2048 is 6e-7 off; they are 1.2e-6 off with chains of 16 to 24 MMAs, whose sums then go to FP32 ones in shared memory (FP32 throughout is 1.0 to 1.8e-6 off).
+// 131072 positions take 41.6 us so and 41.0 with chains twice as long.
+template <int HD, int HPL>
+constexpr int kQ4Chain = HPL == 1 ? 8 : HD == 64 ? 4 : 6;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                 for (int h = 0; h < HPL; h++) offset[h][g] = 0.f;
             }
-            const int first = j, chain_end = min(n_tiles, j + kQ4Chain<HPL>);
+            const int first = j, chain_end = min(n_tiles, j + kQ4Chain<HD, HPL>);
             for (; j < chain_end; j++, pos0 += W * kQ4Tile * kPageTokens) {
                 mbar_wait_bounded(bars + used % kQ4Slots * 8, used / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
                 if (__any_sync(0xffffffffu, failed)) {
@@ -408,8 +409,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                         } else {
                             uint32_t ql[4];  // from shared memory each time: in registers they would push others out (121 us instead of 118, 48 rows of 8192)
                             lds_words<4>(ql, smem_u32(q_s + (HEADS + g8) * Smem::kQueryRow + g * kQ4Group + 8 * t));
-                            mma_f16(c, x0[0], x1[0], x0[1], x1[1], ql[0], ql[1]);
-                            mma_f16(c, x0[2], x1[2], x0[3], x1[3], ql[2], ql[3]);
+                            float low[4];  // sums of their own: the fewer MMAs in a row, the less is cut off
+                            mma_f16_first(low, x0[0], x1[0], x0[1], x1[1], ql[0], ql[1]);
+                            mma_f16(low, x0[2], x1[2], x0[3], x1[3], ql[2], ql[3]);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) c[x] += low[x];
                         }
 #pragma unroll
                         for (int h = 0; h < HPL; h++) {
