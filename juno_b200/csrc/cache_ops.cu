@@ -458,7 +458,8 @@ __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *sums, uns
 }
 
 // One CTA per (sequence, layer, head): which positions stay, in order, and their weights.  The weight that decides (the need-th largest) is found digit by
-// digit, 11, 11 and 10 bits, with a count of every digit in shared memory: three passes over the weights, whatever they are.  Up to kSelectCached weights are
+// digit, 11, 11 and 10 bits, with a count of every digit in shared memory: at most three passes over the weights, whatever they are, two where
+// all weights that share the digits so far stay.  Up to kSelectCached weights are
 // read from memory once.  Six sequences of up to 8192 positions, four layers, eight heads: 20 us, a chain of barriers and passes over shared memory (1024 threads
 // instead of 512 take as long).
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
@@ -474,19 +475,17 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
         return;
     }
     extern __shared__ uint32_t keys[];  // kSelectCached
-    __shared__ unsigned bins[kBins], sums[kSelectWarps], digit_s, left_s;
+    __shared__ unsigned bins[kBins], sums[kSelectWarps], digit_s, left_s, whole_s;
     const int old = r.len - r.recent;  // candidates
     const bool whole = r.len <= kSelectCached;
-    if (whole) {
+    for (int j = tid; j < kBins; j += kSelectThreads) bins[j] = 0;
+    if (whole)
         for (int j = tid; j < r.len; j += kSelectThreads) keys[j] = weight_key(w[j]);
-        __syncthreads();
-    }
+    __syncthreads();
     unsigned need = (unsigned)(r.keep - r.recent), key = 0;
     for (int pass = 0; pass < 3; pass++) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const unsigned mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, digits = pass == 2 ? 1023u : 2047u;
-        for (int j = tid; j < kBins; j += kSelectThreads) bins[j] = 0;
-        __syncthreads();
         if (whole) {
             for (int j = tid; j < old; j += kSelectThreads) {
                 const uint32_t u = keys[j];
@@ -503,7 +502,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
         constexpr int EACH = kBins / kSelectThreads;
         unsigned mine = 0, count[EACH], all;
 #pragma unroll
-        for (int k = 0; k < EACH; k++) mine += count[k] = bins[kBins - 1 - EACH * tid - k];
+        for (int k = 0; k < EACH; k++) {
+            mine += count[k] = bins[kBins - 1 - EACH * tid - k];
+            bins[kBins - 1 - EACH * tid - k] = 0;  // for the next pass
+        }
         unsigned before = block_before(mine, sums, &all);
         if (before < need && need <= before + mine) {
 #pragma unroll
@@ -511,6 +513,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
                 if (before < need && need <= before + count[k]) {
                     digit_s = kBins - 1 - EACH * tid - k;
                     left_s = need - before;
+                    whole_s = left_s == count[k];
                 }
                 before += count[k];
             }
@@ -519,6 +522,11 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
         if (need > 0) {
             key |= digit_s << shift;
             need = left_s;
+            if (whole_s && key > 0) {  // all that begin with these digits stay
+                key--;
+                need = 0;
+                break;
+            }
         } else {
             key = 0xffffffffu;  // no weight has this key
             break;
