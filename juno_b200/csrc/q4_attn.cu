@@ -125,7 +125,7 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
 // eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.  Four heads of 131072 positions take 41 us as the former, 60 as the latter.
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
-// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and 350 of them (four heads of 128, of which 33
+// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and 360 of them (four heads of 128, of which 33
 // MMAs) or 440 (eight) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
 // over 8 of 128: 41 us for 168 MB, 4.1 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 15.7, of which 10 begin and end
 // parts; 48 of up to 8192 with eight heads to a key/value head 117 us for 384 MB.
@@ -689,37 +689,40 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
     }
 }
 
-// The weight that positions have received: a thread has one position of all rows' pages and one key/value head.  Bound by the scores, which come out of L2:
-// 10 us of the 51 that attention and weights of 16 sequences of up to 8192 positions take.
-constexpr int kQ4WeightThreads = 256;
-template <int G>
-__device__ __forceinline__ float weight_of(const float *scores, const float2 *sums, int g_max) {
-    float s[G], sum = 0.f;
-#pragma unroll
-    for (int g = 0; g < G; g++) s[g] = g < g_max ? scores[g] : 0.f;
-#pragma unroll
-    for (int g = 0; g < G; g++)
-        if (g < g_max) sum = fmaf(exp2_fast(s[g] - sums[g].x), sums[g].y, sum);
-    return sum;
-}
+// The weight that positions have received: a thread has four neighbouring positions of all rows' pages and one key/value head, 64 bytes of scores with four heads, which
+// come out of L2.  Attention and weights of 16 sequences of up to 8192 positions: 50.1 us, 51.8 with one position a thread.
+constexpr int kQ4WeightThreads = 128;
 __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __grid_constant__ Q4AttnParams p) {
     pdl_wait();
-    const int kvh = blockIdx.y, at = blockIdx.x * kQ4WeightThreads + threadIdx.x, G = p.n_heads / p.n_kv_heads;
+    const int kvh = blockIdx.y, at = (blockIdx.x * kQ4WeightThreads + threadIdx.x) * 4, G = p.n_heads / p.n_kv_heads;
     if (at >= p.total * kPageTokens) return;
     const int i = cache_find(p.rows, at >> 4);
     const CacheRow r = cache_row(p.rows, i);
-    const int pos = at - r.first * kPageTokens;
-    if (r.track < 0 || pos >= r.upto) return;
+    const int pos = at - r.first * kPageTokens, n = min(4, r.upto - pos);
+    if (r.track < 0 || n <= 0) return;
     const float *scores = p.scores + ((size_t)kvh * p.total * kPageTokens + at) * G;
     const float2 *sums = p.sums + (size_t)i * p.n_heads + kvh * G;
-    float *w = p.weights + (((size_t)r.track * p.n_layers + p.layer) * p.n_kv_heads + kvh) * p.track_tokens + pos;
-    const float old = *w;
-    if (G == 4) {
-        const float4 s = *reinterpret_cast<const float4 *>(scores);  // 16-byte multiples: four heads a position
-        *w = old + fmaf(exp2_fast(s.w - sums[3].x), sums[3].y, fmaf(exp2_fast(s.z - sums[2].x), sums[2].y, fmaf(exp2_fast(s.y - sums[1].x), sums[1].y, exp2_fast(s.x - sums[0].x) * sums[0].y)));
+    float4 *w = reinterpret_cast<float4 *>(p.weights + (((size_t)r.track * p.n_layers + p.layer) * p.n_kv_heads + kvh) * p.track_tokens + pos);
+    const float4 old = *w;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (G == 4) {  // the scores of a position in one load
+        float4 s[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) s[x] = x < n ? reinterpret_cast<const float4 *>(scores)[x] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float2 m0 = sums[0], m1 = sums[1], m2 = sums[2], m3 = sums[3];
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+            sum[x] = fmaf(exp2_fast(s[x].w - m3.x), m3.y, fmaf(exp2_fast(s[x].z - m2.x), m2.y, fmaf(exp2_fast(s[x].y - m1.x), m1.y, exp2_fast(s[x].x - m0.x) * m0.y)));
     } else {
-        *w = old + weight_of<kQ4MaxGroup>(scores, sums, G);
+        for (int g = 0; g < G; g++) {
+            const float2 m = sums[g];
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                if (x < n) sum[x] = fmaf(exp2_fast(scores[x * G + g] - m.x), m.y, sum[x]);
+        }
     }
+    // positions behind the row's end keep what they have
+    *w = make_float4(old.x + sum[0], n > 1 ? old.y + sum[1] : old.y, n > 2 ? old.z + sum[2] : old.z, n > 3 ? old.w + sum[3] : old.w);
 }
 
 template <int HD, int HPL, bool TRACK>
@@ -854,7 +857,7 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
         JUNO_TRY((track ? launch_q4_attn<64, true>(a, G, shares, st) : launch_q4_attn<64, false>(a, G, shares, st)));
     c->kernel_launches++;
     if (!track) return JUNO_OK;
-    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages * kPageTokens + kQ4WeightThreads - 1) / kQ4WeightThreads), (unsigned)H), dim3(kQ4WeightThreads), 0, st, a));
+    JUNO_CUDA_TRY(launch_pdl(q4_weights_kernel, dim3((unsigned)((pages * (kPageTokens / 4) + kQ4WeightThreads - 1) / kQ4WeightThreads), (unsigned)H), dim3(kQ4WeightThreads), 0, st, a));
     c->kernel_launches++;
     return JUNO_OK;
 }
