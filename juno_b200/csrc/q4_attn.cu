@@ -125,8 +125,8 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
 // eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.  Four heads of 131072 positions take 41 us as the former, 60 as the latter.
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
-// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and 360 of them (four heads of 128, of which 33
-// MMAs) or 440 (eight) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
+// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and it takes 360 of them (four heads of 128, of
+// which 17 MMAs) or 440 (eight, 34) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
 // over 8 of 128: 41 us for 168 MB, 4.1 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 15.7, of which 10 begin and end
 // parts; 48 of up to 8192 with eight heads to a key/value head 117 us for 384 MB.
 template <int HD, int HPL>
