@@ -140,8 +140,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // A CTA has R positions, of keys (blockIdx.y = 0) or values.  A lane has eight neighbouring dimensions, four lanes a group: what is stored of a position is
-// contiguous.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found with the estimate
-// of q4_number (a saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided
+// contiguous.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found from an estimate
+// (q4_number_near: a saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided
 // exactly.  131072 positions of eight heads of 128: 1.24 GB in 250 us, 5.0 TB/s; 8156 of them 77 MB in 24 us.
 template <int HD, int R, bool V>
 __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace (&places)[R], int row0) {
@@ -210,13 +210,13 @@ __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace 
             float worst = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float part = __saturatef((x[e] - m) * inv), near = fmaf(part, 15.f, 12582912.f);
-                bits[e] = __float_as_uint(near) - 0x4b400000u;
-                worst = fmaxf(worst, fabsf(fmaf(part, 15.f, 12582912.f - near)));
+                float off;
+                bits[e] = q4_number_near(x[e], m, inv, &off);
+                worst = fmaxf(worst, off);
             }
             auto word = [](const uint32_t (&q)[8]) { return q4_unit(q[0], q[1], q[2], q[3]) | q4_unit(q[4], q[5], q[6], q[7]) << 16; };
             uint32_t w = word(bits);
-            if (worst > 0.49998474f) {  // as in q4_number
+            if (worst > kQ4Near) {
                 uint32_t q[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) q[e] = (uint32_t)q4_number_exact(x[e], m, d, inv * 15.f);

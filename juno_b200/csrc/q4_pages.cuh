@@ -20,6 +20,7 @@
 // Every piece lies as the MMAs of decode attention want it: lane (g, t) of a warp finds the numbers of all groups of position g of the keys at 16 * lane
 // (8 * lane for heads of 64), those of the values come by ldmatrix, and the keys' offsets are operands of an MMA as they are.
 #pragma once
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -57,17 +58,22 @@ JHD int q4_number_exact(float x, float m, float d, float inv) {
     else if (s < below || (s == below && (r < 0.f || (r == 0.f && (q & 1))))) q--;
     return q < 0 ? 0 : q > 15 ? 15 : q;
 }
-// The same where the estimate t = (x - m) inv is enough: t is off by less than 2^-18 (x - m, inv and the product are rounded once each, t <= 15.1), so a t
-// farther than 2^-16 from half-way between two numbers has the right one next to it.  inv is 0 for d = 0.
-JHD int q4_number(float x, float m, float d, float inv) {
-    float t = (x - m) * inv;
-    t = t < 0.f ? 0.f : t > 15.f ? 15.f : t;
-    const float near = t + 12582912.f, off = t - (near - 12582912.f);  // 1.5 * 2^23: the sum's last digit is 1
-    if (off > 0.49998474f || off < -0.49998474f) return q4_number_exact(x, m, d, inv);
+// The same from an estimate (inv is about 1 / (15 d), 0 for d = 0), and how far that lies from its whole number.  t = (x - m) inv 15 is off by less than 2^-17
+// (x - m and the product are rounded once, inv is off by two of its last digits, t <= 15.1), so a t farther than 2^-16 from half-way between two numbers has the
+// right one next to it; where *off is above kQ4Near q4_number_exact decides.
+JHD uint32_t q4_number_near(float x, float m, float inv, float *off) {
+#if defined(__CUDA_ARCH__)
+    const float part = __saturatef((x - m) * inv);
+#else
+    const float t = (x - m) * inv, part = t > 1.f ? 1.f : t > 0.f ? t : 0.f;
+#endif
+    const float near = fmaf(part, 15.f, 12582912.f);  // 1.5 * 2^23: the sum's last digit is 1
+    *off = fabsf(fmaf(part, 15.f, 12582912.f - near));
     uint32_t bits;
     memcpy(&bits, &near, 4);
-    return (int)(bits & 15u);
+    return bits - 0x4b400000u;
 }
+constexpr float kQ4Near = 0.49998474f;
 constexpr float kQ4Most = 65504.f, kQ4Nothing = 8.271806125530277e-25f;  // 2^-80
 
 }  // namespace juno

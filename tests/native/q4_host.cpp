@@ -3,7 +3,11 @@
 
 using namespace juno;
 
-extern "C" int q4_host_number(float x, float m, float d) { return q4_number(x, m, d, d > 0.f ? 1.f / d : 0.f); }
+extern "C" int q4_host_number(float x, float m, float d) {
+    float off;
+    const int q = (int)q4_number_near(x, m, d > 0.f ? 1.f / (15.f * d) : 0.f, &off);
+    return off > kQ4Near ? q4_number_exact(x, m, d, d > 0.f ? 1.f / d : 0.f) : q;
+}
 extern "C" int q4_host_number_exact(float x, float m, float d) { return q4_number_exact(x, m, d, d > 0.f ? 1.f / d : 0.f); }
 extern "C" int q4_host_block_bytes(int hd) { return q4_block_bytes(hd); }
 
