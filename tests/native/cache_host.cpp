@@ -1,0 +1,84 @@
+// Test-only host program: calls on pools and sequences that are put together by hand, without a GPU.  `cache_host NAME` runs one check and exits 0 if it holds.
+#include <cstdio>
+#include <cstring>
+
+#include "../../include/juno_b200.h"
+#include "../../juno_b200/csrc/attn.cuh"
+
+using namespace juno;
+
+#define WANT(x)                                                        \
+    do {                                                               \
+        if (!(x)) {                                                    \
+            printf("line %d: %s (%s)\n", __LINE__, #x, juno_last_error()); \
+            return 1;                                                  \
+        }                                                              \
+    } while (0)
+
+// A pool of 64 pages and 8 slots whose device memory does not exist.
+struct Pool {
+    juno_ctx ctx;
+    juno_kvpool pool;
+    int32_t table[8 * 64];
+    explicit Pool(int dtype) {
+        ctx.magic = kMagicCtx;
+        ctx.device = 0;
+        ctx.sm_count = 148;
+        ctx.stream = nullptr;
+        pool.magic = kMagicPool;
+        pool.ctx = &ctx;
+        pool.n_layers = 2;
+        pool.n_kv_heads = 2;
+        pool.head_dim = 64;
+        pool.n_pages = 64;
+        pool.dtype = dtype;
+        pool.page_tokens = 16;
+        pool.elem_bytes = dtype == 0 ? 2 : dtype == 1 ? 4 : 0;
+        pool.max_slots = 8;
+        pool.max_pages_per_seq = 64;
+        pool.k = pool.v = nullptr;
+        pool.d_table = nullptr;
+        pool.h_table = table;
+        pool.owned_by_model = 0;
+        memset(table, 0, sizeof table);
+        for (int i = 63; i >= 0; i--) pool.free_pages.push_back(i);
+        pool.page_refs.assign(64, 0);
+        for (int i = 7; i >= 0; i--) pool.free_slots.push_back(i);
+    }
+    // a sequence of `len` positions, with their pages; track: its weight plane
+    juno_seq *seq(int len, int track = -1) {
+        juno_seq *s = nullptr;
+        if (juno_kvseq_create(&pool, 512, &s) != JUNO_OK) return nullptr;
+        for (int i = 0; i < (len + 15) / 16; i++) {
+            const int pg = pool.free_pages.back();
+            pool.free_pages.pop_back();
+            pool.page_refs[pg] = 1;
+            s->pages.push_back(pg);
+            table[s->slot * 64 + i] = pg;
+        }
+        s->len = len;
+        s->track = track;
+        return s;
+    }
+};
+
+// Rows of one sequence would add to the same weights: refused, as for device memory.
+static int twice() {
+    Pool p(3);
+    juno_seq *a = p.seq(20, 0), *b = p.seq(20), *two[2] = {a, a}, *mixed[3] = {b, a, a};
+    float x[3 * 256] = {0};
+    WANT(juno_attn_decode(&p.ctx, &p.pool, 0, 2, two, 4, x, x) == JUNO_ERR_INVALID_ARG && strstr(juno_last_error(), "there twice"));
+    WANT(juno_attn_decode(&p.ctx, &p.pool, 0, 3, mixed, 4, x, x) == JUNO_ERR_INVALID_ARG && strstr(juno_last_error(), "there twice"));
+    return 0;
+}
+
+int main(int argc, char **argv) {
+    const struct {
+        const char *name;
+        int (*run)();
+    } checks[] = {{"twice", twice}};
+    for (const auto &c : checks)
+        if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
+    printf("no such check\n");
+    return 2;
+}

@@ -1,0 +1,29 @@
+"""Calls on cache pages that need no GPU: refusals and book-keeping on the host, by a program that links the library (native/cache_host.cpp)."""
+import os
+import subprocess
+
+import pytest
+
+from juno_b200 import _lib, build
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+SRC, EXE = os.path.join(HERE, "native", "cache_host.cpp"), os.path.join(HERE, "native", "build", "cache_host")
+
+
+@pytest.fixture(scope="module")
+def host():
+    lib = build.build()
+    os.makedirs(os.path.dirname(EXE), exist_ok=True)
+    headers = [os.path.join(build.CSRC, f) for f in os.listdir(build.CSRC) if f.endswith(".cuh")]
+    if not os.path.exists(EXE) or os.path.getmtime(EXE) < max(os.path.getmtime(f) for f in (SRC, *headers)):
+        subprocess.check_call(["g++", "-O1", "-std=c++17", "-I/usr/local/cuda/include", "-o", EXE, SRC, lib, f"-Wl,-rpath,{os.path.dirname(lib)}"])
+    assert lib == _lib.LIB_PATH
+
+    def run(name):
+        r = subprocess.run([EXE, name], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+    return run
+
+
+def test_rows_of_one_sequence_do_not_share_weights(host):
+    host("twice")
