@@ -143,8 +143,8 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out);
 int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens, const float *k_host,
                        const float *v_host);
 /* out[i][n_heads*head_dim] = gqa(q[i], K_i, V_i, len_i) for n sequences at one layer
- * (len_i = current length of seqs[i]); host in, host out.  A sequence may be there several times unless one of
- * them keeps weights (juno_seq_track). */
+ * (len_i = current length of seqs[i]); host in, host out.  A sequence may be there several times unless it keeps
+ * weights (juno_seq_track). */
 int juno_attn_decode(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs,
                      int32_t n_heads, const float *q_host, float *out_host);
 

@@ -1433,7 +1433,6 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
     std::lock_guard<std::recursive_mutex> lk(c->mu);
     DeviceGuard g(c->device);
     int max_len = 0;
-    bool track = false;
     std::vector<int32_t> meta(2 * (size_t)n);
     for (int i = 0; i < n; i++) {
         JUNO_TRY(seq_check(seqs[i]));
@@ -1442,10 +1441,8 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
         meta[i] = seqs[i]->slot;
         meta[n + i] = seqs[i]->len;
         max_len = std::max(max_len, seqs[i]->len);
-        track |= seqs[i]->track >= 0;
     }
-    // two rows of one sequence would add to the same weights side by side
-    if (track) JUNO_TRY(guarded([&] { return cache_call_distinct(p, n, seqs); }));
+    JUNO_TRY(guarded([&] { return cache_call_distinct(p, n, seqs, true); }));  // two rows of one sequence would add to the same weights side by side
     const int hd = p->head_dim, qdim = n_heads * hd;
     const size_t qbytes = (size_t)n * qdim * sizeof(float);
     if (p->dtype == kKvQ4) {

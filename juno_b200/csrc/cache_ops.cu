@@ -699,9 +699,10 @@ int cache_call_check(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *co
     return JUNO_OK;
 }
 
-int cache_call_distinct(const juno_kvpool *p, int n, juno_seq *const *seqs) {
+int cache_call_distinct(const juno_kvpool *p, int n, juno_seq *const *seqs, bool weights_only) {
     std::vector<char> seen((size_t)p->max_slots, 0);
     for (int i = 0; i < n; i++) {
+        if (weights_only && seqs[i]->track < 0) continue;
         JUNO_REQUIRE(!seen[(size_t)seqs[i]->slot], "sequence %d is there twice", i);
         seen[(size_t)seqs[i]->slot] = 1;
     }

@@ -56,7 +56,8 @@ private:
 
 // What every such call requires of its handles; a call that writes to a sequence has each one once.
 int cache_call_check(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *seqs);
-int cache_call_distinct(const juno_kvpool *p, int n, juno_seq *const *seqs);
+// weights_only: sequences that keep no weights may be there several times
+int cache_call_distinct(const juno_kvpool *p, int n, juno_seq *const *seqs, bool weights_only = false);
 // JUNO_ERR_INVALID_ARG unless p is memory that this context's device can use (device or managed memory of its own).
 int device_memory(const juno_ctx *c, const void *p, const char *name);
 // The context's working memory, at least `bytes`; what an earlier call left there is gone.

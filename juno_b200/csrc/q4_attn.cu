@@ -879,13 +879,10 @@ extern "C" int juno_attn_decode_device(juno_ctx *c, juno_kvpool *p, int32_t laye
         JUNO_REQUIRE(n_heads > 0 && n_heads % p->n_kv_heads == 0, "n_heads %d is not a multiple of n_kv_heads %d", n_heads, p->n_kv_heads);
         JUNO_REQUIRE(ldq >= (int64_t)n_heads * p->head_dim && ldo >= (int64_t)n_heads * p->head_dim, "rows of %lld and %lld elements hold no %d heads of %d",
                      (long long)ldq, (long long)ldo, n_heads, p->head_dim);
-        bool track = false;
-        for (int i = 0; i < n; i++) {
+        for (int i = 0; i < n; i++)
             JUNO_REQUIRE(!lens || (lens[i] >= 0 && lens[i] <= seqs[i]->len), "sequence %d has %d cached positions, not %d", i, seqs[i]->len, lens ? lens[i] : 0);
-            track |= seqs[i]->track >= 0;
-        }
         DeviceGuard g(c->device);
-        if (track) JUNO_TRY(cache_call_distinct(p, n, seqs));
+        JUNO_TRY(cache_call_distinct(p, n, seqs, true));
         JUNO_TRY(device_memory(c, q_dev, "q"));
         JUNO_TRY(device_memory(c, out_dev, "out"));
         CacheStream s(c, stream);

@@ -72,11 +72,21 @@ static int twice() {
     return 0;
 }
 
+// A sequence without weights may be there several times beside one that has some: what stops such a call here comes after its checks.
+static int beside() {
+    Pool p(3);
+    juno_seq *a = p.seq(20, 0), *b = p.seq(20), *mixed[3] = {b, a, b};
+    float x[3 * 256] = {0};
+    const int rc = juno_attn_decode(&p.ctx, &p.pool, 0, 3, mixed, 4, x, x);
+    WANT(rc != JUNO_OK && !strstr(juno_last_error(), "there twice"));
+    return 0;
+}
+
 int main(int argc, char **argv) {
     const struct {
         const char *name;
         int (*run)();
-    } checks[] = {{"twice", twice}};
+    } checks[] = {{"twice", twice}, {"beside", beside}};
     for (const auto &c : checks)
         if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
     printf("no such check\n");

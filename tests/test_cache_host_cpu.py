@@ -27,3 +27,7 @@ def host():
 
 def test_rows_of_one_sequence_do_not_share_weights(host):
     host("twice")
+
+
+def test_sequences_without_weights_may_be_named_beside_one_with_weights(host):
+    host("beside")
