@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 y[e] = query[n][e] * scale;
-                sum += y[e];
+                sum += y[e] * 0.03125f;  // 32 elements: five powers of two less, no sum overflows
                 top = fmaxf(top, fabsf(y[e]));
             }
 #pragma unroll
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                 if (x < kQ4Group / E) sum += __shfl_xor_sync(0xffffffffu, sum, x);
             }
-            const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127)), up = 13 - e2;
+            const int e2 = max(-100, min(127, (int)(__float_as_uint(top) >> 23) - 127)), up = 13 - e2;
             const float shift = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
             for (int e = 0; e < E; e++) {
@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 to_q[0] = hi;
                 to_q[HEADS * Smem::kQueryRow] = __float2half_rn(whole - __half2float(hi));
             }
-            if (lane % (kQ4Group / E) == 0) {  // 32 elements of up to 2^14: five powers of two less
-                const float whole = sum * (shift * 0.03125f);
+            if (lane % (kQ4Group / E) == 0) {
+                const float whole = sum * shift;
                 const __half hi = __float2half_rn(whole);
                 sums_s[head * 4 + lane / (kQ4Group / E)] = hi;
                 sums_s[(HEADS + head) * 4 + lane / (kQ4Group / E)] = __float2half_rn(whole - __half2float(hi));

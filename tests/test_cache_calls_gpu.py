@@ -5,7 +5,7 @@ import pytest
 from juno_b200.matvec import PagedKvCache
 from oracle import q4_cache_oracle as q4
 from q4util import rows
-from test_q4_cache_gpu import check_attention, check_weights, f32, fill, weights
+from test_q4_cache_gpu import attend, check_attention, check_weights, f32, fill, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -26,4 +26,33 @@ def test_host_attention_names_a_sequence_with_weights_once(ctx):
         w = check_attention(out[i], q[i], q4.held(k), q4.held(v))
         if i == 1:
             check_weights(weights(cache, 0, [a], [40])[0], w, q[i], k)
+    cache.close()
+
+
+# Queries so large that the softmax leaves one position: the result is that position's row.  What the kernel rounds of it: the two limbs of weight times step, 2^-22,
+# and in FP32 the offset's product, the sum of both parts, the warps' merge and the division, four times 2^-24, of terms of up to 3 times the largest value
+# (m and 15 d are up to twice it apart): 3 (2^-22 + 4 2^-24) < 2^-19.  No score comes near the largest: the gap is 1e-3 of it, the scores are off by some 1e-6 of it.
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (8, 2, 128), (16, 2, 128)])
+def test_queries_of_any_size(ctx, heads, kv, dim):
+    rng = np.random.default_rng(52)
+    n = 70
+    cache = PagedKvCache(ctx, 1, kv, dim, 8, "q4")
+    s = cache.new_sequence(n)
+    k, v = f32(rng.standard_normal((n, kv, dim))), f32(rng.standard_normal((n, kv, dim)))
+    fill(cache, 0, [s], [0], [(k, v)])
+    hk, hv = q4.held(k), q4.held(v)
+    q = rng.standard_normal((1, heads, dim))
+    scores = np.einsum("hgd,lhd->hgl", q[0].reshape(kv, -1, dim), hk).reshape(heads, n)
+    first, second = np.sort(scores, -1)[:, -1], np.sort(scores, -1)[:, -2]
+    assert (first - second > 1e-3 * np.abs(scores).max(-1)).all()
+    best = scores.argmax(-1)
+    want = hv[best, np.arange(heads) // (heads // kv)]
+    for size in (1e8, 1e20, 1e30, 1e32, 1e34, 1e36):
+        x = f32(size * q)
+        assert np.isfinite(x).all()
+        got = attend(cache, 0, [s], x)[0]
+        assert np.abs(got - want).max() <= 2.0 ** -19 * np.abs(hv).max(), size
+    for size in (1e-20, 1e-36, 1e-44, 0.0):
+        x = f32(size * q)
+        check_attention(attend(cache, 0, [s], x)[0], x[0], hk, hv)
     cache.close()
