@@ -110,6 +110,13 @@ __device__ __forceinline__ void numbers_of(uint32_t units, uint32_t (&x)[4]) {
     x[2] = KEYS ? units & kTop >> 4 : units << 4 & kTop;
     x[3] = __byte_perm(units, 0, 0x2301) & kTop;
 }
+// A group's scale and the largest step in its range, both as BF16: scale times step is below 1.
+constexpr uint32_t kStepLimits = 0x7eff7effu;
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 // FP32 in two halves' worth: what a half holds of x, towards zero, and the rest.
 __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
@@ -119,7 +126,9 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 //             (q4_unit), after an AND.  A group's result is multiplied by its step d in FP32, and the offsets' part, m times the sum of the query over the group,
 //             comes from one more MMA, whose operand m is as it lies in the page.
 //   O += V P  rows are dimensions, k the positions, columns heads; a weight is multiplied by the step of its position and group first, and the offsets' part
-//             is a sum of its own per lane, in FP32.  The product is scaled by a power of two that follows the largest step, so that it keeps its digits in FP16.
+//             is a sum of its own per lane, in FP32.  The product is scaled by a power of two that follows the largest step of its group, so that it keeps its digits in
+//             FP16 (one scale for all groups: where one group's values were 10^6 times another's, the smaller ones were 5e-3 of their size off; its own for each
+//             takes 43.7 us instead of 42.2 for 131072 positions).  What is left: a position whose step in a group is R times the others' costs them R 2^-30.
 //             The numbers of half the positions count from the other end (q4_v_flip), those positions' products have a minus: the sums stay as small as
 //             the result, where sums of numbers that are all positive would be larger than it by the root of the number of positions that count.
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
@@ -348,8 +357,10 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
             qsum[h] = t < NW ? *reinterpret_cast<const uint32_t *>(sums_s + column * 4 + 2 * t) : 0u;
             back[h] = back_s[HPL * t + h];
         }
-        float m_run[HPL], l_run[HPL], vscale = 0.f;
-        uint32_t limit = 0;  // largest step in the scale's range, in both halves
+        float m_run[HPL], l_run[HPL];
+        uint32_t vscale[NW];  // of each group, as the steps lie: the power of two that its values are scaled by; at first one that no step but 0 stays below
+#pragma unroll
+        for (int g = 0; g < NW; g++) vscale[g] = 0x71807180u;  // 2^100; steps are 2^-84 or more
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
             m_run[h] = -INFINITY;
@@ -437,7 +448,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             for (int x = 0; x < 2; x++)
                                 if (HPL * t + h < G && pos0 + 16 * u + 8 * x + g8 < pos_end) to_s[(16 * u + 8 * x) * G + HPL * t + h] = s[h][u][x];
                 }
-                uint32_t d[kQ4Tile][2][NW], vm[kQ4Tile][2][NW], steps = limit;
+                uint32_t d[kQ4Tile][2][NW], vm[kQ4Tile][2][NW], steps[NW];
 #pragma unroll
                 for (int u = 0; u < kQ4Tile; u++)
 #pragma unroll
@@ -460,13 +471,17 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             }
                         }
                 }
-#pragma unroll
-                for (int u = 0; u < kQ4Tile; u++)
-#pragma unroll
-                    for (int g = 0; g < NW; g++) steps = __vmaxu2(steps, __vmaxu2(d[u][0][g], d[u][1][g]));
-                // a score far above the reference, or a step beyond the scale's range: seldom after the first tile
+                // a score far above the reference, or a step beyond its group's scale: seldom after the first tile
                 float top[HPL];
-                bool grown = steps != limit;
+                bool grown = false;
+#pragma unroll
+                for (int g = 0; g < NW; g++) {
+                    const uint32_t limit = kStepLimits - vscale[g];
+                    steps[g] = limit;
+#pragma unroll
+                    for (int u = 0; u < kQ4Tile; u++) steps[g] = __vmaxu2(steps[g], __vmaxu2(d[u][0][g], d[u][1][g]));
+                    grown |= steps[g] != limit;
+                }
 #pragma unroll
                 for (int h = 0; h < HPL; h++) {
                     top[h] = s[h][0][0];
@@ -475,14 +490,18 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                     grown |= top[h] > m_run[h] + 15.f;
                 }
                 if (__any_sync(0xffffffffu, grown)) {
-                    float fix[HPL], vfix = 1.f;
-                    steps = __reduce_max_sync(0xffffffffu, max(steps & 0xffffu, steps >> 16));
-                    if (steps > (limit & 0xffffu)) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
-                        const int e = max((int)(steps >> 7) - 127, -100);
-                        const float next = __uint_as_float((uint32_t)(127 - 5 - e) << 23);
-                        vfix = vscale == 0.f ? 0.f : next / vscale;
-                        vscale = next;
-                        limit = ((uint32_t)(e + 4 + 127) << 7 | 0x7fu) * 0x10001u;
+                    float fix[HPL], vfix[NG];
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        const int half = 16 * (g & 1);
+                        const uint32_t step = __reduce_max_sync(0xffffffffu, steps[g >> 1] >> half & 0xffffu);
+                        vfix[g] = 1.f;
+                        const uint32_t before = vscale[g >> 1] >> half & 0xffffu;
+                        if (step > (kStepLimits & 0xffffu) - before) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
+                            const uint32_t next = (249u - (step >> 7)) << 7;  // 2^-5 over the step's power of two
+                            vscale[g >> 1] += (next - before) << half;
+                            vfix[g] = __uint_as_float((0x3f80u + next - before) << 16);
+                        }
                     }
 #pragma unroll
                     for (int h = 0; h < HPL; h++) {
@@ -512,7 +531,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                     for (int g = 0; g < NG; g++)
 #pragma unroll
                         for (int x = 0; x < 4; x++) {
-                            const float y = fix[HPL == 1 ? 0 : x & 1] * vfix;
+                            const float y = fix[HPL == 1 ? 0 : x & 1] * vfix[g];
                             o[g][0][x] *= y;
                             o[g][1][x] *= y;
                         }
@@ -522,14 +541,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                     uint32_t v0[NG], v1[NG];  // unit g8 of positions 2t, 2t + 1, and of those eight farther
 #pragma unroll
                     for (int g = 0; g < NG; g += 2) ldmatrix_x4_trans(v0[g], v1[g], v0[g + 1], v1[g + 1], tile + u * BLOCK + (g == 0 ? v_piece : v_piece ^ 32u));
-                    float w[HPL][2], ws[HPL][2];
+                    float w[HPL][2];
 #pragma unroll
                     for (int h = 0; h < HPL; h++) {
 #pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
-                            ws[h][x] = w[h][x] * (x ? -vscale : vscale);  // positions 8..15: 15 - q
-                        }
+                        for (int x = 0; x < 2; x++) w[h][x] = exp2_fast(s[h][u][x] - m_run[h]);
                         l_run[h] += w[h][0] + w[h][1];
                     }
                     // the offsets' part, in FP32: an MMA cuts off what its sum of 22-bit products has below 24 bits, always towards zero, and this part and the
@@ -547,6 +563,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                             }
                         }
                     }
+                    // from here on the steps times their group's scale: exact, a power of two
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int g = 0; g < NW; g++) d[u][x][g] = mul_bf16x2(d[u][x][g], vscale[g]);
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
                         float hi[HPL][2], lo[HPL][2];
@@ -554,7 +575,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                         for (int h = 0; h < HPL; h++)
 #pragma unroll
                             for (int x = 0; x < 2; x++) {
-                                const float y = ws[h][x] * step_of(d[u][x], g);
+                                const float y = (x ? -w[h][x] : w[h][x]) * step_of(d[u][x], g);  // positions 8..15: 15 - q
                                 hi[h][x] = upper_limb(y);
                                 lo[h][x] = y - hi[h][x];
                             }
@@ -580,11 +601,11 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 if (part_issued < part_tiles) issue();
             }
             // a chain's sums, over the lanes that share a head for the offsets' part, to where the warps meet
-            const float unscale = vscale == 0.f ? 0.f : 262144.f / vscale;  // 2^18
 #pragma unroll
             for (int h = 0; h < HPL; h++)
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
+                    const float unscale = __uint_as_float((272u << 23) - __float_as_uint(step_of(vscale, g)));  // 2^18 over the scale
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) offset[h][g] += __shfl_xor_sync(0xffffffffu, offset[h][g], x);
                     float v[4];

@@ -56,3 +56,23 @@ def test_queries_of_any_size(ctx, heads, kv, dim):
         x = f32(size * q)
         check_attention(attend(cache, 0, [s], x)[0], x[0], hk, hv)
     cache.close()
+
+
+# Groups of a value whose sizes lie far apart keep their own digits.  What the kernel rounds relative to a group: the weights, which are off by some 2e-6 as in
+# test_long_sums_are_not_biased, and weight times step in two limbs, 2^-22, both at random over the positions: about 2e-6 of the result's length in the group, and 1e-5 leaves
+# a factor of five.
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9])
+@pytest.mark.parametrize("n,heads,kv,dim", [(300, 8, 2, 64), (300, 8, 2, 128), (5000, 16, 2, 128), (5000, 5, 1, 64)])
+def test_groups_of_values_far_apart(ctx, n, heads, kv, dim, ratio):
+    rng = np.random.default_rng(53)
+    cache = PagedKvCache(ctx, 1, kv, dim, n // 16 + 1, "q4")
+    s = cache.new_sequence(n)
+    size = np.repeat(ratio ** np.linspace(0.5, -0.5, dim // 32), 32)
+    for order in (size, size[::-1]):
+        k, v = rows(rng, n, kv, dim), f32(rng.standard_normal((n, kv, dim)) * order)
+        fill(cache, 0, [s], [0], [(k, v)])
+        q = f32(rng.standard_normal((1, heads, dim)))
+        got, (want, _) = attend(cache, 0, [s], q)[0], q4.attention(q[0], q4.held(k), q4.held(v))
+        of_groups = lambda x: np.linalg.norm(x.reshape(heads, -1, 32), axis=-1)  # noqa: E731
+        assert (of_groups(got - want) <= 1e-5 * of_groups(want)).all(), of_groups(got - want) / of_groups(want)
+    cache.close()
