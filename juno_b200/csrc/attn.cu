@@ -1025,7 +1025,7 @@ int kvpool_destroy(juno_kvpool *p) {
         return JUNO_ERR_CLOSED;
     }
     DeviceGuard g(p->ctx->device);
-    cudaStreamSynchronize(p->ctx->stream);
+    if (ctx_ok(p->ctx)) cudaStreamSynchronize(p->ctx->stream);  // closing a context waits for its work and ends its stream
     cudaFree(p->k);
     cudaFree(p->v);
     if (p->state) cudaFree(p->state);
@@ -1260,6 +1260,7 @@ int juno_kvseq_create(juno_kvpool *p, int32_t max_tokens, juno_seq **out) {
         return JUNO_ERR_CLOSED;
     }
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
+    JUNO_TRY(ctx_check(p->ctx));
     return seq_create(p, max_tokens, out);
 }
 
@@ -1286,6 +1287,7 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
     JUNO_REQUIRE(out, "out is null");
     juno_kvpool *p = src->pool;
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
+    JUNO_TRY(ctx_check(p->ctx));
     JUNO_REQUIRE(n_tokens >= 0 && n_tokens <= src->len, "cannot share %d positions of a sequence that holds %d", n_tokens, src->len);
     DeviceGuard g(p->ctx->device);
     JUNO_TRY(seq_resume_check(p, src->len, n_tokens));
@@ -1338,6 +1340,7 @@ int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens) {
     JUNO_REQUIRE(max_tokens >= 1 && max_tokens <= p->max_pages_per_seq * kPageTokens, "max_tokens %d outside [1,%d]", max_tokens,
                  p->max_pages_per_seq * kPageTokens);
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
+    JUNO_TRY(ctx_check(p->ctx));
     JUNO_REQUIRE(!p->weights, "this pool keeps weights already");
     DeviceGuard g(p->ctx->device);
     JUNO_TRY(guarded([&]() -> int {
@@ -1361,6 +1364,7 @@ int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens) {
 int juno_seq_track(juno_seq *s) {
     JUNO_TRY(seq_check(s));
     std::lock_guard<std::recursive_mutex> lk(s->pool->ctx->mu);
+    JUNO_TRY(ctx_check(s->pool->ctx));
     JUNO_REQUIRE(s->pool->weights, "the pool keeps no weights (juno_kvpool_track)");
     JUNO_REQUIRE(s->track < 0, "this sequence keeps its weights already");
     DeviceGuard g(s->pool->ctx->device);
@@ -1385,6 +1389,7 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     JUNO_REQUIRE(pos >= 0 && n_tokens >= 0, "bad position range");
     if (n_tokens == 0) return JUNO_OK;
     std::lock_guard<std::recursive_mutex> lk(c->mu);
+    JUNO_TRY(ctx_check(c));
     JUNO_REQUIRE(p->dtype != kKvQ4 || pos <= s->len, "position %d is not behind the %d cached ones", pos, s->len);
     DeviceGuard g(c->device);
     JUNO_TRY(seq_reserve(s, pos, pos + n_tokens, c->stream));

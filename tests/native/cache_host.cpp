@@ -82,11 +82,32 @@ static int beside() {
     return 0;
 }
 
+// What reaches a pool's memory through a sequence is refused once the pool, or its context, is closed; a handle of an open pool can be freed then.
+static int closed() {
+    for (int which = 0; which < 2; which++) {
+        Pool p(3);
+        juno_seq *a = p.seq(20), *b = nullptr;
+        float x[2 * 128] = {0}, w = 0;
+        (which ? p.ctx.magic : p.pool.magic) = kMagicDead;
+        WANT(juno_seq_append_kv(a, 0, 3, 1, x, x) == JUNO_ERR_CLOSED);
+        WANT(juno_seq_append_kv(a, 0, 20, 2, x, x) == JUNO_ERR_CLOSED);
+        WANT(juno_seq_fork(a, 0, &b) == JUNO_ERR_CLOSED && !b);
+        WANT(juno_seq_fork(a, 20, &b) == JUNO_ERR_CLOSED && !b);
+        WANT(juno_kvpool_track(&p.pool, 1, 16) == JUNO_ERR_CLOSED);
+        WANT(juno_kvseq_create(&p.pool, 16, &b) == JUNO_ERR_CLOSED && !b);
+        p.pool.weights = &w;
+        WANT(juno_seq_track(a) == JUNO_ERR_CLOSED);
+        WANT(a->len == 20 && a->pages.size() == 2);
+        WANT(which == 0 || (juno_seq_free(a) == JUNO_OK && juno_seq_free(a) == JUNO_ERR_CLOSED));
+    }
+    return 0;
+}
+
 int main(int argc, char **argv) {
     const struct {
         const char *name;
         int (*run)();
-    } checks[] = {{"twice", twice}, {"beside", beside}};
+    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}};
     for (const auto &c : checks)
         if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
     printf("no such check\n");

@@ -31,3 +31,7 @@ def test_rows_of_one_sequence_do_not_share_weights(host):
 
 def test_sequences_without_weights_may_be_named_beside_one_with_weights(host):
     host("beside")
+
+
+def test_sequences_of_a_closed_pool_or_context_are_refused(host):
+    host("closed")
