@@ -1390,6 +1390,7 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     if (n_tokens == 0) return JUNO_OK;
     std::lock_guard<std::recursive_mutex> lk(c->mu);
     JUNO_TRY(ctx_check(c));
+    JUNO_REQUIRE((int64_t)pos + n_tokens <= s->max_tokens, "position %lld is beyond this sequence's limit of %d", (long long)pos + n_tokens - 1, s->max_tokens);
     JUNO_REQUIRE(p->dtype != kKvQ4 || pos <= s->len, "position %d is not behind the %d cached ones", pos, s->len);
     DeviceGuard g(c->device);
     JUNO_TRY(seq_reserve(s, pos, pos + n_tokens, c->stream));

@@ -103,11 +103,26 @@ static int closed() {
     return 0;
 }
 
+// Positions whose end passes 32 bits are beyond the limit, whatever the sum wraps to.
+static int far() {
+    for (int dtype : {0, 1, 3}) {
+        Pool p(dtype);
+        juno_seq *a = p.seq(20);
+        float x[2 * 128] = {0};
+        WANT(juno_seq_append_kv(a, 0, 2147483647, 1, x, x) == JUNO_ERR_INVALID_ARG && strstr(juno_last_error(), "limit of 512"));
+        WANT(juno_seq_append_kv(a, 0, 2147483640, 2147483647, x, x) == JUNO_ERR_INVALID_ARG);
+        WANT(juno_seq_append_kv(a, 0, 5, 2147483647, x, x) == JUNO_ERR_INVALID_ARG);
+        WANT(juno_seq_append_kv(a, 0, 512, 1, x, x) == JUNO_ERR_INVALID_ARG);
+        WANT(a->len == 20 && a->pages.size() == 2);
+    }
+    return 0;
+}
+
 int main(int argc, char **argv) {
     const struct {
         const char *name;
         int (*run)();
-    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}};
+    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}};
     for (const auto &c : checks)
         if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
     printf("no such check\n");

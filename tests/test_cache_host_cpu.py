@@ -35,3 +35,7 @@ def test_sequences_without_weights_may_be_named_beside_one_with_weights(host):
 
 def test_sequences_of_a_closed_pool_or_context_are_refused(host):
     host("closed")
+
+
+def test_positions_beyond_32_bits_are_refused(host):
+    host("far")
