@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <memory>
 #include <type_traits>
 
 #include "attn.cuh"
@@ -908,7 +909,12 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
     JUNO_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim %d is not supported (64, 128)", head_dim);
     JUNO_REQUIRE(dtype == 0 || dtype == 1 || dtype == kKvQ4, "kv_dtype %d (0 = f16, 1 = f32, 3 = 4 bits)", dtype);
     JUNO_REQUIRE(dtype != kKvQ4 || (int64_t)n_pages * n_kv_heads * q4_block_bytes(head_dim) < (1ll << 36), "a layer of 4-bit pages has up to 64 GB");
-    juno_kvpool *p = new juno_kvpool();
+    std::unique_ptr<juno_kvpool> held(new juno_kvpool());
+    juno_kvpool *p = held.get();
+    p->free_pages.reserve(n_pages);
+    for (int i = n_pages - 1; i >= 0; i--) p->free_pages.push_back(i);
+    p->page_refs.assign((size_t)n_pages, 0);
+    for (int i = max_slots - 1; i >= 0; i--) p->free_slots.push_back(i);
     p->magic = kMagicPool;
     p->ctx = ctx;
     p->n_layers = n_layers;
@@ -940,15 +946,10 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
         if (p->v) cudaFree(p->v);
         if (p->d_table) cudaFree(p->d_table);
         if (p->h_table) cudaFreeHost(p->h_table);
-        delete p;
         return e == cudaErrorMemoryAllocation ? JUNO_ERR_OOM : JUNO_ERR_CUDA;
     }
     memset(p->h_table, 0, tbytes);
-    p->free_pages.reserve(n_pages);
-    for (int i = n_pages - 1; i >= 0; i--) p->free_pages.push_back(i);
-    p->page_refs.assign((size_t)n_pages, 0);
-    for (int i = max_slots - 1; i >= 0; i--) p->free_slots.push_back(i);
-    *out = p;
+    *out = held.release();
     return JUNO_OK;
 }
 
@@ -1120,6 +1121,12 @@ static int page_copy(juno_kvpool *p, int dst, int src, cudaStream_t st) {
     return JUNO_OK;
 }
 
+// Room for `more` elements, so that adding them does not throw.
+template <typename T>
+static void make_room(std::vector<T> &v, size_t more) {
+    if (v.capacity() - v.size() < more) v.reserve(std::max(v.size() + more, 2 * v.capacity()));
+}
+
 int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<int32_t> *later) {
     juno_kvpool *p = s->pool;
     JUNO_REQUIRE(upto <= s->max_tokens, "position %d is beyond this sequence's limit of %d", upto - 1, s->max_tokens);
@@ -1135,14 +1142,18 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<in
         set_error("KV pool exhausted: %d pages free, %d needed", (int)p->free_pages.size(), fresh);
         return JUNO_ERR_OOM;
     }
+    // what may throw comes before anything changes: entries that neither the device's table nor the caller has would be missing from then on
+    if (need > have) make_room(s->pages, (size_t)(need - have));
+    if (later) make_room(*later, 2 * (size_t)(need - std::min(first, have)));
     int32_t *row = p->h_table + (size_t)s->slot * p->max_pages_per_seq;
-    int lo = need, hi = -1;  // table entries that change
+    int lo = need, hi = -1, rc = JUNO_OK;  // table entries that change
     for (int i = first; i <= last; i++) {
         const int old = s->pages[(size_t)i];
         if (p->page_refs[(size_t)old] <= 1) continue;
         const int pg = p->free_pages.back();
+        rc = page_copy(p, pg, old, st);
+        if (rc != JUNO_OK) break;
         p->free_pages.pop_back();
-        JUNO_TRY(page_copy(p, pg, old, st));
         p->page_refs[(size_t)old]--;
         p->page_refs[(size_t)pg] = 1;
         s->pages[(size_t)i] = pg;
@@ -1150,7 +1161,7 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<in
         lo = std::min(lo, i);
         hi = std::max(hi, i);
     }
-    for (int i = have; i < need; i++) {
+    for (int i = have; rc == JUNO_OK && i < need; i++) {
         int pg = p->free_pages.back();
         p->free_pages.pop_back();
         p->page_refs[(size_t)pg] = 1;
@@ -1164,9 +1175,10 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<in
             later->push_back(s->slot * p->max_pages_per_seq + i);
             later->push_back(row[i]);
         }
-        return JUNO_OK;
+        return rc;
     }
-    return table_store(p, s->slot, lo, hi, st);
+    const int stored = table_store(p, s->slot, lo, hi, st);
+    return rc != JUNO_OK ? rc : stored;
 }
 
 // A sequence's weights, one plane of `room` (a multiple of 16) positions for each layer and head: the first `len` of another one's, zeros behind.
@@ -1236,7 +1248,7 @@ int juno_kvpool_create(juno_ctx *c, int32_t n_layers, int32_t n_kv_heads, int32_
     JUNO_REQUIRE(out, "out is null");
     std::lock_guard<std::recursive_mutex> lk(c->mu);
     DeviceGuard g(c->device);
-    return kvpool_create(c, n_layers, n_kv_heads, head_dim, n_pages, kv_dtype, 256, std::min(n_pages, 8192), out);
+    return guarded([&] { return kvpool_create(c, n_layers, n_kv_heads, head_dim, n_pages, kv_dtype, 256, std::min(n_pages, 8192), out); });
 }
 
 int juno_kvpool_free(juno_kvpool *p) {
@@ -1261,7 +1273,7 @@ int juno_kvseq_create(juno_kvpool *p, int32_t max_tokens, juno_seq **out) {
     }
     std::lock_guard<std::recursive_mutex> lk(p->ctx->mu);
     JUNO_TRY(ctx_check(p->ctx));
-    return seq_create(p, max_tokens, out);
+    return guarded([&] { return seq_create(p, max_tokens, out); });
 }
 
 int juno_seq_free(juno_seq *s) {
@@ -1282,7 +1294,7 @@ int juno_seq_free(juno_seq *s) {
     return JUNO_OK;
 }
 
-int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
+static int seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
     JUNO_TRY(seq_check(src));
     JUNO_REQUIRE(out, "out is null");
     juno_kvpool *p = src->pool;
@@ -1291,6 +1303,8 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
     JUNO_REQUIRE(n_tokens >= 0 && n_tokens <= src->len, "cannot share %d positions of a sequence that holds %d", n_tokens, src->len);
     DeviceGuard g(p->ctx->device);
     JUNO_TRY(seq_resume_check(p, src->len, n_tokens));
+    const int n_pg = (n_tokens + kPageTokens - 1) / kPageTokens;
+    std::vector<int> pages(src->pages.begin(), src->pages.begin() + n_pg);
     juno_seq *s = nullptr;
     JUNO_TRY(seq_create(p, src->max_tokens, &s));
     if (p->state) {  // the state is small and changes every step: each holder has its own
@@ -1304,14 +1318,13 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
             JUNO_CUDA_TRY(e);
         }
     }
-    const int n_pg = (n_tokens + kPageTokens - 1) / kPageTokens;
     int32_t *row = p->h_table + (size_t)s->slot * p->max_pages_per_seq;
     for (int i = 0; i < n_pg; i++) {
-        const int pg = src->pages[(size_t)i];
+        const int pg = pages[(size_t)i];
         p->page_refs[(size_t)pg]++;
-        s->pages.push_back(pg);
         row[i] = pg;
     }
+    s->pages = std::move(pages);
     s->len = n_tokens;
     const int rc = src->track >= 0 ? seq_track(s, src) : n_pg ? table_store(p, s->slot, 0, n_pg - 1, p->ctx->stream) : JUNO_OK;
     if (rc != JUNO_OK) {
@@ -1323,6 +1336,10 @@ int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
     }
     *out = s;
     return JUNO_OK;
+}
+
+int juno_seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
+    return guarded([&] { return seq_fork(src, n_tokens, out); });
 }
 
 int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens) {
@@ -1378,8 +1395,7 @@ int juno_seq_length(juno_seq *s, int32_t *n_tokens) {
     return JUNO_OK;
 }
 
-int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens, const float *k_host,
-                       const float *v_host) {
+static int append_kv(juno_seq *s, int layer, int pos, int n_tokens, const float *k_host, const float *v_host) {
     JUNO_TRY(seq_check(s));
     juno_kvpool *p = s->pool;
     juno_ctx *c = p->ctx;
@@ -1423,8 +1439,12 @@ int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens
     return JUNO_OK;
 }
 
-int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs, int32_t n_heads,
-                     const float *q_host, float *out_host) {
+int juno_seq_append_kv(juno_seq *s, int32_t layer, int32_t pos, int32_t n_tokens, const float *k_host,
+                       const float *v_host) {
+    return guarded([&] { return append_kv(s, layer, pos, n_tokens, k_host, v_host); });
+}
+
+static int attn_decode(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *seqs, int n_heads, const float *q_host, float *out_host) {
     JUNO_TRY(ctx_check(c));
     JUNO_REQUIRE(p && seqs && q_host && out_host, "null argument");
     if (p->magic != kMagicPool) {
@@ -1448,7 +1468,7 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
         meta[n + i] = seqs[i]->len;
         max_len = std::max(max_len, seqs[i]->len);
     }
-    JUNO_TRY(guarded([&] { return cache_call_distinct(p, n, seqs, true); }));  // two rows of one sequence would add to the same weights side by side
+    JUNO_TRY(cache_call_distinct(p, n, seqs, true));  // two rows of one sequence would add to the same weights side by side
     const int hd = p->head_dim, qdim = n_heads * hd;
     const size_t qbytes = (size_t)n * qdim * sizeof(float);
     if (p->dtype == kKvQ4) {
@@ -1458,7 +1478,7 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
         JUNO_TRY(ensure_device(&py, &c->stage_y_bytes, qbytes));
         c->stage_y = (float *)py;
         JUNO_CUDA_TRY(cudaMemcpyAsync(c->stage_x, q_host, qbytes, cudaMemcpyHostToDevice, c->stream));
-        JUNO_TRY(guarded([&] { return q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, WAIT_BLOCKING, c->stream); }));
+        JUNO_TRY(q4_attend(c, p, layer, n, seqs, nullptr, n_heads, c->stage_x, qdim, c->stage_y, qdim, WAIT_BLOCKING, c->stream));
         JUNO_CUDA_TRY(cudaMemcpyAsync(out_host, c->stage_y, qbytes, cudaMemcpyDeviceToHost, c->stream));
         JUNO_CUDA_TRY(cudaStreamSynchronize(c->stream));
         JUNO_TRY(wait_status(c, WAIT_BLOCKING));
@@ -1501,6 +1521,10 @@ int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno
     return JUNO_OK;
 }
 
+int juno_attn_decode(juno_ctx *c, juno_kvpool *p, int32_t layer, int32_t n, juno_seq *const *seqs, int32_t n_heads,
+                     const float *q_host, float *out_host) {
+    return guarded([&] { return attn_decode(c, p, layer, n, seqs, n_heads, q_host, out_host); });
+}
 
 // ── attention without any allocation ─────────────────────────────────────────────────────────
 // Scratch for juno_attn_decode_static: the per-split partial outputs, the (max, sum) pairs and the per-sequence

@@ -1,11 +1,24 @@
 // Test-only host program: calls on pools and sequences that are put together by hand, without a GPU.  `cache_host NAME` runs one check and exits 0 if it holds.
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
+#include <new>
 
 #include "../../include/juno_b200.h"
 #include "../../juno_b200/csrc/attn.cuh"
 
 using namespace juno;
+
+// The program's own allocation, which the library uses too: the one after `g_left` others fails.
+static long g_left = -1;
+void *operator new(size_t n) {
+    if (g_left == 0) throw std::bad_alloc();
+    if (g_left > 0) g_left--;
+    if (void *p = malloc(n ? n : 1)) return p;
+    throw std::bad_alloc();
+}
+void operator delete(void *p) noexcept { free(p); }
+void operator delete(void *p, size_t) noexcept { free(p); }
 
 #define WANT(x)                                                        \
     do {                                                               \
@@ -118,11 +131,71 @@ static int far() {
     return 0;
 }
 
+// A call that runs out of host memory says so, and leaves pages, slots and the list of changes as they were.
+static int memory() {
+    for (long n = 0;; n++) {
+        Pool p(3);
+        juno_seq *a = p.seq(20), *b = nullptr;
+        std::vector<int32_t> later(3, 7);
+        const size_t pages = p.pool.free_pages.size();
+        bool thrown = false;
+        int rc = JUNO_OK;
+        g_left = n;
+        try {
+            rc = seq_reserve(a, 20, 300, nullptr, &later);
+        } catch (const std::bad_alloc &) {
+            thrown = true;
+        }
+        g_left = -1;
+        if (!thrown) {
+            WANT(rc == JUNO_OK && a->pages.size() == 19 && later.size() == 3 + 2 * 17 && p.pool.free_pages.size() == pages - 17);
+            WANT(n > 0);
+            break;
+        }
+        WANT(a->pages.size() == 2 && later.size() == 3 && p.pool.free_pages.size() == pages);
+    }
+    for (long n = 0;; n++) {
+        Pool p(3);
+        juno_seq *a = p.seq(20), *b = nullptr;
+        const size_t slots = p.pool.free_slots.size();
+        g_left = n;
+        const int rc = juno_seq_fork(a, 20, &b);  // without a GPU the page table does not reach it: an error, too
+        g_left = -1;
+        WANT(rc != JUNO_OK && !b && p.pool.free_slots.size() == slots && p.pool.page_refs[a->pages[0]] == 1 && p.pool.page_refs[a->pages[1]] == 1);
+        if (rc != JUNO_ERR_OOM) {
+            WANT(n > 0);
+            break;
+        }
+    }
+    for (long n = 0;; n++) {
+        Pool p(0);
+        juno_seq *b = nullptr;
+        g_left = n;
+        const int rc = juno_kvseq_create(&p.pool, 16, &b);
+        g_left = -1;
+        WANT((rc == JUNO_OK) == (b != nullptr) && p.pool.free_slots.size() == (b ? 7 : 8));
+        if (b) break;
+        WANT(rc == JUNO_ERR_OOM);
+    }
+    for (long n = 0; n < 2; n++) {
+        Pool p(n ? 0 : 3);
+        juno_seq *a = p.seq(20);
+        float x[256] = {0};
+        g_left = 0;
+        const int decode = juno_attn_decode(&p.ctx, &p.pool, 0, 1, &a, 4, x, x), append = juno_seq_append_kv(a, 0, 20, 100, x, x);
+        juno_kvpool *q = nullptr;
+        const int create = juno_kvpool_create(&p.ctx, 1, 1, 64, 4, 0, &q);
+        g_left = -1;
+        WANT(decode == JUNO_ERR_OOM && append == JUNO_ERR_OOM && create == JUNO_ERR_OOM && !q && a->pages.size() == 2);
+    }
+    return 0;
+}
+
 int main(int argc, char **argv) {
     const struct {
         const char *name;
         int (*run)();
-    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}};
+    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}, {"memory", memory}};
     for (const auto &c : checks)
         if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
     printf("no such check\n");

@@ -39,3 +39,7 @@ def test_sequences_of_a_closed_pool_or_context_are_refused(host):
 
 def test_positions_beyond_32_bits_are_refused(host):
     host("far")
+
+
+def test_host_memory_that_runs_out_is_an_error_and_changes_nothing(host):
+    host("memory")
