@@ -1289,7 +1289,7 @@ int juno_seq_free(juno_seq *s) {
     p->free_slots.push_back(s->slot);
     if (s->track >= 0) p->free_tracks.push_back(s->track);
     s->track = -1;
-    s->pages.clear();
+    std::vector<int>().swap(s->pages);  // the handle stays, so that its later use is seen; its list of pages does not
     s->magic = kMagicDead;
     return JUNO_OK;
 }

@@ -191,11 +191,21 @@ static int memory() {
     return 0;
 }
 
+// A freed sequence keeps its handle, and nothing that grows with its length.
+static int freed() {
+    Pool p(3);
+    juno_seq *a = p.seq(300);
+    WANT(a->pages.capacity() >= 19);
+    WANT(juno_seq_free(a) == JUNO_OK && a->pages.capacity() == 0);
+    WANT(p.pool.free_pages.size() == 64 && p.pool.free_slots.size() == 8);
+    return 0;
+}
+
 int main(int argc, char **argv) {
     const struct {
         const char *name;
         int (*run)();
-    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}, {"memory", memory}};
+    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}, {"memory", memory}, {"freed", freed}};
     for (const auto &c : checks)
         if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
     printf("no such check\n");

@@ -43,3 +43,7 @@ def test_positions_beyond_32_bits_are_refused(host):
 
 def test_host_memory_that_runs_out_is_an_error_and_changes_nothing(host):
     host("memory")
+
+
+def test_a_freed_sequence_gives_its_list_of_pages_back(host):
+    host("freed")
