@@ -173,7 +173,7 @@ int juno_attn_decode_static(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_
  * streams are: a call on another stream waits for what the context's stream has, and the context's stream waits for it.  The caller's own
  * work on q, k, v and results is ordered by that stream only.  A stream that is being captured, or one of another device, gives
  * JUNO_ERR_INVALID_ARG: a graph would hold the page table of the moment.  Working memory belongs to the context and grows with the largest
- * call.  Arrays of sequences, positions, counts and lengths are host memory and are not used after the call.  n <= 4096.
+ * call, to twice its size at least; a call that makes it grow waits for the device.  Arrays of sequences, positions, counts and lengths are host memory and are not used after the call.  n <= 4096.
  * Not for pools of a model. */
 
 /* Writes counts[i] positions of keys and values, the first at positions[i] (at most the sequence's length), for every

@@ -56,8 +56,16 @@ int device_memory(const juno_ctx *c, const void *p, const char *name) {
     return JUNO_OK;
 }
 
+// Growing waits for the device, so it is done seldom: to twice the room that there was where the device has as much, and 1 MB at first.  A sequence that keeps weights
+// asks for more with every page.
+int cache_room(void **ptr, size_t *cur, size_t bytes) {
+    if (*ptr && *cur >= bytes) return JUNO_OK;
+    if (ensure_device(ptr, cur, std::max({bytes, 2 * *cur, (size_t)1 << 20})) == JUNO_OK) return JUNO_OK;
+    return ensure_device(ptr, cur, bytes);
+}
+
 int cache_scratch(juno_ctx *c, size_t bytes, uint8_t **out) {
-    JUNO_TRY(ensure_device(&c->cache_scratch, &c->cache_scratch_bytes, bytes));
+    JUNO_TRY(cache_room(&c->cache_scratch, &c->cache_scratch_bytes, bytes));
     *out = static_cast<uint8_t *>(c->cache_scratch);
     return JUNO_OK;
 }

@@ -62,6 +62,8 @@ int cache_call_distinct(const juno_kvpool *p, int n, juno_seq *const *seqs, bool
 int device_memory(const juno_ctx *c, const void *p, const char *name);
 // The context's working memory, at least `bytes`; what an earlier call left there is gone.
 int cache_scratch(juno_ctx *c, size_t bytes, uint8_t **out);
+// Grows a piece of working memory to `bytes` or more.
+int cache_room(void **ptr, size_t *cur, size_t bytes);
 // Fills `out` for `n` rows; `far`: room for them in the working memory when they are more than kInlineRows.
 int cache_rows(juno_ctx *c, const CacheRow *rows, int n, CacheRow *far, CacheRows *out, cudaStream_t st);
 inline size_t cache_rows_bytes(int n) { return n > kInlineRows ? ((size_t)n * sizeof(CacheRow) + 255) & ~(size_t)255 : 0; }

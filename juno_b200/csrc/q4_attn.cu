@@ -805,7 +805,7 @@ static bool q4_whole(const std::vector<CacheRow> &rows, const std::vector<int32_
 static int arrival_words(juno_ctx *c, size_t n, cudaStream_t st) {
     if (c->cache_arrived && c->cache_arrived_bytes >= n * sizeof(unsigned)) return JUNO_OK;
     void *words = c->cache_arrived;
-    JUNO_TRY(ensure_device(&words, &c->cache_arrived_bytes, std::max<size_t>(n * sizeof(unsigned), 16384)));
+    JUNO_TRY(cache_room(&words, &c->cache_arrived_bytes, n * sizeof(unsigned)));
     c->cache_arrived = static_cast<unsigned *>(words);
     JUNO_CUDA_TRY(cudaMemsetAsync(words, 0, c->cache_arrived_bytes, st));
     return JUNO_OK;

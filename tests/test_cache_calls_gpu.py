@@ -1,13 +1,30 @@
 """Calls on 4-bit cache pages in the forms that one operator's tests do not have: from host memory, beyond usual sizes, after failures, with pages shared in part."""
+import ctypes as C
+import os
+import subprocess
+
 import numpy as np
 import pytest
+import torch
 
-from juno_b200.matvec import PagedKvCache
+from juno_b200.matvec import GpuContext, PagedKvCache
 from oracle import q4_cache_oracle as q4
 from q4util import rows
-from test_q4_cache_gpu import attend, check_attention, check_weights, f32, fill, weights
+from test_q4_cache_gpu import attend, check_attention, check_weights, f32, fill, settle, weights
 
 pytestmark = pytest.mark.gpu
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@pytest.fixture(scope="module")
+def words():
+    src, so = (os.path.join(HERE, "native", f) for f in ("cache_words.cpp", "libcache_words.so"))
+    header = os.path.join(HERE, "..", "juno_b200", "csrc", "common.cuh")
+    if not os.path.exists(so) or os.path.getmtime(so) < max(os.path.getmtime(src), os.path.getmtime(header)):
+        subprocess.check_call(["g++", "-O2", "-std=c++17", "-I/usr/local/cuda/include", "-shared", "-fPIC", "-o", so, src])
+    L = C.CDLL(so)
+    L.cache_scratch_bytes.restype, L.cache_scratch_bytes.argtypes = C.c_longlong, [C.c_void_p]
+    return L
 
 
 def test_host_attention_names_a_sequence_with_weights_once(ctx):
@@ -76,3 +93,24 @@ def test_groups_of_values_far_apart(ctx, n, heads, kv, dim, ratio):
         of_groups = lambda x: np.linalg.norm(x.reshape(heads, -1, 32), axis=-1)  # noqa: E731
         assert (of_groups(got - want) <= 1e-5 * of_groups(want)).all(), of_groups(got - want) / of_groups(want)
     cache.close()
+
+
+def test_a_growing_sequence_with_weights_seldom_grows_the_working_memory(words):
+    """Growing waits for the whole device: to twice the size each time, so that 400 steps do it a few times."""
+    rng = np.random.default_rng(54)
+    own = GpuContext(0)
+    kv, dim, n = 2, 64, 16 * 400
+    cache = PagedKvCache(own, 1, kv, dim, 400, "q4", track_seqs=1, track_tokens=n)
+    s = cache.new_sequence(n, track=True)
+    k, q, out = (torch.from_numpy(f32(rng.standard_normal((16, w)))).cuda() for w in (kv * dim, 16 * dim, 16 * dim))
+    settle()
+    sizes = []
+    for at in range(0, n, 16):
+        cache.append_device(0, [s], [at], [16], k, k)
+        cache.attention_device(0, [s], q[:1], 16, out[:1])
+        sizes.append(words.cache_scratch_bytes(own.handle))
+    own.synchronize()
+    need = n * 16 * 4  # the scores
+    assert need <= sizes[-1] <= 4 * need + (1 << 20) and len(set(sizes)) <= 6, sorted(set(sizes))
+    cache.close()
+    own.close()
