@@ -196,7 +196,7 @@ int juno_attn_decode_device(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_
 /* Accumulated attention weight.  juno_kvpool_track gives a JUNO_KV_Q4 pool room for the weights of n_seqs sequences of up to
  * max_tokens positions (n_layers*n_kv_heads*max_tokens FP32 each); once per pool.  juno_seq_track has a sequence keep them, zeros at
  * first: from then on each decode attention over it adds, for every layer, key/value head and attended position, the softmax weights that
- * the head's query heads gave to that position.  A fork of such a sequence has weights of its own, a copy.  JUNO_ERR_OOM when the
+ * the head's query heads gave to that position.  A call that gave up a wait (JUNO_ERR_TIMEOUT) adds nothing.  A fork of such a sequence has weights of its own, a copy.  JUNO_ERR_OOM when the
  * room is taken. */
 int juno_kvpool_track(juno_kvpool *p, int32_t n_seqs, int32_t max_tokens);
 int juno_seq_track(juno_seq *s);

@@ -93,7 +93,8 @@ struct juno_ctx {
     // working memory of the calls on cache pages that take a stream, and the events that order them (cache_ops.cuh)
     void *cache_scratch = nullptr;
     size_t cache_scratch_bytes = 0;
-    unsigned *cache_arrived = nullptr;  // decode attention's counts of finished parts, zero between launches
+    unsigned *cache_arrived = nullptr;  // decode attention: the last call that gave up a wait (64 bits, 16 bytes of room), then counts of finished parts, zero between launches
+    uint64_t cache_calls = 0;           // calls of decode attention
     size_t cache_arrived_bytes = 0;
     cudaEvent_t cache_events[2] = {nullptr, nullptr};
     // per-kernel timing (off by default): event pairs around launches, summed at read time

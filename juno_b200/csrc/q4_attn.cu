@@ -29,6 +29,7 @@ struct Q4AttnParams {
     float *part_o, *part_ml;  // [part][head][hd], [part][head][max, sum]
     float2 *sums;             // sequences that keep weights: [row][head] largest score of all, 1 / sum
     unsigned *arrived;        // [row][kv_head]: parts that are done, zero between launches
+    unsigned long long *gave_up, call;  // sequences that keep weights: the last call that gave up a wait; the number of this one
     float *scores;            // sequences that keep weights: [kv_head][position of all rows' pages][G], log2 domain
     float *weights;
     int track_tokens;
@@ -686,6 +687,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         }
     }
     if (failed) {  // the parts that are left count as done, so that the next launch finds zeros
+        if (TRACK && lane == 0) *reinterpret_cast<volatile unsigned long long *>(p.gave_up) = p.call;
         for (unsigned j = ring_open((int)issued, (int)used, kQ4Slots); j < issued; j++)
             mbar_wait_bounded(bars + j % kQ4Slots * 8, j / kQ4Slots & 1u, 0, p.err, failed, kErrCacheWait);
         if (tid == 0)
@@ -721,6 +723,8 @@ __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __gr
     const CacheRow r = cache_row(p.rows, i);
     const int pos = at - r.first * kPageTokens, n = min(4, r.upto - pos);
     if (r.track < 0 || n <= 0) return;
+    // the sums and scores of a call that gave up a wait are in part those of an earlier one: none of its rows adds anything
+    const bool valid = __ldcg(p.gave_up) != p.call;
     const float *scores = p.scores + ((size_t)kvh * p.total * kPageTokens + at) * G;
     const float2 *sums = p.sums + (size_t)i * p.n_heads + kvh * G;
     float4 *w = reinterpret_cast<float4 *>(p.weights + (((size_t)r.track * p.n_layers + p.layer) * p.n_kv_heads + kvh) * p.track_tokens + pos);
@@ -743,7 +747,7 @@ __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __gr
         }
     }
     // positions behind the row's end keep what they have
-    *w = make_float4(old.x + sum[0], n > 1 ? old.y + sum[1] : old.y, n > 2 ? old.z + sum[2] : old.z, n > 3 ? old.w + sum[3] : old.w);
+    if (valid) *w = make_float4(old.x + sum[0], n > 1 ? old.y + sum[1] : old.y, n > 2 ? old.z + sum[2] : old.z, n > 3 ? old.w + sum[3] : old.w);
 }
 
 template <int HD, int HPL, bool TRACK>
@@ -801,8 +805,10 @@ static bool q4_whole(const std::vector<CacheRow> &rows, const std::vector<int32_
     return true;
 }
 
-// Zeros, once; every launch leaves them so.
+// Zeros, once; every launch leaves the counts so.
+constexpr size_t kArrivedAt = 4;  // words before the counts
 static int arrival_words(juno_ctx *c, size_t n, cudaStream_t st) {
+    n += kArrivedAt;
     if (c->cache_arrived && c->cache_arrived_bytes >= n * sizeof(unsigned)) return JUNO_OK;
     void *words = c->cache_arrived;
     JUNO_TRY(cache_room(&words, &c->cache_arrived_bytes, n * sizeof(unsigned)));
@@ -835,7 +841,7 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     q4_cut(rows, (int)pages, std::max(1, c->sm_count * ctas / H), warps * kQ4Tile, &cuts);
     const int shares = (int)cuts.size() - 1;
     const bool whole = shares == 1 || q4_whole(rows, cuts);
-    if (!whole) JUNO_TRY(arrival_words(c, (size_t)n * H, st));
+    if (track || !whole) JUNO_TRY(arrival_words(c, whole ? 0 : (size_t)n * H, st));
     Q4AttnParams a;
     auto padded = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t parts = whole ? 0 : (size_t)(n + shares), row_b = cache_rows_bytes(n), cut_b = shares + 1 > kInlineCuts ? padded(cuts.size() * sizeof(int32_t)) : 0,
@@ -869,7 +875,9 @@ int q4_attend(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *se
     a.sums = track ? reinterpret_cast<float2 *>(scratch + far_b + ml_b + o_b + s_b) : nullptr;
     a.weights = p->weights;
     a.track_tokens = p->track_tokens;
-    a.arrived = c->cache_arrived;
+    a.arrived = c->cache_arrived ? c->cache_arrived + kArrivedAt : nullptr;
+    a.gave_up = reinterpret_cast<unsigned long long *>(c->cache_arrived);
+    a.call = ++c->cache_calls;
     a.err = c->gemv_scratch.qerr + word;
     ProfScope prof(c, st, PROF_ATTN, (double)bytes * H * p->row_bytes());
     if (hd == 128)

@@ -23,7 +23,8 @@ def words():
     if not os.path.exists(so) or os.path.getmtime(so) < max(os.path.getmtime(src), os.path.getmtime(header)):
         subprocess.check_call(["g++", "-O2", "-std=c++17", "-I/usr/local/cuda/include", "-shared", "-fPIC", "-o", so, src])
     L = C.CDLL(so)
-    L.cache_scratch_bytes.restype, L.cache_scratch_bytes.argtypes = C.c_longlong, [C.c_void_p]
+    for f, t in (("cache_scratch_bytes", C.c_longlong), ("cache_gave_up", C.c_void_p), ("cache_calls", C.c_ulonglong)):
+        getattr(L, f).restype, getattr(L, f).argtypes = t, [C.c_void_p]
     return L
 
 
@@ -114,3 +115,23 @@ def test_a_growing_sequence_with_weights_seldom_grows_the_working_memory(words):
     assert need <= sizes[-1] <= 4 * need + (1 << 20) and len(set(sizes)) <= 6, sorted(set(sizes))
     cache.close()
     own.close()
+
+
+def test_a_call_that_gave_up_a_wait_adds_no_weights(ctx, words):
+    """The word that such a call's kernel leaves is put there for the next call: its weights stay as they are, those of the call after it are added."""
+    rng = np.random.default_rng(55)
+    cache = PagedKvCache(ctx, 1, 2, 64, 200, "q4", track_seqs=2, track_tokens=1000)
+    lens = [1000, 33]
+    seqs, parts = [cache.new_sequence(1000, track=True) for _ in lens], [(rows(rng, n, 2, 64), rows(rng, n, 2, 64)) for n in lens]
+    fill(cache, 0, seqs, [0, 0], parts)
+    q = f32(rng.standard_normal((2, 8, 64)))
+    want = [check_attention(o, x, q4.held(p[0]), q4.held(p[1])) for o, x, p in zip(attend(cache, 0, seqs, q), q, parts)]
+    settle()
+    number = C.c_ulonglong(words.cache_calls(ctx.handle) + 1)
+    assert C.CDLL("libcuda.so.1").cuMemcpyHtoD_v2(C.c_ulonglong(words.cache_gave_up(ctx.handle)), C.byref(number), C.c_size_t(8)) == 0
+    for times in (1, 2):  # the call that is marked, and the next one
+        attend(cache, 0, seqs, q)
+        w = weights(cache, 0, seqs, lens)
+        for i, n in enumerate(lens):
+            check_weights(w[i][:, :n], times * want[i], q[i], parts[i][0])
+    cache.close()
