@@ -7,10 +7,11 @@ import numpy as np
 import pytest
 import torch
 
+from juno_b200._lib import JunoError
 from juno_b200.matvec import GpuContext, PagedKvCache
 from oracle import q4_cache_oracle as q4
 from q4util import rows
-from test_q4_cache_gpu import attend, check_attention, check_weights, f32, fill, settle, weights
+from test_q4_cache_gpu import attend, check_attention, check_weights, dev, expected, f32, fill, read, settle, some_weights, weights
 
 pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -134,4 +135,74 @@ def test_a_call_that_gave_up_a_wait_adds_no_weights(ctx, words):
         w = weights(cache, 0, seqs, lens)
         for i, n in enumerate(lens):
             check_weights(w[i][:, :n], times * want[i], q[i], parts[i][0])
+    cache.close()
+
+
+def free_pages(cache, most):
+    """How many pages of the pool are free: as many as a sequence of `most` pages can get."""
+    s, wide = cache.new_sequence(16 * most), cache.n_kv_heads * cache.head_dim
+    x, n = torch.zeros((16, wide), device="cuda"), 0
+    settle()
+    try:
+        for n in range(most + 1):
+            cache.append_device(0, [s], [16 * n], [16], x, x)
+    except JunoError as e:
+        assert "pages free" in str(e)
+    except ValueError as e:
+        assert "limit" in str(e)
+    cache.ctx.synchronize()
+    cache.free_sequence(s)
+    return n
+
+
+@pytest.mark.parametrize("both,free", [(False, 3), (False, 2), (True, 5), (True, 4)])
+@pytest.mark.parametrize("kv,dim", [(2, 64), (3, 128)])
+def test_eviction_with_room_for_shared_pages_alone(ctx, kv, dim, both, free):
+    """A branch shares the first two of its pages, and the pool has room for those two but not for all that stay: some pages are fresh, the others are filled in place;
+    alone, and together with the sequence that it came from.  With one page less the call is refused."""
+    rng = np.random.default_rng(56)
+    layers, lens, keep, recent = 2, [160, 140], 100, 17
+    cache = PagedKvCache(ctx, layers, kv, dim, 10 + 7 + free, "q4", track_seqs=3, track_tokens=160)
+    s = cache.new_sequence(160, track=True)
+    have = [[(rows(rng, n, kv, dim), rows(rng, n, kv, dim)) for _ in range(layers)] for n in lens]
+    for l in range(layers):
+        fill(cache, l, [s], [0], [have[0][l]])
+    b = cache.fork(s, 40)
+    for l in range(layers):  # the third page is copied when the branch writes to it
+        fill(cache, l, [b], [40], [tuple(x[40:] for x in have[1][l])])
+        have[1][l] = tuple(np.concatenate([x[:40], y[40:]]) for x, y in zip(have[0][l], have[1][l]))
+    w = [some_weights(rng, (layers, kv, n)) for n in lens]
+    for l in range(layers):
+        for seq, x in ((s, w[0]), (b, w[1])):
+            t = dev(x[l][None])
+            settle()
+            cache.weights_device(l, [seq], [x.shape[-1]], t, store=True)
+            settle()
+    assert free_pages(cache, 12) == free
+    cut = [s, b] if both else [b]
+    if free in (2, 4):  # one page less
+        other, x = cache.new_sequence(16), torch.zeros((1, kv * dim), device="cuda")
+        settle()
+        cache.append_device(0, [other], [0], [1], x, x)
+        with pytest.raises(JunoError, match="pages free"):
+            cache.evict(cut, keep, recent)
+        assert [cache.length(q) for q in (s, b)] == lens
+        cache.free_sequence(other)
+    kept = torch.full((layers, len(cut), kv, keep), 99, dtype=torch.int32, device="cuda")
+    settle()
+    cache.evict(cut, keep, recent, kept=kept)
+    settle()
+    for i, seq in enumerate((s, b)):
+        if seq in cut:
+            want = expected(have[i], w[i], keep, recent)
+        else:
+            want = [(None, *have[i][l], w[i][l]) for l in range(layers)]
+        for l, (at, k, v, wl) in enumerate(want):
+            got = read(cache, l, [seq], [0], [len(k)])
+            assert np.array_equal(got[0], f32(q4.held(k))) and np.array_equal(got[1], f32(q4.held(v)))
+            assert np.array_equal(weights(cache, l, [seq], [len(k)])[0], wl, equal_nan=True)
+            if at is not None:
+                assert np.array_equal(kept[l, cut.index(seq)].cpu().numpy(), at)
+    # the branch needs two fresh pages and gives its last two back; with its source, that gives its last three back and both leave the shared two
+    assert free_pages(cache, 12) == free + (3 if both else 0)
     cache.close()
