@@ -12,6 +12,7 @@ from juno_b200.matvec import GpuContext, PagedKvCache
 from oracle import q4_cache_oracle as q4
 from q4util import rows
 from test_q4_cache_gpu import attend, check_attention, check_weights, dev, expected, f32, fill, read, settle, some_weights, weights
+from test_readme_cpu import cache_example
 
 pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -206,3 +207,24 @@ def test_eviction_with_room_for_shared_pages_alone(ctx, kv, dim, both, free):
     # the branch needs two fresh pages and gives its last two back; with its source, that gives its last three back and both leave the shared two
     assert free_pages(cache, 12) == free + (3 if both else 0)
     cache.close()
+
+
+def test_the_example_of_the_readme_follows_the_tensors(ctx):
+    """On a stream of its own, behind work that takes longer than the calls: the rows are not there yet when they are made."""
+    rng = np.random.default_rng(57)
+    k, v, q = f32(rng.standard_normal((5, 8, 128))), f32(rng.standard_normal((5, 8, 128))), f32(rng.standard_normal((1, 32, 128)))
+    source = [dev(x.reshape(len(x), -1)) for x in (k, v, q)]
+    names = dict(zip("kvq", (torch.full_like(x, 77.0) for x in source)), layer=3, pos=0, n=5, out=torch.full((1, 4096), 77.0, device="cuda"))
+    busy = torch.randn((8192, 8192), device="cuda")
+    settle()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(8):
+            busy = busy @ busy * 1e-2
+        for name, x in zip("kvq", source):
+            names[name].copy_(x)
+        exec(cache_example(), names)
+        out = names["out"].clone()
+    stream.synchronize()
+    check_attention(out.cpu().numpy().reshape(32, 128), q[0], q4.held(k), q4.held(v))
+    names["cache"].close()
