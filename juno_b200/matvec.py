@@ -206,6 +206,13 @@ def _whole_ptr(x, name: str, kind: str, lead: tuple):
     return x.data_ptr()
 
 
+def _in_32_bits(x: int, name: str) -> int:
+    """ctypes would take the lower 32 bits of any whole number."""
+    if not -0x80000000 <= x <= 0x7fffffff:
+        raise ValueError(f"{name} {x}: a whole number of 32 bits is wanted")
+    return x
+
+
 class SequenceBatch:
     """Sequences of one cache in the order in which a step names them."""
 
@@ -257,7 +264,7 @@ class PagedKvCache:
     def fork(self, seq, n_tokens: int):
         """A sequence that starts with the first n_tokens cached positions of another one (juno_seq_fork)."""
         h = C.c_void_p()
-        check(self._L.juno_seq_fork(seq, int(n_tokens), C.byref(h)), "juno_seq_fork")
+        check(self._L.juno_seq_fork(seq, _in_32_bits(int(n_tokens), "n_tokens"), C.byref(h)), "juno_seq_fork")
         return h
 
     def length(self, seq) -> int:
@@ -308,7 +315,7 @@ class PagedKvCache:
         vp, ldv = _device_ptr(v, "v", rows, width)
         if ld != ldv:
             raise ValueError(f"the rows of k and v lie {ld} and {ldv} elements apart")
-        rc = call(self.ctx.handle, self.handle, layer, b.n, b.handles, positions.tobytes(), counts.tobytes(), kp, vp, ld, None if stream is None else self._stream(stream))
+        rc = call(self.ctx.handle, self.handle, _in_32_bits(layer, "layer"), b.n, b.handles, positions.tobytes(), counts.tobytes(), kp, vp, ld, None if stream is None else self._stream(stream))
         if rc:
             check(rc, name)
 
@@ -327,7 +334,7 @@ class PagedKvCache:
         qp, ldq = _device_ptr(q, "q", b.n, width)
         op, ldo = _device_ptr(out, "out", b.n, width)
         lens = None if lens is None else self._ints(lens, b.n, "lens").tobytes()
-        rc = self._L.juno_attn_decode_device(self.ctx.handle, self.handle, layer, b.n, b.handles, lens, n_heads, qp, ldq, op, ldo,
+        rc = self._L.juno_attn_decode_device(self.ctx.handle, self.handle, _in_32_bits(layer, "layer"), b.n, b.handles, lens, n_heads, qp, ldq, op, ldo,
                                              None if stream is None else self._stream(stream))
         if rc:
             check(rc, "juno_attn_decode_device")
@@ -339,7 +346,7 @@ class PagedKvCache:
         wp = _whole_ptr(w, "w", "float32", (b.n, self.n_kv_heads))
         ld = w.shape[2]
         counts = self._ints(counts, b.n, "counts").tobytes()
-        rc = self._L.juno_kv_weights_device(self.ctx.handle, self.handle, layer, b.n, b.handles, counts, wp, ld, 1 if store else 0,
+        rc = self._L.juno_kv_weights_device(self.ctx.handle, self.handle, _in_32_bits(layer, "layer"), b.n, b.handles, counts, wp, ld, 1 if store else 0,
                                             None if stream is None else self._stream(stream))
         if rc:
             check(rc, "juno_kv_weights_device")
@@ -348,8 +355,8 @@ class PagedKvCache:
         """Cuts sequences down to the `keep` positions of most weight, the newest `recent` among them, in every layer and key/value head; kept:
         int32 [n_layers, sequences, n_kv_heads, keep] gets their places (juno_kv_evict)."""
         b, kp = seqs if type(seqs) is SequenceBatch else SequenceBatch(seqs), None
-        if keep >= 1 << 31 or recent >= 1 << 31:
-            raise ValueError(f"keep {keep}, recent {recent}: whole numbers of 32 bits are wanted")
+        _in_32_bits(keep, "keep")
+        _in_32_bits(recent, "recent")
         if kept is not None:
             kp = _whole_ptr(kept, "kept", "int32", (self.n_layers, b.n, self.n_kv_heads))
             if kept.shape[3] != keep:
