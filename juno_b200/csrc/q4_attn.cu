@@ -86,6 +86,7 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+constexpr float kLargest = 3.4028234663852886e38f;
 // N words that lie together in shared memory
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t a) {
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
         for (int g = 0; g < NW; g++) vscale[g] = 0x71807180u;  // 2^100; steps are 2^-84 or more
 #pragma unroll
         for (int h = 0; h < HPL; h++) {
-            m_run[h] = -INFINITY;
+            m_run[h] = -kLargest;  // finite: scores that overflowed to -infinity weigh nothing, also where a tile has no others
             l_run[h] = 0.f;
         }
         int pos0 = pos_first + warp * kQ4Tile * kPageTokens;
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                         mx -= 11.f;
-                        fix[h] = m_run[h] == -INFINITY ? 0.f : exp2_fast(m_run[h] - mx);
+                        fix[h] = exp2_fast(m_run[h] - mx);
                         m_run[h] = mx;
                         l_run[h] *= fix[h];
                     }

@@ -228,3 +228,22 @@ def test_the_example_of_the_readme_follows_the_tensors(ctx):
     stream.synchronize()
     check_attention(out.cpu().numpy().reshape(32, 128), q[0], q4.held(k), q4.held(v))
     names["cache"].close()
+
+
+# Scores beyond FP32 below zero weigh nothing: the result is the mean of the other positions' rows, whose keys are zero.  What the kernel rounds: weights of 2^11 each are
+# exact, their products with steps in two limbs 2^-22, the sums of 16 positions a tile and of tiles, warps and parts 2^-24 each, fewer than 30 of them in a row:
+# below 2^-18 of terms of up to 3 times the largest value.
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (4, 1, 128), (8, 1, 128)])
+@pytest.mark.parametrize("n,bad", [(300, 64), (300, 299), (40, 33), (20000, 15000)])
+def test_scores_that_overflow_below_zero(ctx, heads, kv, dim, n, bad):
+    rng = np.random.default_rng(58)
+    cache = PagedKvCache(ctx, 1, kv, dim, n // 16 + 1, "q4")
+    s = cache.new_sequence(n)
+    k, v = np.zeros((n, kv, dim), np.float32), f32(rng.standard_normal((n, kv, dim)))
+    k[:bad] = -60000.0
+    fill(cache, 0, [s], [0], [(k, v)])
+    q = np.full((1, heads, dim), 1e37, np.float32)
+    want = np.repeat(q4.held(v)[bad:].mean(0), heads // kv, 0)
+    got = attend(cache, 0, [s], q)[0]
+    assert np.abs(got - want).max() <= 3 * 2.0 ** -18 * np.abs(v).max()
+    cache.close()
