@@ -130,7 +130,8 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 //   O += V P  rows are dimensions, k the positions, columns heads; a weight is multiplied by the step of its position and group first, and the offsets' part
 //             is a sum of its own per lane, in FP32.  The product is scaled by a power of two that follows the largest step of its group, so that it keeps its digits in
 //             FP16 (one scale for all groups: where one group's values were 10^6 times another's, the smaller ones were 5e-3 of their size off; its own for each
-//             takes 43.7 us instead of 42.2 for 131072 positions).  What is left: a position whose step in a group is R times the others' costs them R 2^-30.
+//             takes 43.7 us instead of 42.2 for 131072 positions).  What is left: a position whose step in a group is R times the others' costs them
+//             some R 2^-30 (one of 10^4 times their size that weighs nothing: 2e-5 of the result).
 //             The numbers of half the positions count from the other end (q4_v_flip), those positions' products have a minus: the sums stay as small as
 //             the result, where sums of numbers that are all positive would be larger than it by the root of the number of positions that count.
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to

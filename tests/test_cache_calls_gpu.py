@@ -247,3 +247,26 @@ def test_scores_that_overflow_below_zero(ctx, heads, kv, dim, n, bad):
     got = attend(cache, 0, [s], q)[0]
     assert np.abs(got - want).max() <= 3 * 2.0 ** -18 * np.abs(v).max()
     cache.close()
+
+
+# Short contexts, every number of heads to a key/value head, rows whole and cut across, by the result's length in each group of a head's dimensions.  A score has up to nine
+# sums and products in FP32, each off by 2^-24 of terms up to 30 in size: a weight by 1.6e-5 at most, the limbs of queries, weights and steps add 2^-22 each.  Over positions
+# and dimensions that goes both ways; 2e-5 is ten times what such sums are off together.
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("kv,dim", [(2, 64), (2, 128)])
+def test_digits_of_every_group_size(ctx, kv, dim, G):
+    rng = np.random.default_rng(59 + G)
+    lens = [1, 15, 16, 17, 33, 256, 300, 1000, 2500]
+    heads = kv * G
+    cache = PagedKvCache(ctx, 1, kv, dim, sum(n // 16 + 1 for n in lens), "q4")
+    seqs = [cache.new_sequence(n) for n in lens]
+    parts = [(rows(rng, n, kv, dim), f32(rng.standard_normal((n, kv, dim)))) for n in lens]
+    fill(cache, 0, seqs, [0] * len(lens), parts)
+    q = f32(1.5 * rng.standard_normal((len(lens), heads, dim)))
+    whole = [attend(cache, 0, [s], q[i:i + 1])[0] for i, s in enumerate(seqs)]
+    for out in (attend(cache, 0, seqs, q), whole):
+        for i, (k, v) in enumerate(parts):
+            want, _ = q4.attention(q[i], q4.held(k), q4.held(v))
+            norm = lambda x: np.linalg.norm(x.reshape(heads, -1, 32), axis=-1)  # noqa: E731
+            assert (norm(out[i] - want) <= 2e-5 * norm(want)).all(), (lens[i], (norm(out[i] - want) / norm(want)).max())
+    cache.close()
