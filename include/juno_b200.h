@@ -172,7 +172,8 @@ int juno_attn_decode_static(juno_ctx *ctx, juno_kvpool *p, int32_t layer, int32_
  * handles) and the call returns before it is done.  Calls of one context take effect in the order in which they are made, whatever their
  * streams are: a call on another stream waits for what the context's stream has, and the context's stream waits for it.  The caller's own
  * work on q, k, v and results is ordered by that stream only.  A stream that is being captured, or one of another device, gives
- * JUNO_ERR_INVALID_ARG: a graph would hold the page table of the moment.  Working memory belongs to the context and grows with the largest
+ * JUNO_ERR_INVALID_ARG: a graph would hold the page table of the moment (juno_seq_fork, juno_seq_track and the host-memory calls above,
+ * too, while the context's stream is captured).  Working memory belongs to the context and grows with the largest
  * call, to twice its size at least; a call that makes it grow waits for the device.  Arrays of sequences, positions, counts and lengths are host memory and are not used after the call.  n <= 4096.
  * Not for pools of a model. */
 

@@ -1302,6 +1302,7 @@ static int seq_fork(juno_seq *src, int32_t n_tokens, juno_seq **out) {
     JUNO_TRY(ctx_check(p->ctx));
     JUNO_REQUIRE(n_tokens >= 0 && n_tokens <= src->len, "cannot share %d positions of a sequence that holds %d", n_tokens, src->len);
     DeviceGuard g(p->ctx->device);
+    if (!p->owned_by_model) JUNO_TRY(cache_call_outside_graph(p->ctx));
     JUNO_TRY(seq_resume_check(p, src->len, n_tokens));
     const int n_pg = (n_tokens + kPageTokens - 1) / kPageTokens;
     std::vector<int> pages(src->pages.begin(), src->pages.begin() + n_pg);
@@ -1385,6 +1386,7 @@ int juno_seq_track(juno_seq *s) {
     JUNO_REQUIRE(s->pool->weights, "the pool keeps no weights (juno_kvpool_track)");
     JUNO_REQUIRE(s->track < 0, "this sequence keeps its weights already");
     DeviceGuard g(s->pool->ctx->device);
+    JUNO_TRY(cache_call_outside_graph(s->pool->ctx));
     return seq_track(s, nullptr);
 }
 
@@ -1409,6 +1411,7 @@ static int append_kv(juno_seq *s, int layer, int pos, int n_tokens, const float 
     JUNO_REQUIRE((int64_t)pos + n_tokens <= s->max_tokens, "position %lld is beyond this sequence's limit of %d", (long long)pos + n_tokens - 1, s->max_tokens);
     JUNO_REQUIRE(p->dtype != kKvQ4 || pos <= s->len, "position %d is not behind the %d cached ones", pos, s->len);
     DeviceGuard g(c->device);
+    JUNO_TRY(cache_call_outside_graph(c));
     JUNO_TRY(seq_reserve(s, pos, pos + n_tokens, c->stream));
     const int kvdim = p->n_kv_heads * p->head_dim;
     const size_t bytes = (size_t)n_tokens * kvdim * sizeof(float);
@@ -1469,6 +1472,7 @@ static int attn_decode(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *
         max_len = std::max(max_len, seqs[i]->len);
     }
     JUNO_TRY(cache_call_distinct(p, n, seqs, true));  // two rows of one sequence would add to the same weights side by side
+    JUNO_TRY(cache_call_outside_graph(c));
     const int hd = p->head_dim, qdim = n_heads * hd;
     const size_t qbytes = (size_t)n * qdim * sizeof(float);
     if (p->dtype == kKvQ4) {

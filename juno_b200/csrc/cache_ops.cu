@@ -15,16 +15,25 @@ namespace juno {
 // ───────────────────────────── what the calls share ───────────────────────────────────────
 CacheStream::CacheStream(juno_ctx *c, void *stream) : st(stream ? (cudaStream_t)stream : c->stream), c_(c) { status = join(); }
 
-int CacheStream::join() {
-    auto refuse = [](int rc, const char *what) {
-        cudaGetLastError();
-        set_error("%s", what);
-        return rc;
-    };
+static int refuse(int rc, const char *what) {
+    cudaGetLastError();
+    set_error("%s", what);
+    return rc;
+}
+
+int cache_call_outside_graph(const juno_ctx *c) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(c_->stream, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone)
+    const cudaError_t e = cudaStreamIsCapturing(c->stream, &cap);
+    if (e != cudaSuccess) cudaGetLastError();  // but for a capture elsewhere that this stream would join, what is wrong shows in the next call
+    if (e == cudaErrorStreamCaptureImplicit || (e == cudaSuccess && cap != cudaStreamCaptureStatusNone))
         return refuse(JUNO_ERR_INVALID_ARG, "the context's stream is being captured: calls on cache pages cannot be part of a graph");
+    return JUNO_OK;
+}
+
+int CacheStream::join() {
+    JUNO_TRY(cache_call_outside_graph(c_));
     if (st == c_->stream) return JUNO_OK;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone)
         return refuse(JUNO_ERR_INVALID_ARG, "the stream is being captured: calls on cache pages cannot be part of a graph");
     int dev = -1;

@@ -54,6 +54,8 @@ private:
     bool joined_ = false;
 };
 
+// JUNO_ERR_INVALID_ARG while the context's stream is being captured: changes of the page table would be part of the graph, and be missing where they are due.
+int cache_call_outside_graph(const juno_ctx *c);
 // What every such call requires of its handles; a call that writes to a sequence has each one once.
 int cache_call_check(juno_ctx *c, juno_kvpool *p, int layer, int n, juno_seq *const *seqs);
 // weights_only: sequences that keep no weights may be there several times

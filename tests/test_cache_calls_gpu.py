@@ -270,3 +270,37 @@ def test_digits_of_every_group_size(ctx, kv, dim, G):
             norm = lambda x: np.linalg.norm(x.reshape(heads, -1, 32), axis=-1)  # noqa: E731
             assert (norm(out[i] - want) <= 2e-5 * norm(want)).all(), (lens[i], (norm(out[i] - want) / norm(want)).max())
     cache.close()
+
+
+def test_nothing_of_a_cache_goes_into_a_graph_of_the_contexts_stream(ctx):
+    """Forks, tracking and the host-memory calls change page tables on that stream: refused while it is captured, and as usual afterwards."""
+    rng = np.random.default_rng(60)
+    handle = C.c_void_p()
+    own = GpuContext(0)
+    assert own._L.juno_ctx_stream(own.handle, C.byref(handle)) == 0
+    stream = torch.cuda.ExternalStream(handle.value)
+    cache = PagedKvCache(own, 1, 2, 64, 16, "q4", track_seqs=2, track_tokens=64)
+    s, t = cache.new_sequence(64), cache.new_sequence(64, track=True)
+    k = rows(rng, 40, 2, 64)
+    cache.append(s, 0, 0, k.reshape(40, -1), k.reshape(40, -1))
+    q = f32(rng.standard_normal((1, 8, 64)))
+    x = torch.zeros(4, device="cuda")
+    settle()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream, capture_error_mode="relaxed"):
+        y = x + 1
+        for call in (lambda: cache.fork(s, 20), lambda: cache.fork(t, 0), lambda: cache.new_sequence(64, track=True), lambda: cache.attention(0, [s], q.reshape(1, -1), 8),
+                     lambda: cache.append(s, 0, 40, k[:8].reshape(8, -1), k[:8].reshape(8, -1)), lambda: cache.evict([t], 1)):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+    g.replay()
+    settle()
+    assert (y == 1).all() and cache.length(s) == 40
+    b = cache.fork(s, 20)
+    cache.append(b, 0, 20, k[:8].reshape(8, -1), k[:8].reshape(8, -1))
+    both = np.concatenate([k[:20], k[:8]])
+    check_attention(cache.attention(0, [b], q.reshape(1, -1), 8).reshape(8, 64), q[0], q4.held(both), q4.held(both))
+    cache.free_sequence(cache.new_sequence(64, track=True))
+    del g
+    cache.close()
+    own.close()
