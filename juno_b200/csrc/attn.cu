@@ -1062,37 +1062,22 @@ int seq_create(juno_kvpool *p, int max_tokens, juno_seq **out) {
 
 // Entries [lo, hi] of the sequence's row of the page table, from the mirror to the device.  The calls on a pool of its own return before the device
 // is done with them, and the mirror may have changed again by then: the entries travel with the launch.  A model's calls wait for their work.
-struct TableWords {
-    int32_t v[2000];  // 8 KB of parameters
-};
-static __global__ void table_store_kernel(int32_t *dst, const __grid_constant__ TableWords w, int n) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = w.v[i];
-}
 int table_store(const juno_kvpool *p, int slot, int lo, int hi, cudaStream_t st) {
     const size_t at = (size_t)slot * p->max_pages_per_seq;
     if (p->latent || p->owned_by_model) {
         JUNO_CUDA_TRY(cudaMemcpyAsync(p->d_table + at + lo, p->h_table + at + lo, (size_t)(hi - lo + 1) * sizeof(int32_t), cudaMemcpyHostToDevice, st));
         return JUNO_OK;
     }
-    constexpr int kWords = (int)(sizeof(TableWords) / sizeof(int32_t));
-    for (; lo <= hi; lo += kWords) {
-        TableWords w;
-        const int n = std::min(kWords, hi - lo + 1);
-        memcpy(w.v, p->h_table + at + lo, (size_t)n * sizeof(int32_t));
-        table_store_kernel<<<1, 256, 0, st>>>(p->d_table + at + lo, w, n);
-        JUNO_CUDA_TRY(cudaGetLastError());
-        p->ctx->kernel_launches++;
-    }
-    return JUNO_OK;
+    return cache_words(p->ctx, p->h_table + at + lo, (size_t)(hi - lo + 1), p->d_table + at + lo, st);
 }
 
-static __global__ void table_pairs_kernel(int32_t *table, const __grid_constant__ TableWords w, int n) {
+static __global__ void table_pairs_kernel(int32_t *table, const __grid_constant__ WordsByValue w, int n) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) table[w.v[2 * i]] = w.v[2 * i + 1];
 }
 int table_store_pairs(const juno_kvpool *p, const std::vector<int32_t> &pairs, cudaStream_t st) {
-    constexpr size_t kWords = sizeof(TableWords) / sizeof(int32_t);
+    constexpr size_t kWords = sizeof(WordsByValue) / sizeof(int32_t);
     for (size_t at = 0; at < pairs.size(); at += kWords) {
-        TableWords w;
+        WordsByValue w;
         const size_t n = std::min(kWords, pairs.size() - at);
         memcpy(w.v, pairs.data() + at, n * sizeof(int32_t));
         table_pairs_kernel<<<1, 256, 0, st>>>(p->d_table, w, (int)(n / 2));
@@ -1182,7 +1167,7 @@ int seq_reserve(juno_seq *s, int from, int upto, cudaStream_t st, std::vector<in
 }
 
 // A sequence's weights, one plane of `room` (a multiple of 16) positions for each layer and head: the first `len` of another one's, zeros behind.
-static __global__ void track_kernel(float *own, const float *from, int room, int len, int32_t *table, const __grid_constant__ TableWords w, int n) {
+static __global__ void track_kernel(float *own, const float *from, int room, int len, int32_t *table, const __grid_constant__ WordsByValue w, int n) {
     if (blockIdx.x == 0 && blockIdx.y == 0)
         for (int i = threadIdx.x; i < n; i += blockDim.x) table[i] = w.v[i];
     const int pos = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -1210,10 +1195,10 @@ static int seq_track(juno_seq *s, const juno_seq *src) {
     const size_t planes = (size_t)p->n_layers * p->n_kv_heads;
     float *own = p->weights + track * p->track_stride();
     const dim3 grid((unsigned)((p->track_tokens / 4 + 255) / 256), (unsigned)planes);
-    constexpr size_t kWords = sizeof(TableWords) / sizeof(int32_t);
+    constexpr size_t kWords = sizeof(WordsByValue) / sizeof(int32_t);
     const size_t at = (size_t)s->slot * p->max_pages_per_seq, n = src ? std::min(s->pages.size(), kWords) : 0;
     if (src && s->pages.size() > kWords) JUNO_TRY(table_store(p, s->slot, (int)kWords, (int)s->pages.size() - 1, p->ctx->stream));
-    TableWords w;
+    WordsByValue w;
     memcpy(w.v, p->h_table + at, n * sizeof(int32_t));
     track_kernel<<<grid, 256, 0, p->ctx->stream>>>(own, src ? p->weights + src->track * p->track_stride() : nullptr, p->track_tokens, src ? s->len : 0, p->d_table + at, w,
                                                    (int)n);

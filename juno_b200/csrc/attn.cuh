@@ -4,6 +4,10 @@
 
 #include "common.cuh"
 
+namespace juno {
+constexpr int kKvQ4 = 3;  // juno_kvpool::dtype of 4-bit pages
+}
+
 // Page layout (both K and V): [layer][page][kv_head][page_tokens=16][head_dim], FP16 or FP32.  A 4-bit pool has the keys and values of a head and
 // page in one block (q4_pages.cuh): [layer][page][kv_head][block] in `k`, `v` is null.
 //
@@ -38,9 +42,9 @@ struct juno_kvpool {
     int track_tokens = 0;
     std::vector<int> free_tracks;
     // bytes of a cached position and key/value head, key and value together
-    double row_bytes() const { return dtype == 3 ? 1.25 * head_dim : 2.0 * head_dim * elem_bytes; }
+    double row_bytes() const { return dtype == juno::kKvQ4 ? 1.25 * head_dim : 2.0 * head_dim * elem_bytes; }
     // bytes of a page and layer: of keys and of values each, of both together for 4 bits
-    size_t page_bytes() const { return (size_t)n_kv_heads * head_dim * (dtype == 3 ? 20 : page_tokens * elem_bytes); }
+    size_t page_bytes() const { return (size_t)n_kv_heads * head_dim * (dtype == juno::kKvQ4 ? 20 : page_tokens * elem_bytes); }
     size_t track_stride() const { return (size_t)n_layers * n_kv_heads * track_tokens; }
 };
 

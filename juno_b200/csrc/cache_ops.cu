@@ -79,10 +79,6 @@ int cache_scratch(juno_ctx *c, size_t bytes, uint8_t **out) {
     return JUNO_OK;
 }
 
-// By value: neither the caller's memory nor a staging buffer has to outlive the call.
-struct WordsByValue {
-    int32_t v[2000];  // 8 KB of parameters
-};
 static __global__ void words_kernel(int32_t *dst, const __grid_constant__ WordsByValue w, int n) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = w.v[i];
 }

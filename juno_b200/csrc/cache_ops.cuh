@@ -69,7 +69,11 @@ int cache_room(void **ptr, size_t *cur, size_t bytes);
 // Fills `out` for `n` rows; `far`: room for them in the working memory when they are more than kInlineRows.
 int cache_rows(juno_ctx *c, const CacheRow *rows, int n, CacheRow *far, CacheRows *out, cudaStream_t st);
 inline size_t cache_rows_bytes(int n) { return n > kInlineRows ? ((size_t)n * sizeof(CacheRow) + 255) & ~(size_t)255 : 0; }
-// The same for whole numbers that a kernel reads from memory.
+// Whole numbers that travel with a launch: neither the caller's memory nor a staging buffer has to outlive the call.
+struct WordsByValue {
+    int32_t v[2000];  // 8 KB of parameters
+};
+// Whole numbers to device memory.
 int cache_words(juno_ctx *c, const int32_t *words, size_t n, int32_t *dst, cudaStream_t st);
 
 // Rows [n_tokens][ld] of keys and values into the pages: row j belongs to the sequence of `rows` that holds unit j.  The pages exist and are writable.

@@ -29,7 +29,6 @@
 namespace juno {
 
 constexpr int kQ4Group = 32;
-constexpr int kKvQ4 = 3;  // juno_kvpool::dtype
 
 JHD int q4_block_bytes(int hd) { return 20 * hd; }
 JHD int q4_k_code(int hd, int p, int t, int g) { return ((p * 4 + t) * (hd / kQ4Group) + g) * 4; }
