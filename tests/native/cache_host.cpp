@@ -202,6 +202,7 @@ static int freed() {
 }
 
 int main(int argc, char **argv) {
+    setenv("CUDA_VISIBLE_DEVICES", "", 1);  // the pools' device memory does not exist: nothing may be launched, on a machine with a GPU neither
     const struct {
         const char *name;
         int (*run)();

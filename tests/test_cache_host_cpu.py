@@ -20,7 +20,7 @@ def host():
     assert lib == _lib.LIB_PATH
 
     def run(name):
-        r = subprocess.run([EXE, name], capture_output=True, text=True, timeout=120)
+        r = subprocess.run([EXE, name], capture_output=True, text=True, timeout=120, env=os.environ | {"CUDA_VISIBLE_DEVICES": ""})
         assert r.returncode == 0, r.stdout + r.stderr
     return run
 
