@@ -476,15 +476,16 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 }
                 // a score far above the reference, or a step beyond its group's scale: seldom after the first tile
                 float top[HPL];
-                bool grown = false;
+                uint32_t beyond = 0u;
 #pragma unroll
                 for (int g = 0; g < NW; g++) {
                     const uint32_t limit = kStepLimits - vscale[g];
                     steps[g] = limit;
 #pragma unroll
                     for (int u = 0; u < kQ4Tile; u++) steps[g] = __vmaxu2(steps[g], __vmaxu2(d[u][0][g], d[u][1][g]));
-                    grown |= steps[g] != limit;
+                    beyond |= steps[g] ^ limit;
                 }
+                bool grown = beyond != 0u;
 #pragma unroll
                 for (int h = 0; h < HPL; h++) {
                     top[h] = s[h][0][0];
@@ -494,17 +495,21 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
                 }
                 if (__any_sync(0xffffffffu, grown)) {
                     float fix[HPL], vfix[NG];
+                    uint32_t most[NG];
 #pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        const int half = 16 * (g & 1);
-                        const uint32_t step = __reduce_max_sync(0xffffffffu, steps[g >> 1] >> half & 0xffffu);
-                        vfix[g] = 1.f;
-                        const uint32_t before = vscale[g >> 1] >> half & 0xffffu;
-                        if (step > (kStepLimits & 0xffffu) - before) {  // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
-                            const uint32_t next = (249u - (step >> 7)) << 7;  // 2^-5 over the step's power of two
-                            vscale[g >> 1] += (next - before) << half;
-                            vfix[g] = __uint_as_float((0x3f80u + next - before) << 16);
+                    for (int g = 0; g < NG; g++) most[g] = __reduce_max_sync(0xffffffffu, steps[g >> 1] >> 16 * (g & 1) & 0xffffu);
+#pragma unroll
+                    for (int w = 0; w < NW; w++) {
+                        uint32_t next = 0u;
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const uint32_t before = vscale[w] >> 16 * x & 0xffffu, step = most[2 * w + x];
+                            // the largest step to 2^-5 .. 2^-4, up to 1 in range: times weights of up to 2^15
+                            const uint32_t now = step > (kStepLimits & 0xffffu) - before ? (249u - (step >> 7)) << 7 : before;
+                            next |= now << 16 * x;
+                            vfix[2 * w + x] = __uint_as_float((0x3f80u + now - before) << 16);
                         }
+                        vscale[w] = next;
                     }
 #pragma unroll
                     for (int h = 0; h < HPL; h++) {
