@@ -155,7 +155,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // A CTA has R positions, of keys (blockIdx.y = 0) or values.  A lane has eight neighbouring dimensions, four lanes a group: what is stored of a position is
 // contiguous.  The arithmetic is what bounds it, so each element costs a dozen instructions: the number is found from an estimate
 // (q4_number_near: a saturating product and one sum that rounds), and only where a lane has an estimate too close to half-way are its eight numbers decided
-// exactly.  131072 positions of eight heads of 128: 1.24 GB in 250 us, 5.0 TB/s; 8156 of them 77 MB in 24 us.
+// exactly.  131000 positions of eight heads of 128: 1.24 GB in 235 us, 5.3 TB/s; 8156 of them 77 MB in 23 us.
 template <int HD, int R, bool V>
 __device__ __forceinline__ void append_rows(const RowsParams &p, const RowPlace (&places)[R], int row0) {
     constexpr int LPV = HD / 8;  // lanes per vector
@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(256) q4_append_kernel(const __grid_constant__ 
 __device__ __forceinline__ float bits_as_float(uint32_t w, uint32_t mask) { return __uint_as_float((w & mask) | 0x4b000000u) - 8388608.f; }
 
 // A CTA has kReadRows positions, of keys (blockIdx.y = 0) or values; a lane has eight neighbouring dimensions, which it writes at once where they are aligned, and
-// the loads of all positions are under way together.  8156 positions of eight heads of 128, 77 MB, with their append: 33.7 us (four dimensions of two groups a lane
-// 34.2, of one group 34.9).
+// the loads of all positions are under way together.  8156 positions of eight heads of 128, 77 MB, with their append: 32.0 us (0.5 more with four dimensions of two groups a
+// lane, 1.2 more of one group).
 constexpr int kAppendRows = 4, kReadRows = 4;
 __device__ __forceinline__ void store8(float *to, const float (&x)[8], int wide) {
     if (wide == 2) {

@@ -56,7 +56,7 @@ constexpr int kQ4Ctas = HPL == 1 || HD == 64 ? 2 : 3;
 // Tiles whose products are added up in an MMA's sums.  An MMA cuts off what lies more than 24 bits below its largest term or sum, always towards zero, so
 // that a long chain of them falls behind by some 2^-25 of the sum a time: 48 requests of 8192 positions were 5.8e-6 of the result off without a limit, where one
 // request of 2048 is 6e-7 off; they are 1.2e-6 off with chains of 16 to 24 MMAs, whose sums then go to FP32 ones in shared memory (FP32 throughout is 1.0 to 1.8e-6 off).
-// 131072 positions take 41.6 us so and 41.0 with chains twice as long.
+// Chains twice as long save 0.6 us of 131072 positions.
 template <int HD, int HPL>
 constexpr int kQ4Chain = HPL == 1 ? 8 : HD == 64 ? 4 : 6;
 
@@ -130,17 +130,17 @@ __device__ __forceinline__ float upper_limb(float x) { return __uint_as_float(__
 //   O += V P  rows are dimensions, k the positions, columns heads; a weight is multiplied by the step of its position and group first, and the offsets' part
 //             is a sum of its own per lane, in FP32.  The product is scaled by a power of two that follows the largest step of its group, so that it keeps its digits in
 //             FP16 (one scale for all groups: where one group's values were 10^6 times another's, the smaller ones were 5e-3 of their size off; its own for each
-//             takes 43.7 us instead of 42.2 for 131072 positions).  What is left: a position whose step in a group is R times the others' costs them
+//             takes 43.5 us instead of 42.4 for 131072 positions).  What is left: a position whose step in a group is R times the others' costs them
 //             some R 2^-30 (one of 10^4 times their size that weighs nothing: 2e-5 of the result).
 //             The numbers of half the positions count from the other end (q4_v_flip), those positions' products have a minus: the sums stay as small as
 //             the result, where sums of numbers that are all positive would be larger than it by the root of the number of positions that count.
 // Queries and weights are two FP16 limbs.  HPL = 1: up to four heads, columns 2h and 2h + 1 are the limbs of head h, and a lane has one head.  HPL = 2: up to
-// eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.  Four heads of 131072 positions take 41 us as the former, 60 as the latter.
+// eight heads, a column each, the limbs in MMAs of their own; a lane has two heads.  Four heads of 131072 positions took 41 us as the former, 60 as the latter.
 // Scores come out of an MMA with positions in the rows and go into the next with positions along k: movmatrix turns them.
-// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and it takes 360 of them (four heads of 128, of
-// which 17 MMAs) or 440 (eight, 34) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
-// over 8 of 128: 41 us for 168 MB, 4.1 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 15.7, of which 10 begin and end
-// parts; 48 of up to 8192 with eight heads to a key/value head 117 us for 384 MB.
+// What bounds it: instructions.  A page of a head is 2560 bytes, 1.0 us of an SM's share of 6.55 TB/s for 17 pages, and it takes 368 of them (four heads of 128, of
+// which 17 MMAs) or 455 (eight, 34) a warp; with less arithmetic the same kernel streams the pages of 131072 positions in 34 us.  One request of 131072 positions, 32 heads
+// over 8 of 128: 43.4 us for 168 MB, 3.9 TB/s (FP16 pages would be 537 MB, 82 us at the rate of a copy); 8 requests of up to 4096 16.5, of which 10 begin and end
+// parts; 48 of up to 8192 with eight heads to a key/value head 118 us for 384 MB.
 template <int HD, int HPL>
 struct Q4Smem {  // bytes
     static constexpr int kRing = kQ4Warps<HD, HPL> * kQ4Slots * kQ4Tile * 20 * HD, kBars = kRing, kMerge = kBars + kQ4Warps<HD, HPL> * kQ4Slots * 8, kMergeRow = HD + 8,  // floats; the pads keep rows on different banks
@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(kQ4Warps<HD, HPL> * 32, kQ4Ctas<HD, HPL>) q4_a
 }
 
 // The weight that positions have received: a thread has four neighbouring positions of all rows' pages and one key/value head, 64 bytes of scores with four heads, which
-// come out of L2.  Attention and weights of 16 sequences of up to 8192 positions: 50.1 us, 51.8 with one position a thread.
+// come out of L2.  Attention and weights of 16 sequences of up to 8192 positions: 50.2 us, some 1.7 more with one position a thread.
 constexpr int kQ4WeightThreads = 128;
 __global__ void __launch_bounds__(kQ4WeightThreads) q4_weights_kernel(const __grid_constant__ Q4AttnParams p) {
     pdl_wait();
