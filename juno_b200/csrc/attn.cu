@@ -911,10 +911,6 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
     JUNO_REQUIRE(dtype != kKvQ4 || (int64_t)n_pages * n_kv_heads * q4_block_bytes(head_dim) < (1ll << 36), "a layer of 4-bit pages has up to 64 GB");
     std::unique_ptr<juno_kvpool> held(new juno_kvpool());
     juno_kvpool *p = held.get();
-    p->free_pages.reserve(n_pages);
-    for (int i = n_pages - 1; i >= 0; i--) p->free_pages.push_back(i);
-    p->page_refs.assign((size_t)n_pages, 0);
-    for (int i = max_slots - 1; i >= 0; i--) p->free_slots.push_back(i);
     p->magic = kMagicPool;
     p->ctx = ctx;
     p->n_layers = n_layers;
@@ -939,14 +935,21 @@ int kvpool_create(juno_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int
     if (e == cudaSuccess) e = cudaMemsetAsync(p->k, 0, bytes, ctx->stream);
     if (e == cudaSuccess && p->v) e = cudaMemsetAsync(p->v, 0, bytes, ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
-    if (e != cudaSuccess) {
+    const int listed = e != cudaSuccess ? JUNO_OK : guarded([&]() -> int {  // once the device has the room: the lists are as long as the pool
+        p->free_pages.reserve(n_pages);
+        for (int i = n_pages - 1; i >= 0; i--) p->free_pages.push_back(i);
+        p->page_refs.assign((size_t)n_pages, 0);
+        for (int i = max_slots - 1; i >= 0; i--) p->free_slots.push_back(i);
+        return JUNO_OK;
+    });
+    if (e != cudaSuccess || listed != JUNO_OK) {
         cudaGetLastError();
-        set_error("cudaMalloc of the KV pool (%s%zu bytes) failed: %s", dtype == kKvQ4 ? "" : "2 x ", bytes, cudaGetErrorString(e));
+        if (listed == JUNO_OK) set_error("cudaMalloc of the KV pool (%s%zu bytes) failed: %s", dtype == kKvQ4 ? "" : "2 x ", bytes, cudaGetErrorString(e));
         if (p->k) cudaFree(p->k);
         if (p->v) cudaFree(p->v);
         if (p->d_table) cudaFree(p->d_table);
         if (p->h_table) cudaFreeHost(p->h_table);
-        return e == cudaErrorMemoryAllocation ? JUNO_ERR_OOM : JUNO_ERR_CUDA;
+        return listed != JUNO_OK ? listed : e == cudaErrorMemoryAllocation ? JUNO_ERR_OOM : JUNO_ERR_CUDA;
     }
     memset(p->h_table, 0, tbytes);
     *out = held.release();

@@ -201,12 +201,23 @@ static int freed() {
     return 0;
 }
 
+// The lists of a pool are as long as it: they are made once the device has room for its pages, so that a pool that is far too large costs the host nothing.
+static int huge() {
+    Pool p(0);
+    juno_kvpool *q = nullptr;
+    g_left = 1;  // the pool itself
+    const int rc = juno_kvpool_create(&p.ctx, 1, 1, 64, 2000000000, 0, &q);
+    g_left = -1;
+    WANT(rc != JUNO_OK && !q && strstr(juno_last_error(), "cudaMalloc of the KV pool"));
+    return 0;
+}
+
 int main(int argc, char **argv) {
     setenv("CUDA_VISIBLE_DEVICES", "", 1);  // the pools' device memory does not exist: nothing may be launched, on a machine with a GPU neither
     const struct {
         const char *name;
         int (*run)();
-    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}, {"memory", memory}, {"freed", freed}};
+    } checks[] = {{"twice", twice}, {"beside", beside}, {"closed", closed}, {"far", far}, {"memory", memory}, {"freed", freed}, {"huge", huge}};
     for (const auto &c : checks)
         if (argc == 2 && !strcmp(argv[1], c.name)) return c.run();
     printf("no such check\n");

@@ -47,3 +47,7 @@ def test_host_memory_that_runs_out_is_an_error_and_changes_nothing(host):
 
 def test_a_freed_sequence_gives_its_list_of_pages_back(host):
     host("freed")
+
+
+def test_a_pool_that_is_far_too_large_costs_the_host_nothing(host):
+    host("huge")
